@@ -54,6 +54,7 @@ typedef int rfsn_status;
 #define RFSN_F32 0
 #define RFSN_F16 1
 #define RFSN_BF16 2
+#define RFSN_E4M3 3 /* 8-bit floating point (4 exponent, 3 mantissa bits, no infinity): packed archives only */
 
 /* Keys per attention tile. Page-table tile prefix sums are in these units. */
 #define RFSN_TILE_KEYS 64
@@ -430,6 +431,124 @@ RFSN_API rfsn_status rfsn_paged_attention_peer(const rfsn_arena* arena,
                                                float* out, float* lse,
                                                void* workspace, size_t workspace_bytes,
                                                int max_splits, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Packed archive: archived blocks in 8 bits, one power-of-two scale for each
+ * (64-token tile, KV head) of K and of V. No counterpart in the reference
+ * (its blocks keep the cache dtype, cache.py:324-339); a cache that opts in
+ * halves the bytes an attention call has to read.
+ *
+ * For a tile with a = max |x| over its finite elements the scale is the
+ * smallest power of two s with a / s <= 448 (1 when a = 0), the codes are
+ * e4m3(x / s), rounded to nearest even. x / s is exact, so an element is off
+ * by at most half an e4m3 step (2^-4 of its magnitude, or s * 2^-10 for
+ * subnormal codes). NaN stays NaN; an infinity becomes NaN.
+ *
+ * k_codes, v_codes: device uint8 [batch_kv_heads][rows][head_dim], scales:
+ * device float32 [batch_kv_heads][rows / 64][4] = {K scale, V scale, 0, 0}.
+ * All 16-byte aligned; rows a multiple of 64; head_dim 64 or 128. A block
+ * starts at a row that is a multiple of 64 and owns its last tile whole: the
+ * rows of that tile behind the block's last token must hold zero codes
+ * (rfsn_pack_rows writes them).
+ * ---------------------------------------------------------------------- */
+typedef struct rfsn_packed_archive rfsn_packed_archive;
+
+RFSN_API rfsn_status rfsn_packed_archive_create(void* k_codes, void* v_codes, float* scales, int batch_kv_heads,
+                                                int rows, int head_dim, rfsn_packed_archive** out);
+RFSN_API rfsn_status rfsn_packed_archive_destroy(rfsn_packed_archive* archive);
+
+/* K/V rows to pack: element [b][h][i] of a token i is at base + b * stride_b +
+ * h * stride_h + row(i) * stride_t (elements; innermost stride 1), row(i) =
+ * offset + i, modulo wrap when wrap > 0 (a ring whose oldest token is at
+ * offset). dtype RFSN_F32 / F16 / BF16. */
+typedef struct rfsn_kv_rows {
+    const void* k; /* device */
+    const void* v;
+    int64_t k_stride_b, k_stride_h, k_stride_t;
+    int64_t v_stride_b, v_stride_h, v_stride_t;
+    int32_t dtype;
+    int32_t kv_heads;
+    int32_t offset;
+    int32_t wrap;
+} rfsn_kv_rows;
+
+/* Pack count tokens into archive rows dst_row0 .. (dst_row0 a multiple of 64),
+ * in tiles of 64 from the first token on; the rest of the last tile is zeroed.
+ * bounds (optional): device uint8 [batch_kv_heads][rows / 64][2][head_dim],
+ * receives the smallest and the largest K code of each channel of each tile
+ * (for rfsn_select_tiles). Counterpart of the seal copy, cache.py:324-339. */
+RFSN_API rfsn_status rfsn_pack_rows(const rfsn_packed_archive* archive, int dst_row0, const rfsn_kv_rows* src,
+                                    int count, void* bounds, void* stream);
+
+/* code * scale of count rows from src_row0 on, rounded once to out_dtype (exact
+ * in float32 and bfloat16; saturating in float16), to k_out / v_out: device,
+ * 16-byte aligned, row r of (batch, kv head) g at g * out_stride + r * head_dim
+ * (out_stride in elements, its bytes a multiple of 16). */
+RFSN_API rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* archive, int src_row0, int count, void* k_out,
+                                      void* v_out, int out_dtype, int64_t out_stride, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention to a list of archived tiles and the hot window. Semantics and
+ * q / out / lse / hot / workspace conventions of rfsn_paged_attention, except:
+ *   - the archived keys are the listed tiles: of `packed` when it is given
+ *     (K = code * scale, V = code * scale), else of `arena` itself;
+ *   - the hot window is always `arena`'s (the cache's 16-bit type);
+ *   - head_dim 64 or 128, bf16/f16 arenas; any q_len and GQA ratio, with
+ *     K/V read again for every 8 query slots (q_len * q_heads / kv_heads).
+ * Scores are accurate to float32 rounding (q and p are split into two float16
+ * or three bfloat16 terms for the tensor cores).
+ * ---------------------------------------------------------------------- */
+typedef struct rfsn_tile_list {
+    const int32_t* tiles; /* device int32 [n][4] = {row, pos, len, tile}: row of the tile's first token (a multiple
+                           * of 64 for packed archives and for selection), its position, its tokens (0..64; 0: the
+                           * entry is skipped), its number */
+    int32_t n;
+    int32_t per_query; /* 0: one list for all heads and queries; 1: [batch * kv_heads][q_len][n][4], a list for each
+                        * (batch, kv head, query row), as rfsn_select_tiles writes it */
+} rfsn_tile_list;
+
+RFSN_API rfsn_status rfsn_archive_attention(const rfsn_arena* arena, const rfsn_packed_archive* packed,
+                                            const float* q, int batch, int q_heads, int kv_heads, int q_len,
+                                            int q_pos0, const rfsn_tile_list* tiles, const rfsn_hot_window* hot,
+                                            float* out, float* lse, void* workspace, size_t workspace_bytes,
+                                            int max_splits, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Tile selection for sparse attention. For each (batch, kv head, query row):
+ *   score(tile) = max over the kv head's q heads of
+ *                 sum_d max(q_d * lo_d, q_d * hi_d)
+ * with lo, hi the tile's channel-wise key bounds: no key of the tile has a
+ * larger q . k. The products and sums are taken in 64 bits and the score
+ * rounded to float32. The n_select tiles with the largest scores are written
+ * in tile order, equal scores won by the lower tile; tiles that begin behind
+ * the query (pos > its position), are empty or score -inf are never taken,
+ * NaN scores are taken first. Unused entries are {0, 0, 0, -1}.
+ *
+ * bounds: device [batch * kv_heads][rows / 64][2][head_dim] of bounds_dtype:
+ * RFSN_F16 / BF16 (rfsn_tile_bounds), or RFSN_E4M3 codes (rfsn_pack_rows) that
+ * are multiplied by the K scales of `scales` (the packed archive's); the tile
+ * of a list entry is its row / 64. step_state (device int32, may be NULL):
+ * RFSN_STEP_POS replaces q_pos0 when the kernel runs. out: device int32
+ * [batch * kv_heads * q_len][n_select][4].
+ * ---------------------------------------------------------------------- */
+RFSN_API rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float* scales, int rows,
+                                       const float* q, int batch, int q_heads, int kv_heads, int q_len, int head_dim,
+                                       int q_pos0, const rfsn_tile_list* tiles, int n_select, int32_t* out,
+                                       const int32_t* step_state, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* Channel-wise smallest and largest key of each 64-row tile of rows row0 ..
+ * row0 + count of an arena (row0 a multiple of 64; the last tile may be
+ * shorter), in the arena's type (bf16/f16, head_dim 64 or 128); NaN keys give
+ * NaN bounds. bounds: device [batch_kv_heads][rows / 64][2][head_dim]. */
+RFSN_API rfsn_status rfsn_tile_bounds(const rfsn_arena* arena, int row0, int count, void* bounds, void* stream);
+
+/* Workspace bytes of rfsn_archive_attention (n_select = 0: shared lists;
+ * > 0: lists per query) and rfsn_select_tiles (n_select > 0) over up to n_tiles
+ * tiles. Conventions as for rfsn_attention_workspace_size; one workspace
+ * serves all attention calls ordered on one stream. */
+RFSN_API rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim,
+                                                 int n_tiles, int n_select, size_t* bytes);
 
 /* Reads the device error word of a workspace (after synchronising `stream`,
  * bounded by timeout_us) and clears it. RFSN_ERR_DEVICE if a kernel set it. */

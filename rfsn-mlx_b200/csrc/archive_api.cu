@@ -1,0 +1,331 @@
+// C entry points of the packed archive, tile selection and the attention over
+// tile lists (include/rfsn_b200.h): argument checks and launch plans.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+
+#include "archive.cuh"
+
+using namespace rfsn;
+
+namespace {
+
+constexpr int kMaxLists = 65535;  // grid dimension y
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+rfsn_status check_device(int device, const char* what) {
+    int dev = 0;
+    RFSN_CUDA(cudaGetDevice(&dev));
+    RFSN_CHECK_ARG(dev == device, "%s: called with device %d current, the buffers are on device %d", what, dev, device);
+    return RFSN_OK;
+}
+
+// Query slots of one list, column blocks of 4 slots per CTA and CTAs (z) per list.
+struct SlotPlan {
+    int lists, slots, nb, zblocks;
+};
+
+SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, bool per_query) {
+    SlotPlan s;
+    const int G = q_heads / kv_heads;
+    s.lists = batch * kv_heads * (per_query ? q_len : 1);
+    s.slots = per_query ? G : G * q_len;
+    s.nb = s.slots <= 4 ? 1 : 2;
+    s.zblocks = (s.slots + 4 * s.nb - 1) / (4 * s.nb);
+    return s;
+}
+
+// Splits of a list's items: two CTAs per SM over all lists.
+int split_limit(const SlotPlan& sp, int head_dim, int max_splits) {
+    const int sms = std::max(device_sms(), 1);
+    int s = std::max(1, 2 * sms / std::max(1, sp.lists * sp.zblocks));
+    s = std::min(s, head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64);
+    if (max_splits > 0) s = std::min(s, max_splits);
+    return s;
+}
+
+WsLayout attention_ws(const SlotPlan& sp, int splits, int head_dim) {
+    return ws_layout(splits > 1 ? sp.lists * sp.zblocks : 0, 1, splits, 4 * sp.nb, head_dim);
+}
+
+size_t select_scores_offset() { return align_up(256 + sizeof(int) * (size_t)kMaxCounters, 256); }
+
+rfsn_status check_shape(int batch, int q_heads, int kv_heads, int q_len, int head_dim, const char* what) {
+    RFSN_CHECK_ARG(batch > 0 && q_heads > 0 && kv_heads > 0 && q_len > 0, "%s: non-positive shape", what);
+    RFSN_CHECK_ARG(q_heads % kv_heads == 0, "num_heads (%d) must be divisible by num_kv_heads (%d)", q_heads, kv_heads);
+    if (head_dim != 64 && head_dim != 128) {
+        set_error("%s: head_dim %d is not supported (64 or 128)", what, head_dim);
+        return RFSN_ERR_UNSUPPORTED;
+    }
+    RFSN_CHECK_ARG((long long)batch * kv_heads * q_len <= kMaxLists && (long long)q_len * q_heads <= (1 << 22),
+                   "%s: batch * kv_heads * q_len above %d", what, kMaxLists);
+    return RFSN_OK;
+}
+
+rfsn_status check_tiles(const rfsn_tile_list* t, const char* what) {
+    RFSN_CHECK_ARG(t != nullptr && t->n >= 0 && t->n <= (1 << 25) && (t->n == 0 || t->tiles != nullptr) &&
+                       aligned16(t->tiles) && (t->per_query == 0 || t->per_query == 1),
+                   "%s: bad tile list", what);
+    return RFSN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+rfsn_status rfsn_packed_archive_create(void* k_codes, void* v_codes, float* scales, int batch_kv_heads, int rows,
+                                       int head_dim, rfsn_packed_archive** out) {
+    RFSN_CHECK_ARG(out != nullptr, "rfsn_packed_archive_create: out is NULL");
+    RFSN_CHECK_ARG(k_codes != nullptr && v_codes != nullptr && scales != nullptr,
+                   "rfsn_packed_archive_create: NULL pointer");
+    RFSN_CHECK_ARG(aligned16(k_codes) && aligned16(v_codes) && aligned16(scales),
+                   "rfsn_packed_archive_create: pointers must be 16-byte aligned");
+    RFSN_CHECK_ARG(batch_kv_heads > 0 && batch_kv_heads <= kMaxLists && rows > 0 && rows % kTile == 0,
+                   "rfsn_packed_archive_create: rows (%d) must be a positive multiple of %d, batch_kv_heads (%d) in "
+                   "1..%d", rows, kTile, batch_kv_heads, kMaxLists);
+    RFSN_CHECK_ARG((long long)batch_kv_heads * rows < (1LL << 31),
+                   "rfsn_packed_archive_create: batch_kv_heads * rows above 2^31 - 1");
+    if (head_dim != 64 && head_dim != 128) {
+        set_error("rfsn_packed_archive_create: head_dim %d is not supported (64 or 128)", head_dim);
+        return RFSN_ERR_UNSUPPORTED;
+    }
+    rfsn_packed_archive* a = new (std::nothrow) rfsn_packed_archive();
+    if (a == nullptr) {
+        set_error("rfsn_packed_archive_create: out of host memory");
+        return RFSN_ERR_OVERFLOW;
+    }
+    a->k = static_cast<uint8_t*>(k_codes);
+    a->v = static_cast<uint8_t*>(v_codes);
+    a->scales = reinterpret_cast<float4*>(scales);
+    a->groups = batch_kv_heads;
+    a->rows = rows;
+    a->head_dim = head_dim;
+    a->device = 0;
+    cudaGetDevice(&a->device);
+    rfsn_status st = encode_rows_map(&a->maps[0], k_codes, RFSN_E4M3, batch_kv_heads, rows, head_dim, kTile);
+    if (st == RFSN_OK) st = encode_rows_map(&a->maps[1], v_codes, RFSN_E4M3, batch_kv_heads, rows, head_dim, kTile);
+    if (st != RFSN_OK) {
+        delete a;
+        return st;
+    }
+    *out = a;
+    return RFSN_OK;
+}
+
+rfsn_status rfsn_packed_archive_destroy(rfsn_packed_archive* archive) {
+    delete archive;
+    return RFSN_OK;
+}
+
+rfsn_status rfsn_pack_rows(const rfsn_packed_archive* a, int dst_row0, const rfsn_kv_rows* src, int count,
+                           void* bounds, void* stream) {
+    RFSN_CHECK_ARG(a != nullptr && src != nullptr, "rfsn_pack_rows: NULL archive or source");
+    RFSN_CHECK_ARG(count >= 0 && dst_row0 >= 0 && dst_row0 % kTile == 0 && dst_row0 <= a->rows &&
+                       count <= a->rows - dst_row0,
+                   "rfsn_pack_rows: rows [%d, +%d) must start at a multiple of %d inside the archive (%d rows)",
+                   dst_row0, count, kTile, a->rows);
+    RFSN_CHECK_ARG(src->dtype == RFSN_F32 || src->dtype == RFSN_F16 || src->dtype == RFSN_BF16,
+                   "rfsn_pack_rows: unknown dtype %d", src->dtype);
+    RFSN_CHECK_ARG(src->kv_heads > 0 && a->groups % src->kv_heads == 0,
+                   "rfsn_pack_rows: %d KV heads do not divide the archive's %d", src->kv_heads, a->groups);
+    RFSN_CHECK_ARG(src->offset >= 0 && src->wrap >= 0 &&
+                       (src->wrap == 0 || (src->offset < src->wrap && count <= src->wrap)),
+                   "rfsn_pack_rows: bad offset or wrap");
+    RFSN_CHECK_ARG(bounds == nullptr || aligned16(bounds), "rfsn_pack_rows: bounds must be 16-byte aligned");
+    if (count == 0) return RFSN_OK;
+    RFSN_CHECK_ARG(src->k != nullptr && src->v != nullptr, "rfsn_pack_rows: NULL K or V");
+    rfsn_status st = check_device(a->device, "rfsn_pack_rows");
+    if (st != RFSN_OK) return st;
+    return pack_rows_launch(a, dst_row0, src, count, bounds, static_cast<cudaStream_t>(stream));
+}
+
+rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* a, int src_row0, int count, void* k_out, void* v_out,
+                             int out_dtype, int64_t out_stride, void* stream) {
+    RFSN_CHECK_ARG(a != nullptr, "rfsn_unpack_rows: NULL archive");
+    RFSN_CHECK_ARG(count >= 0 && src_row0 >= 0 && src_row0 <= a->rows && count <= a->rows - src_row0,
+                   "rfsn_unpack_rows: rows [%d, +%d) outside the archive (%d rows)", src_row0, count, a->rows);
+    RFSN_CHECK_ARG(out_dtype == RFSN_F32 || out_dtype == RFSN_F16 || out_dtype == RFSN_BF16,
+                   "rfsn_unpack_rows: unknown dtype %d", out_dtype);
+    if (count == 0) return RFSN_OK;
+    RFSN_CHECK_ARG(k_out != nullptr && v_out != nullptr && aligned16(k_out) && aligned16(v_out) &&
+                       out_stride * dtype_size(out_dtype) % 16 == 0 && out_stride >= 0,
+                   "rfsn_unpack_rows: outputs and their stride must be 16-byte aligned");
+    RFSN_CHECK_ARG(a->groups == 1 || out_stride >= (int64_t)count * a->head_dim,
+                   "rfsn_unpack_rows: out_stride %lld overlaps rows of the next head", (long long)out_stride);
+    rfsn_status st = check_device(a->device, "rfsn_unpack_rows");
+    if (st != RFSN_OK) return st;
+    return unpack_rows_launch(a, src_row0, count, k_out, v_out, out_dtype, out_stride, static_cast<cudaStream_t>(stream));
+}
+
+rfsn_status rfsn_tile_bounds(const rfsn_arena* arena, int row0, int count, void* bounds, void* stream) {
+    RFSN_CHECK_ARG(arena != nullptr && bounds != nullptr && aligned16(bounds), "rfsn_tile_bounds: NULL or misaligned pointer");
+    if (!arena->has_items) {
+        set_error("rfsn_tile_bounds: needs a bf16/f16 arena with head_dim 64 or 128");
+        return RFSN_ERR_UNSUPPORTED;
+    }
+    RFSN_CHECK_ARG(count >= 0 && row0 >= 0 && row0 % kTile == 0 && row0 <= arena->rows && count <= arena->rows - row0,
+                   "rfsn_tile_bounds: rows [%d, +%d) must start at a multiple of %d inside the arena (%d rows)", row0,
+                   count, kTile, arena->rows);
+    RFSN_CHECK_ARG(arena->rows % kTile == 0, "rfsn_tile_bounds: the arena's rows (%d) must be a multiple of %d",
+                   arena->rows, kTile);
+    RFSN_CHECK_ARG(arena->groups <= kMaxLists, "rfsn_tile_bounds: more than %d heads", kMaxLists);
+    if (count == 0) return RFSN_OK;
+    rfsn_status st = check_device(arena->device, "rfsn_tile_bounds");
+    if (st != RFSN_OK) return st;
+    return tile_bounds_launch(arena, row0, count, bounds, static_cast<cudaStream_t>(stream));
+}
+
+rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim, int n_tiles,
+                                        int n_select, size_t* bytes) {
+    RFSN_CHECK_ARG(bytes != nullptr, "rfsn_archive_workspace_size: bytes is NULL");
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, "rfsn_archive_workspace_size");
+    if (st != RFSN_OK) return st;
+    RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0, "rfsn_archive_workspace_size: negative tile count");
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, n_select > 0);
+    // at least 148 SMs are assumed, so a size computed without a device serves a B200
+    const int units = std::max(1, sp.lists * sp.zblocks);
+    const int limit = std::max(split_limit(sp, head_dim, 0),
+                               std::min(head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64,
+                                        std::max(1, 2 * 148 / units)));
+    size_t need = attention_ws(sp, limit, head_dim).total;
+    if (n_select > 0) need = std::max(need, select_scores_offset() + sizeof(float) * (size_t)sp.lists * n_tiles);
+    *bytes = need;
+    return RFSN_OK;
+}
+
+rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float* scales, int rows, const float* q,
+                              int batch, int q_heads, int kv_heads, int q_len, int head_dim, int q_pos0,
+                              const rfsn_tile_list* tiles, int n_select, int32_t* out, const int32_t* step_state,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "rfsn_select_tiles";
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, what);
+    if (st == RFSN_OK) st = check_tiles(tiles, what);
+    if (st != RFSN_OK) return st;
+    RFSN_CHECK_ARG(tiles->per_query == 0, "%s: selects from one list for all heads and queries", what);
+    RFSN_CHECK_ARG(q != nullptr && out != nullptr && aligned16(out) && workspace != nullptr && aligned16(workspace),
+                   "%s: NULL or misaligned pointer", what);
+    RFSN_CHECK_ARG(bounds_dtype == RFSN_F16 || bounds_dtype == RFSN_BF16 || bounds_dtype == RFSN_E4M3,
+                   "%s: bounds must be f16, bf16 or e4m3", what);
+    RFSN_CHECK_ARG(tiles->n == 0 || (bounds != nullptr && aligned16(bounds)), "%s: NULL or misaligned bounds", what);
+    RFSN_CHECK_ARG(tiles->n == 0 || bounds_dtype != RFSN_E4M3 || (scales != nullptr && aligned16(scales)),
+                   "%s: e4m3 bounds need the archive's scales", what);
+    RFSN_CHECK_ARG(rows >= 0 && rows % kTile == 0, "%s: rows (%d) must be a multiple of %d", what, rows, kTile);
+    RFSN_CHECK_ARG(n_select > 0 && n_select <= (1 << 20), "%s: n_select %d outside [1, %d]", what, n_select, 1 << 20);
+    const int lists = batch * kv_heads * q_len;
+    RFSN_CHECK_ARG(lists <= kMaxCounters, "%s: batch * kv_heads * q_len above %d", what, kMaxCounters);
+    const size_t off = select_scores_offset(), need = off + sizeof(float) * (size_t)lists * tiles->n;
+    if (workspace_bytes < need) {
+        set_error("%s: workspace too small: need %zu bytes, have %zu", what, need, workspace_bytes);
+        return RFSN_ERR_OVERFLOW;
+    }
+    char* ws = static_cast<char*>(workspace);
+    archive::SelectParams p;
+    memset(&p, 0, sizeof(p));
+    p.bounds = bounds;
+    p.scales = reinterpret_cast<const float4*>(scales);
+    p.tile_slots = rows / kTile;
+    p.q = q;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.q_len = q_len;
+    p.q_pos0 = q_pos0;
+    p.G = q_heads / kv_heads;
+    p.tiles = reinterpret_cast<const int4*>(tiles->tiles);
+    p.n_tiles = tiles->n;
+    p.n_select = n_select;
+    p.out = reinterpret_cast<int4*>(out);
+    p.scores = reinterpret_cast<float*>(ws + off);
+    p.counters = reinterpret_cast<int*>(ws + 256);
+    p.error = reinterpret_cast<int*>(ws);
+    p.dyn = step_state;
+    // two CTAs per SM over all lists, at least the 32 tiles that the CTA's warps score at once
+    const int want = std::max(1, 2 * device_sms() / lists);
+    p.tiles_per_cta = std::max(32, (tiles->n + want - 1) / want);
+    const int chunks = std::max(1, (tiles->n + p.tiles_per_cta - 1) / p.tiles_per_cta);
+    return select_tiles_launch(bounds_dtype, head_dim, p, lists, chunks, static_cast<cudaStream_t>(stream));
+}
+
+rfsn_status rfsn_archive_attention(const rfsn_arena* arena, const rfsn_packed_archive* packed, const float* q,
+                                   int batch, int q_heads, int kv_heads, int q_len, int q_pos0,
+                                   const rfsn_tile_list* tiles, const rfsn_hot_window* hot, float* out, float* lse,
+                                   void* workspace, size_t workspace_bytes, int max_splits, void* stream) {
+    const char* what = "rfsn_archive_attention";
+    RFSN_CHECK_ARG(arena != nullptr && hot != nullptr, "%s: NULL arena or hot window", what);
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, arena->head_dim, what);
+    if (st == RFSN_OK) st = check_tiles(tiles, what);
+    if (st != RFSN_OK) return st;
+    if (!arena->has_items) {
+        set_error("%s: needs a bf16/f16 arena with head_dim 64 or 128", what);
+        return RFSN_ERR_UNSUPPORTED;
+    }
+    const int groups = batch * kv_heads;
+    RFSN_CHECK_ARG(groups == arena->groups, "%s: batch*kv_heads %d != arena groups %d", what, groups, arena->groups);
+    RFSN_CHECK_ARG(packed == nullptr || (packed->groups == groups && packed->head_dim == arena->head_dim &&
+                                         packed->device == arena->device),
+                   "%s: the packed archive's heads, head_dim or device differ from the arena's", what);
+    RFSN_CHECK_ARG(q != nullptr && out != nullptr && aligned16(out) && workspace != nullptr && aligned16(workspace),
+                   "%s: NULL or misaligned pointer", what);
+    RFSN_CHECK_ARG(hot->length >= 0 && hot->length <= hot->capacity && hot->head_index >= 0 &&
+                       hot->head_index < (hot->capacity > 0 ? hot->capacity : 1) && hot->ring_row0 >= 0 &&
+                       hot->ring_row0 + hot->capacity <= arena->rows,
+                   "%s: bad hot window", what);
+    const bool stepped = hot->step_state != nullptr;
+    if (tiles->n == 0 && hot->length == 0 && !stepped) {
+        set_error("run_segmented_attention requires at least one KV segment");
+        return RFSN_ERR_INVALID_ARG;
+    }
+    st = check_device(arena->device, what);
+    if (st != RFSN_OK) return st;
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, tiles->per_query != 0);
+    RFSN_CHECK_ARG(sp.zblocks <= kMaxLists, "%s: too many query rows", what);
+    const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
+    const int per_tile = packed != nullptr ? 1 : kTile / hk;
+    RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
+    const int first = std::min(hot->length, hot->capacity - hot->head_index);
+    // with a device step state the window is only known when the kernel runs: planned for the largest
+    const int hot_items = stepped ? (hot->capacity + hk - 1) / hk + 1
+                                  : (first + hk - 1) / hk + (hot->length - first + hk - 1) / hk;
+    const int total = std::max(1, tiles->n * per_tile + hot_items);
+    int splits = std::min(split_limit(sp, arena->head_dim, max_splits), total);
+    const int per = (total + splits - 1) / splits;
+    splits = (total + per - 1) / per;
+    // more than one split only where all lists leave SMs idle: far fewer lists than arrival counters
+    RFSN_CHECK_ARG(splits == 1 || (long long)sp.lists * sp.zblocks <= kMaxCounters, "%s: too many lists", what);
+    const WsLayout w = attention_ws(sp, splits, arena->head_dim);
+    if (w.total > workspace_bytes) {
+        set_error("%s: workspace too small: need %zu bytes, have %zu", what, w.total, workspace_bytes);
+        return RFSN_ERR_OVERFLOW;
+    }
+    archive::Params p;
+    memset(&p, 0, sizeof(p));
+    p.q = q;
+    p.out = out;
+    p.lse = lse;
+    p.tiles = reinterpret_cast<const int4*>(tiles->tiles);
+    p.n_tiles = tiles->n;
+    p.per_query = tiles->per_query;
+    p.ring_row0 = hot->ring_row0;
+    p.capacity = hot->capacity;
+    p.head = hot->head_index;
+    p.hlen = hot->length;
+    p.hstart = hot->start_pos;
+    p.rows = arena->rows;
+    p.packed_rows = packed != nullptr ? packed->rows : 0;
+    p.scales = packed != nullptr ? packed->scales : nullptr;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.q_len = q_len;
+    p.q_pos0 = q_pos0;
+    p.G = q_heads / kv_heads;
+    p.slots = sp.slots;
+    p.items_per_split = per;
+    p.splits = splits;
+    p.qscale = (float)(1.0 / std::sqrt((double)arena->head_dim)) * 1.4426950408889634f;
+    p.ws = ws_view(workspace, w);
+    p.dyn = hot->step_state;
+    return archive_attn_launch(arena, packed, p, sp.lists, sp.nb, sp.zblocks, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

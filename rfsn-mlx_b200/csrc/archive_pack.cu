@@ -1,0 +1,348 @@
+// Packing of archived K/V rows into 8 bits and back, and the per-tile key
+// bounds that tile selection scores.
+//
+// A tile is 64 consecutive tokens of a block. For each (tile, KV head), K and
+// V apart, with a = the largest finite |x| of the tile:
+//   s = 2^e, the smallest power of two with a / s <= 448 (1 when a = 0)
+//   code = round-to-nearest-even e4m3(x / s)
+// A power of two makes x / s exact, so packing rounds once (at most half an
+// e4m3 step, 2^-4 of the value, or 2^-10 * s below e4m3's normal range), a
+// packed value is exact in bfloat16, and packing an unpacked tile again gives
+// the same values. It costs no precision against a / 448: the codes are
+// floating-point numbers, only the point where they turn subnormal moves.
+// NaN stays NaN, infinities become NaN (e4m3 has none, and saturating them
+// would hide them).
+#include <math_constants.h>
+
+#include "archive.cuh"
+
+namespace rfsn {
+namespace archive {
+
+constexpr int kPackThreads = 256;
+
+struct RowSource {
+    const void* p;
+    long long sb, sh, st;  // strides in elements: batch, head, token
+    int kv_heads, offset, wrap;
+    int vec;               // rows may be read as 16-byte vectors
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int vec, float (&x)[8]) {
+    if (vec) {
+        constexpr int N = 8 * sizeof(T) / 16;
+        uint4 w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+    }
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t x) {
+    return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)x, __NV_E4M3));
+}
+
+// The scale of a tile whose largest finite magnitude is a: from the exponent
+// and mantissa of a = m * 2^e, m in [1, 2): 448 = 1.75 * 2^8.
+__device__ __forceinline__ float tile_scale(float a) {
+    if (!(a > 0.f)) return 1.f;
+    const uint32_t b = __float_as_uint(a);
+    int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    if (e < -126) e = -126;  // also subnormal a
+    return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// One CTA per (tile, KV head, K or V): the tile stays in registers between
+// the maximum and the conversion, so it is read once. Bound by memory. Rows
+// of the tile behind `count` become zero codes (the attention kernel reads
+// whole tiles and multiplies them by zero weights).
+template <typename T, int D>
+__global__ void __launch_bounds__(kPackThreads) pack_kernel(RowSource ks, RowSource vs, uint8_t* __restrict__ kd,
+                                                            uint8_t* __restrict__ vd, float* __restrict__ scales,
+                                                            uint8_t* __restrict__ bounds, int rows, int dst_row0,
+                                                            int count) {
+    constexpr int VPR = D / 8;                    // 8-element vectors per row
+    constexpr int RPP = kPackThreads / VPR;       // rows per pass
+    constexpr int PASSES = kTile / RPP;
+    const int tile = blockIdx.x, bh = blockIdx.y, is_v = blockIdx.z;
+    const RowSource src = is_v ? vs : ks;
+    const int len = min(kTile, count - tile * kTile);
+    const int c8 = threadIdx.x % VPR, r0 = threadIdx.x / VPR;
+    const T* base = static_cast<const T*>(src.p) + (bh / src.kv_heads) * src.sb + (bh % src.kv_heads) * src.sh + 8 * c8;
+    float x[PASSES][8];
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int r = r0 + i * RPP;
+        if (r < len) {
+            long long t = (long long)src.offset + (long long)tile * kTile + r;
+            if (src.wrap > 0) t %= src.wrap;
+            load8<T>(base + t * src.st, src.vec, x[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float m = fabsf(x[i][e]);
+            a = fmaxf(a, m < CUDART_INF_F ? m : 0.f);
+        }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+    __shared__ float part[kPackThreads / 32];
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = part[0];
+#pragma unroll
+    for (int i = 1; i < kPackThreads / 32; ++i) a = fmaxf(a, part[i]);
+    const float s = tile_scale(a), inv = 1.f / s;  // both powers of two
+    const int row0 = dst_row0 + tile * kTile;
+    uint8_t* dst = (is_v ? vd : kd) + ((size_t)bh * rows + row0) * D + 8 * c8;
+    __half2 lo[4], hi[4];
+    const __half2 top = __half2half2(__ushort_as_half(0x7c00)), bottom = __half2half2(__ushort_as_half(0xfc00));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        lo[j] = top;
+        hi[j] = bottom;
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int r = r0 + i * RPP;
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float y[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float v = x[i][2 * j + e];
+                y[e] = fabsf(v) == CUDART_INF_F ? CUDART_NAN_F : v * inv;
+            }
+            c[j] = e4m3x2(y[0], y[1]);
+            if (r < len) {
+                const __half2 h = half2_of_e4m3x2(c[j]);
+                lo[j] = __hmin2_nan(lo[j], h);
+                hi[j] = __hmax2_nan(hi[j], h);
+            }
+        }
+        *reinterpret_cast<uint2*>(dst + (size_t)r * D) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    }
+    const size_t slot = (size_t)bh * (rows / kTile) + row0 / kTile;
+    if (threadIdx.x == 0) scales[4 * slot + is_v] = s;
+    if (bounds == nullptr || is_v) return;
+    // channel-wise smallest and largest code of the tile's keys
+    __shared__ __half2 red[2][RPP][D / 2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        red[0][r0][4 * c8 + j] = lo[j];
+        red[1][r0][4 * c8 + j] = hi[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < D) {  // 2 bounds x D / 2 channel pairs
+        const int w = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
+        __half2 m = red[w][0][j];
+#pragma unroll 4
+        for (int r = 1; r < RPP; ++r) m = w ? __hmax2_nan(m, red[w][r][j]) : __hmin2_nan(m, red[w][r][j]);
+        const float2 f = __half22float2(m);
+        reinterpret_cast<uint16_t*>(bounds)[(slot * 2 + w) * (D / 2) + j] = (uint16_t)e4m3x2(f.x, f.y);
+    }
+}
+
+// value = code * scale, rounded once to T (exact for float32 and bfloat16;
+// finite values saturate at float16's largest number).
+template <typename T> __device__ __forceinline__ T unpacked(float x) { return from_f32<T>(x); }
+template <> __device__ __forceinline__ __half unpacked<__half>(float x) {
+    if (fabsf(x) > 65504.f) x = copysignf(65504.f, x);
+    return __float2half_rn(x);
+}
+
+// 16 codes per thread: one 16-byte load, 32 (64) bytes stored. Bound by memory.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                     const float4* __restrict__ scales, T* __restrict__ ko,
+                                                     T* __restrict__ vo, int rows, int row0, int count,
+                                                     long long group_stride) {
+    constexpr int VPR = D / 16;
+    const int bh = blockIdx.y, is_v = blockIdx.z;
+    const long long total = (long long)count * VPR;
+    const uint8_t* src = (is_v ? vc : kc) + ((size_t)bh * rows + row0) * D;
+    T* dst = (is_v ? vo : ko) + (size_t)bh * group_stride;
+    const float4* sc = scales + (size_t)bh * (rows / kTile);
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const int r = (int)(i / VPR);
+        const float4 s4 = __ldg(sc + (row0 + r) / kTile);
+        const float s = is_v ? s4.y : s4.x;
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        alignas(16) T o[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = __half22float2(half2_of_e4m3x2((w[j >> 1] >> (16 * (j & 1))) & 0xffffu));
+            o[2 * j] = unpacked<T>(f.x * s);
+            o[2 * j + 1] = unpacked<T>(f.y * s);
+        }
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4*>(dst + 16 * i)[j] = reinterpret_cast<uint4*>(o)[j];
+    }
+}
+
+// Channel-wise smallest and largest key of each tile of an exact (16-bit)
+// block: one CTA per (tile, KV head); NaN keys give NaN bounds.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) bounds_kernel(const T* __restrict__ k, T* __restrict__ bounds, int rows,
+                                                     int row0, int count) {
+    constexpr int VPR = D / 8, RPP = 256 / VPR;
+    const int tile = blockIdx.x, bh = blockIdx.y;
+    const int len = min(kTile, count - tile * kTile);
+    const int c8 = threadIdx.x % VPR, r0 = threadIdx.x / VPR;
+    const T* src = k + ((size_t)bh * rows + row0 + tile * kTile) * D + 8 * c8;
+    float lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        lo[e] = CUDART_INF_F;
+        hi[e] = -CUDART_INF_F;
+    }
+#pragma unroll
+    for (int i = 0; i < kTile / RPP; ++i) {
+        const int r = r0 + i * RPP;
+        if (r < len) {
+            float x[8];
+            load8<T>(src + (size_t)r * D, 1, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lo[e] = (x[e] < lo[e] || x[e] != x[e]) ? x[e] : lo[e];
+                hi[e] = (x[e] > hi[e] || x[e] != x[e]) ? x[e] : hi[e];
+            }
+        }
+    }
+    __shared__ float red[2][RPP][D];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        red[0][r0][8 * c8 + e] = lo[e];
+        red[1][r0][8 * c8 + e] = hi[e];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += 256) {
+        const int w = i / D, d = i % D;
+        float m = red[w][0][d];
+        for (int r = 1; r < RPP; ++r) {
+            const float x = red[w][r][d];
+            // a NaN met first stays (comparisons with it are false), one met later replaces m
+            m = ((w ? x > m : x < m) || x != x) ? x : m;
+        }
+        bounds[(((size_t)bh * (rows / kTile) + (row0 + tile * kTile) / kTile) * 2 + w) * D + d] = from_f32<T>(m);
+    }
+}
+
+template <typename T, int D>
+rfsn_status pack_launch(const rfsn_packed_archive* a, int dst_row0, const RowSource& ks, const RowSource& vs,
+                        int count, void* bounds, cudaStream_t s) {
+    const dim3 grid((count + kTile - 1) / kTile, a->groups, 2);
+    pack_kernel<T, D><<<grid, kPackThreads, 0, s>>>(ks, vs, a->k, a->v, reinterpret_cast<float*>(a->scales),
+                                                    static_cast<uint8_t*>(bounds), a->rows, dst_row0, count);
+    RFSN_CUDA(cudaGetLastError());
+    note_launch();
+    return RFSN_OK;
+}
+
+template <typename T, int D>
+rfsn_status unpack_launch(const rfsn_packed_archive* a, int row0, int count, void* k, void* v, long long gs,
+                          cudaStream_t s) {
+    const long long per = ((long long)count * (D / 16) + 255) / 256;
+    const dim3 grid((unsigned)(per < 2048 ? per : 2048), a->groups, 2);
+    unpack_kernel<T, D><<<grid, 256, 0, s>>>(a->k, a->v, a->scales, static_cast<T*>(k), static_cast<T*>(v), a->rows,
+                                             row0, count, gs);
+    RFSN_CUDA(cudaGetLastError());
+    note_launch();
+    return RFSN_OK;
+}
+
+template <typename T, int D>
+rfsn_status bounds_launch(const rfsn_arena* a, int row0, int count, void* bounds, cudaStream_t s) {
+    const dim3 grid((count + kTile - 1) / kTile, a->groups);
+    bounds_kernel<T, D><<<grid, 256, 0, s>>>(static_cast<const T*>(a->k), static_cast<T*>(bounds), a->rows, row0,
+                                             count);
+    RFSN_CUDA(cudaGetLastError());
+    note_launch();
+    return RFSN_OK;
+}
+
+template <typename T, int D>
+void preload() {
+    cudaFuncAttributes a;
+    cudaFuncGetAttributes(&a, pack_kernel<T, D>);
+    cudaFuncGetAttributes(&a, unpack_kernel<T, D>);
+    if constexpr (sizeof(T) == 2) cudaFuncGetAttributes(&a, bounds_kernel<T, D>);
+}
+
+}  // namespace archive
+
+void preload_pack_kernels() {
+    using namespace archive;
+    preload<float, 64>();
+    preload<float, 128>();
+    preload<__half, 64>();
+    preload<__half, 128>();
+    preload<__nv_bfloat16, 64>();
+    preload<__nv_bfloat16, 128>();
+}
+
+rfsn_status pack_rows_launch(const rfsn_packed_archive* a, int dst_row0, const rfsn_kv_rows* src, int count,
+                             void* bounds, cudaStream_t s) {
+    using namespace archive;
+    const int es = dtype_size(src->dtype);
+    auto make = [&](const void* p, int64_t sb, int64_t sh, int64_t st) {
+        const bool vec = ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(sb * es) | (uintptr_t)(sh * es) |
+                           (uintptr_t)(st * es)) & 15) == 0;
+        return RowSource{p, sb, sh, st, src->kv_heads, src->offset, src->wrap, vec ? 1 : 0};
+    };
+    const RowSource ks = make(src->k, src->k_stride_b, src->k_stride_h, src->k_stride_t);
+    const RowSource vs = make(src->v, src->v_stride_b, src->v_stride_h, src->v_stride_t);
+    const bool d128 = a->head_dim == 128;
+    if (src->dtype == RFSN_F32)
+        return d128 ? pack_launch<float, 128>(a, dst_row0, ks, vs, count, bounds, s)
+                    : pack_launch<float, 64>(a, dst_row0, ks, vs, count, bounds, s);
+    if (src->dtype == RFSN_F16)
+        return d128 ? pack_launch<__half, 128>(a, dst_row0, ks, vs, count, bounds, s)
+                    : pack_launch<__half, 64>(a, dst_row0, ks, vs, count, bounds, s);
+    return d128 ? pack_launch<__nv_bfloat16, 128>(a, dst_row0, ks, vs, count, bounds, s)
+                : pack_launch<__nv_bfloat16, 64>(a, dst_row0, ks, vs, count, bounds, s);
+}
+
+rfsn_status unpack_rows_launch(const rfsn_packed_archive* a, int row0, int count, void* k, void* v, int dtype,
+                               long long gs, cudaStream_t s) {
+    using namespace archive;
+    const bool d128 = a->head_dim == 128;
+    if (dtype == RFSN_F32)
+        return d128 ? unpack_launch<float, 128>(a, row0, count, k, v, gs, s)
+                    : unpack_launch<float, 64>(a, row0, count, k, v, gs, s);
+    if (dtype == RFSN_F16)
+        return d128 ? unpack_launch<__half, 128>(a, row0, count, k, v, gs, s)
+                    : unpack_launch<__half, 64>(a, row0, count, k, v, gs, s);
+    return d128 ? unpack_launch<__nv_bfloat16, 128>(a, row0, count, k, v, gs, s)
+                : unpack_launch<__nv_bfloat16, 64>(a, row0, count, k, v, gs, s);
+}
+
+rfsn_status tile_bounds_launch(const rfsn_arena* a, int row0, int count, void* bounds, cudaStream_t s) {
+    using namespace archive;
+    const bool d128 = a->head_dim == 128;
+    if (a->dtype == RFSN_F16)
+        return d128 ? bounds_launch<__half, 128>(a, row0, count, bounds, s)
+                    : bounds_launch<__half, 64>(a, row0, count, bounds, s);
+    return d128 ? bounds_launch<__nv_bfloat16, 128>(a, row0, count, bounds, s)
+                : bounds_launch<__nv_bfloat16, 64>(a, row0, count, bounds, s);
+}
+
+}  // namespace rfsn

@@ -74,13 +74,17 @@ rfsn_status encode_map(CUtensorMap* map, void* base, int dtype, int groups, int 
         set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
         return RFSN_ERR_CUDA;
     }
-    const int es = dtype_size(dtype);
+    const int es = dtype == RFSN_E4M3 ? 1 : dtype_size(dtype);
     cuuint64_t gdim[2] = {(cuuint64_t)head_dim, (cuuint64_t)groups * (cuuint64_t)rows};
     cuuint64_t gstride[1] = {(cuuint64_t)head_dim * es};
-    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    // 16-bit rows in boxes of 64 columns, 8-bit rows whole
+    cuuint32_t box[2] = {es == 1 ? (cuuint32_t)head_dim : 64u, (cuuint32_t)box_rows};
     cuuint32_t estride[2] = {1, 1};
-    CUresult r = fn(map, dtype == RFSN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base,
-                    gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUtensorMapDataType type = es == 1              ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : dtype == RFSN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapSwizzle swizzle = box[0] * es == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    CUresult r = fn(map, type, 2, base, gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
@@ -142,6 +146,7 @@ void preload_kernels_once(int dev) {
     preload_merge_kernels();
     preload_prefill_kernels();
     preload_model_kernels();
+    preload_archive_kernels();
     cudaGetLastError();  // a kernel that cannot be loaded here reports the error at its launch
 }
 
@@ -252,6 +257,13 @@ PrefillPlan plan_prefill(int nqb, int groups, int ppc, int q_len, int q_pos0, in
 
 }  // namespace
 
+int rfsn::device_sms() { return sm_count_cached(); }
+
+rfsn_status rfsn::encode_rows_map(CUtensorMap* map, void* base, int dtype, int groups, int rows, int head_dim,
+                                  int box_rows) {
+    return encode_map(map, base, dtype, groups, rows, head_dim, box_rows);
+}
+
 extern "C" {
 
 const char* rfsn_last_error(void) { return g_last_error.c_str(); }
@@ -297,6 +309,12 @@ rfsn_status rfsn_arena_create(void* k_arena, void* v_arena, int dtype, int batch
             return st;
         }
         a->has_tma = true;
+    }
+    a->has_items = false;
+    if ((dtype == RFSN_BF16 || dtype == RFSN_F16) && (head_dim == 64 || head_dim == 128)) {
+        const int box = head_dim == 128 ? 32 : 64;
+        a->has_items = encode_map(&a->item_maps[0], k_arena, dtype, batch_kv_heads, rows, head_dim, box) == RFSN_OK &&
+                       encode_map(&a->item_maps[1], v_arena, dtype, batch_kv_heads, rows, head_dim, box) == RFSN_OK;
     }
     *out = a;
     return RFSN_OK;

@@ -15,6 +15,8 @@ struct rfsn_arena {
     int device;
     bool has_tma;
     CUtensorMap maps[4];  // K 64-row box, V 64-row box, K 8-row box, V 8-row box
+    bool has_items;             // 16-bit K/V, head_dim 64 or 128: maps of archive_attn.cu's items
+    CUtensorMap item_maps[2];   // K and V, boxes of 32 rows (head_dim 64: 64 rows)
 };
 
 namespace rfsn {
@@ -82,6 +84,9 @@ int fast_max_splits();
 rfsn_status fast_launch(int dtype, const CUtensorMap* maps, const fast::Params& p, int stages, cudaStream_t stream);
 // generic_attn.cu
 rfsn_status generic_launch(int dtype, bool paged, const generic::Params& p, int groups, cudaStream_t stream);
+// capi.cu: SM count of the current device; a 2-D TMA map of a 16-bit or 8-bit [groups * rows][head_dim] array
+int device_sms();
+rfsn_status encode_rows_map(CUtensorMap* map, void* base, int dtype, int groups, int rows, int head_dim, int box_rows);
 // capi.cu: shared body of the paged-attention entry points (peer may be NULL)
 rfsn_status paged_attention_impl(const rfsn_arena* arena, const float* q, int batch, int q_heads, int kv_heads,
                                  int q_len, int q_pos0, const rfsn_page_table* table, const rfsn_hot_window* hot,
@@ -116,6 +121,7 @@ void preload_ring_kernels();
 void preload_merge_kernels();
 void preload_prefill_kernels();
 void preload_model_kernels();
+void preload_archive_kernels();
 
 rfsn_status rms_norm_dispatch(int dtype, const void* x, const void* res, const void* w, void* s_out, void* y, int rows,
                               int n, float eps, cudaStream_t s);

@@ -12,6 +12,7 @@ from .config import RFSNConfig, RuntimeMode, resolve_dtype, validate_session_id 
 from .block_manager import BlockId, BlockLocation, BlockManager, BlockManifest, BlockSpan, PageTable  # noqa: F401
 from .storage import BlockStorage  # noqa: F401
 from .residency import ResidencyManager, ResidencyMetrics  # noqa: F401
+from .archive import PackedArchive  # noqa: F401
 from .cache import LayerKVCache, PagedSegments, RFSNCache, derive_model_id  # noqa: F401
 from .attention_exact import (  # noqa: F401
     build_causal_mask,
@@ -30,6 +31,7 @@ __all__ = [
     "RFSNCache",
     "LayerKVCache",
     "PagedSegments",
+    "PackedArchive",
     "BlockId",
     "BlockLocation",
     "BlockManager",

@@ -34,6 +34,7 @@ RFSN_ERR_DEVICE = 6
 RFSN_F32 = 0
 RFSN_F16 = 1
 RFSN_BF16 = 2
+RFSN_E4M3 = 3  # packed archives only
 TILE_KEYS = 64
 
 DTYPE_CODE = {torch.float32: RFSN_F32, torch.float16: RFSN_F16, torch.bfloat16: RFSN_BF16}
@@ -71,6 +72,14 @@ EXPORTED_SYMBOLS = (
     "rfsn_rms_norm",
     "rfsn_silu_mul",
     "rfsn_gemv",
+    "rfsn_packed_archive_create",
+    "rfsn_packed_archive_destroy",
+    "rfsn_pack_rows",
+    "rfsn_unpack_rows",
+    "rfsn_tile_bounds",
+    "rfsn_select_tiles",
+    "rfsn_archive_attention",
+    "rfsn_archive_workspace_size",
 )
 
 
@@ -118,6 +127,31 @@ class SegmentDescC(ctypes.Structure):
         ("len", ctypes.c_int32),
         ("tile_begin", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
+    ]
+
+
+class KvRowsC(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride_b", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("k_stride_t", ctypes.c_int64),
+        ("v_stride_b", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("offset", ctypes.c_int32),
+        ("wrap", ctypes.c_int32),
+    ]
+
+
+class TileListC(ctypes.Structure):
+    _fields_ = [
+        ("tiles", ctypes.c_void_p),  # device int32 [n][4] = {row, pos, len, tile}
+        ("n", ctypes.c_int32),
+        ("per_query", ctypes.c_int32),
     ]
 
 
@@ -186,6 +220,16 @@ def load_library() -> ctypes.CDLL:
             [vp, vp, i32, i32, i32, i32, i32, ctypes.POINTER(PageTableC), ctypes.POINTER(HotWindowC), vp, vp, i32, vp],
         ),
         "rfsn_noalloc_check": (i32, [vp, i64]),
+        "rfsn_packed_archive_create": (i32, [vp, vp, vp, i32, i32, i32, ctypes.POINTER(vp)]),
+        "rfsn_packed_archive_destroy": (i32, [vp]),
+        "rfsn_pack_rows": (i32, [vp, i32, ctypes.POINTER(KvRowsC), i32, vp, vp]),
+        "rfsn_unpack_rows": (i32, [vp, i32, i32, vp, vp, i32, i64, vp]),
+        "rfsn_tile_bounds": (i32, [vp, i32, i32, vp, vp]),
+        "rfsn_select_tiles": (i32, [vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, ctypes.POINTER(TileListC), i32,
+                                    vp, vp, vp, sz, vp]),
+        "rfsn_archive_attention": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, ctypes.POINTER(TileListC),
+                                         ctypes.POINTER(HotWindowC), vp, vp, vp, sz, i32, vp]),
+        "rfsn_archive_workspace_size": (i32, [i32] * 7 + [ctypes.POINTER(sz)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -243,6 +287,24 @@ def stream_ptr(stream: Optional[torch.cuda.Stream] = None) -> int:
     if _raw_current_stream is not None and _current_device is not None:
         return int(_raw_current_stream(_current_device()))
     return int(torch.cuda.current_stream().cuda_stream)
+
+
+class _Nothing:
+    def __enter__(self) -> None:
+        return None
+
+    def __exit__(self, *exc) -> None:
+        return None
+
+
+_nothing = _Nothing()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current CUDA device (a no-op when it
+    already is): launches go to its current stream."""
+    current = _current_device() if _current_device is not None else torch.cuda.current_device()
+    return _nothing if device.index is None or device.index == current else torch.cuda.device(device)
 
 
 def host_device_pointer(t: torch.Tensor) -> int:

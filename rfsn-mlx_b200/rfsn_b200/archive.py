@@ -1,0 +1,246 @@
+"""Packed (8-bit) archives, tile selection and attention over lists of tiles.
+
+No counterpart in the reference: its archived blocks keep the cache dtype
+(cache.py:324-339) and every query attends to all of them. Two opt-in
+extensions of ``LayerKVCache`` live here:
+
+* **Packed archive** (``archive_dtype="float8_e4m3fn"``): archived K/V are held
+  as e4m3 codes with one power-of-two scale per (64-token tile, KV head), for K
+  and for V, so an attention call reads half the bytes. The hot ring keeps the
+  cache dtype. ``PackedArchive`` owns the codes; ``pack`` and ``unpack`` convert.
+* **Tile selection** (``tile_index=True``): the cache keeps the channel-wise
+  smallest and largest key of every archived tile. ``select_tiles`` bounds the
+  logits of each tile with them and picks the ``top_tiles`` best for each query
+  and KV head; attention then reads those tiles and the hot window only. The
+  result is the exact softmax over the keys that are read; the tiles left out
+  are the approximation.
+
+Everything runs on ``librfsn_b200.so``; there is no CPU fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import Optional
+
+import torch
+
+from . import _native as native
+
+TILE = native.TILE_KEYS
+ARCHIVE_DTYPES = {"float8_e4m3fn": torch.float8_e4m3fn}
+# Query rows of one sparse call: every row reads tiles of its own.
+SPARSE_MAX_ROWS = 64
+
+
+def padded_rows(n: int) -> int:
+    """Rows of a block of n tokens in an archive of whole tiles."""
+    return (n + TILE - 1) // TILE * TILE
+
+
+def check_archive_options(dtype: torch.dtype, head_dim: int, archive_dtype: Optional[str], tile_index: bool) -> None:
+    if archive_dtype is not None and archive_dtype not in ARCHIVE_DTYPES:
+        raise ValueError(f"archive_dtype must be None or one of {set(ARCHIVE_DTYPES)}, got {archive_dtype!r}")
+    if (archive_dtype is not None or tile_index) and (
+            dtype not in (torch.bfloat16, torch.float16) or head_dim not in (64, 128)):
+        raise ValueError("a packed archive or a tile index needs a float16 or bfloat16 model_dtype and head_dim 64 or "
+                         f"128, got {dtype} and {head_dim}")
+
+
+def kv_rows(k: torch.Tensor, v: torch.Tensor, offset: int = 0, wrap: int = 0) -> native.KvRowsC:
+    """Description of K/V [B, Hkv, n, D] for ``rfsn_pack_rows`` (innermost stride 1)."""
+    ks, vs = k.stride(), v.stride()
+    return native.KvRowsC(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                          native.dtype_code(k.dtype), int(k.shape[1]), offset, wrap)
+
+
+class PackedArchive:
+    """e4m3 codes ``k``, ``v`` [groups, rows, head_dim] and float32 ``k_scale``,
+    ``v_scale`` [groups, rows / 64] of one layer (groups = batch * kv_heads).
+
+    A tile is 64 rows; value = code * scale of its tile. ``rows`` is rounded up
+    to whole tiles."""
+
+    def __init__(self, groups: int, rows: int, head_dim: int, *,
+                 device: Optional[torch.device | str] = None) -> None:
+        native.lib()
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        if dev.type != "cuda":
+            raise native.NativeUnavailable("a packed archive lives on a CUDA device (no CPU path)")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.device = dev
+        self.groups, self.rows, self.head_dim = int(groups), padded_rows(int(rows)), int(head_dim)
+        if self.groups <= 0 or self.rows <= 0:
+            raise ValueError("a packed archive needs at least one head and one row")
+        shape = (self.groups, self.rows, self.head_dim)
+        self.k = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        self.v = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        self.scales = torch.ones((self.groups, self.rows // TILE, 4), dtype=torch.float32, device=dev)
+        self.k_scale, self.v_scale = self.scales[..., 0], self.scales[..., 1]
+        handle = ctypes.c_void_p()
+        with native.on_device(dev):
+            native.check(
+                native.lib().rfsn_packed_archive_create(self.k.data_ptr(), self.v.data_ptr(), self.scales.data_ptr(),
+                                                        self.groups, self.rows, self.head_dim, ctypes.byref(handle)),
+                "rfsn_packed_archive_create",
+            )
+        self.handle = handle
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            native.load_library().rfsn_packed_archive_destroy(self.handle)
+            self.handle = ctypes.c_void_p()
+
+    def __del__(self) -> None:  # pragma: no cover - interpreter shutdown order
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def clear(self) -> None:
+        """Zero codes and unit scales (the state of a new archive)."""
+        self.k.view(torch.uint8).zero_()
+        self.v.view(torch.uint8).zero_()
+        self.scales.fill_(1.0)
+
+    def pack(self, k: torch.Tensor, v: torch.Tensor, row: int = 0, *,
+             bounds: Optional[torch.Tensor] = None) -> None:
+        """Pack the tokens of k, v [B, Hkv, n, D] (float32, float16 or bfloat16,
+        any strides with a contiguous last dimension) into rows row .. row + n
+        (``row`` a multiple of 64), in tiles of 64 from the first token on. The
+        rest of the last tile is zeroed. ``bounds`` (uint8 [groups, rows / 64,
+        2, D]) receives the channel-wise smallest and largest K codes."""
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("pack needs k and v of one shape [B, Hkv, n, D] and one dtype")
+        if k.shape[0] * k.shape[1] != self.groups or k.shape[3] != self.head_dim:
+            raise ValueError(f"K/V of shape {tuple(k.shape)} do not fit {self.groups} heads of {self.head_dim}")
+        if k.device != self.device or v.device != self.device:
+            raise ValueError(f"K/V must be on {self.device}")
+        self._check_bounds(bounds)
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        if v.stride(3) != 1:
+            v = v.contiguous()
+        self._pack(kv_rows(k, v), int(row), int(k.shape[2]), bounds)
+
+    def pack_ring(self, k: torch.Tensor, v: torch.Tensor, offset: int, wrap: int, row: int, count: int, *,
+                  bounds: Optional[torch.Tensor] = None) -> None:
+        """``pack`` of ``count`` ring tokens: k, v [groups, ring rows, D], the
+        oldest token at ``offset``, wrapping at ``wrap``."""
+        self._check_bounds(bounds)
+        self._pack(kv_rows(k[None], v[None], offset, wrap), row, count, bounds)
+
+    def _check_bounds(self, bounds: Optional[torch.Tensor]) -> None:
+        shape = (self.groups, self.rows // TILE, 2, self.head_dim)
+        if bounds is not None and (tuple(bounds.shape) != shape or bounds.dtype != torch.uint8
+                                   or bounds.device != self.device or not bounds.is_contiguous()):
+            raise ValueError(f"bounds must be a contiguous uint8 tensor of shape {shape} on {self.device}")
+
+    def _pack(self, rows: native.KvRowsC, row: int, count: int, bounds: Optional[torch.Tensor]) -> None:
+        with native.on_device(self.device):
+            native.check(
+                native.lib().rfsn_pack_rows(self.handle, row, ctypes.byref(rows), count,
+                                            bounds.data_ptr() if bounds is not None else None, native.stream_ptr()),
+                "rfsn_pack_rows",
+            )
+
+    def unpack(self, row: int, n: int, dtype: torch.dtype, *, out: Optional[tuple] = None):
+        """(k, v) [groups, n, D] of rows row .. row + n in ``dtype`` (exact in
+        float32 and bfloat16; float16 rounds and saturates). ``out``: a pair of
+        [groups, n, D] views with one stride between heads to write instead."""
+        if out is None:
+            shape = (self.groups, n, self.head_dim)
+            out = (torch.empty(shape, dtype=dtype, device=self.device),
+                   torch.empty(shape, dtype=dtype, device=self.device))
+        k, v = out
+        for t in (k, v):
+            if tuple(t.shape) != (self.groups, n, self.head_dim) or t.dtype != dtype or t.device != self.device \
+                    or t.stride() != k.stride() or (n > 0 and t.stride()[1:] != (self.head_dim, 1)):
+                raise ValueError(f"out must be two [{self.groups}, {n}, {self.head_dim}] tensors of {dtype} with "
+                                 "contiguous rows and one stride between heads")
+        with native.on_device(self.device):
+            native.check(
+                native.lib().rfsn_unpack_rows(self.handle, int(row), int(n), k.data_ptr(), v.data_ptr(),
+                                              native.dtype_code(dtype), k.stride(0), native.stream_ptr()),
+                "rfsn_unpack_rows",
+            )
+        return k, v
+
+
+@lru_cache(maxsize=4096)
+def workspace_bytes(batch: int, q_heads: int, kv_heads: int, q_len: int, head_dim: int, n_tiles: int,
+                    n_select: int = 0) -> int:
+    out = ctypes.c_size_t()
+    native.check(
+        native.load_library().rfsn_archive_workspace_size(batch, q_heads, kv_heads, q_len, head_dim, n_tiles, n_select,
+                                                          ctypes.byref(out)),
+        "rfsn_archive_workspace_size",
+    )
+    return int(out.value)
+
+
+def select_tiles(cache, q: torch.Tensor, q_start_pos: int, segments, top_tiles: int, *,
+                 workspace: Optional[native.Workspace] = None,
+                 step_state: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Tile list int32 [B, Hkv, q_len, top_tiles, 4] = {row, pos, len, tile} of
+    the ``top_tiles`` archived tiles with the largest logit bound for each query
+    row and KV head (``rfsn_select_tiles``); unused entries are {0, 0, 0, -1}.
+    q: float32 [B, H, q_len, D] on the cache's device. Call with the cache's
+    device current."""
+    if cache.tile_bounds is None:
+        raise ValueError("tile selection needs a cache built with tile_index=True")
+    B, H, Lq, D = q.shape
+    if not 1 <= top_tiles <= 1 << 20:
+        raise ValueError(f"top_tiles must be at least 1, got {top_tiles}")
+    if Lq > SPARSE_MAX_ROWS:
+        raise ValueError(f"tile selection takes up to {SPARSE_MAX_ROWS} query rows a call, got {Lq}")
+    tiles_dev, n_tiles = segments.tile_list
+    tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
+    out = torch.empty((B, cache.num_kv_heads, Lq, top_tiles, 4), dtype=torch.int32, device=cache.device)
+    ws = workspace if workspace is not None else native.default_workspace(cache.device)
+    buf = ws.get(workspace_bytes(B, H, cache.num_kv_heads, Lq, D, n_tiles, top_tiles))
+    bounds = cache.tile_bounds
+    packed = cache.archive is not None
+    native.check(
+        native.lib().rfsn_select_tiles(
+            bounds.data_ptr(), native.RFSN_E4M3 if packed else native.dtype_code(bounds.dtype),
+            cache.archive.scales.data_ptr() if packed else None, int(bounds.shape[1]) * TILE, q.data_ptr(), B, H,
+            cache.num_kv_heads, Lq, D, int(q_start_pos), ctypes.byref(tiles), top_tiles, out.data_ptr(),
+            step_state.data_ptr() if step_state is not None else None, buf.data_ptr(), buf.numel(),
+            native.stream_ptr()),
+        "rfsn_select_tiles",
+    )
+    return out
+
+
+def tile_attention(cache, q: torch.Tensor, q_start_pos: int, segments, out_ptr: int, lse: Optional[torch.Tensor],
+                   hot: native.HotWindowC, *, top_tiles: int, max_splits: int,
+                   workspace: Optional[native.Workspace], step_state: Optional[torch.Tensor]) -> None:
+    """Attention of float32 q over the segments' archived tiles (all of them, or
+    the ``top_tiles`` best of each query and KV head) and the hot window,
+    written to ``out_ptr``: the packed or sparse form of
+    ``cache.paged_attention``, which checks the arguments."""
+    B, H, Lq, D = q.shape
+    Hkv = cache.num_kv_heads
+    tiles_dev, n_tiles = segments.tile_list
+    if top_tiles > 0 and n_tiles > 0:
+        chosen = select_tiles(cache, q, q_start_pos, segments, top_tiles, workspace=workspace, step_state=step_state)
+        tiles = native.TileListC(chosen.data_ptr(), top_tiles, 1)
+    else:
+        top_tiles = 0
+        tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
+    ws = workspace if workspace is not None else native.default_workspace(cache.device)
+    buf = ws.get(workspace_bytes(B, H, Hkv, Lq, D, n_tiles, top_tiles))
+    native.check(
+        native.lib().rfsn_archive_attention(
+            cache.arena.handle, cache.archive.handle if cache.archive is not None else None, q.data_ptr(), B, H, Hkv,
+            Lq, int(q_start_pos), ctypes.byref(tiles), ctypes.byref(hot), out_ptr,
+            lse.data_ptr() if lse is not None else None, buf.data_ptr(), buf.numel(), max_splits,
+            native.stream_ptr()),
+        "rfsn_archive_attention",
+    )
+
+
+__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "select_tiles", "tile_attention", "workspace_bytes"]

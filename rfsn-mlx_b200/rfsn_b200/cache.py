@@ -46,6 +46,7 @@ import numpy as np
 import torch
 
 from . import _native as native
+from .archive import PackedArchive, check_archive_options, padded_rows, select_tiles, tile_attention
 from .block_manager import BlockId, BlockLocation, BlockManager, BlockManifest, BlockSpan
 from .config import RFSNConfig, RuntimeMode, resolve_dtype, validate_session_id
 from .residency import ResidencyManager
@@ -255,6 +256,17 @@ class DeviceOps:
     def new_table(self, rows: int) -> torch.Tensor:
         return torch.zeros((rows, 4), dtype=torch.int32, device=self.device)
 
+    def new_archive(self, groups: int, rows: int, head_dim: int) -> PackedArchive:
+        return PackedArchive(groups, rows, head_dim, device=self.device)
+
+    def tile_bounds(self, row: int, count: int, bounds: torch.Tensor) -> None:
+        """Channel-wise key bounds of the arena rows row .. row + count."""
+        with native.on_device(self.device):
+            native.check(
+                native.lib().rfsn_tile_bounds(self.arena.handle, row, count, bounds.data_ptr(), native.stream_ptr()),
+                "rfsn_tile_bounds",
+            )
+
 
 class PagedSegments(Sequence):
     """Segments of one layer: archived blocks (page-table order) then hot pieces.
@@ -271,6 +283,8 @@ class PagedSegments(Sequence):
         self.n_archived = len(archived)
         self.table = table                    # (device records, n_blocks, archived_tokens, archived_tiles) or None
         self.hot_state = hot_state            # (head_index, length, start) or None when hot pieces excluded
+        # (device int32 [n, 4] tiles, n) of the archived spans: packed caches and caches with a tile index
+        self.tile_list = cache.tile_snapshot() if table is not None else (cache.tile_snapshot()[0], 0)
 
     def __len__(self) -> int:
         return len(self.spans)
@@ -278,6 +292,10 @@ class PagedSegments(Sequence):
     def _view(self, i: int) -> tuple[torch.Tensor, torch.Tensor, int]:
         row, start, n = self.spans[i]
         c = self.cache
+        if c.archive is not None and i < self.n_archived:  # a copy in the cache dtype
+            k, v = c.archive.unpack(row, n, c.dtype)
+            return (k.unflatten(0, (c.batch_size, c.num_kv_heads)), v.unflatten(0, (c.batch_size, c.num_kv_heads)),
+                    start)
         k = c._arena_k[:, row:row + n, :].unflatten(0, (c.batch_size, c.num_kv_heads))
         v = c._arena_v[:, row:row + n, :].unflatten(0, (c.batch_size, c.num_kv_heads))
         return k, v, start
@@ -314,9 +332,21 @@ class LayerKVCache:
         ops: Optional[Any] = None,
         host_tier: bool = False,
         persist_async: bool = False,
+        archive_dtype: Optional[str] = None,
+        tile_index: bool = False,
+        top_tiles: int = 0,
     ) -> None:
+        """``archive_dtype="float8_e4m3fn"`` holds archived blocks in 8 bits (the
+        ring keeps the model dtype); ``tile_index=True`` keeps the key bounds that
+        ``attend(..., top_tiles=n)`` selects tiles with; ``top_tiles=n`` makes that
+        choice for every decode token of ``attention_step`` (and implies the
+        index). All need a 16-bit model dtype and head_dim 64 or 128."""
         if persist_async and not host_tier:
             raise ValueError("persist_async requires host_tier=True (the pinned copy serves reloads meanwhile)")
+        if top_tiles < 0:
+            raise ValueError(f"top_tiles must be >= 0, got {top_tiles}")
+        tile_index = tile_index or top_tiles > 0
+        check_archive_options(resolve_dtype(config.model_dtype), config.head_dim, archive_dtype, tile_index)
         self.config = config
         self.batch_size = batch_size
         self.num_heads = num_heads
@@ -333,8 +363,34 @@ class LayerKVCache:
         biggest_block = max(cap, config.block_size_seq)
         pool = pool_tokens if pool_tokens is not None else config.warm_capacity + 2 * biggest_block
         self._ring_rows = cap
-        self._alloc = _RowAllocator(cap, cap + max(pool, 1))
-        self._make_arena(cap + max(pool, 1))
+        # Packed archives and tile indexes work on whole tiles: blocks start at
+        # rows that are multiples of 64 (of the archive, or of the arena behind
+        # the ring) and own their last tile.
+        self.top_tiles = int(top_tiles)
+        self._whole_tiles = archive_dtype is not None or tile_index
+        self.archive: Optional[PackedArchive] = None
+        self.tile_bounds: Optional[torch.Tensor] = None
+        self._tiles_dev: Optional[torch.Tensor] = None
+        self._n_tiles = 0
+        self._table_serial = 0  # counts page-table refreshes
+        self._pass_cache: Optional[tuple] = None
+        if not self._whole_tiles:
+            self._alloc = _RowAllocator(cap, cap + max(pool, 1))
+            self._make_arena(cap + max(pool, 1))
+        else:
+            if pool_tokens is None:  # each block is rounded up to whole tiles
+                bs = max(1, min(config.block_size_seq, cap))
+                pool = (pool + bs - 1) // bs * padded_rows(bs)
+            pool = padded_rows(max(pool, 1))
+            if archive_dtype is not None:
+                self._alloc = _RowAllocator(0, pool)
+                self._make_arena(cap)
+                self.archive = self._ops.new_archive(batch_size * self.num_kv_heads, pool, config.head_dim)
+            else:
+                self._alloc = _RowAllocator(padded_rows(cap), padded_rows(cap) + pool)
+                self._make_arena(padded_rows(cap) + pool)
+            if tile_index:
+                self.tile_bounds = self._new_bounds()
 
         self.hot_seq_len = 0
         self.hot_start = 0
@@ -379,17 +435,49 @@ class LayerKVCache:
         groups = self.batch_size * self.num_kv_heads
         self._arena_k, self._arena_v = self._ops.new_arena(groups, rows, self.config.head_dim, self.dtype)
 
+    def _block_rows(self, n: int) -> int:
+        """Rows that a block of n tokens occupies."""
+        return padded_rows(n) if self._whole_tiles else n
+
+    def _new_bounds(self) -> torch.Tensor:
+        rows = self.archive.rows if self.archive is not None else int(self._arena_k.shape[1])
+        dtype = torch.uint8 if self.archive is not None else self.dtype  # e4m3 codes: scaled like the keys
+        shape = (self.batch_size * self.num_kv_heads, rows // native.TILE_KEYS, 2, self.config.head_dim)
+        return torch.zeros(shape, dtype=dtype, device=self.device)
+
+    def _grow_bounds(self) -> None:
+        if self.tile_bounds is not None:
+            old = self.tile_bounds
+            self.tile_bounds = self._new_bounds()
+            self.tile_bounds[:, :old.shape[1]].copy_(old)
+
+    def _grow_archive(self, min_extra: int) -> None:
+        old = self.archive
+        new_rows = padded_rows(max(old.rows * 2, old.rows + min_extra))
+        self.archive = self._ops.new_archive(old.groups, new_rows, old.head_dim)
+        for a, b in ((self.archive.k, old.k), (self.archive.v, old.v)):
+            a.view(torch.uint8)[:, :old.rows].copy_(b.view(torch.uint8))
+        self.archive.scales[:, :old.scales.shape[1]].copy_(old.scales)
+        self._alloc.grow(new_rows)
+        self._grow_bounds()
+        self._dirty = True
+
     def _grow_arena(self, min_extra: int) -> None:
+        if self.archive is not None:
+            self._grow_archive(min_extra)
+            return
         old_rows = self._arena_k.shape[1]
-        new_rows = max(old_rows * 2, old_rows + min_extra)
+        new_rows = self._block_rows(max(old_rows * 2, old_rows + min_extra))
         old_k, old_v = self._arena_k, self._arena_v
         self._make_arena(new_rows)
         self._arena_k[:, :old_rows].copy_(old_k)
         self._arena_v[:, :old_rows].copy_(old_v)
         self._alloc.grow(new_rows)
+        self._grow_bounds()
         self._dirty = True
 
     def _allocate_rows(self, n: int) -> int:
+        n = self._block_rows(n)
         row = self._alloc.allocate(n)
         if row is None:
             self._grow_arena(n)
@@ -398,7 +486,7 @@ class LayerKVCache:
         return row
 
     def _free_rows(self, row: int, n: int) -> None:
-        self._deferred_free.append((row, n))
+        self._deferred_free.append((row, self._block_rows(n)))
 
     def _flush_deferred_free(self) -> None:
         for row, n in self._deferred_free:
@@ -440,6 +528,8 @@ class LayerKVCache:
     def _clear_device_state(self) -> None:
         self._arena_k.zero_()
         self._arena_v.zero_()
+        if self.archive is not None:
+            self.archive.clear()
         self._alloc.reset()
         self._resident_rows.clear()
         if self._host_tier is not None:
@@ -603,10 +693,45 @@ class LayerKVCache:
             if m.residency == BlockLocation.WARM_RAM
         )
 
+    # ------------------------------------------------------------------ block rows
+    def _index_block(self, row: int, n: int) -> None:
+        """Key bounds of a block just written to the arena (packing computes its own)."""
+        if self.tile_bounds is not None and self.archive is None:
+            self._ops.tile_bounds(row, n, self.tile_bounds)
+
+    def _read_block(self, row: int, n: int, out_dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        """A block's K/V on the host in ``out_dtype``."""
+        if self.archive is None:
+            return self._ops.download(row, n, out_dtype)
+        k, v = self.archive.unpack(row, n, out_dtype)
+        return k.cpu(), v.cpu()
+
+    def _read_block_pinned(self, row: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """A block's K/V in pinned host memory in the cache dtype."""
+        if self.archive is None:
+            return self._ops.download_pinned(row, n)
+        k, v = self.archive.unpack(row, n, self.dtype)
+        k_host, v_host = torch.empty(k.shape, dtype=k.dtype, pin_memory=True), torch.empty(v.shape, dtype=v.dtype,
+                                                                                           pin_memory=True)
+        k_host.copy_(k)
+        v_host.copy_(v)
+        return k_host, v_host
+
+    def _write_block(self, row: int, n: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Host K/V [groups, n, D] into block rows (packing values that were
+        unpacked before gives the same codes up to the choice of scale, and the
+        same values)."""
+        if self.archive is None:
+            self._ops.upload(row, n, k, v)
+            self._index_block(row, n)
+            return
+        kd, vd = k.to(self.device, non_blocking=True), v.to(self.device, non_blocking=True)
+        self.archive.pack(kd[None], vd[None], row, bounds=self.tile_bounds)
+
     # ------------------------------------------------------------------ warm <-> cold
     def _download_block(self, row: int, n: int) -> dict[str, np.ndarray]:
         out_dtype = torch.float16 if self.storage_array_dtype == np.float16 else torch.float32
-        k_host, v_host = self._ops.download(row, n, out_dtype)
+        k_host, v_host = self._read_block(row, n, out_dtype)
         shape = (self.batch_size, self.num_kv_heads, n, self.config.head_dim)
         return {"keys": k_host.numpy().reshape(shape), "values": v_host.numpy().reshape(shape)}
 
@@ -636,7 +761,7 @@ class LayerKVCache:
                 else:
                     self.storage.write_manifest(manifest)
                 return
-            k_pin, v_pin = self._ops.download_pinned(row, n)
+            k_pin, v_pin = self._read_block_pinned(row, n)
             self._free_rows(row, n)
             self._host_tier[manifest.block_id] = (k_pin, v_pin)
             out = np.float16 if self.storage_array_dtype == np.float16 else np.float32
@@ -693,7 +818,7 @@ class LayerKVCache:
             k = torch.as_tensor(np.asarray(keys)).reshape(groups, n, D)
             v = torch.as_tensor(np.asarray(values)).reshape(groups, n, D)
         row = self._allocate_rows(n)
-        self._ops.upload(row, n, k, v)
+        self._write_block(row, n, k, v)
         self._resident_rows[manifest.block_id] = row
         manifest.residency = BlockLocation.WARM_RAM
         manifest.touch()
@@ -707,7 +832,12 @@ class LayerKVCache:
         """cache.py:324-339: the oldest prefix_len ring tokens become a block."""
         start, end = self.hot_start, self.hot_start + prefix_len
         row = self._allocate_rows(prefix_len)
-        self._ops.copy_rows(0, self.hot_head_index, self.config.hot_capacity, row, prefix_len)
+        if self.archive is not None:
+            self.archive.pack_ring(self._arena_k, self._arena_v, self.hot_head_index, self.config.hot_capacity, row,
+                                   prefix_len, bounds=self.tile_bounds)
+        else:
+            self._ops.copy_rows(0, self.hot_head_index, self.config.hot_capacity, row, prefix_len)
+            self._index_block(row, prefix_len)
         manifest = self._next_block_manifest(start, end, self._storage_dtype_name())
         self.block_manager.register_block(manifest)
         self._resident_rows[manifest.block_id] = row
@@ -814,8 +944,12 @@ class LayerKVCache:
         self.block_manager.register_block(manifest)
         row = self._allocate_rows(n)
         groups, D = self.batch_size * self.num_kv_heads, self.config.head_dim
-        self._arena_k[:, row:row + n].copy_(kc.reshape(groups, n, D))
-        self._arena_v[:, row:row + n].copy_(vc.reshape(groups, n, D))
+        if self.archive is not None:
+            self.archive.pack(kc, vc, row, bounds=self.tile_bounds)
+        else:
+            self._arena_k[:, row:row + n].copy_(kc.reshape(groups, n, D))
+            self._arena_v[:, row:row + n].copy_(vc.reshape(groups, n, D))
+            self._index_block(row, n)
         self._resident_rows[manifest.block_id] = row
         self._dirty = True
         return manifest
@@ -886,11 +1020,78 @@ class LayerKVCache:
         if self._table_dev.shape[0] < records.shape[0]:
             self._table_dev = self._ops.new_table(max(records.shape[0], 2 * self._table_dev.shape[0]))
         self._table_dev[: records.shape[0]].copy_(torch.from_numpy(records))
+        if self._whole_tiles:
+            self._table_serial += 1
+            self._refresh_tiles(records)
         self._attended, self._attended_spans = attended, spans
         self._table_meta = (len(spans), sum(n for _, _, n in spans), tile)
         # every block still attended must be resident for the fast path to stay valid
         self._dirty = any(m.block_id not in self._resident_rows for m in attended)
         self._seen_version = self.block_manager.version
+
+    def _refresh_tiles(self, records: np.ndarray) -> None:
+        """The page table tile by tile: int32 {row, pos, len, tile} on the device."""
+        T = native.TILE_KEYS
+        per = (records[:-1, 2] + T - 1) // T
+        block = np.repeat(np.arange(len(per)), per)
+        tile = np.arange(len(block), dtype=np.int32)
+        off = (tile - records[block, 3]) * T
+        tiles = np.stack([records[block, 0] + off, records[block, 1] + off, np.minimum(records[block, 2] - off, T),
+                          tile], axis=1).astype(np.int32)
+        if self._tiles_dev is None or self._tiles_dev.shape[0] < len(tiles):
+            self._tiles_dev = self._ops.new_table(max(len(tiles), 64 if self._tiles_dev is None
+                                                      else 2 * self._tiles_dev.shape[0]))
+        self._tiles_dev[:len(tiles)].copy_(torch.from_numpy(tiles))
+        self._n_tiles = len(tiles)
+
+    def pass_tables(self, spans: list, row0: int, keys: int) -> tuple[list, torch.Tensor]:
+        """The archived spans as page tables of at most ``keys`` tokens each, for
+        rows shifted by ``row0``: [(first record, records, tokens, tiles)] and the
+        device records (kept until the page table changes)."""
+        key = (self._table_serial, row0, keys, len(spans))
+        if self._pass_cache is not None and self._pass_cache[0] == key:
+            return self._pass_cache[1]
+        passes, records, blocks, room = [], [], [], keys
+        for row, start, n in spans:
+            at = 0
+            while at < n:
+                take = min(room, n - at)
+                blocks.append((row0 + row + at, start + at, take))
+                at += take
+                room -= take
+                if room == 0:
+                    passes.append(blocks)
+                    blocks, room = [], keys
+        if blocks:
+            passes.append(blocks)
+        out = []
+        for blocks in passes:
+            first, tile = len(records), 0
+            for row, start, n in blocks:
+                records.append((row, start, n, tile))
+                tile += _tiles(n)
+            records.append((0, 0, 0, tile))
+            out.append((first, len(blocks), sum(n for _, _, n in blocks), tile))
+        dev = self._ops.new_table(len(records))
+        dev.copy_(torch.tensor(records, dtype=torch.int32))
+        self._pass_cache = (key, (out, dev))
+        return out, dev
+
+    def tile_snapshot(self) -> tuple[Optional[torch.Tensor], int]:
+        """Device tile list of the attended archived blocks and its length (packed
+        caches and caches with a tile index)."""
+        if self._whole_tiles and self._tiles_dev is None:
+            self._tiles_dev = self._ops.new_table(64)
+        return self._tiles_dev, self._n_tiles
+
+    def capture_key(self) -> tuple:
+        """Device addresses, beyond the arena's and the page table's, that a
+        captured attention call of this layer holds by value."""
+        if not self._whole_tiles:
+            return ()
+        return (self.tile_snapshot()[0].data_ptr(), self._n_tiles, self.top_tiles,
+                self.archive.k.data_ptr() if self.archive is not None else 0,
+                self.tile_bounds.data_ptr() if self.tile_bounds is not None else 0)
 
     def _archived_current(self) -> None:
         self.residency_manager.drain_completed_prefetches(self)
@@ -972,18 +1173,104 @@ class LayerKVCache:
 
     # ------------------------------------------------------------------ attention
     def attend(self, q: torch.Tensor, q_start_pos: int, segments: Optional[PagedSegments] = None,
-               *, want_lse: bool = False, max_splits: int = 0):
+               *, want_lse: bool = False, max_splits: int = 0, top_tiles: int = 0):
         """Exact attention of float32 q [B, H, Lq, D] against this layer's
-        archived blocks and hot window (the work of layer.py:139-162)."""
+        archived blocks and hot window (the work of layer.py:139-162). With
+        ``top_tiles`` only the best tiles of each query and KV head are read
+        (``paged_attention``)."""
         if segments is None:
             segments = self.get_attention_segments()
-        return paged_attention(self, q, q_start_pos, segments, want_lse=want_lse, max_splits=max_splits)
+        return paged_attention(self, q, q_start_pos, segments, want_lse=want_lse, max_splits=max_splits,
+                               top_tiles=top_tiles)
+
+    def select_tiles(self, q: torch.Tensor, q_start_pos: int, top_tiles: int,
+                     segments: Optional[PagedSegments] = None) -> torch.Tensor:
+        """Numbers of the archived 64-token tiles (counted through the blocks in
+        page-table order) that ``attend(..., top_tiles=n)`` reads: int32
+        [B, Hkv, Lq, top_tiles], ascending, -1 behind them. Needs
+        ``tile_index=True``."""
+        if segments is None:
+            segments = self.get_attention_segments()
+        qf = _query(self, q)
+        with native.on_device(self.device):
+            return select_tiles(self, qf, q_start_pos, segments, int(top_tiles))[..., 3]
+
+
+def _query(cache: LayerKVCache, q: torch.Tensor) -> torch.Tensor:
+    if q.dim() != 4 or q.shape[0] != cache.batch_size or q.shape[3] != cache.config.head_dim:
+        raise ValueError(f"q must be [batch={cache.batch_size}, heads, q_len, head_dim={cache.config.head_dim}]")
+    return _as(q, cache.device, torch.float32)
+
+
+# Keys of one pass of _unpacked_attention. The prefill kernel adds every tile's
+# P V to one float32 accumulator on the tensor cores, whose rounding error grows
+# with the number of additions: 4e-5 of the result over 17K keys, about 5e-6
+# over 2K. Shorter passes cost launches (512 queries x 17K keys: see
+# _unpacked_attention).
+_PASS_KEYS = 2048
+_MERGE_PARTS = 8
+_CHUNK_ROWS = 64  # query rows from which the tensor-core prefill kernel runs (head_dim 128)
+
+
+def _unpacked_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segments: PagedSegments,
+                        out_ptr: int, lse: Optional[torch.Tensor], hot: native.HotWindowC,
+                        workspace: Optional[native.Workspace]) -> None:
+    """A prompt chunk over a packed cache: products outweigh bytes, so the
+    archive's used rows are unpacked once, behind a copy of the ring, into a
+    temporary arena in the cache dtype that the tensor-core prefill kernel
+    reads, in passes of at most ``_PASS_KEYS`` archived keys (the last one with
+    the ring) merged by their log-sum-exps in float32."""
+    cap, archive = cache._ring_rows, cache.archive
+    spans = segments.spans[:segments.n_archived]
+    used = max(row + n for row, _, n in spans)
+    k = torch.empty((archive.groups, cap + used, archive.head_dim), dtype=cache.dtype, device=cache.device)
+    v = torch.empty_like(k)
+    k[:, :cap].copy_(cache._arena_k[:, :cap])
+    v[:, :cap].copy_(cache._arena_v[:, :cap])
+    archive.unpack(0, used, cache.dtype, out=(k[:, cap:], v[:, cap:]))
+    arena = native.Arena(k, v)
+    passes, records = cache.pass_tables(spans, cap, _PASS_KEYS)
+    B, H, Lq, D = (int(x) for x in q.shape)
+    rows = B * H * Lq
+    ws = workspace if workspace is not None else native.default_workspace(cache.device)
+    buf = ws.get(native.workspace_bytes(B, H, cache.num_kv_heads, Lq, D, 0))
+    parts = min(len(passes), _MERGE_PARTS)
+    no_hot = native.HotWindowC(0, cap, 0, 0, 0, 0, None)
+    o = torch.empty((parts, rows, D), dtype=torch.float32, device=cache.device) if parts > 1 else None
+    m = torch.empty((parts, rows), dtype=torch.float32, device=cache.device) if parts > 1 else None
+    lse_ptr = lse.data_ptr() if lse is not None else None
+    filled = 0
+    for i, (first, n, tokens, tiles) in enumerate(passes):
+        last = i == len(passes) - 1
+        table = native.PageTableC(records.data_ptr() + 16 * first, n, tokens, tiles, 0)
+        native.check(
+            native.lib().rfsn_paged_attention(
+                arena.handle, q.data_ptr(), B, H, cache.num_kv_heads, Lq, int(q_start_pos),
+                native.ctypes.byref(table), native.ctypes.byref(hot if last else no_hot),
+                o[filled].data_ptr() if parts > 1 else out_ptr, m[filled].data_ptr() if parts > 1 else lse_ptr,
+                buf.data_ptr(), buf.numel(), 0, native.stream_ptr()),
+            "rfsn_paged_attention",
+        )
+        filled += 1
+        if parts == 1 or not (last or filled == parts):
+            continue
+        if last:
+            dst, dst_lse = out_ptr, lse_ptr
+        else:  # more passes than parts: what is merged becomes the first part of the next merge
+            merged, merged_lse = torch.empty_like(o[0]), torch.empty_like(m[0])
+            dst, dst_lse = merged.data_ptr(), merged_lse.data_ptr()
+        native.check(native.lib().rfsn_lse_merge(o.data_ptr(), m.data_ptr(), filled, rows, D, dst, dst_lse,
+                                                 native.stream_ptr()), "rfsn_lse_merge")
+        if not last:
+            o[0].copy_(merged)
+            m[0].copy_(merged_lse)
+            filled = 1
 
 
 def paged_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segments: PagedSegments,
                     *, want_lse: bool = False, max_splits: int = 0, workspace: Optional[native.Workspace] = None,
                     peers: Optional[Any] = None, step_state: Optional[torch.Tensor] = None,
-                    out: Optional[torch.Tensor] = None):
+                    out: Optional[torch.Tensor] = None, top_tiles: int = 0):
     """Exact attention of q over a layer's page table + hot window.
 
     With ``peers`` (a ``sharded.PeerGroup``) the kernel also merges the
@@ -998,12 +1285,16 @@ def paged_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
 
     ``out`` (float32 [B, H, Lq, D], contiguous) receives the result instead of
     a new tensor: a tensor on the cache's device, or a pinned CPU tensor that
-    the kernel writes across the bus (no separate copy back)."""
+    the kernel writes across the bus (no separate copy back).
+
+    A cache with a packed archive attends to the packed values. With
+    ``top_tiles`` (a cache with a tile index; up to 64 query rows) each query
+    row reads, per KV head, only the ``top_tiles`` archived 64-token tiles with
+    the largest logit bounds (``LayerKVCache.select_tiles``) and the hot window:
+    the softmax over those keys."""
     if len(segments) == 0 and peers is None:
         raise RuntimeError("run_segmented_attention requires at least one KV segment")
-    if q.dim() != 4 or q.shape[0] != cache.batch_size or q.shape[3] != cache.config.head_dim:
-        raise ValueError(f"q must be [batch={cache.batch_size}, heads, q_len, head_dim={cache.config.head_dim}]")
-    qf = _as(q, cache.device, torch.float32)
+    qf = _query(cache, q)
     B, H, Lq, D = (int(x) for x in qf.shape)
     if out is None:
         out = torch.empty((B, H, Lq, D), dtype=torch.float32, device=cache.device)
@@ -1032,6 +1323,19 @@ def paged_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
             head, hlen, hstart = cache.hot_head_index, cache.hot_seq_len, cache.hot_start
     hot = native.HotWindowC(0, cache.config.hot_capacity, head, hlen, hstart, 0,
                             step_state.data_ptr() if step_state is not None else None)
+    if top_tiles or cache.archive is not None:
+        if peers is not None:
+            raise NotImplementedError("the merge across GPUs inside the kernel reads exact archives in full: no packed "
+                                      "archive and no tile selection")
+        if top_tiles < 0 or (top_tiles and cache.tile_bounds is None):
+            raise ValueError("top_tiles needs a cache built with tile_index=True and a count >= 0")
+        with native.on_device(cache.device):
+            if not top_tiles and segments.n_archived and step_state is None and Lq >= _CHUNK_ROWS and D == 128:
+                _unpacked_attention(cache, qf, q_start_pos, segments, out_ptr, lse, hot, workspace)
+            else:
+                tile_attention(cache, qf, q_start_pos, segments, out_ptr, lse, hot, top_tiles=int(top_tiles),
+                               max_splits=max_splits, workspace=workspace, step_state=step_state)
+        return (out, lse) if want_lse else out
     ws = workspace if workspace is not None else native.default_workspace(cache.device)
     nbytes = native.workspace_bytes(B, H, cache.num_kv_heads, Lq, D, max_splits)
     buf = ws.get(nbytes)
@@ -1074,6 +1378,9 @@ class RFSNCache:
         ops_factory: Optional[Any] = None,
         host_tier: bool = False,
         persist_async: bool = False,
+        archive_dtype: Optional[str] = None,
+        tile_index: bool = False,
+        top_tiles: int = 0,
     ) -> None:
         self.config = config
         self.model_id = model_id or derive_model_id(config)
@@ -1092,6 +1399,9 @@ class RFSNCache:
                 ops=ops_factory() if ops_factory is not None else None,
                 host_tier=host_tier,
                 persist_async=persist_async,
+                archive_dtype=archive_dtype,
+                tile_index=tile_index,
+                top_tiles=top_tiles,
             )
             for i in range(config.num_layers)
         ]

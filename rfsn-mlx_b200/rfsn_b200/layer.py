@@ -46,7 +46,7 @@ def attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Lay
     if seq_len == 1:
         cache.maybe_prefetch_for_decode(start_pos)
     segments = cache.get_attention_segments()
-    return paged_attention(cache, q_rot, start_pos, segments)
+    return paged_attention(cache, q_rot, start_pos, segments, top_tiles=cache.top_tiles if seq_len == 1 else 0)
 
 
 def attention_step_tables(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: LayerKVCache, start_pos: int,
@@ -61,7 +61,7 @@ def attention_step_tables(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cac
     if seq_len == 1:
         cache.maybe_prefetch_for_decode(start_pos)
     segments = cache.get_attention_segments()
-    return paged_attention(cache, q_rot, start_pos, segments)
+    return paged_attention(cache, q_rot, start_pos, segments, top_tiles=cache.top_tiles if seq_len == 1 else 0)
 
 
 def capture_graph(fn, stream: torch.cuda.Stream) -> torch.cuda.CUDAGraph:
@@ -164,7 +164,7 @@ class GraphedDecodeStep:
             "rfsn_rope_append_step",
         )
         return paged_attention(c, q_rot, 0, segs, workspace=self.workspace, step_state=self.state_dev,
-                               out=self.out_host)
+                               out=self.out_host, top_tiles=c.top_tiles)
 
     def step(self, pos: int) -> torch.Tensor:
         from . import _native as native
@@ -189,7 +189,8 @@ class GraphedDecodeStep:
         st = self._state_np
         st[0], st[1], st[2], st[3], st[4] = pos, write_index, head, hlen, hstart
         key = (c.arena.handle.value, c._arena_k.data_ptr(),
-               (segs.table[0].data_ptr(),) + tuple(segs.table[1:]) if segs.table is not None else None)
+               (segs.table[0].data_ptr(),) + tuple(segs.table[1:]) if segs.table is not None else None,
+               c.capture_key())
         if key != self.key or self.graph is None:
             # run this step op by op on the side stream first (the warm-up a
             # capture wants; it also produces this step's result), then capture

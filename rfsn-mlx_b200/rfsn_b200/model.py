@@ -536,7 +536,7 @@ class _DecodeGraph:
         B = int(token_id.numel())
         key = (B,) + tuple((lc.arena.handle.value if hasattr(lc.arena.handle, "value") else id(lc.arena),
                             lc._arena_k.data_ptr(), sg.table[0].data_ptr() if sg.table is not None else 0,
-                            sg.table[1:] if sg.table is not None else None) for lc, sg in zip(cache.layers, segs))
+                            sg.table[1:] if sg.table is not None else None, lc.capture_key()) for lc, sg in zip(cache.layers, segs))
         if self.tok.numel() != B:
             self.tok = torch.zeros((B,), dtype=torch.long, device=model.device)
         self.tok.copy_(token_id.reshape(-1).to(device=model.device, dtype=torch.long), non_blocking=True)
@@ -569,7 +569,8 @@ class _DecodeGraph:
                 lc.config.hot_capacity, native.stream_ptr()),
             "rfsn_rope_append_step",
         )
-        return paged_attention(lc, q_rot, 0, segs, workspace=self.workspace, step_state=self.state_dev)
+        return paged_attention(lc, q_rot, 0, segs, workspace=self.workspace, step_state=self.state_dev,
+                               top_tiles=lc.top_tiles)
 
     def _capture(self, segs) -> None:
         """Run this step once op by op on a side stream (the warm-up torch asks

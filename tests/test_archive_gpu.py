@@ -1,0 +1,505 @@
+"""Packed archives, tile selection and attention over tiles on the GPU, against plain 64-bit forms.
+
+Tolerance of the attention outputs, by arithmetic: a logit is a sum of D / 16 tensor-core steps of products that carry
+at least 22 significant bits of q (K enters exactly), so its error is below (D / 16 + 4) 2^-23 sum |q_d k_d| / sqrt(D).
+With |q_d k_d| summing to at most ~2 D for N(0, 1) data (checked below through the data itself) that is 12 * 2^-23 * 2
+* sqrt(128) < 2^-15 for D = 128; the probabilities get that relative error twice (p and its sum), the split of p 2^-21,
+the exponentials 2^-22, and the sums over a split's keys at most N / 64 steps of 2^-23 each (N <= 2^14 here: 2^-15).
+Together below 2^-13 of the largest |v|.
+"""
+
+import math
+import tempfile
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+REL = 2.0 ** -13
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def make(dtype="bfloat16", B=1, H=8, Hkv=2, D=128, lens=(100, 64, 1), hot=50, hot_cap=None, wrap=0, seed=0,
+         archive_dtype="float8_e4m3fn", tile_index=False, top_tiles=0, scale=1.0, **kw):
+    """A layer cache with the given archived blocks and ``hot`` ring tokens (the ring's oldest at slot ``wrap``), and
+    its keys and values [B, Hkv, N + hot, D]."""
+    torch = _torch()
+    from rfsn_b200 import LayerKVCache, RFSNConfig
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n, cap = sum(lens) + hot, hot_cap or max(hot + wrap, 1)
+    room = max(cap, sum(lens), 1)
+    cfg = RFSNConfig(hidden_dim=H * D, num_heads=H, num_kv_heads=Hkv, head_dim=D, num_layers=1, hot_capacity=cap,
+                     warm_capacity=room, cold_capacity=room, block_size_seq=min(64, cap), model_dtype=dtype,
+                     disk_cache_dir=tempfile.mkdtemp(prefix="rfsn_archive_"))
+    cache = LayerKVCache(cfg, B, H, Hkv, session_id="t", archive_dtype=archive_dtype, tile_index=tile_index,
+                         top_tiles=top_tiles, **kw)
+    k = (torch.randn(B, Hkv, n, D, generator=g, device="cuda") * scale).to(cache.dtype)
+    v = torch.randn(B, Hkv, n, D, generator=g, device="cuda").to(cache.dtype)
+    at = 0
+    for length in lens:
+        cache.import_block(k[:, :, at:at + length], v[:, :, at:at + length], at)
+        at += length
+    cache.hot_start, cache.hot_head_index = at, wrap % cap
+    if hot:
+        cache.append_exact(k[:, :, at:], v[:, :, at:])
+    return cache, k, v
+
+
+def held(cache, k, v, lens):
+    """The keys and values as the cache holds them (float64), from the plain form of packing."""
+    torch = _torch()
+    import archive_ref as ref
+
+    out = []
+    for x in (k, v):
+        x = x.double().cpu()
+        if cache.archive is not None:
+            B, Hkv, n, D = x.shape
+            at = 0
+            for length in lens:
+                part = ref.pack(x[:, :, at:at + length].reshape(B * Hkv, length, D))[0]
+                x[:, :, at:at + length] = part.reshape(B, Hkv, length, D)
+                at += length
+        out.append(x)
+    return out
+
+
+def same(a, b):
+    """Equal values, NaN where the other has NaN (fp16 input of the packing tests overflows to infinity in places)."""
+    torch = _torch()
+    return a.shape == b.shape and torch.allclose(a.double(), b.double(), rtol=0, atol=0, equal_nan=True)
+
+
+def queries(B, H, Lq, D, seed=7, scale=1.0):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(B, H, Lq, D, generator=g, device="cuda") * scale
+
+
+def check_out(out, lse, want, want_lse, v):
+    torch = _torch()
+    tol = REL * float(v.abs().max())
+    err = float((out.double().cpu() - want).abs().max())
+    assert err <= tol
+    if lse is not None:
+        got, fine = lse.double().cpu(), torch.isfinite(want_lse)
+        assert torch.equal(torch.isfinite(got), fine)
+        assert float((got - want_lse)[fine].abs().max() if fine.any() else 0.0) <= REL * 4
+
+
+# ------------------------------------------------------------------ packing
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,row", [(1, 0), (64, 64), (65, 128), (300, 0)])
+def test_pack_gives_the_codes_scales_and_bounds_of_the_formula(dtype, D, n, row):
+    torch = _torch()
+    import archive_ref as ref
+    from rfsn_b200 import PackedArchive
+
+    g = torch.Generator().manual_seed(n + D)
+    x = [torch.randn(2, 3, n, D, generator=g) * torch.exp(3 * torch.randn(2, 3, n, 1, generator=g)) for _ in range(2)]
+    x = [t.to(getattr(torch, dtype)) for t in x]
+    x[0][0, 0, 0, 0] = 0.0
+    x[0][1, 1] = 0.0  # a tile of zeros
+    a = PackedArchive(6, 512, D)
+    a.k.view(torch.uint8).fill_(0x7f)  # NaN codes: what is not written stays, what belongs to the block is overwritten
+    a.v.view(torch.uint8).fill_(0x7f)
+    bounds = torch.zeros(6, 8, 2, D, dtype=torch.uint8, device="cuda")
+    # token-major memory: [B, n, Hkv, D] seen as [B, Hkv, n, D]
+    kv = [t.transpose(1, 2).contiguous().cuda().transpose(1, 2) for t in x]
+    a.pack(kv[0], kv[1], row, bounds=bounds)
+    end = (n + 63) // 64 * 64
+    for t, got, scale in ((x[0], a.k, a.k_scale), (x[1], a.v, a.v_scale)):
+        values, scales, codes = ref.pack(t.reshape(6, n, D))
+        assert same(scale[:, row // 64:(row + end) // 64].double().cpu(), scales)
+        assert same(got[:, row:row + n].double().cpu(), codes)
+        assert (got[:, row + n:row + end].view(torch.uint8) == 0).all()
+        assert (got[:, row + end:].view(torch.uint8) == 0x7f).all() and (got[:, :row].view(torch.uint8) == 0x7f).all()
+        if t is x[0]:
+            lo, hi, _ = ref.bounds(codes.reshape(2, 3, n, D), [n])
+            b = bounds[:, row // 64:(row + end) // 64].view(torch.float8_e4m3fn).double().cpu()
+            assert same(b[:, :, 0], lo.reshape(6, -1, D)) and same(b[:, :, 1], hi.reshape(6, -1, D))
+    for out_dtype in (torch.float32, torch.bfloat16, torch.float16):
+        k, v = a.unpack(row, n, out_dtype)
+        top = torch.finfo(out_dtype).max  # finite values saturate
+        assert same(k.cpu(), ref.pack(x[0].reshape(6, n, D))[0].clamp(-top, top).to(out_dtype))
+        assert same(v.cpu(), ref.pack(x[1].reshape(6, n, D))[0].clamp(-top, top).to(out_dtype))
+
+
+def test_pack_of_unpacked_values_changes_nothing():
+    torch = _torch()
+    from rfsn_b200 import PackedArchive
+
+    x = (torch.randn(1, 2, 640, 128, device="cuda") * 3).to(torch.bfloat16)
+    a, b = PackedArchive(2, 640, 128), PackedArchive(2, 640, 128)
+    a.pack(x, -x)
+    k, v = a.unpack(0, 640, torch.bfloat16)
+    b.pack(k[None], v[None])
+    k2, v2 = b.unpack(0, 640, torch.bfloat16)
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+def test_pack_extremes():
+    """NaN stays, infinities become NaN and do not count for the scale; the smallest and largest magnitudes of each
+    type; a maximum that just reaches the next scale."""
+    torch = _torch()
+    import archive_ref as ref
+    from rfsn_b200 import PackedArchive
+
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        info = torch.finfo(dtype)
+        x = torch.zeros(1, 8, 64, 64)
+        x[0, 0, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, 2.0])
+        x[0, 1, 3, 5] = info.max
+        x[0, 2, 3, 5] = info.smallest_normal
+        x[0, 3, 3, :2] = torch.tensor([448.0, -1.0])
+        x[0, 4, 3, :2] = torch.tensor([449.0 if dtype == torch.float32 else 452.0, 2.0 ** -9])
+        x[0, 5, :, :] = math.inf
+        x[0, 6, 9, 9] = 1.75
+        x[0, 7, 9, 9] = 1.75 + 4 * info.eps
+        x = x.to(dtype)
+        a = PackedArchive(8, 64, 64)
+        a.pack(x.cuda(), x.cuda())
+        values, scales, codes = ref.pack(x[0])
+        assert torch.equal(a.k_scale.double().cpu(), scales), dtype
+        got = a.v.double().cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(codes)) and torch.equal(got.nan_to_num(), codes.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("head,count", [(0, 40), (90, 70), (60, 100)])
+def test_seal_of_a_wrapped_ring_packs_its_oldest_tokens(dtype, head, count):
+    torch = _torch()
+    import archive_ref as ref
+
+    cache, k, v = make(dtype, lens=(), hot=100, hot_cap=100, wrap=head)
+    cache._seal_hot_prefix(count)
+    want = ref.pack(k[0, :, :count])[0]
+    got = cache.get_archived_attention_segments()[0]
+    assert torch.equal(got[0][0].double().cpu(), want) and got[2] == 0
+    assert cache.hot_seq_len == 100 - count
+
+
+# ------------------------------------------------------------------ attention
+CASES = [
+    # dtype, B, H, Hkv, D, lens, hot, wrap, Lq
+    ("bfloat16", 1, 32, 8, 128, (256,) * 5, 200, 0, 1),
+    ("float16", 1, 32, 8, 128, (256,) * 5, 200, 100, 1),
+    ("bfloat16", 1, 8, 8, 64, (65, 1, 64, 130), 3, 2, 1),
+    ("float16", 2, 8, 2, 64, (1000, 37), 129, 60, 3),
+    ("bfloat16", 2, 12, 4, 128, (63, 64, 65), 33, 30, 5),
+    ("bfloat16", 1, 16, 1, 128, (700,), 1, 0, 2),      # 32 slots of one KV head
+    ("float16", 1, 6, 2, 128, (), 100, 40, 1),         # nothing archived
+    ("bfloat16", 1, 4, 4, 128, (900, 130), 0, 0, 1),   # nothing hot
+    ("float16", 3, 4, 2, 64, (1,), 1, 0, 1),
+    ("bfloat16", 1, 32, 8, 128, (512,) * 20 + (77,), 500, 400, 20),   # long chunk: unpacked
+    ("float16", 1, 32, 8, 128, (512, 33), 256, 0, 200),               # tensor-core prefill over unpacked tiles
+    ("bfloat16", 1, 8, 4, 64, (300,), 64, 0, 50),
+]
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("dtype,B,H,Hkv,D,lens,hot,wrap,Lq", CASES)
+def test_attention_over_the_archive_and_the_ring(dtype, B, H, Hkv, D, lens, hot, wrap, Lq, packed):
+    torch = _torch()
+    import archive_ref as ref
+
+    cache, k, v = make(dtype, B, H, Hkv, D, lens, hot, wrap=wrap, hot_cap=max(1, hot), seed=Lq,
+                       archive_dtype="float8_e4m3fn" if packed else None, tile_index=not packed)
+    n = sum(lens) + hot
+    q = queries(B, H, Lq, D)
+    kk, vv = held(cache, k, v, lens)
+    want, want_lse = ref.attention(q, kk, vv, torch.arange(n), n - Lq)
+    if packed:
+        out, lse = cache.attend(q, n - Lq, want_lse=True)
+        check_out(out, lse, want, want_lse, vv)
+    elif Lq <= 64:  # every tile selected: the exact archive through the tile kernel
+        out, lse = cache.attend(q, n - Lq, want_lse=True, top_tiles=len(ref.tiles_of(lens)) + 3)
+        check_out(out, lse, want, want_lse, vv)
+    if packed and 0 < len(lens):  # any split count gives the same softmax
+        for splits in (1, 3):
+            out, lse = cache.attend(q, n - Lq, want_lse=True, max_splits=splits)
+            check_out(out, lse, want, want_lse, vv)
+
+
+@pytest.mark.parametrize("q_pos", [-1, 0, 63, 64, 100, 250])
+def test_queries_among_the_keys_see_the_earlier_ones_only(q_pos):
+    """Positions inside the archive mask part of a tile, whole tiles and the ring; a row before every key gives zeros
+    and -inf."""
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (100, 90)
+    cache, k, v = make("float16", 1, 8, 2, 128, lens, 60)
+    q = queries(1, 8, 3, 128)
+    kk, vv = held(cache, k, v, lens)
+    want, want_lse = ref.attention(q, kk, vv, torch.arange(250), q_pos)
+    out, lse = cache.attend(q, q_pos, want_lse=True)
+    check_out(out, lse, want, want_lse, vv)
+    if q_pos == -1:
+        assert float(out[:, :, 0].abs().max()) == 0.0 and bool((lse[:, :, 0] == -math.inf).all())
+
+
+def test_what_is_masked_or_behind_the_ends_does_not_reach_the_result():
+    """NaN and infinity in ring slots outside the live window, in the tile rows behind a block's end (other than the
+    zero codes that packing writes) and in keys after the query."""
+    torch = _torch()
+
+    lens = (70,)
+    cache, k, v = make("bfloat16", 1, 4, 2, 128, lens, 40, hot_cap=100, wrap=30)
+    q = queries(1, 4, 1, 128)
+    want = cache.attend(q, 109).clone()
+    cache._arena_k[:, :30] = math.nan
+    cache._arena_v[:, :30] = math.nan
+    cache._arena_k[:, 70:] = math.inf
+    cache._arena_v[:, 70:] = math.nan
+    assert torch.equal(cache.attend(q, 109), want)
+    before = cache.attend(q, 50).clone()  # a query inside the archive: the ring lies behind it
+    cache._arena_k[:, 30:70] = math.nan
+    assert torch.equal(cache.attend(q, 50), before)
+
+
+def test_nan_keys_and_values_that_are_seen_reach_the_result():
+    torch = _torch()
+    cache, k, v = make("float16", 1, 4, 2, 128, (70, 64), 40)
+    q = queries(1, 4, 1, 128)
+    kn = k[:, :, :70].clone()
+    kn[0, 1, 3, 5] = math.inf
+    cache.archive.pack(kn, v[:, :, :70], cache._attended_spans[0][0] if cache._attended_spans else 0)
+    out = cache.attend(q, 173)
+    assert bool(torch.isnan(out[0, 2:]).all()) and bool(torch.isfinite(out[0, :2]).all())
+
+
+def test_values_of_very_different_size_and_large_logits():
+    """V scales from 2^-20 to 2^12 from tile to tile, and logits of some hundreds."""
+    torch = _torch()
+    import archive_ref as ref
+    from rfsn_b200 import LayerKVCache  # noqa: F401
+
+    lens = (64,) * 12
+    cache, k, v = make("bfloat16", 1, 4, 1, 128, (), 0, hot_cap=8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = (torch.randn(1, 1, 768, 128, generator=g, device="cuda")).to(torch.bfloat16)
+    level = torch.exp2(torch.tensor([-8, 0, 12, -20, 3, 3, -9, 12, -1, 0, 5, 2.0], device="cuda"))
+    v = (torch.randn(1, 1, 768, 128, generator=g, device="cuda") * level.repeat_interleave(64)[:, None]).to(torch.bfloat16)
+    for i in range(12):
+        cache.import_block(k[:, :, 64 * i:64 * i + 64], v[:, :, 64 * i:64 * i + 64], 64 * i)
+    for scale in (1.0, 60.0, 1e-30, 0.0):
+        q = queries(1, 4, 1, 128, scale=scale)
+        kk, vv = held(cache, k, v, lens)
+        want, want_lse = ref.attention(q, kk, vv, torch.arange(768), 767)
+        out, lse = cache.attend(q, 767, want_lse=True)
+        # logits of `scale` times the usual size carry that many times the error
+        tol = REL * max(1.0, scale) * float(vv.abs().max())
+        assert float((out.double().cpu() - want).abs().max()) <= tol
+        assert float((lse.double().cpu() - want_lse).abs().max()) <= REL * 4 * max(1.0, scale)
+
+
+# ------------------------------------------------------------------ selection
+SELECT = [
+    # dtype, packed, B, H, Hkv, D, lens, hot, Lq, top
+    ("bfloat16", False, 1, 32, 8, 128, (256,) * 6, 100, 1, 5),
+    ("float16", False, 2, 8, 2, 64, (65, 1, 200), 10, 3, 2),
+    ("bfloat16", True, 1, 32, 8, 128, (1000,) * 4 + (24,), 70, 1, 16),
+    ("float16", True, 2, 4, 4, 64, (130, 64), 5, 2, 100),   # more than there are
+    ("bfloat16", False, 1, 32, 1, 128, (500,), 3, 4, 3),     # 32 heads of one KV head
+    ("bfloat16", True, 1, 4, 2, 128, (1,), 1, 1, 1),
+    ("bfloat16", False, 1, 4, 2, 128, (64,) * 300, 1, 1, 37),
+]
+
+
+@pytest.mark.parametrize("dtype,packed,B,H,Hkv,D,lens,hot,Lq,top", SELECT)
+def test_selected_tiles_and_the_attention_over_them(dtype, packed, B, H, Hkv, D, lens, hot, Lq, top):
+    torch = _torch()
+    import archive_ref as ref
+
+    cache, k, v = make(dtype, B, H, Hkv, D, lens, hot, seed=top, tile_index=True,
+                       archive_dtype="float8_e4m3fn" if packed else None)
+    N = sum(lens)
+    n = N + hot
+    q = queries(B, H, Lq, D, seed=top)
+    kk, vv = held(cache, k, v, lens)
+    lo, hi, pos = ref.bounds(kk[:, :, :N], lens)
+    for q_pos in (n - Lq, N // 2):
+        want = ref.select(q, lo, hi, pos, q_pos, top)
+        got = cache.select_tiles(q, q_pos, top)
+        assert got.dtype == torch.int32 and torch.equal(got.cpu().long(), want)
+        tile_of = torch.cat([torch.full((c,), i) for i, (_, _, c) in enumerate(ref.tiles_of(lens))])
+        T = len(ref.tiles_of(lens))
+        chosen = torch.zeros(B, Hkv, Lq, T + 1, dtype=torch.bool).scatter(3, torch.where(want < 0, T, want), True)
+        seen = torch.cat([chosen[..., tile_of], torch.ones(B, Hkv, Lq, hot, dtype=torch.bool)], 3)
+        ref_out, ref_lse = ref.attention(q, kk, vv, torch.arange(n), q_pos, seen)
+        out, lse = cache.attend(q, q_pos, want_lse=True, top_tiles=top)
+        check_out(out, lse, ref_out, ref_lse, vv)
+
+
+def test_equal_scores_go_to_the_lowest_tiles_and_nan_comes_first():
+    torch = _torch()
+    lens = (64,) * 50
+    cache, k, v = make("bfloat16", 1, 4, 1, 64, lens, 1, archive_dtype=None, tile_index=True)
+    row = cache._attended_spans or cache.get_attention_segments().spans
+    cache._arena_k[:, 64:] = 1.0
+    cache._ops.tile_bounds(64, 50 * 64, cache.tile_bounds)
+    q = queries(1, 4, 1, 64)
+    assert cache.select_tiles(q, 5000, 7)[0, 0, 0].tolist() == list(range(7))
+    last = row[49][0]
+    cache._arena_k[0, last + 3, 9] = math.nan
+    cache._ops.tile_bounds(last, 64, cache.tile_bounds)
+    assert cache.select_tiles(q, 5000, 3)[0, 0, 0].tolist() == [0, 1, 49]
+    q[0, 2, 0, 3] = math.nan  # a NaN query: every score is NaN
+    assert cache.select_tiles(q, 5000, 3)[0, 0, 0].tolist() == [0, 1, 2]
+
+
+def test_selection_over_more_tiles_than_fit_shared_memory():
+    torch = _torch()
+    lens = (64 * 13000,)
+    cache, k, v = make("bfloat16", 1, 2, 1, 64, (), 0, hot_cap=8, archive_dtype=None, tile_index=True,
+                       pool_tokens=64 * 13000)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k = torch.randn(1, 1, lens[0], 64, generator=g, device="cuda").to(torch.bfloat16)
+    cache.import_block(k, k, 0)
+    q = queries(1, 2, 1, 64)
+    t = k[0, 0].double().reshape(13000, 64, 64)
+    x = q[0, :, 0].double()
+    score = torch.maximum(x[:, None] * t.amin(1), x[:, None] * t.amax(1)).sum(-1).amax(0).float()
+    want = torch.sort(torch.topk(score, 100).indices).values
+    assert torch.equal(cache.select_tiles(q, lens[0], 100)[0, 0, 0].long(), want)
+
+
+# ------------------------------------------------------------------ in the cache
+@pytest.mark.parametrize("host_tier", [False, True])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_blocks_that_went_cold_come_back_with_the_same_values(dtype, host_tier):
+    torch = _torch()
+    lens = (100, 64, 30)
+    cache, k, v = make(dtype, 1, 8, 2, 128, lens, 20, tile_index=True, host_tier=host_tier)
+    q = queries(1, 8, 1, 128)
+    want = cache.attend(q, 213).clone()
+    tiles = cache.select_tiles(q, 213, 2).clone()
+    for m in list(cache.block_manager.iter_blocks(layer_id=0)):
+        cache.demote_manifest_to_cold(m)
+    cache._flush_deferred_free()
+    cache.archive.clear()
+    cache.tile_bounds.zero_()
+    # the blocks return to other rows, in the same order
+    assert torch.equal(cache.attend(q, 213), want)
+    assert torch.equal(cache.select_tiles(q, 213, 2), tiles)
+
+
+def test_the_archive_grows_and_keeps_its_blocks():
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (100, 64, 30, 500, 70)
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, lens, 20, tile_index=True, pool_tokens=128)
+    assert cache.archive.rows > 128
+    q = queries(1, 8, 1, 128)
+    kk, vv = held(cache, k, v, lens)
+    want, lse = ref.attention(q, kk, vv, torch.arange(784), 783)
+    check_out(cache.attend(q, 783), None, want, lse, vv)
+    lo, hi, pos = ref.bounds(kk[:, :, :764], lens)
+    assert torch.equal(cache.select_tiles(q, 783, 4).cpu().long(), ref.select(q, lo, hi, pos, 783, 4))
+
+
+def test_a_tile_outside_the_archive_is_reported_and_skipped():
+    torch = _torch()
+    from rfsn_b200 import _native as native
+
+    cache, k, v = make("bfloat16", 1, 4, 2, 128, (64, 64, 64), 20, tile_index=True)
+    q = queries(1, 4, 1, 128)
+    segs = cache.get_attention_segments()
+    for bad in (-64, 1 << 20, 7):
+        saved = cache._tiles_dev.clone()
+        cache._tiles_dev[1, 0] = bad
+        ws = native.Workspace(cache.device)
+        from rfsn_b200.cache import paged_attention
+
+        out = paged_attention(cache, q, 211, segs, workspace=ws)
+        with pytest.raises(RuntimeError):
+            ws.check()
+        assert bool(torch.isfinite(out).all())
+        paged_attention(cache, q, 211, segs, workspace=ws, top_tiles=2)
+        with pytest.raises(RuntimeError):
+            ws.check()
+        cache._tiles_dev.copy_(saved)
+        paged_attention(cache, q, 211, segs, workspace=ws)
+        ws.check()
+
+
+def test_calls_on_another_stream_and_back():
+    torch = _torch()
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (300,), 20, tile_index=True)
+    q = queries(1, 8, 1, 128)
+    want = cache.attend(q, 319).clone()
+    from rfsn_b200 import _native as native
+    from rfsn_b200.cache import paged_attention
+
+    s = torch.cuda.Stream()
+    ws = native.Workspace(cache.device)
+    segs = cache.get_attention_segments()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a = paged_attention(cache, q, 319, segs, workspace=ws)
+        b = paged_attention(cache, q, 319, segs, workspace=ws, top_tiles=3)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(a, want) and torch.equal(b, cache.attend(q, 319, top_tiles=3))
+
+
+@pytest.mark.parametrize("top_tiles", [0, 3])
+@pytest.mark.parametrize("packed", [True, False])
+def test_graphed_decode_step_equals_the_op_by_op_step(packed, top_tiles):
+    """Tokens through the seal rule, captured steps against attention_step on a second cache."""
+    torch = _torch()
+    if not packed and not top_tiles:
+        pytest.skip("the exact dense path has its own tests")
+    from rfsn_b200.layer import GraphedDecodeStep, attention_step
+
+    caches = [make("bfloat16", 1, 8, 2, 128, (), 0, hot_cap=96, wrap=0, top_tiles=top_tiles,
+                   archive_dtype="float8_e4m3fn" if packed else None, pool_tokens=2048)[0] for _ in range(2)]
+    step = GraphedDecodeStep(caches[0], 8)
+    g = torch.Generator().manual_seed(11)
+    for pos in range(330):
+        q, k, v = (torch.randn(1, h, 1, 128, generator=g).to(torch.bfloat16) for h in (8, 2, 2))
+        step.q_host.copy_(q)
+        step.k_host.copy_(k)
+        step.v_host.copy_(v)
+        got = step.step(pos).clone()
+        want = attention_step(q.cuda(), k.cuda(), v.cuda(), caches[1], pos)
+        # the split plans differ (a graph plans for a full ring): the same softmax, rounded in another order
+        assert float((got - want.cpu()).abs().max()) <= REL * 5.0, pos
+    # blocks beyond the warm capacity of 96 tokens go cold: the steps that reload them run op by op
+    assert step.replays > 100 and step.captures >= 2 and step.fallbacks > 0
+
+
+@pytest.mark.parametrize("kw", [dict(archive_dtype="float8_e4m3fn"), dict(top_tiles=2),
+                                dict(archive_dtype="float8_e4m3fn", top_tiles=2)])
+def test_model_generates_through_a_packed_and_a_sparse_cache(kw):
+    """The whole path: chunked prefill, seals, graphed and op-by-op decode give the same tokens and nearly the same
+    logits."""
+    torch = _torch()
+    from rfsn_b200 import RFSNCache, RFSNConfig, RFSNModel
+
+    cfg = RFSNConfig(hidden_dim=512, num_heads=4, num_kv_heads=2, head_dim=128, num_layers=2, vocab_size=300,
+                     hot_capacity=64, warm_capacity=1024, cold_capacity=1024, block_size_seq=32, ffn_dim=256,
+                     model_dtype="bfloat16", disk_cache_dir=tempfile.mkdtemp(prefix="rfsn_archive_"))
+    model = RFSNModel(cfg, seed=3)
+    prompt = torch.randint(0, 300, (1, 200), generator=torch.Generator().manual_seed(0))
+    logits = []
+    for graphs in (True, False):
+        model.use_graphs, model._graph = graphs, None
+        cache = RFSNCache(cfg, 1, **kw)
+        out = [model.prefill(prompt, cache)[:, -1]]
+        for i in range(60):
+            tok = torch.tensor([(17 * i) % 300], dtype=torch.int32)
+            out.append(model.decode_step(tok, cache, 200 + i))
+        logits.append(torch.stack(out).float())
+        assert cache.layer(0)._n_tiles >= 3
+    assert torch.isfinite(logits[0]).all()
+    # bf16 activations: the two runs differ by roundings of one bf16 step here and there
+    scale = float(logits[0].abs().max())
+    assert float((logits[0] - logits[1]).abs().max()) <= 16 * 2.0 ** -8 * scale
