@@ -543,9 +543,29 @@ RFSN_API rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, con
  * NaN bounds. bounds: device [batch_kv_heads][rows / 64][2][head_dim]. */
 RFSN_API rfsn_status rfsn_tile_bounds(const rfsn_arena* arena, int row0, int count, void* bounds, void* stream);
 
+/* A prepared call for a context that several queries attend to: what stays the
+ * same from query to query. With top_tiles > 0 every (batch, kv head, query
+ * row) attends to the top_tiles best of `tiles` only: rfsn_select_tiles with
+ * `bounds` (of the packed archive's codes when packed is given, else of the
+ * arena's type) followed by rfsn_archive_attention on the lists, which stay in
+ * the workspace. */
+typedef struct rfsn_archive_call {
+    const rfsn_arena* arena;
+    const rfsn_packed_archive* packed; /* may be NULL */
+    const void* bounds;                /* device; NULL when top_tiles is 0 */
+    rfsn_tile_list tiles;              /* per_query 0 */
+    rfsn_hot_window hot;
+    int32_t batch, q_heads, kv_heads, q_len;
+    int32_t top_tiles;
+    int32_t max_splits;
+} rfsn_archive_call;
+
+RFSN_API rfsn_status rfsn_archive_attend(const rfsn_archive_call* call, const float* q, int q_pos0, float* out,
+                                         float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Workspace bytes of rfsn_archive_attention (n_select = 0: shared lists;
- * > 0: lists per query) and rfsn_select_tiles (n_select > 0) over up to n_tiles
- * tiles. Conventions as for rfsn_attention_workspace_size; one workspace
+ * > 0: lists per query), rfsn_select_tiles (n_select > 0) and
+ * rfsn_archive_attend (n_select = top_tiles) over up to n_tiles tiles. Conventions as for rfsn_attention_workspace_size; one workspace
  * serves all attention calls ordered on one stream. */
 RFSN_API rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim,
                                                  int n_tiles, int n_select, size_t* bytes);

@@ -23,8 +23,6 @@ struct rfsn_packed_archive {
 namespace rfsn {
 namespace archive {
 
-constexpr int kNCW = 4;                         // consumer warps, one 16-key strip of a tile each
-constexpr int kThreads = (kNCW + 1) * 32;       // + one producer warp
 constexpr int kStageBytes = 16384;              // one item: 64 packed keys, or 32 (head_dim 64: 64) 16-bit keys
 constexpr int kMaxSplits128 = 240, kMaxSplits64 = 120;  // bounded by the merge weights kept in shared memory
 
@@ -75,7 +73,8 @@ void preload_pack_kernels();
 void preload_select_kernels();
 rfsn_status select_tiles_launch(int bounds_dtype, int head_dim, const archive::SelectParams& p, int lists, int chunks,
                                 cudaStream_t stream);
-// archive_attn.cu
+// archive_attn.cu: nb = column blocks of 4 query slots per CTA (1, 2 or 4); CTAs per SM of that variant
+int archive_attn_ctas(int nb);
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int nb, int zblocks, cudaStream_t stream);
 

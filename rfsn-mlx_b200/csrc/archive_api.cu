@@ -27,20 +27,20 @@ struct SlotPlan {
     int lists, slots, nb, zblocks;
 };
 
-SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, bool per_query) {
+SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, int head_dim, bool per_query) {
     SlotPlan s;
     const int G = q_heads / kv_heads;
     s.lists = batch * kv_heads * (per_query ? q_len : 1);
     s.slots = per_query ? G : G * q_len;
-    s.nb = s.slots <= 4 ? 1 : 2;
+    s.nb = s.slots <= 4 ? 1 : s.slots <= 8 || head_dim == 128 ? 2 : 4;
     s.zblocks = (s.slots + 4 * s.nb - 1) / (4 * s.nb);
     return s;
 }
 
-// Splits of a list's items: two CTAs per SM over all lists.
+// Splits of a list's items: the CTAs that are resident at once, over all lists.
 int split_limit(const SlotPlan& sp, int head_dim, int max_splits) {
     const int sms = std::max(device_sms(), 1);
-    int s = std::max(1, 2 * sms / std::max(1, sp.lists * sp.zblocks));
+    int s = std::max(1, archive_attn_ctas(sp.nb) * sms / std::max(1, sp.lists * sp.zblocks));
     s = std::min(s, head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64);
     if (max_splits > 0) s = std::min(s, max_splits);
     return s;
@@ -48,6 +48,24 @@ int split_limit(const SlotPlan& sp, int head_dim, int max_splits) {
 
 WsLayout attention_ws(const SlotPlan& sp, int splits, int head_dim) {
     return ws_layout(splits > 1 ? sp.lists * sp.zblocks : 0, 1, splits, 4 * sp.nb, head_dim);
+}
+
+// Largest attention workspace of a shape: every split count it may choose (at
+// least 148 SMs are assumed, so a size computed without a device serves a B200).
+size_t attention_ws_limit(const SlotPlan& sp, int head_dim) {
+    const int units = std::max(1, sp.lists * sp.zblocks);
+    const int limit = std::max(split_limit(sp, head_dim, 0),
+                               std::min(head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64,
+                                        std::max(1, archive_attn_ctas(sp.nb) * 148 / units)));
+    return attention_ws(sp, limit, head_dim).total;
+}
+
+size_t select_scores_offset();
+
+// Selected lists of rfsn_archive_attend: behind everything its two kernels write.
+size_t lists_offset(const SlotPlan& sp, int head_dim, int n_tiles) {
+    return align_up(std::max(attention_ws_limit(sp, head_dim),
+                             select_scores_offset() + sizeof(float) * (size_t)sp.lists * n_tiles), 256);
 }
 
 size_t select_scores_offset() { return align_up(256 + sizeof(int) * (size_t)kMaxCounters, 256); }
@@ -69,6 +87,89 @@ rfsn_status check_tiles(const rfsn_tile_list* t, const char* what) {
                        aligned16(t->tiles) && (t->per_query == 0 || t->per_query == 1),
                    "%s: bad tile list", what);
     return RFSN_OK;
+}
+
+// check_only: every argument check of the call, without a launch
+rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed, const float* q, int batch, int q_heads,
+                      int kv_heads, int q_len, int q_pos0, const rfsn_tile_list* tiles, const rfsn_hot_window* hot,
+                      float* out, float* lse, void* workspace, size_t workspace_bytes, int max_splits, void* stream,
+                      bool check_only) {
+    const char* what = "rfsn_archive_attention";
+    RFSN_CHECK_ARG(arena != nullptr && hot != nullptr, "%s: NULL arena or hot window", what);
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, arena->head_dim, what);
+    if (st == RFSN_OK) st = check_tiles(tiles, what);
+    if (st != RFSN_OK) return st;
+    if (!arena->has_items) {
+        set_error("%s: needs a bf16/f16 arena with head_dim 64 or 128", what);
+        return RFSN_ERR_UNSUPPORTED;
+    }
+    const int groups = batch * kv_heads;
+    RFSN_CHECK_ARG(groups == arena->groups, "%s: batch*kv_heads %d != arena groups %d", what, groups, arena->groups);
+    RFSN_CHECK_ARG(packed == nullptr || (packed->groups == groups && packed->head_dim == arena->head_dim &&
+                                         packed->device == arena->device),
+                   "%s: the packed archive's heads, head_dim or device differ from the arena's", what);
+    RFSN_CHECK_ARG(q != nullptr && aligned16(q) && out != nullptr && aligned16(out) && workspace != nullptr &&
+                       aligned16(workspace), "%s: NULL or misaligned pointer (q, out and workspace: 16 bytes)", what);
+    RFSN_CHECK_ARG(hot->length >= 0 && hot->length <= hot->capacity && hot->head_index >= 0 &&
+                       hot->head_index < (hot->capacity > 0 ? hot->capacity : 1) && hot->ring_row0 >= 0 &&
+                       hot->ring_row0 + hot->capacity <= arena->rows,
+                   "%s: bad hot window", what);
+    const bool stepped = hot->step_state != nullptr;
+    if (tiles->n == 0 && hot->length == 0 && !stepped) {
+        set_error("run_segmented_attention requires at least one KV segment");
+        return RFSN_ERR_INVALID_ARG;
+    }
+    st = check_device(arena->device, what);
+    if (st != RFSN_OK) return st;
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, arena->head_dim, tiles->per_query != 0);
+    RFSN_CHECK_ARG(sp.zblocks <= kMaxLists, "%s: too many query rows", what);
+    const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
+    const int per_tile = packed != nullptr ? 1 : kTile / hk;
+    RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
+    const int first = std::min(hot->length, hot->capacity - hot->head_index);
+    // with a device step state the window is only known when the kernel runs: planned for the largest
+    const int hot_items = stepped ? (hot->capacity + hk - 1) / hk + 1
+                                  : (first + hk - 1) / hk + (hot->length - first + hk - 1) / hk;
+    const int total = std::max(1, tiles->n * per_tile + hot_items);
+    int splits = std::min(split_limit(sp, arena->head_dim, max_splits), total);
+    const int per = (total + splits - 1) / splits;
+    splits = (total + per - 1) / per;
+    // more than one split only where all lists leave SMs idle: far fewer lists than arrival counters
+    RFSN_CHECK_ARG(splits == 1 || (long long)sp.lists * sp.zblocks <= kMaxCounters, "%s: too many lists", what);
+    const WsLayout w = attention_ws(sp, splits, arena->head_dim);
+    if (w.total > workspace_bytes) {
+        set_error("%s: workspace too small: need %zu bytes, have %zu", what, w.total, workspace_bytes);
+        return RFSN_ERR_OVERFLOW;
+    }
+    if (check_only) return RFSN_OK;
+    archive::Params p;
+    memset(&p, 0, sizeof(p));
+    p.q = q;
+    p.out = out;
+    p.lse = lse;
+    p.tiles = reinterpret_cast<const int4*>(tiles->tiles);
+    p.n_tiles = tiles->n;
+    p.per_query = tiles->per_query;
+    p.ring_row0 = hot->ring_row0;
+    p.capacity = hot->capacity;
+    p.head = hot->head_index;
+    p.hlen = hot->length;
+    p.hstart = hot->start_pos;
+    p.rows = arena->rows;
+    p.packed_rows = packed != nullptr ? packed->rows : 0;
+    p.scales = packed != nullptr ? packed->scales : nullptr;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.q_len = q_len;
+    p.q_pos0 = q_pos0;
+    p.G = q_heads / kv_heads;
+    p.slots = sp.slots;
+    p.items_per_split = per;
+    p.splits = splits;
+    p.qscale = (float)(1.0 / std::sqrt((double)arena->head_dim)) * 1.4426950408889634f;
+    p.ws = ws_view(workspace, w);
+    p.dyn = hot->step_state;
+    return archive_attn_launch(arena, packed, p, sp.lists, sp.nb, sp.zblocks, static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace
@@ -183,14 +284,9 @@ rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, in
     rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, "rfsn_archive_workspace_size");
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0, "rfsn_archive_workspace_size: negative tile count");
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, n_select > 0);
-    // at least 148 SMs are assumed, so a size computed without a device serves a B200
-    const int units = std::max(1, sp.lists * sp.zblocks);
-    const int limit = std::max(split_limit(sp, head_dim, 0),
-                               std::min(head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64,
-                                        std::max(1, 2 * 148 / units)));
-    size_t need = attention_ws(sp, limit, head_dim).total;
-    if (n_select > 0) need = std::max(need, select_scores_offset() + sizeof(float) * (size_t)sp.lists * n_tiles);
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, n_select > 0);
+    size_t need = attention_ws_limit(sp, head_dim);
+    if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
     *bytes = need;
     return RFSN_OK;
 }
@@ -204,8 +300,8 @@ rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float*
     if (st == RFSN_OK) st = check_tiles(tiles, what);
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(tiles->per_query == 0, "%s: selects from one list for all heads and queries", what);
-    RFSN_CHECK_ARG(q != nullptr && out != nullptr && aligned16(out) && workspace != nullptr && aligned16(workspace),
-                   "%s: NULL or misaligned pointer", what);
+    RFSN_CHECK_ARG(q != nullptr && aligned16(q) && out != nullptr && aligned16(out) && workspace != nullptr &&
+                       aligned16(workspace), "%s: NULL or misaligned pointer (q, out and workspace: 16 bytes)", what);
     RFSN_CHECK_ARG(bounds_dtype == RFSN_F16 || bounds_dtype == RFSN_BF16 || bounds_dtype == RFSN_E4M3,
                    "%s: bounds must be f16, bf16 or e4m3", what);
     RFSN_CHECK_ARG(tiles->n == 0 || (bounds != nullptr && aligned16(bounds)), "%s: NULL or misaligned bounds", what);
@@ -240,9 +336,9 @@ rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float*
     p.counters = reinterpret_cast<int*>(ws + 256);
     p.error = reinterpret_cast<int*>(ws);
     p.dyn = step_state;
-    // two CTAs per SM over all lists, at least the 32 tiles that the CTA's warps score at once
-    const int want = std::max(1, 2 * device_sms() / lists);
-    p.tiles_per_cta = std::max(32, (tiles->n + want - 1) / want);
+    // four CTAs per SM over all lists, in steps of the 32 tiles that a CTA scores at once
+    const int want = std::max(1, 4 * device_sms() / lists);
+    p.tiles_per_cta = std::max(32, ((tiles->n + want - 1) / want + 31) / 32 * 32);
     const int chunks = std::max(1, (tiles->n + p.tiles_per_cta - 1) / p.tiles_per_cta);
     return select_tiles_launch(bounds_dtype, head_dim, p, lists, chunks, static_cast<cudaStream_t>(stream));
 }
@@ -251,81 +347,46 @@ rfsn_status rfsn_archive_attention(const rfsn_arena* arena, const rfsn_packed_ar
                                    int batch, int q_heads, int kv_heads, int q_len, int q_pos0,
                                    const rfsn_tile_list* tiles, const rfsn_hot_window* hot, float* out, float* lse,
                                    void* workspace, size_t workspace_bytes, int max_splits, void* stream) {
-    const char* what = "rfsn_archive_attention";
-    RFSN_CHECK_ARG(arena != nullptr && hot != nullptr, "%s: NULL arena or hot window", what);
-    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, arena->head_dim, what);
-    if (st == RFSN_OK) st = check_tiles(tiles, what);
+    return attention(arena, packed, q, batch, q_heads, kv_heads, q_len, q_pos0, tiles, hot, out, lse, workspace,
+                     workspace_bytes, max_splits, stream, false);
+}
+
+rfsn_status rfsn_archive_attend(const rfsn_archive_call* c, const float* q, int q_pos0, float* out, float* lse,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "rfsn_archive_attend";
+    RFSN_CHECK_ARG(c != nullptr && c->arena != nullptr && c->top_tiles >= 0, "%s: NULL call or negative top_tiles", what);
+    if (c->top_tiles == 0 || c->tiles.n == 0)
+        return rfsn_archive_attention(c->arena, c->packed, q, c->batch, c->q_heads, c->kv_heads, c->q_len, q_pos0,
+                                      &c->tiles, &c->hot, out, lse, workspace, workspace_bytes, c->max_splits, stream);
+    const int head_dim = c->arena->head_dim;
+    rfsn_status st = check_shape(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, what);
     if (st != RFSN_OK) return st;
-    if (!arena->has_items) {
-        set_error("%s: needs a bf16/f16 arena with head_dim 64 or 128", what);
-        return RFSN_ERR_UNSUPPORTED;
-    }
-    const int groups = batch * kv_heads;
-    RFSN_CHECK_ARG(groups == arena->groups, "%s: batch*kv_heads %d != arena groups %d", what, groups, arena->groups);
-    RFSN_CHECK_ARG(packed == nullptr || (packed->groups == groups && packed->head_dim == arena->head_dim &&
-                                         packed->device == arena->device),
-                   "%s: the packed archive's heads, head_dim or device differ from the arena's", what);
-    RFSN_CHECK_ARG(q != nullptr && out != nullptr && aligned16(out) && workspace != nullptr && aligned16(workspace),
-                   "%s: NULL or misaligned pointer", what);
-    RFSN_CHECK_ARG(hot->length >= 0 && hot->length <= hot->capacity && hot->head_index >= 0 &&
-                       hot->head_index < (hot->capacity > 0 ? hot->capacity : 1) && hot->ring_row0 >= 0 &&
-                       hot->ring_row0 + hot->capacity <= arena->rows,
-                   "%s: bad hot window", what);
-    const bool stepped = hot->step_state != nullptr;
-    if (tiles->n == 0 && hot->length == 0 && !stepped) {
-        set_error("run_segmented_attention requires at least one KV segment");
-        return RFSN_ERR_INVALID_ARG;
-    }
-    st = check_device(arena->device, what);
-    if (st != RFSN_OK) return st;
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, tiles->per_query != 0);
-    RFSN_CHECK_ARG(sp.zblocks <= kMaxLists, "%s: too many query rows", what);
-    const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
-    const int per_tile = packed != nullptr ? 1 : kTile / hk;
-    RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
-    const int first = std::min(hot->length, hot->capacity - hot->head_index);
-    // with a device step state the window is only known when the kernel runs: planned for the largest
-    const int hot_items = stepped ? (hot->capacity + hk - 1) / hk + 1
-                                  : (first + hk - 1) / hk + (hot->length - first + hk - 1) / hk;
-    const int total = std::max(1, tiles->n * per_tile + hot_items);
-    int splits = std::min(split_limit(sp, arena->head_dim, max_splits), total);
-    const int per = (total + splits - 1) / splits;
-    splits = (total + per - 1) / per;
-    // more than one split only where all lists leave SMs idle: far fewer lists than arrival counters
-    RFSN_CHECK_ARG(splits == 1 || (long long)sp.lists * sp.zblocks <= kMaxCounters, "%s: too many lists", what);
-    const WsLayout w = attention_ws(sp, splits, arena->head_dim);
-    if (w.total > workspace_bytes) {
-        set_error("%s: workspace too small: need %zu bytes, have %zu", what, w.total, workspace_bytes);
+    RFSN_CHECK_ARG(c->tiles.n > 0 && c->tiles.per_query == 0 && c->top_tiles <= (1 << 20), "%s: bad tile list", what);
+    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, true);
+    const size_t off = lists_offset(sp, head_dim, c->tiles.n);
+    const size_t need = off + sizeof(int4) * (size_t)sp.lists * c->top_tiles;
+    if (workspace == nullptr || workspace_bytes < need) {
+        set_error("%s: workspace too small: need %zu bytes, have %zu", what, need,
+                  workspace == nullptr ? (size_t)0 : workspace_bytes);
         return RFSN_ERR_OVERFLOW;
     }
-    archive::Params p;
-    memset(&p, 0, sizeof(p));
-    p.q = q;
-    p.out = out;
-    p.lse = lse;
-    p.tiles = reinterpret_cast<const int4*>(tiles->tiles);
-    p.n_tiles = tiles->n;
-    p.per_query = tiles->per_query;
-    p.ring_row0 = hot->ring_row0;
-    p.capacity = hot->capacity;
-    p.head = hot->head_index;
-    p.hlen = hot->length;
-    p.hstart = hot->start_pos;
-    p.rows = arena->rows;
-    p.packed_rows = packed != nullptr ? packed->rows : 0;
-    p.scales = packed != nullptr ? packed->scales : nullptr;
-    p.q_heads = q_heads;
-    p.kv_heads = kv_heads;
-    p.q_len = q_len;
-    p.q_pos0 = q_pos0;
-    p.G = q_heads / kv_heads;
-    p.slots = sp.slots;
-    p.items_per_split = per;
-    p.splits = splits;
-    p.qscale = (float)(1.0 / std::sqrt((double)arena->head_dim)) * 1.4426950408889634f;
-    p.ws = ws_view(workspace, w);
-    p.dyn = hot->step_state;
-    return archive_attn_launch(arena, packed, p, sp.lists, sp.nb, sp.zblocks, static_cast<cudaStream_t>(stream));
+    rfsn_tile_list chosen;
+    chosen.tiles = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + off);
+    chosen.n = c->top_tiles;
+    chosen.per_query = 1;
+    // Everything the attention would refuse is refused before the selection is launched.
+    st = attention(c->arena, c->packed, q, c->batch, c->q_heads, c->kv_heads, c->q_len, q_pos0, &chosen, &c->hot, out,
+                   lse, workspace, off, c->max_splits, stream, true);
+    if (st != RFSN_OK) return st;
+    const rfsn_packed_archive* pk = c->packed;
+    st = rfsn_select_tiles(c->bounds, pk != nullptr ? RFSN_E4M3 : c->arena->dtype,
+                           pk != nullptr ? reinterpret_cast<const float*>(pk->scales) : nullptr,
+                           pk != nullptr ? pk->rows : c->arena->rows, q, c->batch, c->q_heads, c->kv_heads, c->q_len,
+                           head_dim, q_pos0, &c->tiles, c->top_tiles, const_cast<int32_t*>(chosen.tiles),
+                           c->hot.step_state, workspace, off, stream);
+    if (st != RFSN_OK) return st;
+    return attention(c->arena, c->packed, q, c->batch, c->q_heads, c->kv_heads, c->q_len, q_pos0, &chosen, &c->hot, out,
+                     lse, workspace, off, c->max_splits, stream, false);
 }
 
 }  // extern "C"

@@ -7,8 +7,8 @@
 // {row, pos, len}: the archived blocks of the page table (one list for all
 // heads and queries), or the tiles selected for each query and KV head. A
 // producer warp streams them (and then the hot window) with TMA as 16 KB
-// items: 64 packed keys, or 32 16-bit keys (64 with head_dim 64). Four
-// consumer warps each own a 16-key strip:
+// items: 64 packed keys, or 32 16-bit keys (64 with head_dim 64). Consumer
+// warps in groups of four take items in turn, a 16-key strip each:
 //   S^T[16 keys x 8] = K[16 x D] . Q^T[D x 8]       (mma.sync m16n8k16)
 //   O^T[D x 8]      += V^T[D x 16] . P^T[16 x 8]
 // A column pair (2s, 2s + 1) is query slot s twice: the 16-bit head and the
@@ -33,6 +33,8 @@
 // The softmax keeps a reference maximum per query slot that moves only when a
 // logit exceeds it by more than 2^8 (in powers of two), so most strips need
 // one vote instead of a reduction over the lanes and a rescale.
+#include <atomic>
+
 #include <math_constants.h>
 
 #include "archive.cuh"
@@ -51,18 +53,21 @@ template <int D> struct Geometry {
     static constexpr int kVPacked = kTile * D;            // V offset inside a packed item
 };
 
-template <int D, int NB, int STAGES, bool PACKED, bool BF16>
+template <int D, int NB, int GROUPS, int STAGES, bool PACKED, bool BF16>
 struct Smem {
     static constexpr int SL = 4 * NB;
-    // 16-bit tiles: head|remainder fragments, and for bfloat16 the third terms; packed tiles: float16 head|remainder
-    static constexpr int kSets = (BF16 ? 2 : 1) + (PACKED ? 1 : 0);
+    static constexpr int kNCW = 4 * GROUPS;
+    static constexpr int kRow = D + 8;  // row stride of red_o: the slots' rows start in different banks
     uint8_t stage[STAGES][kStageBytes];
     alignas(16) float4 meta[STAGES];  // scales of a packed tile, by bulk copy with the tile
     int4 info[STAGES];                // {packed, position of the first key, valid keys, 0}
-    uint4 qf[kSets][NB][D / 32][32];  // Q^T operand fragments of two k-steps per entry
-    alignas(16) float red_o[kNCW][SL][D];
+    alignas(16) float red_o[kNCW][SL][kRow];
     float red_m[kNCW][SL], red_l[kNCW][SL], red_u[kNCW];
-    float qmul[SL];
+    int red_packed[kNCW];             // order of red_o's channels (packed_pos)
+    // With several column blocks the Q^T fragments of all warps live here (16-bit tiles: head and remainder, third
+    // terms of bfloat16; packed tiles), with one in each warp's registers.
+    static constexpr int kSets = (BF16 ? 2 : 1) + (PACKED ? 1 : 0);
+    uint2 qf[NB > 1 ? kSets : 1][NB > 1 ? NB : 1][D / 16][32];
     uint64_t full[STAGES], empty[STAGES];
     int flag, abort;
 };
@@ -93,6 +98,84 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
         "l"(src), "r"(bytes), "r"(smem_u32(bar))
         : "memory");
+}
+
+// Channel group (D / 8 consecutive channels, 16-byte chunk or half of one) that
+// lane group g takes of a packed V row, and, for head_dim 128, the key of a
+// strip's row g: a permutation that spreads a shared-memory phase over all banks.
+template <int D> __device__ __forceinline__ int spread(int g) { return D == 128 ? ((g & 1) << 2 | g >> 1) : g; }
+template <int D> __device__ __forceinline__ int unspread(int c) { return D == 128 ? ((c & 3) << 1 | c >> 2) : c; }
+
+// Place of channels c, c + 1 (c even) in a row of red_o written in the order of
+// packed tiles' accumulators: lane group major, so that a warp's stores meet all banks.
+template <int D> __device__ __forceinline__ int packed_pos(int c) {
+    return (((c & (D / 8 - 1)) >> 1) * 8 + unspread<D>(c / (D / 8))) * 2;
+}
+
+// A warp's Q^T operand fragments: column n = lane / 4 is query slot
+// 4 nb + n / 2, the head (n even) or the remainder (n odd) of q times a power
+// of two that puts the row's largest magnitude into [2^4, 2^5). a: k-steps of
+// head and remainder, c: third terms (bfloat16). mul[nb]: for the lane's own
+// softmax slot 4 nb + lane % 4, what turns products into log2 units.
+template <int D, int NB>
+struct QFrag {
+    uint32_t a[NB][D / 16][2], c[NB][D / 16][2];
+    float mul[NB];
+};
+
+// Fragments of one set (a or c) of all column blocks -> shared memory.
+template <int D, int NB>
+__device__ __forceinline__ void store_q(uint2 (*dst)[D / 16][32], const uint32_t (&f)[NB][D / 16][2]) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) dst[nb][kk][threadIdx.x & 31] = make_uint2(f[nb][kk][0], f[nb][kk][1]);
+}
+
+// Channels of k-step kk, register h, of lane t: packed tiles 64 (kk / 4) + 16 t + 4 (kk % 4) + 2 h (the lane's 16
+// consecutive codes), 16-bit tiles 16 kk + 2 t + 8 h (ldmatrix).
+template <typename T, int D, int NB, bool PACKED_TILE, bool THIRD>
+__device__ __forceinline__ void load_q(QFrag<D, NB>& q, const float* __restrict__ base, const OutMap& om, int bh,
+                                       int slot0, int nslots, float qscale) {
+    const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int sl = 4 * nb + (n >> 1);
+        const bool live = sl < nslots;
+        const float* row = base + om.row(bh, live ? slot0 + sl : slot0) * D;
+        float x[D / 16][4];
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            const int d0 = PACKED_TILE ? 64 * (kk >> 2) + 16 * t + 4 * (kk & 3) : 16 * kk + 2 * t;
+            const int d1 = PACKED_TILE ? d0 + 2 : d0 + 8;
+            const float2 u = *reinterpret_cast<const float2*>(row + d0), v = *reinterpret_cast<const float2*>(row + d1);
+            x[kk][0] = live ? u.x : 0.f;
+            x[kk][1] = live ? u.y : 0.f;
+            x[kk][2] = live ? v.x : 0.f;
+            x[kk][3] = live ? v.y : 0.f;
+        }
+        float a = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a = fmaxf(a, fabsf(x[kk][j]));
+        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+        int e = a > 0.f ? 4 + 127 - (int)(__float_as_uint(a) >> 23) : 0;  // a infinite: 2^-124, q stays infinite
+        e = max(-126, min(126, e));
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+        q.mul[nb] = __shfl_sync(0xffffffffu, qscale * __uint_as_float((uint32_t)(127 - e) << 23), 8 * t);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float x0 = x[kk][2 * h] * up, x1 = x[kk][2 * h + 1] * up;
+                const float h0 = round16<T>(x0), h1 = round16<T>(x1);
+                const float r0 = x0 - h0, r1 = x1 - h1;
+                q.a[nb][kk][h] = (n & 1) ? pack2<T>(r0, r1) : pack2<T>(h0, h1);
+                if (THIRD) q.c[nb][kk][h] = (n & 1) ? 0u : pack2<T>(r0 - round16<T>(r0), r1 - round16<T>(r1));
+            }
+    }
 }
 
 // Online-softmax state of a warp, one value per lane and column block: lane
@@ -158,14 +241,18 @@ __device__ __forceinline__ void softmax_strip(State<D, NB>& st, const float (&s0
     }
 }
 
-template <typename T, int D, int NB, int STAGES, bool PACKED>
-__global__ void __launch_bounds__(kThreads, 2)
+// Consumer warps come in GROUPS of four; item i of a split belongs to group
+// i % GROUPS (a divisor of STAGES, so each stage has one group of its own).
+template <typename T, int D, int NB, int GROUPS, int STAGES, int CTAS, bool PACKED>
+__global__ void __launch_bounds__((4 * GROUPS + 1) * 32, CTAS)
 archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_constant__ CUtensorMap mapV16,
                     const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ CUtensorMap mapV8,
                     const Params p) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using Geo = Geometry<D>;
-    using Sm = Smem<D, NB, STAGES, PACKED, BF16>;
+    using Sm = Smem<D, NB, GROUPS, STAGES, PACKED, BF16>;
+    static_assert(STAGES % GROUPS == 0, "a stage belongs to one group");
+    constexpr int kNCW = Sm::kNCW;
     constexpr int SL = Sm::SL;
     constexpr int HK = Geo::kHotKeys;
     extern __shared__ uint8_t smem_raw[];
@@ -205,7 +292,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&sm.full[s], 1);
-            mbar_init(&sm.empty[s], kNCW);
+            mbar_init(&sm.empty[s], 4);
         }
         sm.abort = 0;
         fence_mbar_init();
@@ -314,66 +401,36 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     if (p.dyn != nullptr) read_state(threadIdx.x == 0 && split == 0 && list == 0 && zb == 0);
     const int nitems = min(p.items_per_split, total - item0);
 
-    // Q: each slot's row scaled by the power of two that puts its largest
-    // magnitude into [2^4, 2^5), then split into fragments.
-    float* qn = &sm.red_o[0][0][0];  // [SL][D]
-    for (int sl = warp; sl < SL; sl += kNCW) {
-        const bool live = sl < nslots;
-        const float* qrow = p.q + om.row(bh, live ? slot0 + sl : slot0) * D;
-        float x[D / 32];
-        float a = 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            x[j] = live ? qrow[lane + 32 * j] : 0.f;
-            a = fmaxf(a, fabsf(x[j]));
+    QFrag<D, NB> q;
+    bool packed_order = PACKED && nitems > 0 && item0 < arch_items;
+    constexpr bool QS = NB > 1;
+    constexpr int kPackedSet = Sm::kSets - 1;
+    if constexpr (QS) {
+        if (!PACKED || warp != 1) load_q<T, D, NB, false, BF16>(q, p.q, om, bh, slot0, nslots, p.qscale);
+        if (warp == 0) {
+            store_q<D, NB>(sm.qf[0], q.a);
+            if constexpr (BF16) store_q<D, NB>(sm.qf[1], q.c);
         }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
-        int e = a > 0.f ? 4 + 127 - (int)(__float_as_uint(a) >> 23) : 0;  // a infinite: 2^-124, q stays infinite
-        e = max(-126, min(126, e));
-        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) qn[sl * D + lane + 32 * j] = x[j] * up;
-        if (lane == 0) sm.qmul[sl] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
-    }
-    named_barrier_sync(1, kNCW * 32);
-    for (int i = threadIdx.x; i < Sm::kSets * NB * (D / 32) * 32; i += kNCW * 32) {
-        const int ln = i & 31, pair = (i >> 5) % (D / 32), nb = (i >> 5) / (D / 32) % NB, set = (i >> 5) / (D / 32) / NB;
-        const int n = ln >> 2, t = ln & 3;
-        const float* row = qn + (4 * nb + (n >> 1)) * D;
-        const bool packed_set = PACKED && set == Sm::kSets - 1;
-        const bool third_set = BF16 && set == 1;
-        uint32_t w[4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const int kk = 2 * pair + (h >> 1);
-            // packed: lane t reads codes 16 t .. of a 64-channel half, four per k-step
-            const int d = packed_set ? 64 * (kk >> 2) + 16 * t + 4 * (kk & 3) + 2 * (h & 1)
-                                     : 16 * kk + 2 * t + 8 * (h & 1);
-            const float x0 = row[d], x1 = row[d + 1];
-            if (packed_set) {
-                const float h0 = round16<__half>(x0), h1 = round16<__half>(x1);
-                w[h] = (n & 1) ? pack2<__half>(x0 - h0, x1 - h1) : pack2<__half>(h0, h1);
-            } else {
-                const float h0 = round16<T>(x0), h1 = round16<T>(x1);
-                const float r0 = x0 - h0, r1 = x1 - h1;
-                if (third_set)
-                    w[h] = (n & 1) ? 0u : pack2<T>(r0 - round16<T>(r0), r1 - round16<T>(r1));
-                else
-                    w[h] = (n & 1) ? pack2<T>(r0, r1) : pack2<T>(h0, h1);
-            }
+        if (PACKED && warp == 1) {
+            load_q<__half, D, NB, true, false>(q, p.q, om, bh, slot0, nslots, p.qscale);
+            store_q<D, NB>(sm.qf[kPackedSet], q.a);
         }
-        sm.qf[set][nb][pair][ln] = make_uint4(w[0], w[1], w[2], w[3]);
+        named_barrier_sync(1, kNCW * 32);
+    } else {
+        if (PACKED && packed_order)
+            load_q<__half, D, NB, true, false>(q, p.q, om, bh, slot0, nslots, p.qscale);
+        else
+            load_q<T, D, NB, false, BF16>(q, p.q, om, bh, slot0, nslots, p.qscale);
     }
-    named_barrier_sync(1, kNCW * 32);
-
+    // operand of k-step kk: set 0 head and remainder, 1 third terms (16-bit tiles), kPackedSet packed tiles
+    auto qop = [&](int set, int nb, int kk) {
+        if constexpr (QS) return sm.qf[set][nb][kk][lane];
+        if (BF16 && set == 1 && !(PACKED && kPackedSet == 1)) return make_uint2(q.c[nb][kk][0], q.c[nb][kk][1]);
+        return make_uint2(q.a[nb][kk][0], q.a[nb][kk][1]);
+    };
     int qp[NB];
-    float qm[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        qp[nb] = q_pos0 + (slot0 + 4 * nb + t4) / p.G;
-        qm[nb] = sm.qmul[4 * nb + t4];
-    }
+    for (int nb = 0; nb < NB; ++nb) qp[nb] = q_pos0 + (slot0 + 4 * nb + t4) / p.G;
     State<D, NB> st;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -388,84 +445,91 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     st.inv_u = 0.f;
     // Channel of accumulator row g (+ 8 h) of strip dt: packed tiles
     // chan0 + 2 dt + h, 16-bit tiles 16 dt + 8 h + g.
-    const int cg = D == 128 ? ((g & 1) << 2 | g >> 1) : g;
+    const int cg = spread<D>(g);
     const int chan0 = cg * (D / 8);
-    bool packed_order = PACKED && nitems > 0 && item0 < arch_items;
 
     const int mi = lane >> 3, ri = lane & 7;
-    int consumed = 0;
-    for (int it = 0; it < nitems; ++it) {
+    const int group = warp >> 2, gwarp = warp & 3;
+    int next = group;  // first item of this group not consumed yet
+    for (int it = group; it < nitems; it += GROUPS) {
         const int s = it % STAGES;
         if (!mbar_wait_bounded(&sm.full[s], (it / STAGES) & 1, &sm.abort)) {
             atomicExch(&sm.abort, 1);
             atomicExch(p.ws.error, kDevErrTimeout);
             break;
         }
-        consumed = it + 1;
+        next = it + GROUPS;
         const int4 inf = sm.info[s];
         const uint32_t sb = smem_u32(sm.stage[s]);
         if (PACKED && inf.x) {
-            const int k_strip = 16 * warp;
-            if (inf.z > k_strip) {
+            const int k_strip = 16 * gwarp;
+            const bool mine = inf.z > k_strip;
+            if (mine) {
                 const float4 sc = sm.meta[s];
-                // key of strip row g: a permutation that spreads the 8 lanes of a
-                // shared-memory phase over all banks (head_dim 64: rows alternate halves already)
-                const int ka = k_strip + (D == 128 ? cg : g), kb = ka + 8;
-                float c[NB][4];
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) c[nb][0] = c[nb][1] = c[nb][2] = c[nb][3] = 0.f;
+                const int ka = k_strip + (D == 128 ? cg : g), kb = ka + 8;  // rows ka and kb share the swizzle pattern
+                uint32_t wa[D / 16], wb[D / 16];
 #pragma unroll
                 for (int half = 0; half < D / 64; ++half) {
                     const int ch = t4 + 4 * half;
                     const uint32_t swz = D == 128 ? (ch ^ (ka & 7)) : (ch ^ ((ka >> 1) & 3));
-                    // rows ka and kb = ka + 8 share the swizzle pattern
                     const uint4 xa = lds_u4(sb + ka * D + (swz << 4)), xb = lds_u4(sb + kb * D + (swz << 4));
-                    const uint32_t wa[4] = {xa.x, xa.y, xa.z, xa.w}, wb[4] = {xb.x, xb.y, xb.z, xb.w};
+                    wa[4 * half] = xa.x, wa[4 * half + 1] = xa.y, wa[4 * half + 2] = xa.z, wa[4 * half + 3] = xa.w;
+                    wb[4 * half] = xb.x, wb[4 * half + 1] = xb.y, wb[4 * half + 2] = xb.z, wb[4 * half + 3] = xb.w;
+                }
+                // V: keys of P^T rows 2t, 2t + 1 and 2t + 8, 2t + 9; D / 8 consecutive channels per lane.
+                // With one column block they are fetched before the logits are needed and free the stage early;
+                // with more there are no registers to hold them through the softmax.
+                const int v0 = k_strip + (D == 128 ? t4 : 2 * t4), v1 = D == 128 ? v0 + 4 : v0 + 1;
+                const uint32_t vb = sb + Geo::kVPacked;
+                uint32_t x0[D / 32], x1[D / 32], x2[D / 32], x3[D / 32];
+                auto fetch_v = [&]() {
+                    if constexpr (D == 128) {
+                        const uint4 y0 = lds_u4(vb + v0 * D + ((cg ^ (v0 & 7)) << 4));
+                        const uint4 y1 = lds_u4(vb + v1 * D + ((cg ^ (v1 & 7)) << 4));
+                        const uint4 y2 = lds_u4(vb + (v0 + 8) * D + ((cg ^ (v0 & 7)) << 4));
+                        const uint4 y3 = lds_u4(vb + (v1 + 8) * D + ((cg ^ (v1 & 7)) << 4));
+                        x0[0] = y0.x, x0[1] = y0.y, x0[2] = y0.z, x0[3] = y0.w;
+                        x1[0] = y1.x, x1[1] = y1.y, x1[2] = y1.z, x1[3] = y1.w;
+                        x2[0] = y2.x, x2[1] = y2.y, x2[2] = y2.z, x2[3] = y2.w;
+                        x3[0] = y3.x, x3[1] = y3.y, x3[2] = y3.z, x3[3] = y3.w;
+                    } else {
+                        const int ch = g >> 1, lo = (g & 1) * 8;
+                        auto at = [&](int key) { return lds_u2(vb + key * D + ((ch ^ ((key >> 1) & 3)) << 4) + lo); };
+                        const uint2 y0 = at(v0), y1 = at(v1), y2 = at(v0 + 8), y3 = at(v1 + 8);
+                        x0[0] = y0.x, x0[1] = y0.y, x1[0] = y1.x, x1[1] = y1.y;
+                        x2[0] = y2.x, x2[1] = y2.y, x3[0] = y3.x, x3[1] = y3.y;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.empty[s]);
+                };
+                if (NB == 1) fetch_v();
+                float c[NB][2][4];  // two chains of dependent products
 #pragma unroll
-                    for (int pr = 0; pr < 2; ++pr) {
-                        uint4 qv[NB];
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) qv[nb] = sm.qf[Sm::kSets - 1][nb][2 * half + pr][lane];
+                    for (int j = 0; j < 4; ++j) c[nb][0][j] = c[nb][1][j] = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int w = 2 * pr + j;
-                            const uint32_t a[4] = {f16x2_of_e4m3x2(wa[w]), f16x2_of_e4m3x2(wb[w]),
-                                                   f16x2_of_e4m3x2_hi(wa[w]), f16x2_of_e4m3x2_hi(wb[w])};
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t a[4] = {f16x2_of_e4m3x2(wa[kk]), f16x2_of_e4m3x2(wb[kk]), f16x2_of_e4m3x2_hi(wa[kk]),
+                                           f16x2_of_e4m3x2_hi(wb[kk])};
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb)
-                                MmaOp<__half>::run(c[nb], a, j ? qv[nb].z : qv[nb].x, j ? qv[nb].w : qv[nb].y);
-                        }
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const uint2 o = qop(kPackedSet, nb, kk);
+                        MmaOp<__half>::run(c[nb][kk & 1], a, o.x, o.y);
                     }
                 }
                 float s0[NB], s1[NB];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const float f = qm[nb] * sc.x;
-                    s0[nb] = (ka < inf.z && inf.y + ka <= qp[nb]) ? (c[nb][0] + c[nb][1]) * f : -CUDART_INF_F;
-                    s1[nb] = (kb < inf.z && inf.y + kb <= qp[nb]) ? (c[nb][2] + c[nb][3]) * f : -CUDART_INF_F;
+                    const float f = q.mul[nb] * sc.x;
+                    s0[nb] = (ka < inf.z && inf.y + ka <= qp[nb])
+                                 ? ((c[nb][0][0] + c[nb][1][0]) + (c[nb][0][1] + c[nb][1][1])) * f : -CUDART_INF_F;
+                    s1[nb] = (kb < inf.z && inf.y + kb <= qp[nb])
+                                 ? ((c[nb][0][2] + c[nb][1][2]) + (c[nb][0][3] + c[nb][1][3])) * f : -CUDART_INF_F;
                 }
                 uint32_t b[NB][2], b3[NB][2];
                 softmax_strip<__half, D, NB, false>(st, s0, s1, sc.y, b, b3);
-                // V: keys of P^T rows 2t, 2t + 1 and 2t + 8, 2t + 9; D / 8 consecutive channels per lane
-                const int v0 = k_strip + (D == 128 ? t4 : 2 * t4), v1 = D == 128 ? v0 + 4 : v0 + 1;
-                const uint32_t vb = sb + Geo::kVPacked;
-                uint32_t x0[D / 32], x1[D / 32], x2[D / 32], x3[D / 32];
-                if constexpr (D == 128) {
-                    const uint4 y0 = lds_u4(vb + v0 * D + ((cg ^ (v0 & 7)) << 4));
-                    const uint4 y1 = lds_u4(vb + v1 * D + ((cg ^ (v1 & 7)) << 4));
-                    const uint4 y2 = lds_u4(vb + (v0 + 8) * D + ((cg ^ (v0 & 7)) << 4));
-                    const uint4 y3 = lds_u4(vb + (v1 + 8) * D + ((cg ^ (v1 & 7)) << 4));
-                    x0[0] = y0.x, x0[1] = y0.y, x0[2] = y0.z, x0[3] = y0.w;
-                    x1[0] = y1.x, x1[1] = y1.y, x1[2] = y1.z, x1[3] = y1.w;
-                    x2[0] = y2.x, x2[1] = y2.y, x2[2] = y2.z, x2[3] = y2.w;
-                    x3[0] = y3.x, x3[1] = y3.y, x3[2] = y3.z, x3[3] = y3.w;
-                } else {
-                    const int ch = g >> 1, lo = (g & 1) * 8;
-                    auto at = [&](int key) { return lds_u2(vb + key * D + ((ch ^ ((key >> 1) & 3)) << 4) + lo); };
-                    const uint2 y0 = at(v0), y1 = at(v1), y2 = at(v0 + 8), y3 = at(v1 + 8);
-                    x0[0] = y0.x, x0[1] = y0.y, x1[0] = y1.x, x1[1] = y1.y;
-                    x2[0] = y2.x, x2[1] = y2.y, x3[0] = y3.x, x3[1] = y3.y;
-                }
+                if (NB > 1) fetch_v();
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w) {
                     // interleave the two keys' bytes: each half word is one channel of both
@@ -481,14 +545,17 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                         MmaOp<__half>::run(st.acc[nb][2 * w + 1], a1, b[nb][0], b[nb][1]);
                     }
                 }
+            } else {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.empty[s]);
             }
         } else {
-            // 16-bit item: HK / 16 strips; with two strips the warp pairs take turns
-            const int strip = HK == 64 ? warp : (warp & 1);
-            const bool mine = HK == 64 || (warp >> 1) == (it & 1);
+            // 16-bit item: HK / 16 strips; with two strips the group's warp pairs take turns
+            const int strip = HK == 64 ? gwarp : (gwarp & 1);
+            const bool mine = HK == 64 || (gwarp >> 1) == ((it / GROUPS) & 1);
             const int sv = inf.z - 16 * strip;  // valid keys in the strip
             if (mine && sv > 0) {
-                if (PACKED && packed_order) {  // first 16-bit strip after packed ones: reorder O's channels
+                if (PACKED && packed_order) {  // first 16-bit strip after packed ones: reorder O's channels, q's fragments
                     packed_order = false;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
@@ -509,28 +576,26 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                             st.acc[nb][dt][1] = st.acc[nb][dt][3] = 0.f;
                         }
                     __syncwarp();
+                    if (!QS) load_q<T, D, NB, false, BF16>(q, p.q, om, bh, slot0, nslots, p.qscale);
                 }
-                float c[NB][4];
+                float c[NB][2][4];  // two chains of dependent products
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) c[nb][0] = c[nb][1] = c[nb][2] = c[nb][3] = 0.f;
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[nb][0][j] = c[nb][1][j] = 0.f;
                 const int kkey = 16 * strip + ri + 8 * (mi & 1);
 #pragma unroll
-                for (int pr = 0; pr < D / 32; ++pr) {
-                    uint4 qv[NB], q3[NB];
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const int chunk = (kk & 3) * 2 + (mi >> 1);
+                    uint32_t a[4];
+                    ldmatrix_x4(a, sb + (kk >> 2) * HK * 128 + kkey * 128 + ((chunk ^ (kkey & 7)) << 4));
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        qv[nb] = sm.qf[0][nb][pr][lane];
-                        if (BF16) q3[nb] = sm.qf[Sm::kSets > 1 ? 1 : 0][nb][pr][lane];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int kk = 2 * pr + j, chunk = (kk & 3) * 2 + (mi >> 1);
-                        uint32_t a[4];
-                        ldmatrix_x4(a, sb + (kk >> 2) * HK * 128 + kkey * 128 + ((chunk ^ (kkey & 7)) << 4));
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            MmaOp<T>::run(c[nb], a, j ? qv[nb].z : qv[nb].x, j ? qv[nb].w : qv[nb].y);
-                            if (BF16) MmaOp<T>::run(c[nb], a, j ? q3[nb].z : q3[nb].x, j ? q3[nb].w : q3[nb].y);
+                        const uint2 o = qop(0, nb, kk);
+                        MmaOp<T>::run(c[nb][BF16 ? 0 : kk & 1], a, o.x, o.y);
+                        if (BF16) {
+                            const uint2 o3 = qop(1, nb, kk);
+                            MmaOp<T>::run(c[nb][1], a, o3.x, o3.y);
                         }
                     }
                 }
@@ -538,8 +603,10 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                 float s0[NB], s1[NB];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    s0[nb] = (ka < inf.z && inf.y + ka <= qp[nb]) ? (c[nb][0] + c[nb][1]) * qm[nb] : -CUDART_INF_F;
-                    s1[nb] = (kb < inf.z && inf.y + kb <= qp[nb]) ? (c[nb][2] + c[nb][3]) * qm[nb] : -CUDART_INF_F;
+                    s0[nb] = (ka < inf.z && inf.y + ka <= qp[nb])
+                                 ? ((c[nb][0][0] + c[nb][1][0]) + (c[nb][0][1] + c[nb][1][1])) * q.mul[nb] : -CUDART_INF_F;
+                    s1[nb] = (kb < inf.z && inf.y + kb <= qp[nb])
+                                 ? ((c[nb][0][2] + c[nb][1][2]) + (c[nb][0][3] + c[nb][1][3])) * q.mul[nb] : -CUDART_INF_F;
                 }
                 uint32_t b[NB][2], b3[NB][2];
                 softmax_strip<T, D, NB, BF16>(st, s0, s1, 1.f, b, b3);
@@ -566,15 +633,15 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                     }
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.empty[s]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.empty[s]);
     }
 
     griddep_launch_dependents();
     if (sm.abort) {
         // Drain: wait (bounded) for loads already issued into stages we did not consume.
-        for (int it = consumed; it < min(nitems, consumed + STAGES); ++it)
+        for (int it = next; it < min(nitems, next + STAGES); it += GROUPS)
             mbar_wait_bounded(&sm.full[it % STAGES], (it / STAGES) & 1, nullptr);
     }
 
@@ -584,18 +651,26 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) st.l[nb] += __shfl_xor_sync(0xffffffffu, st.l[nb], off);
         const int sl = 4 * nb + t4;
+        float* row = sm.red_o[warp][sl];
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) {
-            float* o = &sm.red_o[warp][sl][packed_order ? chan0 + 2 * dt : 16 * dt + g];
-            o[0] = st.acc[nb][dt][0] + st.acc[nb][dt][1];
-            o[packed_order ? 1 : 8] = st.acc[nb][dt][2] + st.acc[nb][dt][3];
+            const float o0 = st.acc[nb][dt][0] + st.acc[nb][dt][1], o1 = st.acc[nb][dt][2] + st.acc[nb][dt][3];
+            if (PACKED && packed_order) {
+                *reinterpret_cast<float2*>(row + (dt * 8 + g) * 2) = make_float2(o0, o1);
+            } else {
+                row[16 * dt + g] = o0;
+                row[16 * dt + 8 + g] = o1;
+            }
         }
         if (g == 0) {
             sm.red_m[warp][sl] = st.m[nb];
             sm.red_l[warp][sl] = st.l[nb];
         }
     }
-    if (lane == 0) sm.red_u[warp] = st.u * (1.f / kPScale);
+    if (lane == 0) {
+        sm.red_u[warp] = st.u * (1.f / kPScale);
+        sm.red_packed[warp] = packed_order;
+    }
     named_barrier_sync(1, kNCW * 32);
 
     const int counter = list * gridDim.z + zb;
@@ -613,7 +688,14 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
             // a warp without keys has weight 0; NaN maxima cannot occur (fmaxf drops them), NaN sums stay
             const float wt = M == -CUDART_INF_F ? 1.f : ex2_approx(mw - M);
             const float wo = wt * sm.red_u[w];
-            const float4 o = reinterpret_cast<const float4*>(sm.red_o[w][sl])[d4];
+            float4 o;
+            if (PACKED && sm.red_packed[w]) {
+                const float* r = sm.red_o[w][sl] + packed_pos<D>(4 * d4);
+                const float2 a = *reinterpret_cast<const float2*>(r), b = *reinterpret_cast<const float2*>(r + 16);
+                o = make_float4(a.x, a.y, b.x, b.y);
+            } else {
+                o = reinterpret_cast<const float4*>(sm.red_o[w][sl])[d4];
+            }
             L += wt * sm.red_l[w][sl];
             O.x += wo * o.x;
             O.y += wo * o.y;
@@ -642,25 +724,36 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     if (threadIdx.x == 0) sm.flag = atom_add_acq_rel_gpu(&p.ws.counters[counter], 1) == p.splits - 1;
     named_barrier_sync(1, kNCW * 32);
     if (!sm.flag) return;
-    // The partial outputs of all splits are one contiguous run: with room for
+    // The partials of all splits are contiguous runs (O, m, l): with room for
     // them in the idle stages they come in one round trip of asynchronous copies.
     float* wts = &sm.red_o[0][0][0];  // [SL][splits] weights
     const int parts = p.splits * SL;
-    const bool staged = (size_t)parts * D * 4 <= (size_t)STAGES * kStageBytes;
-    float4* stage = reinterpret_cast<float4*>(&sm.stage[0][0]);
-    const float4* src = reinterpret_cast<const float4*>(p.ws.o + part_base * D);
+    const bool staged = (size_t)parts * (D + 2) * 4 <= (size_t)STAGES * kStageBytes;
+    const float* src_o = p.ws.o + part_base * D;
+    const float* src_m = p.ws.m + part_base;
+    const float* src_l = p.ws.l + part_base;
     if (staged) {
-        for (int i = threadIdx.x; i < parts * V4; i += kNCW * 32) cp_async_16(stage + i, src + i);
+        float4* st_o = reinterpret_cast<float4*>(&sm.stage[0][0]);
+        float4* st_ml = st_o + (size_t)parts * V4;
+        for (int i = threadIdx.x; i < parts / 2; i += kNCW * 32)
+            cp_async_16(st_ml + i, i < parts / 4 ? src_m + 4 * i : src_l + 4 * (i - parts / 4));
+        for (int i = threadIdx.x; i < parts * V4; i += kNCW * 32) cp_async_16(st_o + i, src_o + 4 * (size_t)i);
         cp_async_commit();
+        cp_async_wait_all();
+        named_barrier_sync(1, kNCW * 32);
+        src_o = reinterpret_cast<const float*>(st_o);
+        src_m = reinterpret_cast<const float*>(st_ml);
+        src_l = src_m + parts;
     }
+    auto get = [&](const float* x) { return staged ? *x : __ldcg(x); };
     for (int sl = warp; sl < nslots; sl += kNCW) {
         float M = -CUDART_INF_F, L = 0.f;
-        for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, __ldcg(p.ws.m + part_base + s * SL + sl));
+        for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, get(src_m + s * SL + sl));
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
         for (int s = lane; s < p.splits; s += 32) {
-            const float wt = M == -CUDART_INF_F ? 1.f : ex2_approx(__ldcg(p.ws.m + part_base + s * SL + sl) - M);
-            L += wt * __ldcg(p.ws.l + part_base + s * SL + sl);
+            const float wt = M == -CUDART_INF_F ? 1.f : ex2_approx(get(src_m + s * SL + sl) - M);
+            L += wt * get(src_l + s * SL + sl);
             wts[sl * p.splits + s] = wt;
         }
 #pragma unroll
@@ -672,12 +765,11 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                 p.lse[om.row(bh, slot0 + sl)] = any ? (M + log2f(L)) * 0.69314718055994531f : -CUDART_INF_F;
         }
     }
-    if (staged) cp_async_wait_all();
     named_barrier_sync(1, kNCW * 32);
     for (int i = threadIdx.x; i < nslots * V4; i += kNCW * 32) {
         const int sl = i / V4, d4 = i % V4;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4* from = (staged ? stage : src) + sl * V4 + d4;
+        const float4* from = reinterpret_cast<const float4*>(src_o) + sl * V4 + d4;
 #pragma unroll 8
         for (int s = 0; s < p.splits; ++s) {
             const float4 o = staged ? from[(size_t)s * SL * V4] : __ldcg(from + (size_t)s * SL * V4);
@@ -694,37 +786,79 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     if (threadIdx.x == 0) p.ws.counters[counter] = 0;
 }
 
+// Launch shape by column blocks: consumer groups, stages and CTAs per SM.
+template <int NB> struct Shape;
+#ifndef RFSN_G1
+#define RFSN_G1 1
+#define RFSN_S1 6
+#define RFSN_C1 2
+#endif
+template <> struct Shape<1> { static constexpr int kGroups = RFSN_G1, kStages = RFSN_S1, kCtas = RFSN_C1; };
+#ifndef RFSN_G2
+#define RFSN_G2 2
+#define RFSN_S2 8
+#define RFSN_C2 1
+#endif
+template <> struct Shape<2> { static constexpr int kGroups = RFSN_G2, kStages = RFSN_S2, kCtas = RFSN_C2; };
+template <> struct Shape<4> { static constexpr int kGroups = 2, kStages = 8, kCtas = 1; };
+
 template <typename T, int D, int NB, bool PACKED>
 rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const Params& p, int lists, int zblocks,
                    cudaStream_t s) {
-    constexpr int STAGES = NB == 1 ? 6 : 5;  // two CTAs per SM
-    const size_t smem = sizeof(Smem<D, NB, STAGES, PACKED, std::is_same<T, __nv_bfloat16>::value>) + 1024;
-    auto kern = archive_attn_kernel<T, D, NB, STAGES, PACKED>;
-    RFSN_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    using Sh = Shape<NB>;
+    const size_t smem = sizeof(Smem<D, NB, Sh::kGroups, Sh::kStages, PACKED, std::is_same<T, __nv_bfloat16>::value>) + 1024;
+    auto kern = archive_attn_kernel<T, D, NB, Sh::kGroups, Sh::kStages, Sh::kCtas, PACKED>;
+    static std::atomic<bool> ready[64];  // the attribute stays with the kernel on each device
+    const int dev = arena->device;
+    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+        RFSN_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+    }
     const CUtensorMap& k8 = PACKED ? packed->maps[0] : arena->item_maps[0];
     const CUtensorMap& v8 = PACKED ? packed->maps[1] : arena->item_maps[1];
-    RFSN_CUDA(launch_pdl(kern, dim3(p.splits, lists, zblocks), dim3(kThreads), smem, s, arena->item_maps[0],
-                         arena->item_maps[1], k8, v8, p));
+    RFSN_CUDA(launch_pdl(kern, dim3(p.splits, lists, zblocks), dim3((4 * Sh::kGroups + 1) * 32), smem, s,
+                         arena->item_maps[0], arena->item_maps[1], k8, v8, p));
     note_launch();
     return RFSN_OK;
+}
+
+template <typename T, int D, int NB>
+rfsn_status launch_packed(const rfsn_arena* a, const rfsn_packed_archive* pk, const Params& p, int lists, int zb,
+                          cudaStream_t s) {
+    return pk != nullptr ? launch<T, D, NB, true>(a, pk, p, lists, zb, s) : launch<T, D, NB, false>(a, pk, p, lists, zb, s);
 }
 
 template <typename T, int D>
 rfsn_status launch_nb(const rfsn_arena* a, const rfsn_packed_archive* pk, const Params& p, int lists, int nb, int zb,
                       cudaStream_t s) {
-    if (pk != nullptr)
-        return nb == 1 ? launch<T, D, 1, true>(a, pk, p, lists, zb, s) : launch<T, D, 2, true>(a, pk, p, lists, zb, s);
-    return nb == 1 ? launch<T, D, 1, false>(a, pk, p, lists, zb, s) : launch<T, D, 2, false>(a, pk, p, lists, zb, s);
+    if (nb == 1) return launch_packed<T, D, 1>(a, pk, p, lists, zb, s);
+    if constexpr (D == 64) {  // head_dim 128: the accumulators of 16 slots do not fit the registers
+        if (nb == 4) return launch_packed<T, D, 4>(a, pk, p, lists, zb, s);
+    }
+    return launch_packed<T, D, 2>(a, pk, p, lists, zb, s);
 }
 
 template <typename T, int D, int NB>
-void preload() {
+void preload_nb() {
+    using Sh = Shape<NB>;
     cudaFuncAttributes a;
-    cudaFuncGetAttributes(&a, archive_attn_kernel<T, D, NB, NB == 1 ? 6 : 5, true>);
-    cudaFuncGetAttributes(&a, archive_attn_kernel<T, D, NB, NB == 1 ? 6 : 5, false>);
+    cudaFuncGetAttributes(&a, archive_attn_kernel<T, D, NB, Sh::kGroups, Sh::kStages, Sh::kCtas, true>);
+    cudaFuncGetAttributes(&a, archive_attn_kernel<T, D, NB, Sh::kGroups, Sh::kStages, Sh::kCtas, false>);
+}
+
+template <typename T, int D>
+void preload() {
+    preload_nb<T, D, 1>();
+    preload_nb<T, D, 2>();
+    if constexpr (D == 64) preload_nb<T, D, 4>();
 }
 
 }  // namespace archive
+
+int archive_attn_ctas(int nb) {
+    using namespace archive;
+    return nb == 1 ? Shape<1>::kCtas : nb == 2 ? Shape<2>::kCtas : Shape<4>::kCtas;
+}
 
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int nb, int zblocks, cudaStream_t s) {
@@ -741,14 +875,10 @@ void preload_archive_kernels() {
     using namespace archive;
     preload_pack_kernels();
     preload_select_kernels();
-    preload<__nv_bfloat16, 128, 1>();
-    preload<__nv_bfloat16, 128, 2>();
-    preload<__nv_bfloat16, 64, 1>();
-    preload<__nv_bfloat16, 64, 2>();
-    preload<__half, 128, 1>();
-    preload<__half, 128, 2>();
-    preload<__half, 64, 1>();
-    preload<__half, 64, 2>();
+    preload<__nv_bfloat16, 128>();
+    preload<__nv_bfloat16, 64>();
+    preload<__half, 128>();
+    preload<__half, 64>();
 }
 
 }  // namespace rfsn

@@ -74,7 +74,9 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(RowSource ks, RowSou
     constexpr int VPR = D / 8;                    // 8-element vectors per row
     constexpr int RPP = kPackThreads / VPR;       // rows per pass
     constexpr int PASSES = kTile / RPP;
-    const int tile = blockIdx.x, bh = blockIdx.y, is_v = blockIdx.z;
+    // heads first: the CTAs that run together read neighbouring rows of token-major sources whole
+    const int bh = blockIdx.x >> 1, is_v = blockIdx.x & 1, tile = blockIdx.y + blockIdx.z * gridDim.y;
+    if (tile * kTile >= count) return;
     const RowSource src = is_v ? vs : ks;
     const int len = min(kTile, count - tile * kTile);
     const int c8 = threadIdx.x % VPR, r0 = threadIdx.x / VPR;
@@ -249,7 +251,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(const T* __restrict__ k, T*
 template <typename T, int D>
 rfsn_status pack_launch(const rfsn_packed_archive* a, int dst_row0, const RowSource& ks, const RowSource& vs,
                         int count, void* bounds, cudaStream_t s) {
-    const dim3 grid((count + kTile - 1) / kTile, a->groups, 2);
+    const int tiles = (count + kTile - 1) / kTile, ty = tiles < 32768 ? tiles : 32768;
+    const dim3 grid(2 * a->groups, ty, (tiles + ty - 1) / ty);
     pack_kernel<T, D><<<grid, kPackThreads, 0, s>>>(ks, vs, a->k, a->v, reinterpret_cast<float*>(a->scales),
                                                     static_cast<uint8_t*>(bounds), a->rows, dst_row0, count);
     RFSN_CUDA(cudaGetLastError());

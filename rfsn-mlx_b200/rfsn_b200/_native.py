@@ -79,6 +79,7 @@ EXPORTED_SYMBOLS = (
     "rfsn_tile_bounds",
     "rfsn_select_tiles",
     "rfsn_archive_attention",
+    "rfsn_archive_attend",
     "rfsn_archive_workspace_size",
 )
 
@@ -152,6 +153,22 @@ class TileListC(ctypes.Structure):
         ("tiles", ctypes.c_void_p),  # device int32 [n][4] = {row, pos, len, tile}
         ("n", ctypes.c_int32),
         ("per_query", ctypes.c_int32),
+    ]
+
+
+class ArchiveCallC(ctypes.Structure):
+    _fields_ = [
+        ("arena", ctypes.c_void_p),
+        ("packed", ctypes.c_void_p),
+        ("bounds", ctypes.c_void_p),
+        ("tiles", TileListC),
+        ("hot", HotWindowC),
+        ("batch", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("q_len", ctypes.c_int32),
+        ("top_tiles", ctypes.c_int32),
+        ("max_splits", ctypes.c_int32),
     ]
 
 
@@ -229,6 +246,7 @@ def load_library() -> ctypes.CDLL:
                                     vp, vp, vp, sz, vp]),
         "rfsn_archive_attention": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, ctypes.POINTER(TileListC),
                                          ctypes.POINTER(HotWindowC), vp, vp, vp, sz, i32, vp]),
+        "rfsn_archive_attend": (i32, [ctypes.POINTER(ArchiveCallC), vp, i32, vp, vp, vp, sz, vp]),
         "rfsn_archive_workspace_size": (i32, [i32] * 7 + [ctypes.POINTER(sz)]),
     }
     for name, (res, args) in sig.items():

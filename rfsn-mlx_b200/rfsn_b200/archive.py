@@ -215,32 +215,35 @@ def select_tiles(cache, q: torch.Tensor, q_start_pos: int, segments, top_tiles: 
     return out
 
 
-def tile_attention(cache, q: torch.Tensor, q_start_pos: int, segments, out_ptr: int, lse: Optional[torch.Tensor],
-                   hot: native.HotWindowC, *, top_tiles: int, max_splits: int,
-                   workspace: Optional[native.Workspace], step_state: Optional[torch.Tensor]) -> None:
-    """Attention of float32 q over the segments' archived tiles (all of them, or
-    the ``top_tiles`` best of each query and KV head) and the hot window,
-    written to ``out_ptr``: the packed or sparse form of
-    ``cache.paged_attention``, which checks the arguments."""
-    B, H, Lq, D = q.shape
-    Hkv = cache.num_kv_heads
-    tiles_dev, n_tiles = segments.tile_list
-    if top_tiles > 0 and n_tiles > 0:
-        chosen = select_tiles(cache, q, q_start_pos, segments, top_tiles, workspace=workspace, step_state=step_state)
-        tiles = native.TileListC(chosen.data_ptr(), top_tiles, 1)
-    else:
-        top_tiles = 0
-        tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
-    ws = workspace if workspace is not None else native.default_workspace(cache.device)
-    buf = ws.get(workspace_bytes(B, H, Hkv, Lq, D, n_tiles, top_tiles))
-    native.check(
-        native.lib().rfsn_archive_attention(
-            cache.arena.handle, cache.archive.handle if cache.archive is not None else None, q.data_ptr(), B, H, Hkv,
-            Lq, int(q_start_pos), ctypes.byref(tiles), ctypes.byref(hot), out_ptr,
-            lse.data_ptr() if lse is not None else None, buf.data_ptr(), buf.numel(), max_splits,
-            native.stream_ptr()),
-        "rfsn_archive_attention",
-    )
+class PreparedCall:
+    """``rfsn_archive_call`` of a layer's segments for one query shape, and the
+    buffers it points to (kept alive with it)."""
+
+    __slots__ = ("ref", "nbytes", "keep")
+
+    def __init__(self, cache, segments, hot: native.HotWindowC, q_heads: int, q_len: int, top_tiles: int,
+                 max_splits: int) -> None:
+        if top_tiles and q_len > SPARSE_MAX_ROWS:
+            raise ValueError(f"top_tiles takes up to {SPARSE_MAX_ROWS} query rows a call, got {q_len}")
+        tiles_dev, n_tiles = segments.tile_list
+        archive, bounds = cache.archive, cache.tile_bounds
+        call = native.ArchiveCallC(
+            cache.arena.handle, archive.handle if archive is not None else None,
+            bounds.data_ptr() if top_tiles else None, native.TileListC(tiles_dev.data_ptr(), n_tiles, 0), hot,
+            cache.batch_size, q_heads, cache.num_kv_heads, q_len, top_tiles, max_splits)
+        self.ref = ctypes.byref(call)
+        self.nbytes = workspace_bytes(cache.batch_size, q_heads, cache.num_kv_heads, q_len, cache.config.head_dim,
+                                      n_tiles, top_tiles if n_tiles else 0)
+        self.keep = (call, cache.arena, archive, bounds, tiles_dev)
+
+    def __call__(self, cache, q_ptr: int, q_start_pos: int, out_ptr: int, lse_ptr: Optional[int],
+                 workspace: Optional[native.Workspace]) -> None:
+        ws = workspace if workspace is not None else native.default_workspace(cache.device)
+        buf = ws.get(self.nbytes)
+        status = native.lib().rfsn_archive_attend(self.ref, q_ptr, q_start_pos, out_ptr, lse_ptr, buf.data_ptr(),
+                                                  buf.numel(), native.stream_ptr())
+        if status:
+            native.check(status, "rfsn_archive_attend")
 
 
-__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "select_tiles", "tile_attention", "workspace_bytes"]
+__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "PreparedCall", "select_tiles", "workspace_bytes"]

@@ -46,7 +46,7 @@ import numpy as np
 import torch
 
 from . import _native as native
-from .archive import PackedArchive, check_archive_options, padded_rows, select_tiles, tile_attention
+from .archive import PackedArchive, PreparedCall, check_archive_options, padded_rows, select_tiles
 from .block_manager import BlockId, BlockLocation, BlockManager, BlockManifest, BlockSpan
 from .config import RFSNConfig, RuntimeMode, resolve_dtype, validate_session_id
 from .residency import ResidencyManager
@@ -285,6 +285,7 @@ class PagedSegments(Sequence):
         self.hot_state = hot_state            # (head_index, length, start) or None when hot pieces excluded
         # (device int32 [n, 4] tiles, n) of the archived spans: packed caches and caches with a tile index
         self.tile_list = cache.tile_snapshot() if table is not None else (cache.tile_snapshot()[0], 0)
+        self.calls: dict[tuple, PreparedCall] = {}  # prepared calls over these segments, by query shape
 
     def __len__(self) -> int:
         return len(self.spans)
@@ -1267,6 +1268,64 @@ def _unpacked_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, 
             filled = 1
 
 
+def _out_pointer(cache: LayerKVCache, out: torch.Tensor, shape: tuple) -> int:
+    if out.dtype != torch.float32 or tuple(out.shape) != shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
+    if out.device.type == "cpu":
+        return native.host_device_pointer(out)
+    if out.device == cache.device:
+        return out.data_ptr()
+    raise ValueError(f"out must be on {cache.device} or pinned host memory")
+
+
+def _hot_window(cache: LayerKVCache, segments: PagedSegments,
+                step_state: Optional[torch.Tensor]) -> native.HotWindowC:
+    if segments.hot_state is not None:
+        head, hlen, hstart = segments.hot_state
+    else:
+        head, hlen, hstart = 0, 0, 0
+        if segments.n_archived != len(segments):
+            # hot-only view taken without a snapshot: use the live ring state
+            head, hlen, hstart = cache.hot_head_index, cache.hot_seq_len, cache.hot_start
+    return native.HotWindowC(0, cache.config.hot_capacity, head, hlen, hstart, 0,
+                             step_state.data_ptr() if step_state is not None else None)
+
+
+def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segments: PagedSegments, want_lse: bool,
+                    max_splits: int, workspace: Optional[native.Workspace], peers: Optional[Any],
+                    step_state: Optional[torch.Tensor], out: Optional[torch.Tensor], top_tiles: int):
+    """``paged_attention`` of packed caches and of calls that select tiles. The
+    part of a call that does not depend on the query is prepared once per
+    segments and shape: a decode step's host work is a few microseconds."""
+    if peers is not None:
+        raise NotImplementedError("the merge across GPUs inside the kernel reads exact archives in full: no packed "
+                                  "archive and no tile selection")
+    qf = _query(cache, q)
+    if out is None:
+        out = torch.empty_like(qf)
+        out_ptr = out.data_ptr()
+    else:
+        out_ptr = _out_pointer(cache, out, tuple(qf.shape))
+    _, H, Lq, D = qf.shape
+    lse = torch.empty(qf.shape[:3], dtype=torch.float32, device=cache.device) if want_lse else None
+    key = (H, Lq, top_tiles, max_splits)
+    call = segments.calls.get(key) if step_state is None else None
+    if call is None or call.keep[2] is not cache.archive or call.keep[1] is not cache.arena:
+        if top_tiles < 0 or (top_tiles and cache.tile_bounds is None):
+            raise ValueError("top_tiles needs a cache built with tile_index=True and a count >= 0")
+        hot = _hot_window(cache, segments, step_state)
+        if not top_tiles and segments.n_archived and step_state is None and Lq >= _CHUNK_ROWS and D == 128:
+            with native.on_device(cache.device):
+                _unpacked_attention(cache, qf, q_start_pos, segments, out_ptr, lse, hot, workspace)
+            return (out, lse) if want_lse else out
+        call = PreparedCall(cache, segments, hot, H, Lq, int(top_tiles), max_splits)
+        if step_state is None and segments.hot_state is not None:
+            segments.calls[key] = call
+    with native.on_device(cache.device):
+        call(cache, qf.data_ptr(), int(q_start_pos), out_ptr, lse.data_ptr() if want_lse else None, workspace)
+    return (out, lse) if want_lse else out
+
+
 def paged_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segments: PagedSegments,
                     *, want_lse: bool = False, max_splits: int = 0, workspace: Optional[native.Workspace] = None,
                     peers: Optional[Any] = None, step_state: Optional[torch.Tensor] = None,
@@ -1294,48 +1353,21 @@ def paged_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
     the softmax over those keys."""
     if len(segments) == 0 and peers is None:
         raise RuntimeError("run_segmented_attention requires at least one KV segment")
+    if top_tiles or cache.archive is not None:
+        return _tile_attention(cache, q, q_start_pos, segments, want_lse, max_splits, workspace, peers, step_state, out,
+                               top_tiles)
     qf = _query(cache, q)
     B, H, Lq, D = (int(x) for x in qf.shape)
     if out is None:
         out = torch.empty((B, H, Lq, D), dtype=torch.float32, device=cache.device)
-        out_ptr = out.data_ptr()
-    else:
-        if out.dtype != torch.float32 or tuple(out.shape) != (B, H, Lq, D) or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous float32 tensor of shape {(B, H, Lq, D)}")
-        if out.device.type == "cpu":
-            out_ptr = native.host_device_pointer(out)
-        elif out.device == cache.device:
-            out_ptr = out.data_ptr()
-        else:
-            raise ValueError(f"out must be on {cache.device} or pinned host memory")
+    out_ptr = _out_pointer(cache, out, (B, H, Lq, D))
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=cache.device) if want_lse else None
     if segments.table is not None:
         table_dev, n_blocks, toks, tiles = segments.table
     else:
         table_dev, n_blocks, toks, tiles = cache._table_dev, 0, 0, 0
     table = native.PageTableC(table_dev.data_ptr(), n_blocks, toks, tiles, 0)
-    if segments.hot_state is not None:
-        head, hlen, hstart = segments.hot_state
-    else:
-        head, hlen, hstart = 0, 0, 0
-        if segments.n_archived != len(segments):
-            # hot-only view taken without a snapshot: use the live ring state
-            head, hlen, hstart = cache.hot_head_index, cache.hot_seq_len, cache.hot_start
-    hot = native.HotWindowC(0, cache.config.hot_capacity, head, hlen, hstart, 0,
-                            step_state.data_ptr() if step_state is not None else None)
-    if top_tiles or cache.archive is not None:
-        if peers is not None:
-            raise NotImplementedError("the merge across GPUs inside the kernel reads exact archives in full: no packed "
-                                      "archive and no tile selection")
-        if top_tiles < 0 or (top_tiles and cache.tile_bounds is None):
-            raise ValueError("top_tiles needs a cache built with tile_index=True and a count >= 0")
-        with native.on_device(cache.device):
-            if not top_tiles and segments.n_archived and step_state is None and Lq >= _CHUNK_ROWS and D == 128:
-                _unpacked_attention(cache, qf, q_start_pos, segments, out_ptr, lse, hot, workspace)
-            else:
-                tile_attention(cache, qf, q_start_pos, segments, out_ptr, lse, hot, top_tiles=int(top_tiles),
-                               max_splits=max_splits, workspace=workspace, step_state=step_state)
-        return (out, lse) if want_lse else out
+    hot = _hot_window(cache, segments, step_state)
     ws = workspace if workspace is not None else native.default_workspace(cache.device)
     nbytes = native.workspace_bytes(B, H, cache.num_kv_heads, Lq, D, max_splits)
     buf = ws.get(nbytes)

@@ -355,7 +355,7 @@ def test_equal_scores_go_to_the_lowest_tiles_and_nan_comes_first():
     assert cache.select_tiles(q, 5000, 3)[0, 0, 0].tolist() == [0, 1, 2]
 
 
-def test_selection_over_more_tiles_than_fit_shared_memory():
+def test_selection_over_more_tiles_than_fit_registers():
     torch = _torch()
     lens = (64 * 13000,)
     cache, k, v = make("bfloat16", 1, 2, 1, 64, (), 0, hot_cap=8, archive_dtype=None, tile_index=True,
