@@ -336,9 +336,9 @@ rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float*
     p.counters = reinterpret_cast<int*>(ws + 256);
     p.error = reinterpret_cast<int*>(ws);
     p.dyn = step_state;
-    // four CTAs per SM over all lists, in steps of the 32 tiles that a CTA scores at once
-    const int want = std::max(1, 4 * device_sms() / lists);
-    p.tiles_per_cta = std::max(32, ((tiles->n + want - 1) / want + 31) / 32 * 32);
+    // one CTA per SM over all lists, in steps of the 128 tiles that a CTA scores at once
+    const int want = std::max(1, device_sms() / lists);
+    p.tiles_per_cta = std::max(128, ((tiles->n + want - 1) / want + 127) / 128 * 128);
     const int chunks = std::max(1, (tiles->n + p.tiles_per_cta - 1) / p.tiles_per_cta);
     return select_tiles_launch(bounds_dtype, head_dim, p, lists, chunks, static_cast<cudaStream_t>(stream));
 }

@@ -22,14 +22,14 @@
 namespace rfsn {
 namespace archive {
 
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kHeadsPerPass = 4;
 
 template <typename T> struct BoundVec;  // 8 bounds -> float
 template <> struct BoundVec<__nv_bfloat16> {
-    static constexpr int kBytes = 16;
     uint4 w;
+    __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void load(const void* p) { w = __ldg(static_cast<const uint4*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t x = (&w.x)[i >> 1];
@@ -37,8 +37,8 @@ template <> struct BoundVec<__nv_bfloat16> {
     }
 };
 template <> struct BoundVec<__half> {
-    static constexpr int kBytes = 16;
     uint4 w;
+    __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void load(const void* p) { w = __ldg(static_cast<const uint4*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t x = (&w.x)[i >> 1];
@@ -46,8 +46,8 @@ template <> struct BoundVec<__half> {
     }
 };
 template <> struct BoundVec<uint8_t> {  // e4m3
-    static constexpr int kBytes = 8;
     uint2 w;
+    __device__ __forceinline__ void clear() { w = make_uint2(0, 0); }
     __device__ __forceinline__ void load(const void* p) { w = __ldg(static_cast<const uint2*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t x = (&w.x)[i >> 2] >> (8 * (i & 3));
@@ -64,207 +64,212 @@ __device__ __forceinline__ uint32_t score_key(float s) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Selection of one list by one CTA, up to kSelRegKeys * 256 tiles: the keys
-// stay in registers (key i of a thread is tile 256 i + thread).
-constexpr int kSelRegKeys = 16;
+// Selection of one list by one CTA. Up to kSelRegKeys * kSelThreads tiles the
+// keys stay in registers (key i of a thread is tile kSelThreads i + thread);
+// longer lists read their scores again from the workspace (L2) in each pass.
+constexpr int kSelRegKeys = 8;
+constexpr int kBuckets = 2 * kSelThreads;
 
 struct SelShared {
     int flag;
-    int count[2][kSelWarps];
-    uint32_t any[kSelWarps], all[kSelWarps];
+    uint32_t lo[kSelWarps], hi[kSelWarps];
+    int visible[kSelWarps], total[kSelWarps];
+    int bucket, above, inside;
+    int hist[kBuckets];
     alignas(16) int tally[kSelRegKeys * kSelWarps];  // tiles above (low half) and at (high half) the threshold
 };
 
-// The n-th largest key by bisection over the key's bits, two bits a round: a
-// count for each of three candidate thresholds (packed into one word per warp:
-// a warp holds at most 512 keys), skipping the leading bits that all keys
-// share and stopping as soon as a threshold holds exactly n keys.
-__device__ __forceinline__ void select_in_registers(const SelectParams& p, const float* scores, int4* out,
-                                                    SelShared& sh) {
+// The n-th largest key by narrowing a key range: a histogram of 1,024 equal
+// buckets, the bucket in which the count from the top passes n becomes the
+// range. Two passes as a rule (the first bucket holds a few keys, the second
+// separates them), four at most; integer counts, so any order gives the same.
+template <bool REGS>
+__device__ __forceinline__ void select_list(const SelectParams& p, const float* scores, int4* out, SelShared& sh) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int T_ = p.n_tiles;
-    uint32_t key[kSelRegKeys];
-    uint32_t any = 0u, all = 0xffffffffu;
-    int visible = 0;
+    uint32_t key[REGS ? kSelRegKeys : 1];
+    if (REGS) {
 #pragma unroll
-    for (int i = 0; i < kSelRegKeys; ++i) {
-        const int t = tid + kSelThreads * i;
-        key[i] = t < T_ ? score_key(__ldcg(scores + t)) : 0u;
-    }
-#pragma unroll
-    for (int i = 0; i < kSelRegKeys; ++i)
-        if (key[i] != 0u) {
-            ++visible;
-            any |= key[i];
-            all &= key[i];
+        for (int i = 0; i < kSelRegKeys; ++i) {
+            const int t = tid + kSelThreads * i;
+            key[REGS ? i : 0] = t < T_ ? score_key(__ldcg(scores + t)) : 0u;
         }
-    any = __reduce_or_sync(0xffffffffu, any);
-    all = __reduce_and_sync(0xffffffffu, all);
+    }
+    auto each = [&](auto&& f) {  // f(key) for the thread's keys
+        if (REGS) {
+#pragma unroll
+            for (int i = 0; i < kSelRegKeys; ++i)
+                if (i * kSelThreads < T_) f(key[REGS ? i : 0]);
+        } else {
+            for (int t = tid; t < T_; t += kSelThreads) f(score_key(__ldcg(scores + t)));
+        }
+    };
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    int visible = 0;
+    each([&](uint32_t k) {
+        if (k != 0u) {
+            ++visible;
+            lo = min(lo, k);
+            hi = max(hi, k);
+        }
+    });
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
     visible = __reduce_add_sync(0xffffffffu, visible);
     if (lane == 0) {
-        sh.any[warp] = any;
-        sh.all[warp] = all;
-        sh.count[1][warp] = visible;
+        sh.lo[warp] = lo;
+        sh.hi[warp] = hi;
+        sh.visible[warp] = visible;
     }
+    sh.hist[tid] = sh.hist[tid + kSelThreads] = 0;
     __syncthreads();
     visible = 0;
 #pragma unroll
     for (int w = 0; w < kSelWarps; ++w) {
-        any |= sh.any[w];
-        all &= sh.all[w];
-        visible += sh.count[1][w];
+        lo = min(lo, sh.lo[w]);
+        hi = max(hi, sh.hi[w]);
+        visible += sh.visible[w];
     }
     const int n = min(p.n_select, visible);
     uint32_t thr = 1u;  // every visible tile
     if (n < visible) {
-        const uint32_t differ = any ^ all;
-        int bit = differ ? 31 - __clz(differ) : -1;
-        if (bit >= 0 && !(bit & 1)) ++bit;  // bit pairs: (31, 30) .. (1, 0)
-        thr = bit < 31 ? (any >> (bit + 1)) << (bit + 1) : 0u;  // the bits all keys share
-        int round = 0;
-        for (; bit >= 0; bit -= 2, round ^= 1) {
-            const uint32_t step = 1u << (bit - 1);
-            int c = 0;
+        int need = n;
+        int shift = max(0, 32 - __clz(hi - lo) - 10);  // hi - lo + 1 keys in at most 1,024 buckets
+        for (;;) {
+            each([&](uint32_t k) {
+                const uint32_t d = (k - lo) >> shift;
+                if (k >= lo && d < kBuckets) atomicAdd(&sh.hist[d], 1);
+            });
+            __syncthreads();
+            // counts from the top: thread i has buckets 1023 - 2 i and 1022 - 2 i
+            const int h1 = sh.hist[kBuckets - 1 - 2 * tid], h0 = sh.hist[kBuckets - 2 - 2 * tid];
+            int incl = h0 + h1;
 #pragma unroll
-            for (int i = 0; i < kSelRegKeys; ++i)
-                if (i * kSelThreads < T_)
-                    c += (int)(key[i] >= thr + step) + ((int)(key[i] >= thr + 2 * step) << 10) +
-                         ((int)(key[i] >= thr + 3 * step) << 20);
-            c = __reduce_add_sync(0xffffffffu, c);
-            if (lane == 0) sh.count[round][warp] = c;
-            __syncthreads();  // the other buffer is written only after every thread has passed here again
-            int c1 = 0, c2 = 0, c3 = 0;
-#pragma unroll
-            for (int w = 0; w < kSelWarps; ++w) {
-                const int x = sh.count[round][w];
-                c1 += x & 1023;
-                c2 += (x >> 10) & 1023;
-                c3 += x >> 20;
+            for (int off = 1; off < 32; off <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += v;
             }
-            const int up = c3 >= n ? 3 : c2 >= n ? 2 : c1 >= n ? 1 : 0;
-            thr += up * step;
-            if ((up == 3 && c3 == n) || (up == 2 && c2 == n) || (up == 1 && c1 == n)) break;
+            if (lane == 31) sh.total[warp] = incl;
+            __syncthreads();
+            sh.hist[tid] = sh.hist[tid + kSelThreads] = 0;  // every thread has read its buckets
+#pragma unroll
+            for (int w = 0; w < kSelWarps; ++w)
+                if (w < warp) incl += sh.total[w];
+            const int before = incl - h0 - h1;
+            if (before < need && incl >= need) {
+                const bool first = before + h1 >= need;
+                sh.bucket = kBuckets - (first ? 1 : 2) - 2 * tid;
+                sh.above = before + (first ? 0 : h1);
+                sh.inside = first ? h1 : h0;
+            }
+            __syncthreads();
+            lo += (uint32_t)sh.bucket << shift;
+            need -= sh.above;
+            if (sh.inside == need || shift == 0) break;
+            shift = max(0, shift - 10);
         }
+        thr = lo;
     }
-    // Write in tile order: keys above the threshold all, keys equal to it from the lowest tile on.
-#pragma unroll
-    for (int i = 0; i < kSelRegKeys; ++i) {
-        const unsigned mg = __ballot_sync(0xffffffffu, key[i] > thr), me = __ballot_sync(0xffffffffu, key[i] == thr);
-        if (lane == 0) sh.tally[i * kSelWarps + warp] = __popc(mg) | __popc(me) << 16;
-    }
-    __syncthreads();
-    static_assert(kSelRegKeys * kSelWarps == 128, "four tallies per lane");
-    const int4 four = reinterpret_cast<const int4*>(sh.tally)[lane];
-    int incl = four.x + four.y + four.z + four.w;
-    const int own = incl;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
-    }
-    const int need = n - (__shfl_sync(0xffffffffu, incl, 31) & 0xffff);  // tiles taken among those at the threshold
-    const int part = (warp & 3) > 0 ? four.x + ((warp & 3) > 1 ? four.y : 0) + ((warp & 3) > 2 ? four.z : 0) : 0;
-    const int mine = incl - own + part;  // tallies before (i, warp) when the lane holds that entry
+    // Write in tile order: keys above the threshold all, keys equal to it from
+    // the lowest tile on (all of them, unless the bucket was one key).
     const unsigned below = (1u << lane) - 1u;
+    if (REGS) {
 #pragma unroll
-    for (int i = 0; i < kSelRegKeys; ++i) {
-        if (i * kSelThreads >= T_) break;
-        const int before = __shfl_sync(0xffffffffu, mine, 2 * i + (warp >> 2));
-        const bool gt = key[i] > thr, eq = key[i] == thr;
-        const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-        const int g = (before & 0xffff) + __popc(mg & below), e = (before >> 16) + __popc(me & below);
-        if (gt || (eq && e < need)) {
-            const int t = tid + kSelThreads * i;
-            int4 x = __ldg(p.tiles + t);
-            x.w = t;
-            out[g + min(e, need)] = x;
+        for (int i = 0; i < kSelRegKeys; ++i) {
+            const uint32_t k = key[REGS ? i : 0];
+            const unsigned mg = __ballot_sync(0xffffffffu, k > thr), me = __ballot_sync(0xffffffffu, k == thr);
+            if (lane == 0) sh.tally[i * kSelWarps + warp] = __popc(mg) | __popc(me) << 16;
         }
-    }
-    for (int i = n + tid; i < p.n_select; i += kSelThreads) out[i] = make_int4(0, 0, 0, -1);
-}
-
-// The same for any number of tiles: a bit a round, the scores read again from
-// the workspace (L2) for each.
-__device__ __forceinline__ void select_in_memory(const SelectParams& p, const float* scores, int4* out, SelShared& sh) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int T_ = p.n_tiles;
-    auto key_at = [&](int t) { return score_key(__ldcg(scores + t)); };
-    auto block_sum = [&](int c) {
-        c = __reduce_add_sync(0xffffffffu, c);
-        __syncthreads();  // the previous sum has been read
-        if (lane == 0) sh.count[0][warp] = c;
         __syncthreads();
-        c = 0;
+        static_assert(kSelRegKeys * kSelWarps == 128, "four tallies per lane");
+        const int4 four = reinterpret_cast<const int4*>(sh.tally)[lane];
+        int incl = four.x + four.y + four.z + four.w;
+        const int own = incl;
 #pragma unroll
-        for (int w = 0; w < kSelWarps; ++w) c += sh.count[0][w];
-        return c;
-    };
-    int visible = 0;
-    for (int t = tid; t < T_; t += kSelThreads) visible += key_at(t) != 0u;
-    visible = block_sum(visible);
-    const int n = min(p.n_select, visible);
-    uint32_t thr = 1u;
-    if (n < visible) {
-        thr = 0u;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t cand = thr | (1u << bit);
-            int c = 0;
-            for (int t = tid; t < T_; t += kSelThreads) c += key_at(t) >= cand;
-            c = block_sum(c);
-            if (c >= n) thr = cand;
-            if (c == n) break;
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += v;
         }
-    }
-    // each warp owns a run of tiles
-    const int run = ((T_ + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-    const int r0 = min(warp * run, T_), r1 = min(r0 + run, T_);
-    int gt = 0, eq = 0;
-    for (int t = r0 + lane; t < r1; t += 32) {
-        const uint32_t k = key_at(t);
-        gt += k > thr;
-        eq += k == thr;
-    }
-    gt = __reduce_add_sync(0xffffffffu, gt);
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    if (lane == 0) {
-        sh.tally[warp] = gt;
-        sh.tally[kSelWarps + warp] = eq;
-    }
-    __syncthreads();
-    int gt_before = 0, eq_before = 0, gt_all = 0;
+        const int need = n - (__shfl_sync(0xffffffffu, incl, 31) & 0xffff);  // taken among those at the threshold
+        const int w3 = warp & 3;
+        const int part = (w3 > 0 ? four.x : 0) + (w3 > 1 ? four.y : 0) + (w3 > 2 ? four.z : 0);
+        const int mine = incl - own + part;  // tallies before (i, warp), in the lane that holds that entry
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) {
-        if (w < warp) {
-            gt_before += sh.tally[w];
-            eq_before += sh.tally[kSelWarps + w];
+        for (int i = 0; i < kSelRegKeys; ++i) {
+            if (i * kSelThreads >= T_) break;
+            const uint32_t k = key[REGS ? i : 0];
+            const int before = __shfl_sync(0xffffffffu, mine, (i * kSelWarps + warp) >> 2);
+            const bool gt = k > thr, eq = k == thr;
+            const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+            const int g = (before & 0xffff) + __popc(mg & below), e = (before >> 16) + __popc(me & below);
+            if (gt || (eq && e < need)) {
+                const int t = tid + kSelThreads * i;
+                int4 x = __ldg(p.tiles + t);
+                x.w = t;
+                out[g + min(e, need)] = x;
+            }
         }
-        gt_all += sh.tally[w];
-    }
-    const int need = n - gt_all;
-    const unsigned below = (1u << lane) - 1u;
-    for (int t0 = r0; t0 < r1; t0 += 32) {
-        const int t = t0 + lane;
-        const uint32_t k = t < r1 ? key_at(t) : 0u;
-        const bool is_gt = t < r1 && k > thr, is_eq = t < r1 && k == thr;
-        const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-        const int g = gt_before + __popc(mg & below), e = eq_before + __popc(me & below);
-        if (is_gt || (is_eq && e < need)) {
-            int4 x = __ldg(p.tiles + t);
-            x.w = t;
-            out[g + min(e, need)] = x;
+    } else {
+        // each warp owns a run of tiles
+        const int run = ((T_ + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
+        const int r0 = min(warp * run, T_), r1 = min(r0 + run, T_);
+        int gt = 0, eq = 0;
+        for (int t = r0 + lane; t < r1; t += 32) {
+            const uint32_t k = score_key(__ldcg(scores + t));
+            gt += k > thr;
+            eq += k == thr;
         }
-        gt_before += __popc(mg);
-        eq_before += __popc(me);
+        gt = __reduce_add_sync(0xffffffffu, gt);
+        eq = __reduce_add_sync(0xffffffffu, eq);
+        if (lane == 0) {
+            sh.tally[warp] = gt;
+            sh.tally[kSelWarps + warp] = eq;
+        }
+        __syncthreads();
+        int gt_before = 0, eq_before = 0, gt_all = 0;
+#pragma unroll
+        for (int w = 0; w < kSelWarps; ++w) {
+            if (w < warp) {
+                gt_before += sh.tally[w];
+                eq_before += sh.tally[kSelWarps + w];
+            }
+            gt_all += sh.tally[w];
+        }
+        const int need = n - gt_all;
+        for (int t0 = r0; t0 < r1; t0 += 32) {
+            const int t = t0 + lane;
+            const uint32_t k = t < r1 ? score_key(__ldcg(scores + t)) : 0u;
+            const bool is_gt = t < r1 && k > thr, is_eq = t < r1 && k == thr;
+            const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+            const int g = gt_before + __popc(mg & below), e = eq_before + __popc(me & below);
+            if (is_gt || (is_eq && e < need)) {
+                int4 x = __ldg(p.tiles + t);
+                x.w = t;
+                out[g + min(e, need)] = x;
+            }
+            gt_before += __popc(mg);
+            eq_before += __popc(me);
+        }
     }
     for (int i = n + tid; i < p.n_select; i += kSelThreads) out[i] = make_int4(0, 0, 0, -1);
 }
 
-// Eight lanes score a tile, 32 tiles at a time per CTA; the tile's bounds are
-// requested before the wait for q (they never come from the kernel that this
-// launch overlaps: packing and bounding are launched without that overlap).
+// Eight lanes score kTilesPerLane tiles side by side (each q pair fetched from
+// shared memory serves all of them), kPassTiles at a time per CTA. The first
+// pass's bounds are requested before the wait for q: they never come from the
+// kernel that this launch overlaps (packing and bounding are launched without
+// that overlap).
+constexpr int kTilesPerLane = 2;
+constexpr int kPassTiles = kSelWarps * 4 * kTilesPerLane;
+
+// A bound as a double has an empty low word (8 or 11 significant bits), so the
+// choice between lo and hi by the sign of q is one word.
+__device__ __forceinline__ double pick(bool up, int hi_hi, int hi_lo) { return __hiloint2double(up ? hi_hi : hi_lo, 0); }
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
     constexpr int NV = D / 64;  // vectors of 8 channels per lane
+    constexpr int U = kTilesPerLane;
     __shared__ double2 qs[kHeadsPerPass * D / 2];
     __shared__ SelShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -288,14 +293,19 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         if (t < t_end) f.e = __ldg(p.tiles + t);
         if ((f.e.x & (kTile - 1)) != 0 || f.e.x < 0 || f.e.x / kTile >= p.tile_slots) {
             atomicExch(p.error, kDevErrBadTable);
-            f.e.z = 0;
+            f.e.x = f.e.z = 0;
+        }
+        const size_t slot = (size_t)bh * p.tile_slots + f.e.x / kTile;
+        const char* base = static_cast<const char*>(p.bounds) + slot * 2 * D * sizeof(T);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {  // lanes read consecutive vectors
+            f.lo[v].clear();
+            f.hi[v].clear();
         }
         if (f.e.z > 0) {
-            const size_t slot = (size_t)bh * p.tile_slots + f.e.x / kTile;
             if (sizeof(T) == 1) f.sk = __ldg(p.scales + slot).x;
-            const char* base = static_cast<const char*>(p.bounds) + slot * 2 * D * sizeof(T);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {  // lanes read consecutive vectors
+            for (int v = 0; v < NV; ++v) {
                 const int d0 = 8 * (l8 + 8 * v);
                 f.lo[v].load(base + d0 * sizeof(T));
                 f.hi[v].load(base + (D + d0) * sizeof(T));
@@ -303,17 +313,17 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         }
         return f;
     };
-    Fetched next = fetch(t_begin + 4 * warp + sub);
+    const int t_lane = t_begin + U * (4 * warp + sub);
+    Fetched f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) f[u] = fetch(t_lane + u);
 
     griddep_wait();  // q, the step state and the workspace may belong to the kernel this one overlaps
     griddep_launch_dependents();
     const int qpos = (p.dyn != nullptr ? p.dyn[RFSN_STEP_POS] : p.q_pos0) + row;
     for (int g0 = 0; g0 < p.G; g0 += kHeadsPerPass) {
         const int heads = min(kHeadsPerPass, p.G - g0);
-        if (g0 > 0) {
-            __syncthreads();
-            next = fetch(t_begin + 4 * warp + sub);
-        }
+        if (g0 > 0) __syncthreads();
         for (int i = tid; i < kHeadsPerPass * D / 2; i += kSelThreads) {
             // pairs of channels 8 (l8 + 8 v) + 2 j, + 1 of a head at [head][4 v + j][l8]: lanes side by side
             const int g = i / (D / 2), pr = i % (D / 2);
@@ -325,50 +335,64 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
             qs[i] = make_double2((double)x.x, (double)x.y);
         }
         __syncthreads();
-        for (int t0 = t_begin; t0 < t_end; t0 += kSelWarps * 4) {
-            const int t = t0 + 4 * warp + sub;
-            const Fetched f = next;
-            if (t0 + kSelWarps * 4 < t_end) next = fetch(t + kSelWarps * 4);
-            const bool live = t < t_end && f.e.z > 0 && f.e.y <= qpos;
-            double acc[kHeadsPerPass];
+        for (int t0 = 0; t_begin + t0 < t_end; t0 += kPassTiles) {
+            if (t0 > 0 || g0 > 0) {
 #pragma unroll
-            for (int g = 0; g < kHeadsPerPass; ++g) acc[g] = 0.0;
-            if (live) {
+                for (int u = 0; u < U; ++u) f[u] = fetch(t_lane + t0 + u);
+            }
+            double acc[U][kHeadsPerPass];
 #pragma unroll
-                for (int v = 0; v < NV; ++v)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const double l0 = (double)f.lo[v].get(2 * j), h0 = (double)f.hi[v].get(2 * j);
-                        const double l1 = (double)f.lo[v].get(2 * j + 1), h1 = (double)f.hi[v].get(2 * j + 1);
+                for (int g = 0; g < kHeadsPerPass; ++g) acc[u][g] = 0.0;
 #pragma unroll
-                        for (int g = 0; g < kHeadsPerPass; ++g) {
-                            const double2 q2 = qs[g * (D / 2) + (4 * v + j) * 8 + l8];
-                            acc[g] += q2.x * (q2.x >= 0.0 ? h0 : l0);
-                            acc[g] += q2.y * (q2.y >= 0.0 ? h1 : l1);
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    int lo0[U], hi0[U], lo1[U], hi1[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        lo0[u] = __double2hiint((double)f[u].lo[v].get(2 * j));
+                        hi0[u] = __double2hiint((double)f[u].hi[v].get(2 * j));
+                        lo1[u] = __double2hiint((double)f[u].lo[v].get(2 * j + 1));
+                        hi1[u] = __double2hiint((double)f[u].hi[v].get(2 * j + 1));
+                    }
+#pragma unroll
+                    for (int g = 0; g < kHeadsPerPass; ++g) {
+                        const double2 q2 = qs[g * (D / 2) + (4 * v + j) * 8 + l8];
+                        const bool up0 = q2.x >= 0.0, up1 = q2.y >= 0.0;
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            acc[u][g] += q2.x * pick(up0, hi0[u], lo0[u]);
+                            acc[u][g] += q2.y * pick(up1, hi1[u], lo1[u]);
                         }
                     }
-            }
+                }
             // Sums over the 8 lanes, halving the heads a lane carries: lanes end with head 2 (l8 / 4) + (l8 / 2) % 2.
             static_assert(kHeadsPerPass == 4, "two halvings");
             const bool up4 = l8 & 4, up2 = l8 & 2;
-            const double s0 = __shfl_xor_sync(0xffffffffu, up4 ? acc[0] : acc[2], 4);
-            const double s1 = __shfl_xor_sync(0xffffffffu, up4 ? acc[1] : acc[3], 4);
-            const double a0 = (up4 ? acc[2] : acc[0]) + s0, a1 = (up4 ? acc[3] : acc[1]) + s1;
-            double a = (up2 ? a1 : a0) + __shfl_xor_sync(0xffffffffu, up2 ? a0 : a1, 2);
-            a += __shfl_xor_sync(0xffffffffu, a, 1);
             const int head = (up4 ? 2 : 0) + (up2 ? 1 : 0);
-            float best = head < heads ? (float)(a * (double)f.sk) : -CUDART_INF_F;
-            unsigned nan = __ballot_sync(0xffffffffu, best != best);
-            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
-            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-            if (l8 == 0 && t < t_end) {
-                if ((nan >> (8 * sub)) & 0xffu) best = CUDART_NAN_F;
-                if (!live) best = -CUDART_INF_F;
-                if (g0 > 0) {  // heads of the earlier passes
-                    const float prev = scores[t];
-                    best = (prev != prev || best != best) ? CUDART_NAN_F : fmaxf(prev, best);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int t = t_lane + t0 + u;
+                const double s0 = __shfl_xor_sync(0xffffffffu, up4 ? acc[u][0] : acc[u][2], 4);
+                const double s1 = __shfl_xor_sync(0xffffffffu, up4 ? acc[u][1] : acc[u][3], 4);
+                const double a0 = (up4 ? acc[u][2] : acc[u][0]) + s0, a1 = (up4 ? acc[u][3] : acc[u][1]) + s1;
+                double a = (up2 ? a1 : a0) + __shfl_xor_sync(0xffffffffu, up2 ? a0 : a1, 2);
+                a += __shfl_xor_sync(0xffffffffu, a, 1);
+                float best = head < heads ? (float)(a * (double)f[u].sk) : -CUDART_INF_F;
+                const unsigned nan = __ballot_sync(0xffffffffu, best != best);
+                best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+                best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+                if (l8 == 0 && t < t_end) {
+                    if ((nan >> (8 * sub)) & 0xffu) best = CUDART_NAN_F;
+                    if (f[u].e.z <= 0 || f[u].e.y > qpos) best = -CUDART_INF_F;
+                    if (g0 > 0) {  // heads of the earlier passes
+                        const float prev = scores[t];
+                        best = (prev != prev || best != best) ? CUDART_NAN_F : fmaxf(prev, best);
+                    }
+                    scores[t] = best;
                 }
-                scores[t] = best;
             }
         }
     }
@@ -380,9 +404,9 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
     }
     int4* out = p.out + (size_t)list * p.n_select;
     if (p.n_tiles <= kSelRegKeys * kSelThreads)
-        select_in_registers(p, scores, out, sh);
+        select_list<true>(p, scores, out, sh);
     else
-        select_in_memory(p, scores, out, sh);
+        select_list<false>(p, scores, out, sh);
     if (gridDim.x > 1 && tid == 0) p.counters[list] = 0;
 }
 
