@@ -493,8 +493,10 @@ RFSN_API rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* archive, int sr
  *   - the archived keys are the listed tiles: of `packed` when it is given
  *     (K = code * scale, V = code * scale), else of `arena` itself;
  *   - the hot window is always `arena`'s (the cache's 16-bit type);
- *   - head_dim 64 or 128, bf16/f16 arenas; any q_len and GQA ratio, with
- *     K/V read again for every 8 query slots (q_len * q_heads / kv_heads).
+ *   - head_dim 64 or 128, bf16/f16 arenas; any q_len and GQA ratio. From 64
+ *     query slots (q_len * q_heads / kv_heads) on, a packed archive with
+ *     head_dim 128 runs the tcgen05 kernel; else K/V are read again for every
+ *     8 query slots.
  * Scores are accurate to float32 rounding (q and p are split into two float16
  * or three bfloat16 terms for the tensor cores).
  * ---------------------------------------------------------------------- */
@@ -565,10 +567,11 @@ RFSN_API rfsn_status rfsn_archive_attend(const rfsn_archive_call* call, const fl
 
 /* Workspace bytes of rfsn_archive_attention (n_select = 0: shared lists;
  * > 0: lists per query), rfsn_select_tiles (n_select > 0) and
- * rfsn_archive_attend (n_select = top_tiles) over up to n_tiles tiles. Conventions as for rfsn_attention_workspace_size; one workspace
+ * rfsn_archive_attend (n_select = top_tiles) over up to n_tiles tiles and a
+ * hot window of up to hot_capacity tokens. Conventions as for rfsn_attention_workspace_size; one workspace
  * serves all attention calls ordered on one stream. */
 RFSN_API rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim,
-                                                 int n_tiles, int n_select, size_t* bytes);
+                                                 int hot_capacity, int n_tiles, int n_select, size_t* bytes);
 
 /* Reads the device error word of a workspace (after synchronising `stream`,
  * bounded by timeout_us) and clears it. RFSN_ERR_DEVICE if a kernel set it. */

@@ -23,6 +23,8 @@ struct rfsn_packed_archive {
 namespace rfsn {
 namespace archive {
 
+constexpr float kPScale = 128.f;  // p <= 2^8 (kLazy), p * 2^7 <= 2^15 fits float16
+constexpr float kLazy = 8.f;      // log2 units the running maximum may be exceeded by before it moves
 constexpr int kStageBytes = 16384;              // one item: 64 packed keys, or 32 (head_dim 64: 64) 16-bit keys
 constexpr int kMaxSplits128 = 240, kMaxSplits64 = 120;  // bounded by the merge weights kept in shared memory
 
@@ -77,5 +79,13 @@ rfsn_status select_tiles_launch(int bounds_dtype, int head_dim, const archive::S
 int archive_attn_ctas(int nb);
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int nb, int zblocks, cudaStream_t stream);
+
+// archive_chunk.cu: chunks of queries over a packed archive, head_dim 128. Workspace: partials and a copy of the ring.
+bool archive_chunk_fits(int G);
+size_t archive_chunk_ws(int groups, int hot_capacity);
+rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& a,
+                                 int batch, void* workspace, size_t workspace_bytes, int max_splits,
+                                 cudaStream_t stream);
+void preload_chunk_kernels();
 
 }  // namespace rfsn

@@ -60,6 +60,13 @@ size_t attention_ws_limit(const SlotPlan& sp, int head_dim) {
     return attention_ws(sp, limit, head_dim).total;
 }
 
+// Chunks run on the tcgen05 kernel: it works on 128 query rows whatever the
+// call has, the tile kernel reads K/V again for every 8.
+constexpr int kChunkSlots = 64;
+bool chunk_shape(int head_dim, int G, int q_len) {
+    return head_dim == 128 && q_len * (long long)G >= kChunkSlots && archive_chunk_fits(G);
+}
+
 size_t select_scores_offset();
 
 // Selected lists of rfsn_archive_attend: behind everything its two kernels write.
@@ -121,6 +128,8 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     }
     st = check_device(arena->device, what);
     if (st != RFSN_OK) return st;
+    const bool chunk = packed != nullptr && tiles->per_query == 0 && !stepped && tiles->n > 0 &&
+                       chunk_shape(arena->head_dim, q_heads / kv_heads, q_len);
     const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, arena->head_dim, tiles->per_query != 0);
     RFSN_CHECK_ARG(sp.zblocks <= kMaxLists, "%s: too many query rows", what);
     const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
@@ -137,7 +146,7 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     // more than one split only where all lists leave SMs idle: far fewer lists than arrival counters
     RFSN_CHECK_ARG(splits == 1 || (long long)sp.lists * sp.zblocks <= kMaxCounters, "%s: too many lists", what);
     const WsLayout w = attention_ws(sp, splits, arena->head_dim);
-    if (w.total > workspace_bytes) {
+    if (!chunk && w.total > workspace_bytes) {
         set_error("%s: workspace too small: need %zu bytes, have %zu", what, w.total, workspace_bytes);
         return RFSN_ERR_OVERFLOW;
     }
@@ -169,6 +178,9 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     p.qscale = (float)(1.0 / std::sqrt((double)arena->head_dim)) * 1.4426950408889634f;
     p.ws = ws_view(workspace, w);
     p.dyn = hot->step_state;
+    if (chunk)
+        return archive_chunk_launch(arena, packed, p, batch, workspace, workspace_bytes, max_splits,
+                                    static_cast<cudaStream_t>(stream));
     return archive_attn_launch(arena, packed, p, sp.lists, sp.nb, sp.zblocks, static_cast<cudaStream_t>(stream));
 }
 
@@ -278,15 +290,18 @@ rfsn_status rfsn_tile_bounds(const rfsn_arena* arena, int row0, int count, void*
     return tile_bounds_launch(arena, row0, count, bounds, static_cast<cudaStream_t>(stream));
 }
 
-rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim, int n_tiles,
-                                        int n_select, size_t* bytes) {
+rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim,
+                                        int hot_capacity, int n_tiles, int n_select, size_t* bytes) {
     RFSN_CHECK_ARG(bytes != nullptr, "rfsn_archive_workspace_size: bytes is NULL");
     rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, "rfsn_archive_workspace_size");
     if (st != RFSN_OK) return st;
-    RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0, "rfsn_archive_workspace_size: negative tile count");
+    RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0 && hot_capacity >= 0,
+                   "rfsn_archive_workspace_size: negative count");
     const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, n_select > 0);
     size_t need = attention_ws_limit(sp, head_dim);
     if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
+    else if (chunk_shape(head_dim, q_heads / kv_heads, q_len))
+        need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity));
     *bytes = need;
     return RFSN_OK;
 }

@@ -42,9 +42,6 @@
 namespace rfsn {
 namespace archive {
 
-constexpr float kPScale = 128.f;  // p <= 2^8 (kLazy), p * 2^7 <= 2^15 fits float16
-constexpr float kLazy = 8.f;      // log2 units
-
 template <int D> struct Geometry {
     static constexpr int kHotKeys = D == 128 ? 32 : 64;   // 16-bit keys per item
     static constexpr int kItemsPerTile16 = kTile / kHotKeys;
@@ -875,6 +872,7 @@ void preload_archive_kernels() {
     using namespace archive;
     preload_pack_kernels();
     preload_select_kernels();
+    preload_chunk_kernels();
     preload<__nv_bfloat16, 128>();
     preload<__nv_bfloat16, 64>();
     preload<__half, 128>();

@@ -247,7 +247,7 @@ def load_library() -> ctypes.CDLL:
         "rfsn_archive_attention": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, ctypes.POINTER(TileListC),
                                          ctypes.POINTER(HotWindowC), vp, vp, vp, sz, i32, vp]),
         "rfsn_archive_attend": (i32, [ctypes.POINTER(ArchiveCallC), vp, i32, vp, vp, vp, sz, vp]),
-        "rfsn_archive_workspace_size": (i32, [i32] * 7 + [ctypes.POINTER(sz)]),
+        "rfsn_archive_workspace_size": (i32, [i32] * 8 + [ctypes.POINTER(sz)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -170,12 +170,12 @@ class PackedArchive:
 
 
 @lru_cache(maxsize=4096)
-def workspace_bytes(batch: int, q_heads: int, kv_heads: int, q_len: int, head_dim: int, n_tiles: int,
-                    n_select: int = 0) -> int:
+def workspace_bytes(batch: int, q_heads: int, kv_heads: int, q_len: int, head_dim: int, hot_capacity: int,
+                    n_tiles: int, n_select: int = 0) -> int:
     out = ctypes.c_size_t()
     native.check(
-        native.load_library().rfsn_archive_workspace_size(batch, q_heads, kv_heads, q_len, head_dim, n_tiles, n_select,
-                                                          ctypes.byref(out)),
+        native.load_library().rfsn_archive_workspace_size(batch, q_heads, kv_heads, q_len, head_dim, hot_capacity,
+                                                          n_tiles, n_select, ctypes.byref(out)),
         "rfsn_archive_workspace_size",
     )
     return int(out.value)
@@ -200,7 +200,8 @@ def select_tiles(cache, q: torch.Tensor, q_start_pos: int, segments, top_tiles: 
     tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
     out = torch.empty((B, cache.num_kv_heads, Lq, top_tiles, 4), dtype=torch.int32, device=cache.device)
     ws = workspace if workspace is not None else native.default_workspace(cache.device)
-    buf = ws.get(workspace_bytes(B, H, cache.num_kv_heads, Lq, D, n_tiles, top_tiles))
+    buf = ws.get(workspace_bytes(B, H, cache.num_kv_heads, Lq, D, cache.config.hot_capacity, n_tiles,
+                                 top_tiles))
     bounds = cache.tile_bounds
     packed = cache.archive is not None
     native.check(
@@ -233,7 +234,7 @@ class PreparedCall:
             cache.batch_size, q_heads, cache.num_kv_heads, q_len, top_tiles, max_splits)
         self.ref = ctypes.byref(call)
         self.nbytes = workspace_bytes(cache.batch_size, q_heads, cache.num_kv_heads, q_len, cache.config.head_dim,
-                                      n_tiles, top_tiles if n_tiles else 0)
+                                      cache.config.hot_capacity, n_tiles, top_tiles if n_tiles else 0)
         self.keep = (call, cache.arena, archive, bounds, tiles_dev)
 
     def __call__(self, cache, q_ptr: int, q_start_pos: int, out_ptr: int, lse_ptr: Optional[int],

@@ -373,8 +373,6 @@ class LayerKVCache:
         self.tile_bounds: Optional[torch.Tensor] = None
         self._tiles_dev: Optional[torch.Tensor] = None
         self._n_tiles = 0
-        self._table_serial = 0  # counts page-table refreshes
-        self._pass_cache: Optional[tuple] = None
         if not self._whole_tiles:
             self._alloc = _RowAllocator(cap, cap + max(pool, 1))
             self._make_arena(cap + max(pool, 1))
@@ -1022,7 +1020,6 @@ class LayerKVCache:
             self._table_dev = self._ops.new_table(max(records.shape[0], 2 * self._table_dev.shape[0]))
         self._table_dev[: records.shape[0]].copy_(torch.from_numpy(records))
         if self._whole_tiles:
-            self._table_serial += 1
             self._refresh_tiles(records)
         self._attended, self._attended_spans = attended, spans
         self._table_meta = (len(spans), sum(n for _, _, n in spans), tile)
@@ -1044,39 +1041,6 @@ class LayerKVCache:
                                                       else 2 * self._tiles_dev.shape[0]))
         self._tiles_dev[:len(tiles)].copy_(torch.from_numpy(tiles))
         self._n_tiles = len(tiles)
-
-    def pass_tables(self, spans: list, row0: int, keys: int) -> tuple[list, torch.Tensor]:
-        """The archived spans as page tables of at most ``keys`` tokens each, for
-        rows shifted by ``row0``: [(first record, records, tokens, tiles)] and the
-        device records (kept until the page table changes)."""
-        key = (self._table_serial, row0, keys, len(spans))
-        if self._pass_cache is not None and self._pass_cache[0] == key:
-            return self._pass_cache[1]
-        passes, records, blocks, room = [], [], [], keys
-        for row, start, n in spans:
-            at = 0
-            while at < n:
-                take = min(room, n - at)
-                blocks.append((row0 + row + at, start + at, take))
-                at += take
-                room -= take
-                if room == 0:
-                    passes.append(blocks)
-                    blocks, room = [], keys
-        if blocks:
-            passes.append(blocks)
-        out = []
-        for blocks in passes:
-            first, tile = len(records), 0
-            for row, start, n in blocks:
-                records.append((row, start, n, tile))
-                tile += _tiles(n)
-            records.append((0, 0, 0, tile))
-            out.append((first, len(blocks), sum(n for _, _, n in blocks), tile))
-        dev = self._ops.new_table(len(records))
-        dev.copy_(torch.tensor(records, dtype=torch.int32))
-        self._pass_cache = (key, (out, dev))
-        return out, dev
 
     def tile_snapshot(self) -> tuple[Optional[torch.Tensor], int]:
         """Device tile list of the attended archived blocks and its length (packed
@@ -1203,71 +1167,6 @@ def _query(cache: LayerKVCache, q: torch.Tensor) -> torch.Tensor:
     return _as(q, cache.device, torch.float32)
 
 
-# Keys of one pass of _unpacked_attention. The prefill kernel adds every tile's
-# P V to one float32 accumulator on the tensor cores, whose rounding error grows
-# with the number of additions: 4e-5 of the result over 17K keys, about 5e-6
-# over 2K. Shorter passes cost launches (512 queries x 17K keys: see
-# _unpacked_attention).
-_PASS_KEYS = 2048
-_MERGE_PARTS = 8
-_CHUNK_ROWS = 64  # query rows from which the tensor-core prefill kernel runs (head_dim 128)
-
-
-def _unpacked_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segments: PagedSegments,
-                        out_ptr: int, lse: Optional[torch.Tensor], hot: native.HotWindowC,
-                        workspace: Optional[native.Workspace]) -> None:
-    """A prompt chunk over a packed cache: products outweigh bytes, so the
-    archive's used rows are unpacked once, behind a copy of the ring, into a
-    temporary arena in the cache dtype that the tensor-core prefill kernel
-    reads, in passes of at most ``_PASS_KEYS`` archived keys (the last one with
-    the ring) merged by their log-sum-exps in float32."""
-    cap, archive = cache._ring_rows, cache.archive
-    spans = segments.spans[:segments.n_archived]
-    used = max(row + n for row, _, n in spans)
-    k = torch.empty((archive.groups, cap + used, archive.head_dim), dtype=cache.dtype, device=cache.device)
-    v = torch.empty_like(k)
-    k[:, :cap].copy_(cache._arena_k[:, :cap])
-    v[:, :cap].copy_(cache._arena_v[:, :cap])
-    archive.unpack(0, used, cache.dtype, out=(k[:, cap:], v[:, cap:]))
-    arena = native.Arena(k, v)
-    passes, records = cache.pass_tables(spans, cap, _PASS_KEYS)
-    B, H, Lq, D = (int(x) for x in q.shape)
-    rows = B * H * Lq
-    ws = workspace if workspace is not None else native.default_workspace(cache.device)
-    buf = ws.get(native.workspace_bytes(B, H, cache.num_kv_heads, Lq, D, 0))
-    parts = min(len(passes), _MERGE_PARTS)
-    no_hot = native.HotWindowC(0, cap, 0, 0, 0, 0, None)
-    o = torch.empty((parts, rows, D), dtype=torch.float32, device=cache.device) if parts > 1 else None
-    m = torch.empty((parts, rows), dtype=torch.float32, device=cache.device) if parts > 1 else None
-    lse_ptr = lse.data_ptr() if lse is not None else None
-    filled = 0
-    for i, (first, n, tokens, tiles) in enumerate(passes):
-        last = i == len(passes) - 1
-        table = native.PageTableC(records.data_ptr() + 16 * first, n, tokens, tiles, 0)
-        native.check(
-            native.lib().rfsn_paged_attention(
-                arena.handle, q.data_ptr(), B, H, cache.num_kv_heads, Lq, int(q_start_pos),
-                native.ctypes.byref(table), native.ctypes.byref(hot if last else no_hot),
-                o[filled].data_ptr() if parts > 1 else out_ptr, m[filled].data_ptr() if parts > 1 else lse_ptr,
-                buf.data_ptr(), buf.numel(), 0, native.stream_ptr()),
-            "rfsn_paged_attention",
-        )
-        filled += 1
-        if parts == 1 or not (last or filled == parts):
-            continue
-        if last:
-            dst, dst_lse = out_ptr, lse_ptr
-        else:  # more passes than parts: what is merged becomes the first part of the next merge
-            merged, merged_lse = torch.empty_like(o[0]), torch.empty_like(m[0])
-            dst, dst_lse = merged.data_ptr(), merged_lse.data_ptr()
-        native.check(native.lib().rfsn_lse_merge(o.data_ptr(), m.data_ptr(), filled, rows, D, dst, dst_lse,
-                                                 native.stream_ptr()), "rfsn_lse_merge")
-        if not last:
-            o[0].copy_(merged)
-            m[0].copy_(merged_lse)
-            filled = 1
-
-
 def _out_pointer(cache: LayerKVCache, out: torch.Tensor, shape: tuple) -> int:
     if out.dtype != torch.float32 or tuple(out.shape) != shape or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
@@ -1306,7 +1205,7 @@ def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
         out_ptr = out.data_ptr()
     else:
         out_ptr = _out_pointer(cache, out, tuple(qf.shape))
-    _, H, Lq, D = qf.shape
+    _, H, Lq, _ = qf.shape
     lse = torch.empty(qf.shape[:3], dtype=torch.float32, device=cache.device) if want_lse else None
     key = (H, Lq, top_tiles, max_splits)
     call = segments.calls.get(key) if step_state is None else None
@@ -1314,10 +1213,6 @@ def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
         if top_tiles < 0 or (top_tiles and cache.tile_bounds is None):
             raise ValueError("top_tiles needs a cache built with tile_index=True and a count >= 0")
         hot = _hot_window(cache, segments, step_state)
-        if not top_tiles and segments.n_archived and step_state is None and Lq >= _CHUNK_ROWS and D == 128:
-            with native.on_device(cache.device):
-                _unpacked_attention(cache, qf, q_start_pos, segments, out_ptr, lse, hot, workspace)
-            return (out, lse) if want_lse else out
         call = PreparedCall(cache, segments, hot, H, Lq, int(top_tiles), max_splits)
         if step_state is None and segments.hot_state is not None:
             segments.calls[key] = call

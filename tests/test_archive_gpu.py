@@ -197,8 +197,14 @@ CASES = [
     ("float16", 1, 6, 2, 128, (), 100, 40, 1),         # nothing archived
     ("bfloat16", 1, 4, 4, 128, (900, 130), 0, 0, 1),   # nothing hot
     ("float16", 3, 4, 2, 64, (1,), 1, 0, 1),
-    ("bfloat16", 1, 32, 8, 128, (512,) * 20 + (77,), 500, 400, 20),   # long chunk: unpacked
-    ("float16", 1, 32, 8, 128, (512, 33), 256, 0, 200),               # tensor-core prefill over unpacked tiles
+    # chunks of 64 query slots and more: the tcgen05 kernel
+    ("bfloat16", 1, 32, 8, 128, (512,) * 20 + (77,), 500, 400, 20),
+    ("float16", 1, 32, 8, 128, (512, 33), 256, 0, 200),
+    ("bfloat16", 2, 6, 2, 128, (64, 1, 130), 100, 33, 41),            # 3 heads per KV head: 126 of 128 rows used
+    ("bfloat16", 1, 4, 4, 128, (70,), 128, 100, 128),                 # no GQA
+    ("float16", 1, 32, 1, 128, (1, 63), 1, 0, 2),                     # 32 heads per KV head
+    ("bfloat16", 1, 8, 8, 128, (100,) * 3, 0, 0, 70),                 # nothing hot
+    ("bfloat16", 1, 16, 2, 128, (900,) * 9, 2000, 700, 16),           # few units: the keys are split
     ("bfloat16", 1, 8, 4, 64, (300,), 64, 0, 50),
 ]
 
