@@ -494,9 +494,9 @@ RFSN_API rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* archive, int sr
  *     (K = code * scale, V = code * scale), else of `arena` itself;
  *   - the hot window is always `arena`'s (the cache's 16-bit type);
  *   - head_dim 64 or 128, bf16/f16 arenas; any q_len and GQA ratio. From 64
- *     query slots (q_len * q_heads / kv_heads) on, a packed archive with
- *     head_dim 128 runs the tcgen05 kernel; else K/V are read again for every
- *     8 query slots.
+ *     query slots (q_len * q_heads / kv_heads) on, 24 over 256 tiles and more,
+ *     a packed archive with head_dim 128 runs the tcgen05 kernel; else K/V are
+ *     read again for every 8 query slots.
  * Scores are accurate to float32 rounding (q and p are split into two float16
  * or three bfloat16 terms for the tensor cores).
  * ---------------------------------------------------------------------- */

@@ -75,7 +75,7 @@ void preload_pack_kernels();
 void preload_select_kernels();
 rfsn_status select_tiles_launch(int bounds_dtype, int head_dim, const archive::SelectParams& p, int lists, int chunks,
                                 cudaStream_t stream);
-// archive_attn.cu: nb = column blocks of 4 query slots per CTA (1, 2 or 4); CTAs per SM of that variant
+// archive_attn.cu: nb = column blocks of 4 query slots per CTA (1 or 2); CTAs per SM of that variant
 int archive_attn_ctas(int nb);
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int nb, int zblocks, cudaStream_t stream);

@@ -27,12 +27,12 @@ struct SlotPlan {
     int lists, slots, nb, zblocks;
 };
 
-SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, int head_dim, bool per_query) {
+SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, bool per_query) {
     SlotPlan s;
     const int G = q_heads / kv_heads;
     s.lists = batch * kv_heads * (per_query ? q_len : 1);
     s.slots = per_query ? G : G * q_len;
-    s.nb = s.slots <= 4 ? 1 : s.slots <= 8 || head_dim == 128 ? 2 : 4;
+    s.nb = s.slots <= 4 ? 1 : 2;
     s.zblocks = (s.slots + 4 * s.nb - 1) / (4 * s.nb);
     return s;
 }
@@ -60,11 +60,16 @@ size_t attention_ws_limit(const SlotPlan& sp, int head_dim) {
     return attention_ws(sp, limit, head_dim).total;
 }
 
-// Chunks run on the tcgen05 kernel: it works on 128 query rows whatever the
-// call has, the tile kernel reads K/V again for every 8.
-constexpr int kChunkSlots = 64;
-bool chunk_shape(int head_dim, int G, int q_len) {
-    return head_dim == 128 && q_len * (long long)G >= kChunkSlots && archive_chunk_fits(G);
+// Chunks run on the tcgen05 kernel. It works on 128 query rows whatever the
+// call has and takes about 24 us at least; the tile kernel reads K/V again for
+// every 8 slots. Measured (32 q / 8 KV heads, us, tile / chunk kernel): 32
+// slots over 4K keys 16 / 24, 16K 37 / 38, 132K 217 / 141; 64 slots over 4K
+// 27 / 24, 16K 72 / 38.
+constexpr int kChunkSlots = 64, kChunkSlotsLong = 24, kChunkLongTiles = 256;
+bool chunk_shape(int head_dim, int G, int q_len, int n_tiles) {
+    const long long slots = q_len * (long long)G;
+    return head_dim == 128 && archive_chunk_fits(G) &&
+           (slots >= kChunkSlots || (slots >= kChunkSlotsLong && n_tiles >= kChunkLongTiles));
 }
 
 size_t select_scores_offset();
@@ -129,8 +134,8 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     st = check_device(arena->device, what);
     if (st != RFSN_OK) return st;
     const bool chunk = packed != nullptr && tiles->per_query == 0 && !stepped && tiles->n > 0 &&
-                       chunk_shape(arena->head_dim, q_heads / kv_heads, q_len);
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, arena->head_dim, tiles->per_query != 0);
+                       chunk_shape(arena->head_dim, q_heads / kv_heads, q_len, tiles->n);
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, tiles->per_query != 0);
     RFSN_CHECK_ARG(sp.zblocks <= kMaxLists, "%s: too many query rows", what);
     const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
     const int per_tile = packed != nullptr ? 1 : kTile / hk;
@@ -297,10 +302,10 @@ rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, in
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0 && hot_capacity >= 0,
                    "rfsn_archive_workspace_size: negative count");
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, n_select > 0);
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, n_select > 0);
     size_t need = attention_ws_limit(sp, head_dim);
     if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
-    else if (chunk_shape(head_dim, q_heads / kv_heads, q_len))
+    else if (chunk_shape(head_dim, q_heads / kv_heads, q_len, n_tiles))
         need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity));
     *bytes = need;
     return RFSN_OK;
@@ -377,7 +382,7 @@ rfsn_status rfsn_archive_attend(const rfsn_archive_call* c, const float* q, int 
     rfsn_status st = check_shape(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, what);
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(c->tiles.n > 0 && c->tiles.per_query == 0 && c->top_tiles <= (1 << 20), "%s: bad tile list", what);
-    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, true);
+    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, true);
     const size_t off = lists_offset(sp, head_dim, c->tiles.n);
     const size_t need = off + sizeof(int4) * (size_t)sp.lists * c->top_tiles;
     if (workspace == nullptr || workspace_bytes < need) {

@@ -785,19 +785,8 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
 
 // Launch shape by column blocks: consumer groups, stages and CTAs per SM.
 template <int NB> struct Shape;
-#ifndef RFSN_G1
-#define RFSN_G1 1
-#define RFSN_S1 6
-#define RFSN_C1 2
-#endif
-template <> struct Shape<1> { static constexpr int kGroups = RFSN_G1, kStages = RFSN_S1, kCtas = RFSN_C1; };
-#ifndef RFSN_G2
-#define RFSN_G2 2
-#define RFSN_S2 8
-#define RFSN_C2 1
-#endif
-template <> struct Shape<2> { static constexpr int kGroups = RFSN_G2, kStages = RFSN_S2, kCtas = RFSN_C2; };
-template <> struct Shape<4> { static constexpr int kGroups = 2, kStages = 8, kCtas = 1; };
+template <> struct Shape<1> { static constexpr int kGroups = 1, kStages = 6, kCtas = 2; };
+template <> struct Shape<2> { static constexpr int kGroups = 2, kStages = 8, kCtas = 1; };
 
 template <typename T, int D, int NB, bool PACKED>
 rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const Params& p, int lists, int zblocks,
@@ -829,9 +818,6 @@ template <typename T, int D>
 rfsn_status launch_nb(const rfsn_arena* a, const rfsn_packed_archive* pk, const Params& p, int lists, int nb, int zb,
                       cudaStream_t s) {
     if (nb == 1) return launch_packed<T, D, 1>(a, pk, p, lists, zb, s);
-    if constexpr (D == 64) {  // head_dim 128: the accumulators of 16 slots do not fit the registers
-        if (nb == 4) return launch_packed<T, D, 4>(a, pk, p, lists, zb, s);
-    }
     return launch_packed<T, D, 2>(a, pk, p, lists, zb, s);
 }
 
@@ -847,14 +833,13 @@ template <typename T, int D>
 void preload() {
     preload_nb<T, D, 1>();
     preload_nb<T, D, 2>();
-    if constexpr (D == 64) preload_nb<T, D, 4>();
 }
 
 }  // namespace archive
 
 int archive_attn_ctas(int nb) {
     using namespace archive;
-    return nb == 1 ? Shape<1>::kCtas : nb == 2 ? Shape<2>::kCtas : Shape<4>::kCtas;
+    return nb == 1 ? Shape<1>::kCtas : Shape<2>::kCtas;
 }
 
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,

@@ -59,6 +59,7 @@ constexpr int kSoftmaxThreads = 256, kThreads = 512;
 // registers per thread of the two softmax warpgroups and of the two others: together the 512 x 128 of the launch
 constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;
 constexpr int kConvWarp = 8, kProducerWarp = 12, kMmaWarp = 13;
+constexpr int kMaxSplit = 32;  // key ranges of a unit
 constexpr uint32_t kTmemCols = 512, kColO = 256, kColQhi = 384, kColQlo = 448;
 
 struct Info {
@@ -80,7 +81,7 @@ struct Smem {
     float red[2][2][BM];
     Info info[kInfo];
     uint32_t tmem;
-    int abort, flag, n_arch, n_hot;
+    int abort, n_arch, n_hot;
 };
 
 struct Params {
@@ -126,8 +127,48 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                  : "memory");
 }
-// (a, b) -> two float16 (high parts) and two float16 (remainders)
-__device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint32_t& lo) {
+// Paired float32 arithmetic (PTX .f32x2): two results per issue slot, each rounded as the scalar operation.
+__device__ __forceinline__ uint64_t pair(float2 a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t r) {
+    float2 a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+    return a;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)), "l"(pair(c)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+    return unpair(r);
+}
+
+// (a, b) -> two float16 high parts and two float16 remainders. The high part
+// is the value cut to 11 significant bits (exact in float16, and no
+// conversion back is needed for the remainder), the remainder is exact in
+// float32 and rounded to 11 bits: 21 to 22 bits together. Below float16's
+// normal range bits are lost at 2^-25, 2^-32 of the largest p.
+__device__ __forceinline__ void split_half(float2 x, uint32_t& hi, uint32_t& lo) {
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u),
+                                 __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+    const float2 r = sub2(x, h);
+    hi = pack2<__half>(h.x, h.y);
+    lo = pack2<__half>(r.x, r.y);
+}
+
+// The same rounded to nearest: 24 bits. For q, which is split once per CTA: an error of q moves every logit of its row.
+__device__ __forceinline__ void split_half_rn(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = pack2<__half>(a, b);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     lo = pack2<__half>(a - f.x, b - f.y);
@@ -138,29 +179,40 @@ __device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint3
 // the upper channel half store their two chunks in the other order, so that
 // both the load and the stores meet every bank once. A half without keys is
 // zeroed (its staging holds an earlier tile).
-__device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, const Info& inf) {
+__device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, bool first, bool second) {
     const int th = threadIdx.x & 127, c = th & 7, r0 = th >> 3;
+    const int c0 = (2 * c) & 7, swap = c >> 2;
+    // rows r0 + 16 i share r & 7, so the swizzled chunk offsets are the thread's own
+    const uint32_t from = codes + r0 * 128 + ((c ^ (r0 & 7)) << 4);
+    const uint32_t to = op + (c >> 2) * kHalfBytes + r0 * 128;
+    const uint32_t to0 = to + (((c0 + swap) ^ (r0 & 7)) << 4), to1 = to + (((c0 + 1 - swap) ^ (r0 & 7)) << 4);
 #pragma unroll
-    for (int i = 0; i < BN / 16; ++i) {
-        const int r = r0 + 16 * i;
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
-        if (inf.len[r >> 6] > 0) {
-            const uint4 x = lds_u4(codes + r * 128 + ((c ^ (r & 7)) << 4));
-            a = make_uint4(widen(x.x), widen_hi(x.x), widen(x.y), widen_hi(x.y));
-            b = make_uint4(widen(x.z), widen_hi(x.z), widen(x.w), widen_hi(x.w));
+    for (int h = 0; h < 2; ++h) {  // the two 64-key halves, four loads in flight
+        uint4 x[4];
+        const bool any = h ? second : first;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = any ? lds_u4(from + (64 * h + 16 * i) * 128) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 a = make_uint4(widen(x[i].x), widen_hi(x[i].x), widen(x[i].y), widen_hi(x[i].y));
+            const uint4 b = make_uint4(widen(x[i].z), widen_hi(x[i].z), widen(x[i].w), widen_hi(x[i].w));
+            sts_u4(to0 + (64 * h + 16 * i) * 128, swap ? b : a);
+            sts_u4(to1 + (64 * h + 16 * i) * 128, swap ? a : b);
         }
-        const uint32_t row = op + (c >> 2) * kHalfBytes + r * 128;
-        const int c0 = (2 * c) & 7, swap = c >> 2;
-        sts_u4(row + (((c0 + swap) ^ (r & 7)) << 4), swap ? b : a);
-        sts_u4(row + (((c0 + 1 - swap) ^ (r & 7)) << 4), swap ? a : b);
     }
 }
 
 // A float16 tile that is already in the operand's layout.
 __device__ __forceinline__ void copy_tile(uint32_t from, uint32_t op) {
     const int th = threadIdx.x & 127;
-#pragma unroll 4
-    for (int i = 0; i < 2 * kHalfBytes / 16 / 128; ++i) sts_u4(op + (128 * i + th) * 16, lds_u4(from + (128 * i + th) * 16));
+#pragma unroll
+    for (int i = 0; i < 2 * kHalfBytes / 16 / 128; i += 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = lds_u4(from + (128 * (i + j) + th) * 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sts_u4(op + (128 * (i + j) + th) * 16, x[j]);
+    }
 }
 
 // This warp's generic-proxy writes to an operand buffer are done: visible to
@@ -232,6 +284,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = sm.tmem;
+    griddep_wait();  // q, the hot copy and the workspace belong to the kernels before
+    griddep_launch_dependents();
     // Tiles of 128 keys: archived pairs, then hot pairs; this split's share [t_lo, t_hi).
     const int arch_tiles = (sm.n_arch + 1) / 2, all_tiles = arch_tiles + (sm.n_hot + 1) / 2;
     const int t_lo = (int)((long long)split * all_tiles / p.nsplit);
@@ -252,9 +306,10 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                      warp_wait(&sm.c_full[slot & 1], (slot >> 1) & 1, &sm.abort) &&
                      (t < kStages || warp_wait(&sm.k_empty[s], ph ^ 1, &sm.abort));
                 if (!ok) break;
+                const bool first = sm.info[t % kInfo].len[0] > 0, second = sm.info[t % kInfo].len[1] > 0;
                 const uint32_t k_op = smem_u32(sm.k[s][0]), v_op = smem_u32(sm.v[s][0]);
                 if (arch) {
-                    convert_tile(smem_u32(sm.staged[slot & 1]), k_op, sm.info[t % kInfo]);
+                    convert_tile(smem_u32(sm.staged[slot & 1]), k_op, first, second);
                 } else {
                     copy_tile(smem_u32(sm.staged[slot & 1]), k_op);
                     __syncwarp();
@@ -266,7 +321,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                      (t < kStages || warp_wait(&sm.v_empty[s], ph ^ 1, &sm.abort));
                 if (!ok) break;
                 if (arch)
-                    convert_tile(smem_u32(sm.staged[slot & 1]) + kCodeBytes, v_op, sm.info[t % kInfo]);
+                    convert_tile(smem_u32(sm.staged[slot & 1]) + kCodeBytes, v_op, first, second);
                 else
                     copy_tile(smem_u32(sm.staged[slot & 1]), v_op);
                 publish(&sm.v_full[s]);
@@ -475,8 +530,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             uint32_t hi[32], lo[32];
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
-                split_half(x[c].x * up, x[c].y * up, hi[2 * c], lo[2 * c]);
-                split_half(x[c].z * up, x[c].w * up, hi[2 * c + 1], lo[2 * c + 1]);
+                split_half_rn(x[c].x * up, x[c].y * up, hi[2 * c], lo[2 * c]);
+                split_half_rn(x[c].z * up, x[c].w * up, hi[2 * c + 1], lo[2 * c + 1]);
             }
             tc::st_32x32b_x32(tmem + lane_base + kColQhi + 32 * ch, hi);
             tc::st_32x32b_x32(tmem + lane_base + kColQlo + 32 * ch, lo);
@@ -487,9 +542,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
 
         const int qpos = p.q_pos0 + qrow;
         const uint32_t tO = tmem + kColO + lane_base + 64 * ch;
-        float acc[64];
+        float2 acc[32];  // O of the row's channels 64 ch .. 64 ch + 63
 #pragma unroll
-        for (int i = 0; i < 64; ++i) acc[i] = 0.f;
+        for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
         float m = -CUDART_INF_F, l = 0.f, w_prev = 0.f;
         bool failed = false;
         // acc += w O(t): P V of tile t out of TMEM, 32 columns at a time
@@ -501,7 +556,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                 uint32_t o[32];
                 tc::ld_32x32b_x32_sync(tO + 32 * c, o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(o[i]), w, acc[32 * c + i]);
+                for (int i = 0; i < 16; ++i)
+                    acc[16 * c + i] = fma2(make_float2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])),
+                                           make_float2(w, w), acc[16 * c + i]);
             }
             tc::fence_before_sync();
             mbar_arrive(&sm.o_empty);
@@ -513,7 +570,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             const Info& inf = sm.info[t % kInfo];
             const int pos = inf.pos[ch], len = inf.len[ch];
             const float u = fmaxf(inf.sv[0], inf.sv[1]);
+            // p comes out of the exponential times f = 2^7 s_v / u; the row sum takes f off again once per tile
             const float f = inf.sv[ch] / u * kPScale, c = qmul * inf.sk[ch];
+            const float lf = log2f(f);
             if (!warp_wait(&sm.s_full[s], (t >> 1) & 1, &sm.abort)) { failed = true; break; }
             tc::fence_after_sync();
             const uint32_t tS = tmem + 128 * s + lane_base;
@@ -545,19 +604,21 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                 m = mn;
             }
             const float ms = m == -CUDART_INF_F ? 0.f : m;
-            float rs[2] = {0.f, 0.f};
+            const float2 c2 = make_float2(c, c), b2 = make_float2(lf - ms, lf - ms);
+            float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             uint32_t hi[32], lo[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-                const float p0 = tc::ex2(fmaf(__uint_as_float(sr[2 * e]), c, -ms));
-                const float p1 = tc::ex2(fmaf(__uint_as_float(sr[2 * e + 1]), c, -ms));
-                rs[0] += p0;
-                rs[1] += p1;
-                split_half(p0 * f, p1 * f, hi[e], lo[e]);
+                const float2 x =
+                    fma2(make_float2(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), c2, b2);
+                const float2 pp = make_float2(tc::ex2(x.x), tc::ex2(x.y));
+                rs[e & 1] = add2(rs[e & 1], pp);
+                split_half(pp, hi[e], lo[e]);
             }
             tc::st_32x32b_x32(tS + 32 * ch, hi);
             tc::st_32x32b_x32(tS + 64 + 32 * ch, lo);
-            l = l * alpha + (rs[0] + rs[1]);
+            const float2 sum = add2(rs[0], rs[1]);
+            l = l * alpha + (sum.x + sum.y) * (1.f / f);
             tc::wait_st();
             tc::fence_before_sync();
             mbar_arrive(&sm.p_full[s]);
@@ -566,7 +627,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             w_prev = u * (1.f / kPScale);
             if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) acc[i] *= alpha;
+                for (int i = 0; i < 32; ++i) acc[i] = make_float2(acc[i].x * alpha, acc[i].y * alpha);
             }
         }
         if (!failed && nt > 0 && !drain(nt - 1, w_prev)) failed = true;
@@ -584,57 +645,17 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         const bool any = lt > 0.f || lt != lt;
         const float inv = any ? 1.f / lt : 0.f;
         const float lse = any ? (m + log2f(lt)) * 0.69314718055994531f : -CUDART_INF_F;
-        const size_t orow = ((size_t)b * p.q_heads + hk * G + g) * p.q_len + (row_ok ? qrow : 0);
-        if (p.nsplit == 1) {
-            if (row_ok) {
+        // the call's output, or this split's normalised output and log-sum-exp for chunk_merge_kernel
+        const bool whole = p.nsplit == 1;
+        const size_t orow = whole ? ((size_t)b * p.q_heads + hk * G + g) * p.q_len + qrow : (size_t)blockIdx.x * BM + r;
+        float* dst = (whole ? p.out : p.ws.o) + (!whole || row_ok ? orow : 0) * D + 64 * ch;
+        float* dst_lse = whole ? p.lse : p.ws.m;
+        if (!whole || row_ok) {
 #pragma unroll
-                for (int i = 0; i < 64; i += 4)
-                    *reinterpret_cast<float4*>(p.out + orow * D + 64 * ch + i) =
-                        make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-                if (ch == 0 && p.lse != nullptr) p.lse[orow] = lse;
-            }
-        } else {
-            // normalised output and log-sum-exp of this split; the unit's last CTA combines them
-            const size_t prow = (size_t)blockIdx.x * BM + r;
-#pragma unroll
-            for (int i = 0; i < 64; i += 4)
-                *reinterpret_cast<float4*>(p.ws.o + prow * D + 64 * ch + i) =
-                    make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-            if (ch == 0) p.ws.m[prow] = lse;
-            named_barrier_sync(3, kSoftmaxThreads);
-            if (tid == 0) sm.flag = atom_add_acq_rel_gpu(&p.ws.counters[unit], 1) == p.nsplit - 1;
-            named_barrier_sync(3, kSoftmaxThreads);
-            if (sm.flag) {
-                const size_t base = (size_t)unit * p.nsplit * BM + r;
-                float M = -CUDART_INF_F, L = 0.f;
-                for (int k = 0; k < p.nsplit; ++k) M = fmaxf(M, __ldcg(p.ws.m + base + (size_t)k * BM));
-#pragma unroll
-                for (int i = 0; i < 64; ++i) acc[i] = 0.f;
-                for (int k = 0; k < p.nsplit; ++k) {
-                    const float ls = __ldcg(p.ws.m + base + (size_t)k * BM);
-                    const float wt = ls == -CUDART_INF_F ? 0.f : ex2_approx((ls - M) * 1.4426950408889634f);
-                    L += wt;
-                    const float4* src = reinterpret_cast<const float4*>(p.ws.o + (base + (size_t)k * BM) * D + 64 * ch);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 o = __ldcg(src + i);
-                        acc[4 * i] += wt * o.x;
-                        acc[4 * i + 1] += wt * o.y;
-                        acc[4 * i + 2] += wt * o.z;
-                        acc[4 * i + 3] += wt * o.w;
-                    }
-                }
-                const bool some = L > 0.f || L != L;
-                const float invL = some ? 1.f / L : 0.f;
-                if (row_ok) {
-#pragma unroll
-                    for (int i = 0; i < 64; i += 4)
-                        *reinterpret_cast<float4*>(p.out + orow * D + 64 * ch + i) =
-                            make_float4(acc[i] * invL, acc[i + 1] * invL, acc[i + 2] * invL, acc[i + 3] * invL);
-                    if (ch == 0 && p.lse != nullptr) p.lse[orow] = some ? M + logf(L) : -CUDART_INF_F;
-                }
-                if (tid == 0) p.ws.counters[unit] = 0;
-            }
+            for (int i = 0; i < 32; i += 2)
+                *reinterpret_cast<float4*>(dst + 2 * i) =
+                    make_float4(acc[i].x * inv, acc[i].y * inv, acc[i + 1].x * inv, acc[i + 1].y * inv);
+            if (ch == 0 && dst_lse != nullptr) dst_lse[orow] = lse;
         }
     }
     tc::fence_before_sync();
@@ -644,6 +665,47 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, kTmemCols);
     }
+}
+
+// out = sum_s e^(lse_s - M) O_s / sum_s e^(lse_s - M) over the splits of a unit's
+// keys: one warp per query row, a lane holding 4 channels. Bound by the
+// partials' bytes (64 KB per part, from L2).
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const Params p) {
+    griddep_wait();
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int unit = row / BM, r = row % BM;
+    if (unit >= p.units) return;
+    const int nqb = p.units / p.groups, ppc = BM / p.G;
+    const int qb = nqb - 1 - unit / p.groups, bh = unit % p.groups;
+    const int g = r % p.G, j = r / p.G, qrow = qb * ppc + j;
+    if (j >= ppc || qrow >= p.q_len) return;
+    const size_t base = (size_t)unit * p.nsplit * BM + r;
+    static_assert(kMaxSplit == 32, "a lane per split");
+    const float ls = lane < p.nsplit ? __ldcg(p.ws.m + base + (size_t)lane * BM) : -CUDART_INF_F;
+    float M = ls;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    const float wl = ls == -CUDART_INF_F ? 0.f : expf(ls - M);
+    float L = wl;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4* src = reinterpret_cast<const float4*>(p.ws.o + base * D) + lane;
+#pragma unroll 8
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float4 o = __ldcg(src + (size_t)s * BM * (D / 4));
+        const float wt = __shfl_sync(0xffffffffu, wl, s);
+        acc.x += wt * o.x;
+        acc.y += wt * o.y;
+        acc.z += wt * o.z;
+        acc.w += wt * o.w;
+    }
+    const bool some = L > 0.f || L != L;
+    const float inv = some ? 1.f / L : 0.f;
+    const size_t orow = ((size_t)(bh / p.kv_heads) * p.q_heads + (bh % p.kv_heads) * p.G + g) * p.q_len + qrow;
+    reinterpret_cast<float4*>(p.out + orow * D)[lane] =
+        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (lane == 0 && p.lse != nullptr) p.lse[orow] = some ? M + logf(L) : -CUDART_INF_F;
 }
 
 // The live ring tokens as float16 tiles of 64 with a power-of-two scale s each
@@ -696,7 +758,7 @@ __global__ void __launch_bounds__(256) hot_half_kernel(const T* __restrict__ k, 
 // Splits of each unit's keys: the count (of at most kMaxParts parts per SM)
 // with the shortest run of waves, a part costing its share of the tiles plus
 // about four tiles' time of set-up, partial output and merge.
-constexpr int kMaxParts = 4, kMaxSplit = 32;
+constexpr int kMaxParts = 4;
 constexpr double kPartTiles = 4.0;
 
 int choose_split(int units, double tiles, int sms, int max_splits) {
@@ -704,7 +766,7 @@ int choose_split(int units, double tiles, int sms, int max_splits) {
     double best_t = 1e300;
     for (int s = 1; s <= kMaxSplit; ++s) {
         if (max_splits > 0 && s > max_splits) break;
-        if (s > 1 && ((long long)units * s > (long long)kMaxParts * sms || tiles / s < 4.0 || units > kMaxCounters)) break;
+        if (s > 1 && ((long long)units * s > (long long)kMaxParts * sms || tiles / s < 4.0)) break;
         const double waves = (double)((units * (long long)s + sms - 1) / sms);
         const double t = waves * (tiles / s + kPartTiles * (s > 1 ? 2.0 : 1.0));
         if (t < 0.97 * best_t) {
@@ -767,6 +829,26 @@ rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_arch
     p.nsplit = choose_split(p.units, (a.n_tiles + 1) / 2 + p.hot_rows / (double)BN, device_sms(), max_splits);
     // partials of all parts: outputs [parts][128][128] and log-sum-exps [parts][128] (in the layout's m)
     p.ws = ws_view(workspace, ws_layout(1, 1, p.nsplit > 1 ? p.units * p.nsplit : 1, BM, D));
+    static std::atomic<bool> ready[64];
+    const int dev = arena->device;
+    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+        // setmaxnreg moves registers between the warpgroups of what the block was launched with
+        cudaFuncAttributes attr;
+        RFSN_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel));
+        if (attr.numRegs * kThreads < 256 * (kSoftmaxRegs + kOtherRegs)) {
+            set_error("rfsn_archive_attention: built with %d registers per thread, the chunk kernel needs %d",
+                      attr.numRegs, 256 * (kSoftmaxRegs + kOtherRegs) / kThreads);
+            return RFSN_ERR_UNSUPPORTED;
+        }
+        RFSN_CUDA(cudaFuncSetAttribute(chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(chunk::Smem)));
+        // the small kernels around it with the same split of the SM's memory, or each change of split drains the SMs
+        for (const void* f : {reinterpret_cast<const void*>(hot_half_kernel<__half>),
+                              reinterpret_cast<const void*>(hot_half_kernel<__nv_bfloat16>),
+                              reinterpret_cast<const void*>(chunk_merge_kernel)})
+            RFSN_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                           cudaSharedmemCarveoutMaxShared));
+        if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+    }
     char* hot = static_cast<char*>(workspace) + off;
     const size_t rows = (size_t)groups * p.hot_rows;
     CUtensorMap mk, mv;
@@ -793,30 +875,20 @@ rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_arch
         mk = arena->item_maps[0];  // not used
         mv = arena->item_maps[1];
     }
-    static std::atomic<bool> ready[64];
-    const int dev = arena->device;
-    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
-        // setmaxnreg moves registers between the warpgroups of what the block was launched with
-        cudaFuncAttributes attr;
-        RFSN_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel));
-        if (attr.numRegs * kThreads < 256 * (kSoftmaxRegs + kOtherRegs)) {
-            set_error("rfsn_archive_attention: built with %d registers per thread, the chunk kernel needs %d",
-                      attr.numRegs, 256 * (kSoftmaxRegs + kOtherRegs) / kThreads);
-            return RFSN_ERR_UNSUPPORTED;
-        }
-        RFSN_CUDA(cudaFuncSetAttribute(chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(chunk::Smem)));
-        if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
-    }
-    chunk_kernel<<<p.units * p.nsplit, chunk::kThreads, sizeof(chunk::Smem), s>>>(packed->maps[0], packed->maps[1], mk,
-                                                                                 mv, p);
-    RFSN_CUDA(cudaGetLastError());
+    RFSN_CUDA(launch_pdl(chunk_kernel, dim3(p.units * p.nsplit), dim3(chunk::kThreads), sizeof(chunk::Smem), s,
+                         packed->maps[0], packed->maps[1], mk, mv, p));
     note_launch();
+    if (p.nsplit > 1) {
+        RFSN_CUDA(launch_pdl(chunk_merge_kernel, dim3(p.units * (BM / 8)), dim3(256), 0, s, p));
+        note_launch();
+    }
     return RFSN_OK;
 }
 
 void preload_chunk_kernels() {
     cudaFuncAttributes a;
     cudaFuncGetAttributes(&a, archive::chunk::chunk_kernel);
+    cudaFuncGetAttributes(&a, archive::chunk::chunk_merge_kernel);
     cudaFuncGetAttributes(&a, archive::chunk::hot_half_kernel<__half>);
     cudaFuncGetAttributes(&a, archive::chunk::hot_half_kernel<__nv_bfloat16>);
 }

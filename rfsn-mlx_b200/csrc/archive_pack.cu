@@ -12,6 +12,9 @@
 // floating-point numbers, only the point where they turn subnormal moves.
 // NaN stays NaN, infinities become NaN (e4m3 has none, and saturating them
 // would hide them).
+#include <algorithm>
+#include <cstring>
+
 #include <math_constants.h>
 
 #include "archive.cuh"
@@ -20,6 +23,7 @@ namespace rfsn {
 namespace archive {
 
 constexpr int kPackThreads = 256;
+constexpr int kPackCtas = 8;  // per SM: 65,501 tokens of 8 heads 67.8 us (3: 74.5, 4: 72.1, 6: 77.6)
 
 struct RowSource {
     const void* p;
@@ -28,20 +32,48 @@ struct RowSource {
     int vec;               // rows may be read as 16-byte vectors
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int vec, float (&x)[8]) {
-    if (vec) {
-        constexpr int N = 8 * sizeof(T) / 16;
-        uint4 w[N];
+// 8 elements as they are in memory, and their values
+template <typename T> struct Vec8 {
+    uint4 w[8 * sizeof(T) / 16];
+    __device__ __forceinline__ void load(const T* p, int vec) {
+        if (vec) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const T* e = reinterpret_cast<const T*>(w);
+            for (int i = 0; i < (int)sizeof(w) / 16; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+            T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(p[i]);
+            for (int i = 0; i < 8; ++i) e[i] = p[i];
+        }
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(w) / 16; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T*>(w)[i]); }
+    __device__ __forceinline__ void drop_infinities() {  // to NaN
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (fabsf(get(i)) == CUDART_INF_F) reinterpret_cast<T*>(w)[i] = from_f32<T>(CUDART_NAN_F);
+    }
+    // Largest |x| so far as bit patterns (they order like the magnitudes, infinities and NaN above all numbers): one
+    // per word, two per word for 16-bit types.
+    __device__ __forceinline__ uint32_t abs_max(uint32_t acc) const {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(w) / 4; ++i) {
+            const uint32_t x = (&w[i / 4].x)[i % 4];
+            acc = sizeof(T) == 4 ? max(acc, x & 0x7fffffffu) : __vmaxu2(acc, x & 0x7fff7fffu);
+        }
+        return acc;
+    }
+};
+// The pattern of abs_max as a number, infinite for infinities and NaN alike.
+template <typename T> __device__ __forceinline__ float pattern_value(uint32_t m) {
+    if (sizeof(T) == 4) return m >= 0x7f800000u ? CUDART_INF_F : __uint_as_float(m);
+    const uint16_t h = (uint16_t)m;
+    T x;
+    memcpy(&x, &h, 2);
+    const float f = to_f32<T>(x);
+    return f != f ? CUDART_INF_F : f;
 }
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -62,103 +94,128 @@ __device__ __forceinline__ float tile_scale(float a) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// One CTA per (tile, KV head, K or V): the tile stays in registers between
-// the maximum and the conversion, so it is read once. Bound by memory. Rows
-// of the tile behind `count` become zero codes (the attention kernel reads
-// whole tiles and multiplies them by zero weights).
-template <typename T, int D>
+// A CTA's work item is a (tile, KV head, K or V); the tile stays in registers
+// between the maximum and the conversion, so it is read once, and the next
+// item's tile is requested before this one is converted. Items are numbered K
+// and V fastest, then the heads, so that the CTAs that run together read
+// neighbouring rows of token-major sources. Bound by memory. Rows of the tile
+// behind `count` become zero codes (the attention kernels read whole tiles and
+// multiply them by zero weights).
+template <typename T, int D, bool BOUNDS>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(RowSource ks, RowSource vs, uint8_t* __restrict__ kd,
                                                             uint8_t* __restrict__ vd, float* __restrict__ scales,
                                                             uint8_t* __restrict__ bounds, int rows, int dst_row0,
-                                                            int count) {
+                                                            int count, uint32_t groups, uint32_t items) {
     constexpr int VPR = D / 8;                    // 8-element vectors per row
     constexpr int RPP = kPackThreads / VPR;       // rows per pass
     constexpr int PASSES = kTile / RPP;
-    // heads first: the CTAs that run together read neighbouring rows of token-major sources whole
-    const int bh = blockIdx.x >> 1, is_v = blockIdx.x & 1, tile = blockIdx.y + blockIdx.z * gridDim.y;
-    if (tile * kTile >= count) return;
-    const RowSource src = is_v ? vs : ks;
-    const int len = min(kTile, count - tile * kTile);
     const int c8 = threadIdx.x % VPR, r0 = threadIdx.x / VPR;
-    const T* base = static_cast<const T*>(src.p) + (bh / src.kv_heads) * src.sb + (bh % src.kv_heads) * src.sh + 8 * c8;
-    float x[PASSES][8];
-    float a = 0.f;
+    __shared__ uint32_t part[2][kPackThreads / 32];
+    __shared__ __half2 red[BOUNDS ? 2 : 1][BOUNDS ? RPP : 1][D / 2];
+    struct Place {
+        int is_v, bh, tile;
+    };
+    auto fetch = [&](uint32_t item, Vec8<T> (&x)[PASSES]) {
+        const uint32_t pair = item >> 1, tile_ = pair / groups;
+        const Place at{(int)(item & 1), (int)(pair - tile_ * groups), (int)tile_};
+        const RowSource& src = at.is_v ? vs : ks;
+        const uint32_t b = (uint32_t)at.bh / (uint32_t)src.kv_heads, h = (uint32_t)at.bh - b * src.kv_heads;
+        const T* base = static_cast<const T*>(src.p) + b * src.sb + h * src.sh + 8 * c8;
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = r0 + i * RPP;
-        if (r < len) {
-            long long t = (long long)src.offset + (long long)tile * kTile + r;
-            if (src.wrap > 0) t %= src.wrap;
-            load8<T>(base + t * src.st, src.vec, x[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = at.tile * kTile + r0 + i * RPP;
+            x[i].clear();
+            if (r < count) {
+                long long t = (long long)src.offset + r;
+                if (src.wrap > 0 && t >= src.wrap) t -= src.wrap;
+                x[i].load(base + t * src.st, src.vec);
+            }
         }
-    }
+        return at;
+    };
+    Vec8<T> next[PASSES];
+    uint32_t item = blockIdx.x;
+    Place next_at = fetch(item, next);  // the grid has at most `items` CTAs
+    for (int turn = 0; item < items; item += gridDim.x, turn ^= 1) {
+        Vec8<T> x[PASSES];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i)
+        for (int i = 0; i < PASSES; ++i) x[i] = next[i];
+        const int is_v = next_at.is_v, bh = next_at.bh, tile = next_at.tile;
+        if (item + gridDim.x < items) next_at = fetch(item + gridDim.x, next);
+        const int len = min(kTile, count - tile * kTile);
+        uint32_t m = 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float m = fabsf(x[i][e]);
-            a = fmaxf(a, m < CUDART_INF_F ? m : 0.f);
+        for (int i = 0; i < PASSES; ++i) m = x[i].abs_max(m);
+        if (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
+        m = __reduce_max_sync(0xffffffffu, m);
+        if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = m;
+        __syncthreads();  // also: the previous item's bounds have been reduced
+        m = part[turn][0];
+#pragma unroll
+        for (int i = 1; i < kPackThreads / 32; ++i) m = max(m, part[turn][i]);
+        float a = pattern_value<T>(m);
+        if (a == CUDART_INF_F) {  // infinities or NaN in the tile (all threads agree): the maximum of the rest
+            a = 0.f;
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                x[i].drop_infinities();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[i].get(e)));  // NaN loses
+            }
+            const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = bits;
+            __syncthreads();
+            m = part[turn][0];
+#pragma unroll
+            for (int i = 1; i < kPackThreads / 32; ++i) m = max(m, part[turn][i]);
+            a = __uint_as_float(m);
         }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
-    __shared__ float part[kPackThreads / 32];
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-    __syncthreads();
-    a = part[0];
-#pragma unroll
-    for (int i = 1; i < kPackThreads / 32; ++i) a = fmaxf(a, part[i]);
-    const float s = tile_scale(a), inv = 1.f / s;  // both powers of two
-    const int row0 = dst_row0 + tile * kTile;
-    uint8_t* dst = (is_v ? vd : kd) + ((size_t)bh * rows + row0) * D + 8 * c8;
-    __half2 lo[4], hi[4];
-    const __half2 top = __half2half2(__ushort_as_half(0x7c00)), bottom = __half2half2(__ushort_as_half(0xfc00));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        lo[j] = top;
-        hi[j] = bottom;
-    }
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = r0 + i * RPP;
-        uint32_t c[4];
+        const float s = tile_scale(a), inv = 1.f / s;  // both powers of two
+        const int row0 = dst_row0 + tile * kTile;
+        uint8_t* dst = (is_v ? vd : kd) + ((size_t)bh * rows + row0) * D + 8 * c8;
+        const bool bound = BOUNDS && !is_v;
+        __half2 lo[4], hi[4];
+        const __half2 top = __half2half2(__ushort_as_half(0x7c00)), bottom = __half2half2(__ushort_as_half(0xfc00));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float y[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float v = x[i][2 * j + e];
-                y[e] = fabsf(v) == CUDART_INF_F ? CUDART_NAN_F : v * inv;
-            }
-            c[j] = e4m3x2(y[0], y[1]);
-            if (r < len) {
-                const __half2 h = half2_of_e4m3x2(c[j]);
-                lo[j] = __hmin2_nan(lo[j], h);
-                hi[j] = __hmax2_nan(hi[j], h);
-            }
+            lo[j] = top;
+            hi[j] = bottom;
         }
-        *reinterpret_cast<uint2*>(dst + (size_t)r * D) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-    }
-    const size_t slot = (size_t)bh * (rows / kTile) + row0 / kTile;
-    if (threadIdx.x == 0) scales[4 * slot + is_v] = s;
-    if (bounds == nullptr || is_v) return;
-    // channel-wise smallest and largest code of the tile's keys
-    __shared__ __half2 red[2][RPP][D / 2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        red[0][r0][4 * c8 + j] = lo[j];
-        red[1][r0][4 * c8 + j] = hi[j];
-    }
-    __syncthreads();
-    if (threadIdx.x < D) {  // 2 bounds x D / 2 channel pairs
-        const int w = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
-        __half2 m = red[w][0][j];
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = r0 + i * RPP;
+            uint32_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                c[j] = e4m3x2(x[i].get(2 * j) * inv, x[i].get(2 * j + 1) * inv);
+                if (BOUNDS && bound && r < len) {
+                    const __half2 h = half2_of_e4m3x2(c[j]);
+                    lo[j] = __hmin2_nan(lo[j], h);
+                    hi[j] = __hmax2_nan(hi[j], h);
+                }
+            }
+            *reinterpret_cast<uint2*>(dst + (size_t)r * D) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+        }
+        const size_t slot = (size_t)bh * (rows / kTile) + row0 / kTile;
+        if (threadIdx.x == 0) scales[4 * slot + is_v] = s;
+        if (!BOUNDS || !bound) continue;
+        // channel-wise smallest and largest code of the tile's keys
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            red[0][r0][4 * c8 + j] = lo[j];
+            red[1][r0][4 * c8 + j] = hi[j];
+        }
+        __syncthreads();
+        if (threadIdx.x < D) {  // 2 bounds x D / 2 channel pairs
+            const int w = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
+            __half2 m = red[w][0][j];
 #pragma unroll 4
-        for (int r = 1; r < RPP; ++r) m = w ? __hmax2_nan(m, red[w][r][j]) : __hmin2_nan(m, red[w][r][j]);
-        const float2 f = __half22float2(m);
-        reinterpret_cast<uint16_t*>(bounds)[(slot * 2 + w) * (D / 2) + j] = (uint16_t)e4m3x2(f.x, f.y);
+            for (int r = 1; r < (BOUNDS ? RPP : 1); ++r)
+                m = w ? __hmax2_nan(m, red[w][r][j]) : __hmin2_nan(m, red[w][r][j]);
+            const float2 f = __half22float2(m);
+            reinterpret_cast<uint16_t*>(bounds)[(slot * 2 + w) * (D / 2) + j] = (uint16_t)e4m3x2(f.x, f.y);
+        }
     }
 }
 
@@ -220,12 +277,13 @@ __global__ void __launch_bounds__(256) bounds_kernel(const T* __restrict__ k, T*
     for (int i = 0; i < kTile / RPP; ++i) {
         const int r = r0 + i * RPP;
         if (r < len) {
-            float x[8];
-            load8<T>(src + (size_t)r * D, 1, x);
+            Vec8<T> x;
+            x.load(src + (size_t)r * D, 1);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                lo[e] = (x[e] < lo[e] || x[e] != x[e]) ? x[e] : lo[e];
-                hi[e] = (x[e] > hi[e] || x[e] != x[e]) ? x[e] : hi[e];
+                const float y = x.get(e);
+                lo[e] = (y < lo[e] || y != y) ? y : lo[e];
+                hi[e] = (y > hi[e] || y != y) ? y : hi[e];
             }
         }
     }
@@ -251,10 +309,16 @@ __global__ void __launch_bounds__(256) bounds_kernel(const T* __restrict__ k, T*
 template <typename T, int D>
 rfsn_status pack_launch(const rfsn_packed_archive* a, int dst_row0, const RowSource& ks, const RowSource& vs,
                         int count, void* bounds, cudaStream_t s) {
-    const int tiles = (count + kTile - 1) / kTile, ty = tiles < 32768 ? tiles : 32768;
-    const dim3 grid(2 * a->groups, ty, (tiles + ty - 1) / ty);
-    pack_kernel<T, D><<<grid, kPackThreads, 0, s>>>(ks, vs, a->k, a->v, reinterpret_cast<float*>(a->scales),
-                                                    static_cast<uint8_t*>(bounds), a->rows, dst_row0, count);
+    // groups * rows < 2^31, so the count fits 32 bits
+    const uint32_t items = 2u * (uint32_t)a->groups * (uint32_t)((count + kTile - 1) / kTile);
+    const uint32_t ctas = std::min(items, (uint32_t)(kPackCtas * device_sms()));
+    if (bounds != nullptr)
+        pack_kernel<T, D, true><<<ctas, kPackThreads, 0, s>>>(ks, vs, a->k, a->v, reinterpret_cast<float*>(a->scales),
+                                                              static_cast<uint8_t*>(bounds), a->rows, dst_row0, count,
+                                                              a->groups, items);
+    else
+        pack_kernel<T, D, false><<<ctas, kPackThreads, 0, s>>>(ks, vs, a->k, a->v, reinterpret_cast<float*>(a->scales),
+                                                               nullptr, a->rows, dst_row0, count, a->groups, items);
     RFSN_CUDA(cudaGetLastError());
     note_launch();
     return RFSN_OK;
@@ -285,7 +349,8 @@ rfsn_status bounds_launch(const rfsn_arena* a, int row0, int count, void* bounds
 template <typename T, int D>
 void preload() {
     cudaFuncAttributes a;
-    cudaFuncGetAttributes(&a, pack_kernel<T, D>);
+    cudaFuncGetAttributes(&a, pack_kernel<T, D, false>);
+    cudaFuncGetAttributes(&a, pack_kernel<T, D, true>);
     cudaFuncGetAttributes(&a, unpack_kernel<T, D>);
     if constexpr (sizeof(T) == 2) cudaFuncGetAttributes(&a, bounds_kernel<T, D>);
 }

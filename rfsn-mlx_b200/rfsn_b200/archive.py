@@ -9,7 +9,7 @@ extensions of ``LayerKVCache`` live here:
   and for V, so an attention call reads half the bytes. The hot ring keeps the
   cache dtype. ``PackedArchive`` owns the codes; ``pack`` and ``unpack`` convert.
 * **Tile selection** (``tile_index=True``): the cache keeps the channel-wise
-  smallest and largest key of every archived tile. ``select_tiles`` bounds the
+  smallest and largest key of every archived tile. ``rfsn_select_tiles`` bounds the
   logits of each tile with them and picks the ``top_tiles`` best for each query
   and KV head; attention then reads those tiles and the hot window only. The
   result is the exact softmax over the keys that are read; the tiles left out
@@ -181,39 +181,40 @@ def workspace_bytes(batch: int, q_heads: int, kv_heads: int, q_len: int, head_di
     return int(out.value)
 
 
-def select_tiles(cache, q: torch.Tensor, q_start_pos: int, segments, top_tiles: int, *,
-                 workspace: Optional[native.Workspace] = None,
-                 step_state: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Tile list int32 [B, Hkv, q_len, top_tiles, 4] = {row, pos, len, tile} of
-    the ``top_tiles`` archived tiles with the largest logit bound for each query
-    row and KV head (``rfsn_select_tiles``); unused entries are {0, 0, 0, -1}.
-    q: float32 [B, H, q_len, D] on the cache's device. Call with the cache's
-    device current."""
-    if cache.tile_bounds is None:
-        raise ValueError("tile selection needs a cache built with tile_index=True")
-    B, H, Lq, D = q.shape
-    if not 1 <= top_tiles <= 1 << 20:
-        raise ValueError(f"top_tiles must be at least 1, got {top_tiles}")
-    if Lq > SPARSE_MAX_ROWS:
-        raise ValueError(f"tile selection takes up to {SPARSE_MAX_ROWS} query rows a call, got {Lq}")
-    tiles_dev, n_tiles = segments.tile_list
-    tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
-    out = torch.empty((B, cache.num_kv_heads, Lq, top_tiles, 4), dtype=torch.int32, device=cache.device)
-    ws = workspace if workspace is not None else native.default_workspace(cache.device)
-    buf = ws.get(workspace_bytes(B, H, cache.num_kv_heads, Lq, D, cache.config.hot_capacity, n_tiles,
-                                 top_tiles))
-    bounds = cache.tile_bounds
-    packed = cache.archive is not None
-    native.check(
-        native.lib().rfsn_select_tiles(
-            bounds.data_ptr(), native.RFSN_E4M3 if packed else native.dtype_code(bounds.dtype),
-            cache.archive.scales.data_ptr() if packed else None, int(bounds.shape[1]) * TILE, q.data_ptr(), B, H,
-            cache.num_kv_heads, Lq, D, int(q_start_pos), ctypes.byref(tiles), top_tiles, out.data_ptr(),
-            step_state.data_ptr() if step_state is not None else None, buf.data_ptr(), buf.numel(),
-            native.stream_ptr()),
-        "rfsn_select_tiles",
-    )
-    return out
+class PreparedSelection:
+    """The part of ``rfsn_select_tiles`` that does not depend on the query, for
+    one cache, its segments' tiles and one query shape."""
+
+    __slots__ = ("before", "between", "shape", "nbytes", "keep")
+
+    def __init__(self, cache, segments, q_heads: int, q_len: int, top_tiles: int) -> None:
+        if cache.tile_bounds is None:
+            raise ValueError("tile selection needs a cache built with tile_index=True")
+        if not 1 <= top_tiles <= 1 << 20:
+            raise ValueError(f"top_tiles must be at least 1, got {top_tiles}")
+        if q_len > SPARSE_MAX_ROWS:
+            raise ValueError(f"tile selection takes up to {SPARSE_MAX_ROWS} query rows a call, got {q_len}")
+        B, Hkv, D = cache.batch_size, cache.num_kv_heads, cache.config.head_dim
+        tiles_dev, n_tiles = segments.tile_list
+        tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
+        archive, bounds = cache.archive, cache.tile_bounds
+        self.before = (bounds.data_ptr(), native.RFSN_E4M3 if archive is not None else native.dtype_code(bounds.dtype),
+                       archive.scales.data_ptr() if archive is not None else None, int(bounds.shape[1]) * TILE)
+        self.between = (B, q_heads, Hkv, q_len, D)
+        self.shape = (B, Hkv, q_len, top_tiles, 4)
+        self.nbytes = workspace_bytes(B, q_heads, Hkv, q_len, D, cache.config.hot_capacity, n_tiles, top_tiles)
+        self.keep = (ctypes.byref(tiles), tiles, archive, bounds, tiles_dev)
+
+    def __call__(self, cache, q: torch.Tensor, q_start_pos: int) -> torch.Tensor:
+        """Tile list int32 [B, Hkv, q_len, top_tiles, 4] = {row, pos, len, tile}."""
+        out = torch.empty(self.shape, dtype=torch.int32, device=cache.device)
+        buf = native.default_workspace(cache.device).get(self.nbytes)
+        status = native.lib().rfsn_select_tiles(*self.before, q.data_ptr(), *self.between, q_start_pos, self.keep[0],
+                                                self.shape[3], out.data_ptr(), None, buf.data_ptr(), buf.numel(),
+                                                native.stream_ptr())
+        if status:
+            native.check(status, "rfsn_select_tiles")
+        return out
 
 
 class PreparedCall:
@@ -247,4 +248,4 @@ class PreparedCall:
             native.check(status, "rfsn_archive_attend")
 
 
-__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "PreparedCall", "select_tiles", "workspace_bytes"]
+__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "PreparedCall", "PreparedSelection", "workspace_bytes"]

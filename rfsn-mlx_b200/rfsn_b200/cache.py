@@ -46,7 +46,7 @@ import numpy as np
 import torch
 
 from . import _native as native
-from .archive import PackedArchive, PreparedCall, check_archive_options, padded_rows, select_tiles
+from .archive import PackedArchive, PreparedCall, PreparedSelection, check_archive_options, padded_rows
 from .block_manager import BlockId, BlockLocation, BlockManager, BlockManifest, BlockSpan
 from .config import RFSNConfig, RuntimeMode, resolve_dtype, validate_session_id
 from .residency import ResidencyManager
@@ -285,7 +285,9 @@ class PagedSegments(Sequence):
         self.hot_state = hot_state            # (head_index, length, start) or None when hot pieces excluded
         # (device int32 [n, 4] tiles, n) of the archived spans: packed caches and caches with a tile index
         self.tile_list = cache.tile_snapshot() if table is not None else (cache.tile_snapshot()[0], 0)
-        self.calls: dict[tuple, PreparedCall] = {}  # prepared calls over these segments, by query shape
+        # prepared calls over these segments, by query shape
+        self.calls: dict[tuple, PreparedCall] = {}
+        self.selections: dict[tuple, PreparedSelection] = {}
 
     def __len__(self) -> int:
         return len(self.spans)
@@ -1157,8 +1159,13 @@ class LayerKVCache:
         if segments is None:
             segments = self.get_attention_segments()
         qf = _query(self, q)
+        key = (qf.shape[1], qf.shape[2], top_tiles)
+        call = segments.selections.get(key)
+        if call is None or call.keep[3] is not self.tile_bounds:
+            call = segments.selections[key] = PreparedSelection(self, segments, int(qf.shape[1]), int(qf.shape[2]),
+                                                                int(top_tiles))
         with native.on_device(self.device):
-            return select_tiles(self, qf, q_start_pos, segments, int(top_tiles))[..., 3]
+            return call(self, qf, int(q_start_pos)).select(4, 3)
 
 
 def _query(cache: LayerKVCache, q: torch.Tensor) -> torch.Tensor:
