@@ -82,15 +82,17 @@ size_t lists_offset(const SlotPlan& sp, int head_dim, int n_tiles) {
 
 size_t select_scores_offset() { return align_up(256 + sizeof(int) * (size_t)kMaxCounters, 256); }
 
-rfsn_status check_shape(int batch, int q_heads, int kv_heads, int q_len, int head_dim, const char* what) {
+rfsn_status check_shape(int batch, int q_heads, int kv_heads, int q_len, int head_dim, bool per_query,
+                        const char* what) {
     RFSN_CHECK_ARG(batch > 0 && q_heads > 0 && kv_heads > 0 && q_len > 0, "%s: non-positive shape", what);
     RFSN_CHECK_ARG(q_heads % kv_heads == 0, "num_heads (%d) must be divisible by num_kv_heads (%d)", q_heads, kv_heads);
     if (head_dim != 64 && head_dim != 128) {
         set_error("%s: head_dim %d is not supported (64 or 128)", what, head_dim);
         return RFSN_ERR_UNSUPPORTED;
     }
-    RFSN_CHECK_ARG((long long)batch * kv_heads * q_len <= kMaxLists && (long long)q_len * q_heads <= (1 << 22),
-                   "%s: batch * kv_heads * q_len above %d", what, kMaxLists);
+    RFSN_CHECK_ARG((long long)batch * kv_heads * (per_query ? q_len : 1) <= kMaxLists, "%s: more than %d tile lists", what,
+                   kMaxLists);
+    RFSN_CHECK_ARG((long long)batch * q_heads * q_len < (1LL << 30), "%s: too many query rows", what);
     return RFSN_OK;
 }
 
@@ -108,8 +110,9 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
                       bool check_only) {
     const char* what = "rfsn_archive_attention";
     RFSN_CHECK_ARG(arena != nullptr && hot != nullptr, "%s: NULL arena or hot window", what);
-    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, arena->head_dim, what);
-    if (st == RFSN_OK) st = check_tiles(tiles, what);
+    rfsn_status st = check_tiles(tiles, what);
+    if (st == RFSN_OK)
+        st = check_shape(batch, q_heads, kv_heads, q_len, arena->head_dim, tiles->per_query != 0, what);
     if (st != RFSN_OK) return st;
     if (!arena->has_items) {
         set_error("%s: needs a bf16/f16 arena with head_dim 64 or 128", what);
@@ -136,7 +139,7 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     const bool chunk = packed != nullptr && tiles->per_query == 0 && !stepped && tiles->n > 0 &&
                        chunk_shape(arena->head_dim, q_heads / kv_heads, q_len, tiles->n);
     const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, tiles->per_query != 0);
-    RFSN_CHECK_ARG(sp.zblocks <= kMaxLists, "%s: too many query rows", what);
+    RFSN_CHECK_ARG(chunk || sp.zblocks <= kMaxLists, "%s: too many query rows", what);
     const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
     const int per_tile = packed != nullptr ? 1 : kTile / hk;
     RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
@@ -298,7 +301,7 @@ rfsn_status rfsn_tile_bounds(const rfsn_arena* arena, int row0, int count, void*
 rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim,
                                         int hot_capacity, int n_tiles, int n_select, size_t* bytes) {
     RFSN_CHECK_ARG(bytes != nullptr, "rfsn_archive_workspace_size: bytes is NULL");
-    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, "rfsn_archive_workspace_size");
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, n_select > 0, "rfsn_archive_workspace_size");
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0 && hot_capacity >= 0,
                    "rfsn_archive_workspace_size: negative count");
@@ -316,7 +319,7 @@ rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float*
                               const rfsn_tile_list* tiles, int n_select, int32_t* out, const int32_t* step_state,
                               void* workspace, size_t workspace_bytes, void* stream) {
     const char* what = "rfsn_select_tiles";
-    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, what);
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, true, what);
     if (st == RFSN_OK) st = check_tiles(tiles, what);
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(tiles->per_query == 0, "%s: selects from one list for all heads and queries", what);
@@ -379,7 +382,7 @@ rfsn_status rfsn_archive_attend(const rfsn_archive_call* c, const float* q, int 
         return rfsn_archive_attention(c->arena, c->packed, q, c->batch, c->q_heads, c->kv_heads, c->q_len, q_pos0,
                                       &c->tiles, &c->hot, out, lse, workspace, workspace_bytes, c->max_splits, stream);
     const int head_dim = c->arena->head_dim;
-    rfsn_status st = check_shape(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, what);
+    rfsn_status st = check_shape(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, true, what);
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(c->tiles.n > 0 && c->tiles.per_query == 0 && c->top_tiles <= (1 << 20), "%s: bad tile list", what);
     const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, true);

@@ -266,10 +266,10 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         sm.abort = 0;
         // 64-token tiles up to the causal limit (positions ascend through the list)
         int lo = 0, hi = p.n_tiles;
-        if (hi > 0 && __ldg(p.tiles + hi - 1).y <= qlast) lo = hi;
+        if (hi > 0 && __ldcg(p.tiles + hi - 1).y <= qlast) lo = hi;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (__ldg(p.tiles + mid).y <= qlast) lo = mid + 1; else hi = mid;
+            if (__ldcg(p.tiles + mid).y <= qlast) lo = mid + 1; else hi = mid;
         }
         sm.n_arch = lo;
         const int seen = max(0, min(p.hlen, qlast - p.hstart + 1));
@@ -346,7 +346,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                     if (gt < arch_tiles) {
                         const int i = 2 * gt + half;
                         if (i < sm.n_arch) {
-                            const int4 e = __ldg(p.tiles + i);
+                            const int4 e = __ldcg(p.tiles + i);
                             if (e.x < 0 || e.z < 0 || e.z > kTile || (e.x & (kTile - 1)) != 0 ||
                                 e.x + e.z > p.packed_rows) {
                                 atomicExch(p.ws.error, kDevErrBadTable);  // outside the archive: skipped
@@ -354,7 +354,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                                 row = e.x;
                                 pos = e.y;
                                 len = e.z;
-                                const float4 sc = __ldg(p.scales + (size_t)bh * (p.packed_rows / kTile) + row / kTile);
+                                const float4 sc = __ldcg(p.scales + (size_t)bh * (p.packed_rows / kTile) + row / kTile);
                                 sk = sc.x;
                                 sv = sc.y;
                             }

@@ -30,7 +30,7 @@ template <typename T> struct BoundVec;  // 8 bounds -> float
 template <> struct BoundVec<__nv_bfloat16> {
     uint4 w;
     __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const void* p) { w = __ldg(static_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void load(const void* p) { w = __ldcg(static_cast<const uint4*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t x = (&w.x)[i >> 1];
         return __uint_as_float((i & 1) ? (x & 0xffff0000u) : (x << 16));
@@ -39,7 +39,7 @@ template <> struct BoundVec<__nv_bfloat16> {
 template <> struct BoundVec<__half> {
     uint4 w;
     __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const void* p) { w = __ldg(static_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void load(const void* p) { w = __ldcg(static_cast<const uint4*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t x = (&w.x)[i >> 1];
         return __half2float(__ushort_as_half((unsigned short)((i & 1) ? (x >> 16) : (x & 0xffffu))));
@@ -48,7 +48,7 @@ template <> struct BoundVec<__half> {
 template <> struct BoundVec<uint8_t> {  // e4m3
     uint2 w;
     __device__ __forceinline__ void clear() { w = make_uint2(0, 0); }
-    __device__ __forceinline__ void load(const void* p) { w = __ldg(static_cast<const uint2*>(p)); }
+    __device__ __forceinline__ void load(const void* p) { w = __ldcg(static_cast<const uint2*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         const uint32_t x = (&w.x)[i >> 2] >> (8 * (i & 3));
         return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(x & 0xffu), __NV_E4M3)));
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         Fetched f;
         f.e = make_int4(0, 0, 0, 0);
         f.sk = 1.f;
-        if (t < t_end) f.e = __ldg(p.tiles + t);
+        if (t < t_end) f.e = __ldcg(p.tiles + t);
         if ((f.e.x & (kTile - 1)) != 0 || f.e.x < 0 || f.e.x / kTile >= p.tile_slots) {
             atomicExch(p.error, kDevErrBadTable);
             f.e.x = f.e.z = 0;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
             f.hi[v].clear();
         }
         if (f.e.z > 0) {
-            if (sizeof(T) == 1) f.sk = __ldg(p.scales + slot).x;
+            if (sizeof(T) == 1) f.sk = __ldcg(p.scales + slot).x;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int d0 = 8 * (l8 + 8 * v);

@@ -46,6 +46,10 @@ def build_parser() -> argparse.ArgumentParser:
     bnc.add_argument("--seed-prompt-len", type=int, default=8)
     bnc.add_argument("--archive-seed-steps", type=int, default=0)
     bnc.add_argument("--seed", type=int, default=0, help="random-init seed of the model weights")
+    bnc.add_argument("--archive-dtype", type=str, default="", choices=["", "float8_e4m3fn"],
+                     help="hold archived blocks in 8 bits (default: the model dtype)")
+    bnc.add_argument("--top-tiles", type=int, default=0,
+                     help="archived 64-token tiles that a decode token attends to (0 = all)")
     return ap
 
 
@@ -68,7 +72,8 @@ def cmd_bench(args: argparse.Namespace) -> None:
 
     config = config_from_args(args)
     model = RFSNModel(config, seed=args.seed)
-    cache = RFSNCache(config, batch_size=1, device=model.device)
+    cache = RFSNCache(config, batch_size=1, device=model.device, archive_dtype=args.archive_dtype or None,
+                      top_tiles=args.top_tiles)
     print(
         f"[bench] Model: {config.num_layers}L x {config.hidden_dim}d, "
         f"{config.num_heads}H/{config.num_kv_heads}KVH, "

@@ -233,8 +233,9 @@ def test_attention_over_the_archive_and_the_ring(dtype, B, H, Hkv, D, lens, hot,
             check_out(out, lse, want, want_lse, vv)
 
 
+@pytest.mark.parametrize("Lq", [3, 40])  # the tile kernel and the chunk kernel
 @pytest.mark.parametrize("q_pos", [-1, 0, 63, 64, 100, 250])
-def test_queries_among_the_keys_see_the_earlier_ones_only(q_pos):
+def test_queries_among_the_keys_see_the_earlier_ones_only(q_pos, Lq):
     """Positions inside the archive mask part of a tile, whole tiles and the ring; a row before every key gives zeros
     and -inf."""
     torch = _torch()
@@ -242,7 +243,7 @@ def test_queries_among_the_keys_see_the_earlier_ones_only(q_pos):
 
     lens = (100, 90)
     cache, k, v = make("float16", 1, 8, 2, 128, lens, 60)
-    q = queries(1, 8, 3, 128)
+    q = queries(1, 8, Lq, 128)
     kk, vv = held(cache, k, v, lens)
     want, want_lse = ref.attention(q, kk, vv, torch.arange(250), q_pos)
     out, lse = cache.attend(q, q_pos, want_lse=True)
@@ -251,34 +252,43 @@ def test_queries_among_the_keys_see_the_earlier_ones_only(q_pos):
         assert float(out[:, :, 0].abs().max()) == 0.0 and bool((lse[:, :, 0] == -math.inf).all())
 
 
-def test_what_is_masked_or_behind_the_ends_does_not_reach_the_result():
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_what_is_masked_or_behind_the_ends_does_not_reach_the_result(Lq):
     """NaN and infinity in ring slots outside the live window, in the tile rows behind a block's end (other than the
     zero codes that packing writes) and in keys after the query."""
     torch = _torch()
 
     lens = (70,)
     cache, k, v = make("bfloat16", 1, 4, 2, 128, lens, 40, hot_cap=100, wrap=30)
-    q = queries(1, 4, 1, 128)
-    want = cache.attend(q, 109).clone()
+    q = queries(1, 4, Lq, 128)
+    last = 110 - Lq
+    want = cache.attend(q, last).clone()
     cache._arena_k[:, :30] = math.nan
     cache._arena_v[:, :30] = math.nan
     cache._arena_k[:, 70:] = math.inf
     cache._arena_v[:, 70:] = math.nan
-    assert torch.equal(cache.attend(q, 109), want)
-    before = cache.attend(q, 50).clone()  # a query inside the archive: the ring lies behind it
+    assert torch.equal(cache.attend(q, last), want)
+    early = 60 - Lq  # queries inside the archive: the ring lies behind them
+    before = cache.attend(q, early).clone()
     cache._arena_k[:, 30:70] = math.nan
-    assert torch.equal(cache.attend(q, 50), before)
+    assert torch.equal(cache.attend(q, early), before)
 
 
-def test_nan_keys_and_values_that_are_seen_reach_the_result():
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_nan_keys_and_values_that_are_seen_reach_the_result(Lq):
     torch = _torch()
     cache, k, v = make("float16", 1, 4, 2, 128, (70, 64), 40)
-    q = queries(1, 4, 1, 128)
-    kn = k[:, :, :70].clone()
-    kn[0, 1, 3, 5] = math.inf
-    cache.archive.pack(kn, v[:, :, :70], cache._attended_spans[0][0] if cache._attended_spans else 0)
-    out = cache.attend(q, 173)
-    assert bool(torch.isnan(out[0, 2:]).all()) and bool(torch.isfinite(out[0, :2]).all())
+    q = queries(1, 4, Lq, 128)
+    row = cache.get_attention_segments().spans[0][0]
+    kn, vn = k[:, :, :70].clone(), v[:, :, :70].clone()
+    kn[0, 1, 3, 5] = math.inf  # packed as NaN: every row of KV head 1
+    vn[0, 0, 4, 7] = math.nan  # channel 7 of KV head 0
+    cache.archive.pack(kn, vn, row)
+    out = cache.attend(q, 174 - Lq)
+    assert bool(torch.isnan(out[0, 2:]).all())
+    fine = torch.ones(128, dtype=torch.bool, device="cuda")
+    fine[7] = False
+    assert bool(torch.isfinite(out[0, :2][..., fine]).all()) and bool(torch.isnan(out[0, :2, :, 7]).all())
 
 
 def test_values_of_very_different_size_and_large_logits():
@@ -295,11 +305,11 @@ def test_values_of_very_different_size_and_large_logits():
     v = (torch.randn(1, 1, 768, 128, generator=g, device="cuda") * level.repeat_interleave(64)[:, None]).to(torch.bfloat16)
     for i in range(12):
         cache.import_block(k[:, :, 64 * i:64 * i + 64], v[:, :, 64 * i:64 * i + 64], 64 * i)
-    for scale in (1.0, 60.0, 1e-30, 0.0):
-        q = queries(1, 4, 1, 128, scale=scale)
-        kk, vv = held(cache, k, v, lens)
-        want, want_lse = ref.attention(q, kk, vv, torch.arange(768), 767)
-        out, lse = cache.attend(q, 767, want_lse=True)
+    kk, vv = held(cache, k, v, lens)
+    for scale, Lq in ((1.0, 1), (60.0, 1), (1e-30, 1), (0.0, 1), (1.0, 20), (60.0, 20), (0.0, 20)):
+        q = queries(1, 4, Lq, 128, scale=scale)
+        want, want_lse = ref.attention(q, kk, vv, torch.arange(768), 768 - Lq)
+        out, lse = cache.attend(q, 768 - Lq, want_lse=True)
         # logits of `scale` times the usual size carry that many times the error
         tol = REL * max(1.0, scale) * float(vv.abs().max())
         assert float((out.double().cpu() - want).abs().max()) <= tol
@@ -509,3 +519,167 @@ def test_model_generates_through_a_packed_and_a_sparse_cache(kw):
     # bf16 activations: the two runs differ by roundings of one bf16 step here and there
     scale = float(logits[0].abs().max())
     assert float((logits[0] - logits[1]).abs().max()) <= 16 * 2.0 ** -8 * scale
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_offsets_past_32_bits(packed):
+    """Heads whose rows lie more than 2^31 elements into the archive (or arena), and its bounds."""
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (200,)
+    cache, k, v = make("bfloat16", 1, 8, 8, 128, lens, 10, tile_index=True, pool_tokens=2_500_032,
+                       archive_dtype="float8_e4m3fn" if packed else None)
+    rows = cache.archive.rows if packed else cache._arena_k.shape[1]
+    assert 7 * rows * 128 > 1 << 31
+    q = queries(1, 8, 1, 128)
+    kk, vv = held(cache, k, v, lens)
+    want, lse = ref.attention(q, kk, vv, torch.arange(210), 209)
+    out, got = cache.attend(q, 209, want_lse=True, top_tiles=4)
+    check_out(out, got, want, lse, vv)
+    if packed:
+        check_out(cache.attend(q, 209), None, want, lse, vv)
+        q = queries(1, 8, 70, 128)
+        want, lse = ref.attention(q, kk, vv, torch.arange(210), 140)
+        check_out(cache.attend(q, 140), None, want, lse, vv)
+    lo, hi, pos = ref.bounds(kk[:, :, :200], lens)
+    q = queries(1, 8, 1, 128)
+    assert torch.equal(cache.select_tiles(q, 209, 2).cpu().long(), ref.select(q, lo, hi, pos, 209, 2))
+
+
+def test_results_go_where_the_caller_says():
+    torch = _torch()
+    from rfsn_b200.cache import paged_attention
+
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (300,), 20, tile_index=True)
+    q = queries(1, 8, 1, 128)
+    segs = cache.get_attention_segments()
+    for top in (0, 2):
+        want = cache.attend(q, 319, top_tiles=top)
+        out = torch.empty_like(q)
+        assert paged_attention(cache, q, 319, segs, out=out, top_tiles=top) is out and torch.equal(out, want)
+        host = torch.empty(q.shape).pin_memory()
+        paged_attention(cache, q, 319, segs, out=host, top_tiles=top)
+        torch.cuda.synchronize()
+        assert torch.equal(host, want.cpu())
+        half = cache.attend(q.to(torch.bfloat16), 319, top_tiles=top)  # any float q is taken as float32
+        assert half.dtype == torch.float32 and torch.equal(half, cache.attend(q.to(torch.bfloat16).float(), 319,
+                                                                              top_tiles=top))
+        strided = torch.empty(1, 1, 8, 128, device="cuda").transpose(1, 2)
+        strided.copy_(q)
+        assert torch.equal(cache.attend(strided, 319, top_tiles=top), want)
+
+
+def test_segments_are_a_snapshot_of_the_window():
+    """A prepared call keeps the window of its segments; new segments see the appended token."""
+    torch = _torch()
+    import archive_ref as ref
+
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (300,), 20, hot_cap=64)
+    q = queries(1, 8, 1, 128)
+    old = cache.get_attention_segments()
+    before = cache.attend(q, 1000, old).clone()
+    extra = torch.randn(1, 2, 1, 128, device="cuda").to(torch.bfloat16)
+    cache.append_exact(extra, extra)
+    assert torch.equal(cache.attend(q, 1000, old), before)
+    kk, vv = held(cache, k, v, (300,))
+    kk, vv = (torch.cat([x, extra.double().cpu()], 2) for x in (kk, vv))
+    want, lse = ref.attention(q, kk, vv, torch.arange(321), 1000)
+    check_out(cache.attend(q, 1000), None, want, lse, vv)
+
+
+def test_refusals():
+    torch = _torch()
+    from rfsn_b200 import PackedArchive
+    from rfsn_b200.cache import paged_attention
+
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (300,), 20, tile_index=True)
+    plain, _, _ = make("bfloat16", 1, 8, 2, 128, (300,), 20, archive_dtype=None)
+    q = queries(1, 8, 1, 128)
+    for bad in (queries(2, 8, 1, 128), queries(1, 8, 1, 64), queries(1, 7, 1, 128)):
+        with pytest.raises(ValueError):
+            cache.attend(bad, 319)
+        with pytest.raises(ValueError):
+            cache.select_tiles(bad, 319, 2)
+    with pytest.raises(ValueError, match="tile_index"):
+        plain.attend(q, 319, top_tiles=2)
+    with pytest.raises(ValueError, match="tile_index"):
+        plain.select_tiles(q, 319, 2)
+    for top in (-1, (1 << 20) + 1):
+        with pytest.raises(ValueError):
+            cache.attend(q, 319, top_tiles=top)
+        with pytest.raises(ValueError):
+            cache.select_tiles(q, 319, top)
+    with pytest.raises(ValueError):
+        cache.select_tiles(q, 319, 0)
+    with pytest.raises(ValueError, match="64 query rows"):
+        cache.attend(queries(1, 8, 65, 128), 319, top_tiles=2)
+    with pytest.raises(ValueError, match="64 query rows"):
+        cache.select_tiles(queries(1, 8, 65, 128), 319, 2)
+    segs = cache.get_attention_segments()
+    with pytest.raises(NotImplementedError):
+        paged_attention(cache, q, 319, segs, peers=object())
+    with pytest.raises(ValueError, match="out must"):
+        paged_attention(cache, q, 319, segs, out=torch.empty(1, 8, 2, 128, device="cuda"))
+    empty, _, _ = make("bfloat16", 1, 8, 2, 128, (), 0, hot_cap=8)
+    with pytest.raises(RuntimeError):
+        empty.attend(q, 0)
+    a = PackedArchive(2, 128, 128)
+    x = torch.zeros(1, 2, 64, 128, device="cuda")
+    for bad in ((x[:, :, :, :64], x[:, :, :, :64]), (x[0], x[0]), (x, x[:, :, :32]), (x, x.half()), (x.cpu(), x.cpu()),
+                (x.double(), x.double()), (x[:, :1], x[:, :1])):
+        with pytest.raises(ValueError):
+            a.pack(*bad)
+    for row, n in ((1, 64), (128, 64), (-64, 64), (64, 128)):
+        with pytest.raises(ValueError):
+            a.pack(torch.zeros(1, 2, n, 128, device="cuda"), torch.zeros(1, 2, n, 128, device="cuda"), row)
+    with pytest.raises(ValueError, match="bounds"):
+        a.pack(x, x, bounds=torch.zeros(2, 2, 2, 128, device="cuda"))
+    for row, n in ((0, 129), (-1, 4), (128, 1)):
+        with pytest.raises(ValueError):
+            a.unpack(row, n, torch.float32)
+    with pytest.raises(ValueError):
+        a.unpack(0, 4, torch.float64)
+    with pytest.raises((ValueError, NotImplementedError)):
+        PackedArchive(2, 64, 96)
+    with pytest.raises(ValueError):
+        PackedArchive(0, 64, 128)
+    a.pack(x[:, :, :0], x[:, :, :0])  # nothing to do
+    assert a.unpack(0, 0, torch.float32)[0].shape == (2, 0, 128)
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    torch = _torch()
+    from rfsn_b200 import _native as native
+    from rfsn_b200.cache import paged_attention
+
+    caches = [make("bfloat16", 1, 8, 2, 128, (3000,), 20, tile_index=True, seed=i)[0] for i in range(2)]
+    q = queries(1, 8, 1, 128)
+    want = [[c.attend(q, 3019, top_tiles=top).clone() for top in (0, 5)] for c in caches]
+    streams = [torch.cuda.Stream() for _ in caches]
+    spaces = [native.Workspace(c.device) for c in caches]
+    segs = [c.get_attention_segments() for c in caches]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, c in enumerate(caches):
+            with torch.cuda.stream(streams[i]):
+                got[i].append([paged_attention(c, q, 3019, segs[i], workspace=spaces[i], top_tiles=top)
+                               for top in (0, 5)])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in got[i]:
+            assert torch.equal(pair[0], want[i][0]) and torch.equal(pair[1], want[i][1])
+
+
+def test_the_same_call_gives_the_same_bits():
+    torch = _torch()
+    cache, k, v = make("bfloat16", 1, 32, 8, 128, (1000,) * 8, 200, tile_index=True)
+    for Lq in (1, 4, 64):
+        q = queries(1, 32, Lq, 128)
+        want = cache.attend(q, 8200 - Lq).clone()
+        sparse = cache.attend(q, 8200 - Lq, top_tiles=9).clone()
+        for _ in range(5):
+            assert torch.equal(cache.attend(q, 8200 - Lq), want)
+            assert torch.equal(cache.attend(q, 8200 - Lq, top_tiles=9), sparse)
