@@ -499,11 +499,15 @@ RFSN_API rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* archive, int sr
  *     read again for every 8 query slots.
  * Scores are accurate to float32 rounding (q and p are split into two float16
  * or three bfloat16 terms for the tensor cores).
+ * A key behind a row's position changes nothing in it, with one exception: a
+ * NaN or infinity in its V reaches the rows that are computed together with a
+ * row that does see it (0 * NaN), so finite V is asked for where q_len > 1.
  * ---------------------------------------------------------------------- */
 typedef struct rfsn_tile_list {
     const int32_t* tiles; /* device int32 [n][4] = {row, pos, len, tile}: row of the tile's first token (a multiple
                            * of 64 for packed archives and for selection), its position, its tokens (0..64; 0: the
-                           * entry is skipped), its number */
+                           * entry is skipped), its number. Shared lists are in the order of their positions, a tile
+                           * listed twice counts twice */
     int32_t n;
     int32_t per_query; /* 0: one list for all heads and queries; 1: [batch * kv_heads][q_len][n][4], a list for each
                         * (batch, kv head, query row), as rfsn_select_tiles writes it */

@@ -127,7 +127,7 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
                        aligned16(workspace), "%s: NULL or misaligned pointer (q, out and workspace: 16 bytes)", what);
     RFSN_CHECK_ARG(hot->length >= 0 && hot->length <= hot->capacity && hot->head_index >= 0 &&
                        hot->head_index < (hot->capacity > 0 ? hot->capacity : 1) && hot->ring_row0 >= 0 &&
-                       hot->ring_row0 + hot->capacity <= arena->rows,
+                       hot->ring_row0 <= arena->rows && hot->capacity <= arena->rows - hot->ring_row0,
                    "%s: bad hot window", what);
     const bool stepped = hot->step_state != nullptr;
     if (tiles->n == 0 && hot->length == 0 && !stepped) {

@@ -428,6 +428,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     int qp[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) qp[nb] = q_pos0 + (slot0 + 4 * nb + t4) / p.G;
+    const int qlast = q_pos0 + (slot0 + nslots - 1) / p.G;  // keys behind it reach no slot of the CTA: neither K nor V is used
     State<D, NB> st;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -460,7 +461,8 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
         const uint32_t sb = smem_u32(sm.stage[s]);
         if (PACKED && inf.x) {
             const int k_strip = 16 * gwarp;
-            const bool mine = inf.z > k_strip;
+            const int seen = min(inf.z, qlast - inf.y + 1) - k_strip;
+            const bool mine = seen > 0;
             if (mine) {
                 const float4 sc = sm.meta[s];
                 const int ka = k_strip + (D == 128 ? cg : g), kb = ka + 8;  // rows ka and kb share the swizzle pattern
@@ -495,6 +497,16 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                         const uint2 y0 = at(v0), y1 = at(v1), y2 = at(v0 + 8), y3 = at(v1 + 8);
                         x0[0] = y0.x, x0[1] = y0.y, x1[0] = y1.x, x1[1] = y1.y;
                         x2[0] = y2.x, x2[1] = y2.y, x3[0] = y3.x, x3[1] = y3.y;
+                    }
+                    if (seen < 16) {
+                        const int k0 = v0 - k_strip, k1 = v1 - k_strip;
+#pragma unroll
+                        for (int w = 0; w < D / 32; ++w) {
+                            x0[w] = k0 < seen ? x0[w] : 0u;
+                            x1[w] = k1 < seen ? x1[w] : 0u;
+                            x2[w] = k0 + 8 < seen ? x2[w] : 0u;
+                            x3[w] = k1 + 8 < seen ? x3[w] : 0u;
+                        }
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.empty[s]);
@@ -550,7 +562,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
             // 16-bit item: HK / 16 strips; with two strips the group's warp pairs take turns
             const int strip = HK == 64 ? gwarp : (gwarp & 1);
             const bool mine = HK == 64 || (gwarp >> 1) == ((it / GROUPS) & 1);
-            const int sv = inf.z - 16 * strip;  // valid keys in the strip
+            const int sv = min(inf.z, qlast - inf.y + 1) - 16 * strip;  // keys of the strip that some slot sees
             if (mine && sv > 0) {
                 if (PACKED && packed_order) {  // first 16-bit strip after packed ones: reorder O's channels, q's fragments
                     packed_order = false;
@@ -607,7 +619,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                 }
                 uint32_t b[NB][2], b3[NB][2];
                 softmax_strip<T, D, NB, BF16>(st, s0, s1, 1.f, b, b3);
-                uint32_t m01 = 0xffffffffu, m23 = 0xffffffffu;  // rows behind the span hold anything: zero them
+                uint32_t m01 = 0xffffffffu, m23 = 0xffffffffu;  // rows that no slot sees hold anything: zero them
                 if (sv < 16) {
                     const int k2 = 2 * t4;
                     m01 = (k2 < sv ? 0x0000ffffu : 0u) | (k2 + 1 < sv ? 0xffff0000u : 0u);

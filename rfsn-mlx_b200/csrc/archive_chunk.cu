@@ -60,6 +60,8 @@ constexpr int kSoftmaxThreads = 256, kThreads = 512;
 constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;
 constexpr int kConvWarp = 8, kProducerWarp = 12, kMmaWarp = 13;
 constexpr int kMaxSplit = 32;  // key ranges of a unit
+constexpr float kTiny = 1.17549435e-38f;  // 2^-126
+constexpr float kMinF = 7.8886091e-31f;   // 2^-100
 constexpr uint32_t kTmemCols = 512, kColO = 256, kColQhi = 384, kColQlo = 448;
 
 struct Info {
@@ -177,9 +179,10 @@ __device__ __forceinline__ void split_half_rn(float a, float b, uint32_t& hi, ui
 // Codes of 128 keys -> float16 operand tile: a thread widens 16 codes (one
 // 16-byte chunk of a row) at a time. Eight lanes cover a row, and the lanes of
 // the upper channel half store their two chunks in the other order, so that
-// both the load and the stores meet every bank once. A half without keys is
-// zeroed (its staging holds an earlier tile).
-__device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, bool first, bool second) {
+// both the load and the stores meet every bank once. Rows from first (second)
+// of the two 64-key halves on are zeroed: a half without keys (its staging
+// holds an earlier tile), and V of keys that no query row of the CTA sees.
+__device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, int first, int second) {
     const int th = threadIdx.x & 127, c = th & 7, r0 = th >> 3;
     const int c0 = (2 * c) & 7, swap = c >> 2;
     // rows r0 + 16 i share r & 7, so the swizzled chunk offsets are the thread's own
@@ -189,9 +192,10 @@ __device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, bool f
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // the two 64-key halves, four loads in flight
         uint4 x[4];
-        const bool any = h ? second : first;
+        const int live = (h ? second : first) - r0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = any ? lds_u4(from + (64 * h + 16 * i) * 128) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; ++i)
+            x[i] = 16 * i < live ? lds_u4(from + (64 * h + 16 * i) * 128) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint4 a = make_uint4(widen(x[i].x), widen_hi(x[i].x), widen(x[i].y), widen_hi(x[i].y));
@@ -202,14 +206,17 @@ __device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, bool f
     }
 }
 
-// A float16 tile that is already in the operand's layout.
-__device__ __forceinline__ void copy_tile(uint32_t from, uint32_t op) {
+// A float16 tile that is already in the operand's layout; rows zeroed as above.
+__device__ __forceinline__ void copy_tile(uint32_t from, uint32_t op, int first, int second) {
     const int th = threadIdx.x & 127;
 #pragma unroll
     for (int i = 0; i < 2 * kHalfBytes / 16 / 128; i += 8) {
         uint4 x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = lds_u4(from + (128 * (i + j) + th) * 16);
+        for (int j = 0; j < 8; ++j) {
+            const int r = (16 * (i + j) + (th >> 3)) & (BN - 1);
+            x[j] = (r & 63) < (r < 64 ? first : second) ? lds_u4(from + (128 * (i + j) + th) * 16) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sts_u4(op + (128 * (i + j) + th) * 16, x[j]);
     }
@@ -306,12 +313,14 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                      warp_wait(&sm.c_full[slot & 1], (slot >> 1) & 1, &sm.abort) &&
                      (t < kStages || warp_wait(&sm.k_empty[s], ph ^ 1, &sm.abort));
                 if (!ok) break;
-                const bool first = sm.info[t % kInfo].len[0] > 0, second = sm.info[t % kInfo].len[1] > 0;
+                const Info& inf = sm.info[t % kInfo];
+                const int first = inf.len[0] > 0 ? 64 : 0, second = inf.len[1] > 0 ? 64 : 0;
+                const int v_first = min(inf.len[0], qlast - inf.pos[0] + 1), v_second = min(inf.len[1], qlast - inf.pos[1] + 1);
                 const uint32_t k_op = smem_u32(sm.k[s][0]), v_op = smem_u32(sm.v[s][0]);
                 if (arch) {
                     convert_tile(smem_u32(sm.staged[slot & 1]), k_op, first, second);
                 } else {
-                    copy_tile(smem_u32(sm.staged[slot & 1]), k_op);
+                    copy_tile(smem_u32(sm.staged[slot & 1]), k_op, first, second);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.c_empty[slot & 1]);
                     ++slot;
@@ -321,9 +330,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                      (t < kStages || warp_wait(&sm.v_empty[s], ph ^ 1, &sm.abort));
                 if (!ok) break;
                 if (arch)
-                    convert_tile(smem_u32(sm.staged[slot & 1]) + kCodeBytes, v_op, first, second);
+                    convert_tile(smem_u32(sm.staged[slot & 1]) + kCodeBytes, v_op, v_first, v_second);
                 else
-                    copy_tile(smem_u32(sm.staged[slot & 1]), v_op);
+                    copy_tile(smem_u32(sm.staged[slot & 1]), v_op, v_first, v_second);
                 publish(&sm.v_full[s]);
                 if (lane == 0) mbar_arrive(&sm.c_empty[slot & 1]);
                 ++slot;
@@ -341,7 +350,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                 // lanes 2 j, 2 j + 1 fetch the two halves of tile base + j
                 const int t_mine = base + (lane >> 1), gt = t_lo + t_mine, half = lane & 1;
                 int row = 0, pos = 0, len = 0;
-                float sk = 1.f, sv = 1.f;
+                float sk = 1.f, sv = kTiny;  // a half without keys leaves the unit to the other one
                 if (t_mine < nt) {
                     if (gt < arch_tiles) {
                         const int i = 2 * gt + half;
@@ -373,8 +382,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                 }
                 const int n = min(16, nt - base);
                 for (int j = 0; j < n && !stop; ++j) {
-                    const int t = base + j, s = t & 1;
-                    const uint32_t ph = (t >> 1) & 1;
+                    const int t = base + j;
                     int r[2];
                     Info inf;
 #pragma unroll
@@ -570,8 +578,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             const Info& inf = sm.info[t % kInfo];
             const int pos = inf.pos[ch], len = inf.len[ch];
             const float u = fmaxf(inf.sv[0], inf.sv[1]);
-            // p comes out of the exponential times f = 2^7 s_v / u; the row sum takes f off again once per tile
-            const float f = inf.sv[ch] / u * kPScale, c = qmul * inf.sk[ch];
+            // p comes out of the exponential times f = 2^7 s_v / u; the row sum takes f off again once per tile. Both
+            // factors stay normal numbers: a product below them is lost beside the other half (f) or a logit of 0 (c).
+            const float f = fmaxf(inf.sv[ch] / u * kPScale, kMinF), c = fmaxf(qmul * inf.sk[ch], kTiny);
             const float lf = log2f(f);
             if (!warp_wait(&sm.s_full[s], (t >> 1) & 1, &sm.abort)) { failed = true; break; }
             tc::fence_after_sync();

@@ -291,11 +291,11 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         f.e = make_int4(0, 0, 0, 0);
         f.sk = 1.f;
         if (t < t_end) f.e = __ldcg(p.tiles + t);
-        if ((f.e.x & (kTile - 1)) != 0 || f.e.x < 0 || f.e.x / kTile >= p.tile_slots) {
+        if (f.e.z > 0 && ((f.e.x & (kTile - 1)) != 0 || f.e.x < 0 || f.e.x / kTile >= p.tile_slots)) {
             atomicExch(p.error, kDevErrBadTable);
-            f.e.x = f.e.z = 0;
+            f.e.z = 0;
         }
-        const size_t slot = (size_t)bh * p.tile_slots + f.e.x / kTile;
+        const size_t slot = (size_t)bh * p.tile_slots + (f.e.z > 0 ? f.e.x / kTile : 0);
         const char* base = static_cast<const char*>(p.bounds) + slot * 2 * D * sizeof(T);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {  // lanes read consecutive vectors

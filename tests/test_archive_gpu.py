@@ -24,7 +24,7 @@ def _torch():
 
 
 def make(dtype="bfloat16", B=1, H=8, Hkv=2, D=128, lens=(100, 64, 1), hot=50, hot_cap=None, wrap=0, seed=0,
-         archive_dtype="float8_e4m3fn", tile_index=False, top_tiles=0, scale=1.0, **kw):
+         archive_dtype="float8_e4m3fn", tile_index=False, top_tiles=0, scale=1.0, v_scale=1.0, **kw):
     """A layer cache with the given archived blocks and ``hot`` ring tokens (the ring's oldest at slot ``wrap``), and
     its keys and values [B, Hkv, N + hot, D]."""
     torch = _torch()
@@ -39,7 +39,7 @@ def make(dtype="bfloat16", B=1, H=8, Hkv=2, D=128, lens=(100, 64, 1), hot=50, ho
     cache = LayerKVCache(cfg, B, H, Hkv, session_id="t", archive_dtype=archive_dtype, tile_index=tile_index,
                          top_tiles=top_tiles, **kw)
     k = (torch.randn(B, Hkv, n, D, generator=g, device="cuda") * scale).to(cache.dtype)
-    v = torch.randn(B, Hkv, n, D, generator=g, device="cuda").to(cache.dtype)
+    v = (torch.randn(B, Hkv, n, D, generator=g, device="cuda") * v_scale).to(cache.dtype)
     at = 0
     for length in lens:
         cache.import_block(k[:, :, at:at + length], v[:, :, at:at + length], at)
@@ -683,3 +683,82 @@ def test_the_same_call_gives_the_same_bits():
         for _ in range(5):
             assert torch.equal(cache.attend(q, 8200 - Lq), want)
             assert torch.equal(cache.attend(q, 8200 - Lq, top_tiles=9), sparse)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("Lq", [1, 3, 40])
+def test_keys_and_values_behind_the_queries_are_not_touched(packed, Lq):
+    """NaN K and V at every position behind the last query, in its own tile too."""
+    torch = _torch()
+    lens = (130, 64)
+    tops = (0, 9) if packed else (9,)  # without either option the call is that of an exact cache
+    for last in (20, 129, 150, 200, 215):
+        cache, k, v = make("bfloat16", 1, 4, 2, 128, lens, 40, tile_index=True,
+                           archive_dtype="float8_e4m3fn" if packed else None)
+        q = queries(1, 4, Lq, 128)
+        first = last + 1 - Lq
+        if first < 0:
+            continue
+        want = [cache.attend(q, first, top_tiles=top, want_lse=True) for top in tops]
+        bad_k, bad_v = k.clone(), v.clone()
+        for x in (bad_k, bad_v):
+            x[:, :, last + 1:] = math.nan
+        spans = cache.get_attention_segments().spans
+        for (row, start, n) in spans[:2]:
+            kk, vv = bad_k[:, :, start:start + n], bad_v[:, :, start:start + n]
+            if packed:  # codes only: the scales are those of the finite tiles
+                codes = cache.archive.k.view(torch.uint8), cache.archive.v.view(torch.uint8)
+                for c in codes:
+                    c[:, row:row + n][:, max(0, last + 1 - start):] = 0x7F
+            else:
+                cache._arena_k[:, row:row + n] = kk[0]
+                cache._arena_v[:, row:row + n] = vv[0]
+        ring = max(0, last + 1 - 194)
+        cache._arena_k[:, ring:40] = math.nan
+        cache._arena_v[:, ring:40] = math.nan
+        for top, (out, lse) in zip(tops, want):
+            got, got_lse = cache.attend(q, first, top_tiles=top, want_lse=True)
+            assert torch.equal(got, out) and torch.equal(got_lse, lse), (last, top)
+
+
+@pytest.mark.parametrize("Lq", [1, 40])
+@pytest.mark.parametrize("v_scale", [1e-6, 1e-30, 1e30])
+@pytest.mark.parametrize("lens", [(64,), (64, 64), (50, 64, 64), ()])
+def test_small_and_large_values(Lq, v_scale, lens):
+    """V far from 1, an odd number of tiles: the halves without keys and the ring do not set the unit."""
+    torch = _torch()
+    import archive_ref as ref
+
+    n = sum(lens) + 70
+    torch.manual_seed(5)
+    cache, k, v = make("bfloat16", 1, 4, 1, 128, lens, 70, v_scale=v_scale)
+    q = queries(1, 4, Lq, 128)
+    kk, vv = held(cache, k, v, lens)
+    want, lse = ref.attention(q, kk, vv, torch.arange(n), n - Lq)
+    out, got = cache.attend(q, n - Lq, want_lse=True)
+    check_out(out, got, want, lse, vv)
+
+
+def test_a_vanishing_product_of_scales_masks_like_any_other():
+    """q and K so small that their scales' product underflows: logits 0, masked keys still masked."""
+    torch = _torch()
+    import archive_ref as ref
+
+    cache, k, v = make("bfloat16", 1, 4, 1, 128, (64, 30), 0, hot_cap=8, scale=1e-20)
+    for Lq in (1, 40):
+        q = queries(1, 4, Lq, 128, scale=1e-36)
+        kk, vv = held(cache, k, v, (64, 30))
+        want, lse = ref.attention(q, kk, vv, torch.arange(94), 94 - Lq)
+        out, got = cache.attend(q, 94 - Lq, want_lse=True)
+        check_out(out, got, want, lse, vv)
+
+
+def test_a_selection_from_no_tiles_reports_nothing():
+    torch = _torch()
+    from rfsn_b200 import _native as native
+
+    cache, _, _ = make("bfloat16", 1, 4, 2, 128, (), 20, hot_cap=32, tile_index=True)
+    q = queries(1, 4, 1, 128)
+    assert bool((cache.select_tiles(q, 19, 3) == -1).all())
+    assert torch.equal(cache.attend(q, 19, top_tiles=3), cache.attend(q, 19))
+    native.default_workspace(cache.device).check()
