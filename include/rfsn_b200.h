@@ -569,9 +569,15 @@ typedef struct rfsn_archive_call {
 RFSN_API rfsn_status rfsn_archive_attend(const rfsn_archive_call* call, const float* q, int q_pos0, float* out,
                                          float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The tiles that rfsn_archive_attend of this call (top_tiles > 0) reads for q:
+ * their numbers, int32 [batch * kv_heads][q_len][top_tiles], ascending, -1
+ * behind them. */
+RFSN_API rfsn_status rfsn_archive_select(const rfsn_archive_call* call, const float* q, int q_pos0, int32_t* numbers,
+                                         void* workspace, size_t workspace_bytes, void* stream);
+
 /* Workspace bytes of rfsn_archive_attention (n_select = 0: shared lists;
- * > 0: lists per query), rfsn_select_tiles (n_select > 0) and
- * rfsn_archive_attend (n_select = top_tiles) over up to n_tiles tiles and a
+ * > 0: lists per query), rfsn_select_tiles (n_select > 0), rfsn_archive_attend
+ * and rfsn_archive_select (n_select = top_tiles) over up to n_tiles tiles and a
  * hot window of up to hot_capacity tokens. Conventions as for rfsn_attention_workspace_size; one workspace
  * serves all attention calls ordered on one stream. */
 RFSN_API rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, int q_len, int head_dim,

@@ -55,7 +55,8 @@ struct SelectParams {
     int q_heads, kv_heads, q_len, q_pos0, G;
     const int4* tiles;
     int n_tiles, n_select, tiles_per_cta;
-    int4* out;              // [groups * q_len][n_select]
+    int4* out;              // [groups * q_len][n_select] tiles, or
+    int* numbers;           // their numbers only (out is nullptr)
     float* scores;          // workspace [groups * q_len][n_tiles]
     int* counters;
     int* error;

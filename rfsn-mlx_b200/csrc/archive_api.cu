@@ -192,6 +192,69 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     return archive_attn_launch(arena, packed, p, sp.lists, sp.nb, sp.zblocks, static_cast<cudaStream_t>(stream));
 }
 
+// numbers: out receives the tiles' numbers ([lists][n_select]) instead of their entries
+rfsn_status select(const char* what, const void* bounds, int bounds_dtype, const float* scales, int rows, const float* q,
+                   int batch, int q_heads, int kv_heads, int q_len, int head_dim, int q_pos0,
+                   const rfsn_tile_list* tiles, int n_select, int32_t* out, bool numbers, const int32_t* step_state,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, true, what);
+    if (st == RFSN_OK) st = check_tiles(tiles, what);
+    if (st != RFSN_OK) return st;
+    RFSN_CHECK_ARG(tiles->per_query == 0, "%s: selects from one list for all heads and queries", what);
+    RFSN_CHECK_ARG(q != nullptr && aligned16(q) && out != nullptr && aligned16(out) && workspace != nullptr &&
+                       aligned16(workspace), "%s: NULL or misaligned pointer (q, out and workspace: 16 bytes)", what);
+    RFSN_CHECK_ARG(bounds_dtype == RFSN_F16 || bounds_dtype == RFSN_BF16 || bounds_dtype == RFSN_E4M3,
+                   "%s: bounds must be f16, bf16 or e4m3", what);
+    RFSN_CHECK_ARG(tiles->n == 0 || (bounds != nullptr && aligned16(bounds)), "%s: NULL or misaligned bounds", what);
+    RFSN_CHECK_ARG(tiles->n == 0 || bounds_dtype != RFSN_E4M3 || (scales != nullptr && aligned16(scales)),
+                   "%s: e4m3 bounds need the archive's scales", what);
+    RFSN_CHECK_ARG(rows >= 0 && rows % kTile == 0, "%s: rows (%d) must be a multiple of %d", what, rows, kTile);
+    RFSN_CHECK_ARG(n_select > 0 && n_select <= (1 << 20), "%s: n_select %d outside [1, %d]", what, n_select, 1 << 20);
+    const int lists = batch * kv_heads * q_len;
+    RFSN_CHECK_ARG(lists <= kMaxCounters, "%s: batch * kv_heads * q_len above %d", what, kMaxCounters);
+    const size_t off = select_scores_offset(), need = off + sizeof(float) * (size_t)lists * tiles->n;
+    if (workspace_bytes < need) {
+        set_error("%s: workspace too small: need %zu bytes, have %zu", what, need, workspace_bytes);
+        return RFSN_ERR_OVERFLOW;
+    }
+    char* ws = static_cast<char*>(workspace);
+    archive::SelectParams p;
+    memset(&p, 0, sizeof(p));
+    p.bounds = bounds;
+    p.scales = reinterpret_cast<const float4*>(scales);
+    p.tile_slots = rows / kTile;
+    p.q = q;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.q_len = q_len;
+    p.q_pos0 = q_pos0;
+    p.G = q_heads / kv_heads;
+    p.tiles = reinterpret_cast<const int4*>(tiles->tiles);
+    p.n_tiles = tiles->n;
+    p.n_select = n_select;
+    p.out = numbers ? nullptr : reinterpret_cast<int4*>(out);
+    p.numbers = numbers ? out : nullptr;
+    p.scores = reinterpret_cast<float*>(ws + off);
+    p.counters = reinterpret_cast<int*>(ws + 256);
+    p.error = reinterpret_cast<int*>(ws);
+    p.dyn = step_state;
+    // one CTA per SM over all lists, in steps of the 128 tiles that a CTA scores at once
+    const int want = std::max(1, device_sms() / lists);
+    p.tiles_per_cta = std::max(128, ((tiles->n + want - 1) / want + 127) / 128 * 128);
+    const int chunks = std::max(1, (tiles->n + p.tiles_per_cta - 1) / p.tiles_per_cta);
+    return select_tiles_launch(bounds_dtype, head_dim, p, lists, chunks, static_cast<cudaStream_t>(stream));
+}
+
+rfsn_status select_call(const char* what, const rfsn_archive_call* c, const float* q, int q_pos0, int32_t* out,
+                        bool numbers, void* workspace, size_t workspace_bytes, void* stream) {
+    const rfsn_packed_archive* pk = c->packed;
+    return select(what, c->bounds, pk != nullptr ? RFSN_E4M3 : c->arena->dtype,
+                  pk != nullptr ? reinterpret_cast<const float*>(pk->scales) : nullptr,
+                  pk != nullptr ? pk->rows : c->arena->rows, q, c->batch, c->q_heads, c->kv_heads, c->q_len,
+                  c->arena->head_dim, q_pos0, &c->tiles, c->top_tiles, out, numbers, c->hot.step_state, workspace,
+                  workspace_bytes, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -318,52 +381,8 @@ rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float*
                               int batch, int q_heads, int kv_heads, int q_len, int head_dim, int q_pos0,
                               const rfsn_tile_list* tiles, int n_select, int32_t* out, const int32_t* step_state,
                               void* workspace, size_t workspace_bytes, void* stream) {
-    const char* what = "rfsn_select_tiles";
-    rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, true, what);
-    if (st == RFSN_OK) st = check_tiles(tiles, what);
-    if (st != RFSN_OK) return st;
-    RFSN_CHECK_ARG(tiles->per_query == 0, "%s: selects from one list for all heads and queries", what);
-    RFSN_CHECK_ARG(q != nullptr && aligned16(q) && out != nullptr && aligned16(out) && workspace != nullptr &&
-                       aligned16(workspace), "%s: NULL or misaligned pointer (q, out and workspace: 16 bytes)", what);
-    RFSN_CHECK_ARG(bounds_dtype == RFSN_F16 || bounds_dtype == RFSN_BF16 || bounds_dtype == RFSN_E4M3,
-                   "%s: bounds must be f16, bf16 or e4m3", what);
-    RFSN_CHECK_ARG(tiles->n == 0 || (bounds != nullptr && aligned16(bounds)), "%s: NULL or misaligned bounds", what);
-    RFSN_CHECK_ARG(tiles->n == 0 || bounds_dtype != RFSN_E4M3 || (scales != nullptr && aligned16(scales)),
-                   "%s: e4m3 bounds need the archive's scales", what);
-    RFSN_CHECK_ARG(rows >= 0 && rows % kTile == 0, "%s: rows (%d) must be a multiple of %d", what, rows, kTile);
-    RFSN_CHECK_ARG(n_select > 0 && n_select <= (1 << 20), "%s: n_select %d outside [1, %d]", what, n_select, 1 << 20);
-    const int lists = batch * kv_heads * q_len;
-    RFSN_CHECK_ARG(lists <= kMaxCounters, "%s: batch * kv_heads * q_len above %d", what, kMaxCounters);
-    const size_t off = select_scores_offset(), need = off + sizeof(float) * (size_t)lists * tiles->n;
-    if (workspace_bytes < need) {
-        set_error("%s: workspace too small: need %zu bytes, have %zu", what, need, workspace_bytes);
-        return RFSN_ERR_OVERFLOW;
-    }
-    char* ws = static_cast<char*>(workspace);
-    archive::SelectParams p;
-    memset(&p, 0, sizeof(p));
-    p.bounds = bounds;
-    p.scales = reinterpret_cast<const float4*>(scales);
-    p.tile_slots = rows / kTile;
-    p.q = q;
-    p.q_heads = q_heads;
-    p.kv_heads = kv_heads;
-    p.q_len = q_len;
-    p.q_pos0 = q_pos0;
-    p.G = q_heads / kv_heads;
-    p.tiles = reinterpret_cast<const int4*>(tiles->tiles);
-    p.n_tiles = tiles->n;
-    p.n_select = n_select;
-    p.out = reinterpret_cast<int4*>(out);
-    p.scores = reinterpret_cast<float*>(ws + off);
-    p.counters = reinterpret_cast<int*>(ws + 256);
-    p.error = reinterpret_cast<int*>(ws);
-    p.dyn = step_state;
-    // one CTA per SM over all lists, in steps of the 128 tiles that a CTA scores at once
-    const int want = std::max(1, device_sms() / lists);
-    p.tiles_per_cta = std::max(128, ((tiles->n + want - 1) / want + 127) / 128 * 128);
-    const int chunks = std::max(1, (tiles->n + p.tiles_per_cta - 1) / p.tiles_per_cta);
-    return select_tiles_launch(bounds_dtype, head_dim, p, lists, chunks, static_cast<cudaStream_t>(stream));
+    return select("rfsn_select_tiles", bounds, bounds_dtype, scales, rows, q, batch, q_heads, kv_heads, q_len, head_dim,
+                  q_pos0, tiles, n_select, out, false, step_state, workspace, workspace_bytes, stream);
 }
 
 rfsn_status rfsn_archive_attention(const rfsn_arena* arena, const rfsn_packed_archive* packed, const float* q,
@@ -401,15 +420,23 @@ rfsn_status rfsn_archive_attend(const rfsn_archive_call* c, const float* q, int 
     st = attention(c->arena, c->packed, q, c->batch, c->q_heads, c->kv_heads, c->q_len, q_pos0, &chosen, &c->hot, out,
                    lse, workspace, off, c->max_splits, stream, true);
     if (st != RFSN_OK) return st;
-    const rfsn_packed_archive* pk = c->packed;
-    st = rfsn_select_tiles(c->bounds, pk != nullptr ? RFSN_E4M3 : c->arena->dtype,
-                           pk != nullptr ? reinterpret_cast<const float*>(pk->scales) : nullptr,
-                           pk != nullptr ? pk->rows : c->arena->rows, q, c->batch, c->q_heads, c->kv_heads, c->q_len,
-                           head_dim, q_pos0, &c->tiles, c->top_tiles, const_cast<int32_t*>(chosen.tiles),
-                           c->hot.step_state, workspace, off, stream);
+    st = select_call(what, c, q, q_pos0, const_cast<int32_t*>(chosen.tiles), false, workspace, off, stream);
     if (st != RFSN_OK) return st;
     return attention(c->arena, c->packed, q, c->batch, c->q_heads, c->kv_heads, c->q_len, q_pos0, &chosen, &c->hot, out,
                      lse, workspace, off, c->max_splits, stream, false);
+}
+
+rfsn_status rfsn_archive_select(const rfsn_archive_call* c, const float* q, int q_pos0, int32_t* numbers,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "rfsn_archive_select";
+    RFSN_CHECK_ARG(c != nullptr && c->arena != nullptr, "%s: NULL call", what);
+    RFSN_CHECK_ARG(c->batch > 0 && c->kv_heads > 0 && c->batch * c->kv_heads == c->arena->groups &&
+                       (c->packed == nullptr || (c->packed->groups == c->arena->groups &&
+                                                 c->packed->head_dim == c->arena->head_dim)),
+                   "%s: heads or head_dim differ from the arena's", what);
+    rfsn_status st = check_device(c->arena->device, what);
+    if (st != RFSN_OK) return st;
+    return select_call(what, c, q, q_pos0, numbers, true, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -84,7 +84,7 @@ struct SelShared {
 // range. Two passes as a rule (the first bucket holds a few keys, the second
 // separates them), four at most; integer counts, so any order gives the same.
 template <bool REGS>
-__device__ __forceinline__ void select_list(const SelectParams& p, const float* scores, int4* out, SelShared& sh) {
+__device__ __forceinline__ void select_list(const SelectParams& p, const float* scores, int list, SelShared& sh) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int T_ = p.n_tiles;
     uint32_t key[REGS ? kSelRegKeys : 1];
@@ -173,6 +173,19 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
     // Write in tile order: keys above the threshold all, keys equal to it from
     // the lowest tile on (all of them, unless the bucket was one key).
     const unsigned below = (1u << lane) - 1u;
+    const size_t base = (size_t)list * p.n_select;
+    auto put = [&](int i, int t) {
+        if (p.numbers != nullptr) {
+            p.numbers[base + i] = t;
+            return;
+        }
+        int4 x = make_int4(0, 0, 0, -1);
+        if (t >= 0) {
+            x = __ldg(p.tiles + t);
+            x.w = t;
+        }
+        p.out[base + i] = x;
+    };
     if (REGS) {
 #pragma unroll
         for (int i = 0; i < kSelRegKeys; ++i) {
@@ -202,12 +215,7 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
             const bool gt = k > thr, eq = k == thr;
             const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
             const int g = (before & 0xffff) + __popc(mg & below), e = (before >> 16) + __popc(me & below);
-            if (gt || (eq && e < need)) {
-                const int t = tid + kSelThreads * i;
-                int4 x = __ldg(p.tiles + t);
-                x.w = t;
-                out[g + min(e, need)] = x;
-            }
+            if (gt || (eq && e < need)) put(g + min(e, need), tid + kSelThreads * i);
         }
     } else {
         // each warp owns a run of tiles
@@ -242,16 +250,12 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
             const bool is_gt = t < r1 && k > thr, is_eq = t < r1 && k == thr;
             const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
             const int g = gt_before + __popc(mg & below), e = eq_before + __popc(me & below);
-            if (is_gt || (is_eq && e < need)) {
-                int4 x = __ldg(p.tiles + t);
-                x.w = t;
-                out[g + min(e, need)] = x;
-            }
+            if (is_gt || (is_eq && e < need)) put(g + min(e, need), t);
             gt_before += __popc(mg);
             eq_before += __popc(me);
         }
     }
-    for (int i = n + tid; i < p.n_select; i += kSelThreads) out[i] = make_int4(0, 0, 0, -1);
+    for (int i = n + tid; i < p.n_select; i += kSelThreads) put(i, -1);
 }
 
 // Eight lanes score kTilesPerLane tiles side by side (each q pair fetched from
@@ -402,11 +406,10 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         __syncthreads();
         if (!sh.flag) return;
     }
-    int4* out = p.out + (size_t)list * p.n_select;
     if (p.n_tiles <= kSelRegKeys * kSelThreads)
-        select_list<true>(p, scores, out, sh);
+        select_list<true>(p, scores, list, sh);
     else
-        select_list<false>(p, scores, out, sh);
+        select_list<false>(p, scores, list, sh);
     if (gridDim.x > 1 && tid == 0) p.counters[list] = 0;
 }
 

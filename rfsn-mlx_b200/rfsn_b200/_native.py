@@ -80,6 +80,7 @@ EXPORTED_SYMBOLS = (
     "rfsn_select_tiles",
     "rfsn_archive_attention",
     "rfsn_archive_attend",
+    "rfsn_archive_select",
     "rfsn_archive_workspace_size",
 )
 
@@ -247,6 +248,7 @@ def load_library() -> ctypes.CDLL:
         "rfsn_archive_attention": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, ctypes.POINTER(TileListC),
                                          ctypes.POINTER(HotWindowC), vp, vp, vp, sz, i32, vp]),
         "rfsn_archive_attend": (i32, [ctypes.POINTER(ArchiveCallC), vp, i32, vp, vp, vp, sz, vp]),
+        "rfsn_archive_select": (i32, [ctypes.POINTER(ArchiveCallC), vp, i32, vp, vp, sz, vp]),
         "rfsn_archive_workspace_size": (i32, [i32] * 8 + [ctypes.POINTER(sz)]),
     }
     for name, (res, args) in sig.items():

@@ -9,7 +9,7 @@ extensions of ``LayerKVCache`` live here:
   and for V, so an attention call reads half the bytes. The hot ring keeps the
   cache dtype. ``PackedArchive`` owns the codes; ``pack`` and ``unpack`` convert.
 * **Tile selection** (``tile_index=True``): the cache keeps the channel-wise
-  smallest and largest key of every archived tile. ``rfsn_select_tiles`` bounds the
+  smallest and largest key of every archived tile. The selection bounds the
   logits of each tile with them and picks the ``top_tiles`` best for each query
   and KV head; attention then reads those tiles and the hot window only. The
   result is the exact softmax over the keys that are read; the tiles left out
@@ -50,9 +50,10 @@ def check_archive_options(dtype: torch.dtype, head_dim: int, archive_dtype: Opti
 
 def kv_rows(k: torch.Tensor, v: torch.Tensor, offset: int = 0, wrap: int = 0) -> native.KvRowsC:
     """Description of K/V [B, Hkv, n, D] for ``rfsn_pack_rows`` (innermost stride 1)."""
-    ks, vs = k.stride(), v.stride()
-    return native.KvRowsC(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                          native.dtype_code(k.dtype), int(k.shape[1]), offset, wrap)
+    kb, kh, kt, _ = k.stride()
+    vb, vh, vt, _ = v.stride()
+    return native.KvRowsC(k.data_ptr(), v.data_ptr(), kb, kh, kt, vb, vh, vt, native.dtype_code(k.dtype), k.shape[1],
+                          offset, wrap)
 
 
 class PackedArchive:
@@ -112,39 +113,42 @@ class PackedArchive:
         (``row`` a multiple of 64), in tiles of 64 from the first token on. The
         rest of the last tile is zeroed. ``bounds`` (uint8 [groups, rows / 64,
         2, D]) receives the channel-wise smallest and largest K codes."""
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 4 or v.shape != shape or v.dtype != dtype:
             raise ValueError("pack needs k and v of one shape [B, Hkv, n, D] and one dtype")
-        if k.shape[0] * k.shape[1] != self.groups or k.shape[3] != self.head_dim:
-            raise ValueError(f"K/V of shape {tuple(k.shape)} do not fit {self.groups} heads of {self.head_dim}")
+        if shape[0] * shape[1] != self.groups or shape[3] != self.head_dim:
+            raise ValueError(f"K/V of shape {tuple(shape)} do not fit {self.groups} heads of {self.head_dim}")
         if k.device != self.device or v.device != self.device:
             raise ValueError(f"K/V must be on {self.device}")
-        self._check_bounds(bounds)
+        if bounds is not None:
+            self._check_bounds(bounds)
         if k.stride(3) != 1:
             k = k.contiguous()
         if v.stride(3) != 1:
             v = v.contiguous()
-        self._pack(kv_rows(k, v), int(row), int(k.shape[2]), bounds)
+        self._pack(kv_rows(k, v), int(row), shape[2], bounds)
 
     def pack_ring(self, k: torch.Tensor, v: torch.Tensor, offset: int, wrap: int, row: int, count: int, *,
                   bounds: Optional[torch.Tensor] = None) -> None:
         """``pack`` of ``count`` ring tokens: k, v [groups, ring rows, D], the
         oldest token at ``offset``, wrapping at ``wrap``."""
-        self._check_bounds(bounds)
+        if bounds is not None:
+            self._check_bounds(bounds)
         self._pack(kv_rows(k[None], v[None], offset, wrap), row, count, bounds)
 
-    def _check_bounds(self, bounds: Optional[torch.Tensor]) -> None:
+    def _check_bounds(self, bounds: torch.Tensor) -> None:
         shape = (self.groups, self.rows // TILE, 2, self.head_dim)
-        if bounds is not None and (tuple(bounds.shape) != shape or bounds.dtype != torch.uint8
-                                   or bounds.device != self.device or not bounds.is_contiguous()):
+        if tuple(bounds.shape) != shape or bounds.dtype != torch.uint8 or bounds.device != self.device \
+                or not bounds.is_contiguous():
             raise ValueError(f"bounds must be a contiguous uint8 tensor of shape {shape} on {self.device}")
 
     def _pack(self, rows: native.KvRowsC, row: int, count: int, bounds: Optional[torch.Tensor]) -> None:
         with native.on_device(self.device):
-            native.check(
-                native.lib().rfsn_pack_rows(self.handle, row, ctypes.byref(rows), count,
-                                            bounds.data_ptr() if bounds is not None else None, native.stream_ptr()),
-                "rfsn_pack_rows",
-            )
+            status = native.lib().rfsn_pack_rows(self.handle, row, ctypes.byref(rows), count,
+                                                 bounds.data_ptr() if bounds is not None else None,
+                                                 native.stream_ptr())
+        if status:
+            native.check(status, "rfsn_pack_rows")
 
     def unpack(self, row: int, n: int, dtype: torch.dtype, *, out: Optional[tuple] = None):
         """(k, v) [groups, n, D] of rows row .. row + n in ``dtype`` (exact in
@@ -181,50 +185,19 @@ def workspace_bytes(batch: int, q_heads: int, kv_heads: int, q_len: int, head_di
     return int(out.value)
 
 
-class PreparedSelection:
-    """The part of ``rfsn_select_tiles`` that does not depend on the query, for
-    one cache, its segments' tiles and one query shape."""
-
-    __slots__ = ("before", "between", "shape", "nbytes", "keep")
-
-    def __init__(self, cache, segments, q_heads: int, q_len: int, top_tiles: int) -> None:
-        if cache.tile_bounds is None:
-            raise ValueError("tile selection needs a cache built with tile_index=True")
-        if not 1 <= top_tiles <= 1 << 20:
-            raise ValueError(f"top_tiles must be at least 1, got {top_tiles}")
-        if q_len > SPARSE_MAX_ROWS:
-            raise ValueError(f"tile selection takes up to {SPARSE_MAX_ROWS} query rows a call, got {q_len}")
-        B, Hkv, D = cache.batch_size, cache.num_kv_heads, cache.config.head_dim
-        tiles_dev, n_tiles = segments.tile_list
-        tiles = native.TileListC(tiles_dev.data_ptr(), n_tiles, 0)
-        archive, bounds = cache.archive, cache.tile_bounds
-        self.before = (bounds.data_ptr(), native.RFSN_E4M3 if archive is not None else native.dtype_code(bounds.dtype),
-                       archive.scales.data_ptr() if archive is not None else None, int(bounds.shape[1]) * TILE)
-        self.between = (B, q_heads, Hkv, q_len, D)
-        self.shape = (B, Hkv, q_len, top_tiles, 4)
-        self.nbytes = workspace_bytes(B, q_heads, Hkv, q_len, D, cache.config.hot_capacity, n_tiles, top_tiles)
-        self.keep = (ctypes.byref(tiles), tiles, archive, bounds, tiles_dev)
-
-    def __call__(self, cache, q: torch.Tensor, q_start_pos: int) -> torch.Tensor:
-        """Tile list int32 [B, Hkv, q_len, top_tiles, 4] = {row, pos, len, tile}."""
-        out = torch.empty(self.shape, dtype=torch.int32, device=cache.device)
-        buf = native.default_workspace(cache.device).get(self.nbytes)
-        status = native.lib().rfsn_select_tiles(*self.before, q.data_ptr(), *self.between, q_start_pos, self.keep[0],
-                                                self.shape[3], out.data_ptr(), None, buf.data_ptr(), buf.numel(),
-                                                native.stream_ptr())
-        if status:
-            native.check(status, "rfsn_select_tiles")
-        return out
-
-
 class PreparedCall:
     """``rfsn_archive_call`` of a layer's segments for one query shape, and the
-    buffers it points to (kept alive with it)."""
+    buffers it points to (kept alive with it). ``select_only`` prepares a call
+    of ``select`` (no hot window)."""
 
-    __slots__ = ("ref", "nbytes", "keep")
+    __slots__ = ("ref", "nbytes", "numbers", "keep")
 
     def __init__(self, cache, segments, hot: native.HotWindowC, q_heads: int, q_len: int, top_tiles: int,
-                 max_splits: int) -> None:
+                 max_splits: int, select_only: bool = False) -> None:
+        if (top_tiles or select_only) and cache.tile_bounds is None:
+            raise ValueError("tile selection needs a cache built with tile_index=True")
+        if not int(select_only) <= top_tiles <= 1 << 20:
+            raise ValueError(f"top_tiles must be between {int(select_only)} and {1 << 20}, got {top_tiles}")
         if top_tiles and q_len > SPARSE_MAX_ROWS:
             raise ValueError(f"top_tiles takes up to {SPARSE_MAX_ROWS} query rows a call, got {q_len}")
         tiles_dev, n_tiles = segments.tile_list
@@ -235,8 +208,14 @@ class PreparedCall:
             cache.batch_size, q_heads, cache.num_kv_heads, q_len, top_tiles, max_splits)
         self.ref = ctypes.byref(call)
         self.nbytes = workspace_bytes(cache.batch_size, q_heads, cache.num_kv_heads, q_len, cache.config.head_dim,
-                                      cache.config.hot_capacity, n_tiles, top_tiles if n_tiles else 0)
+                                      cache.config.hot_capacity, n_tiles, top_tiles if n_tiles or select_only else 0)
+        self.numbers = torch.empty((cache.batch_size, cache.num_kv_heads, q_len, top_tiles), dtype=torch.int32,
+                                   device=cache.device) if select_only else None  # shape of a selection
         self.keep = (call, cache.arena, archive, bounds, tiles_dev)
+
+    def current(self, cache) -> bool:
+        """The cache's buffers are still the ones this call points to."""
+        return self.keep[1] is cache.arena and self.keep[2] is cache.archive
 
     def __call__(self, cache, q_ptr: int, q_start_pos: int, out_ptr: int, lse_ptr: Optional[int],
                  workspace: Optional[native.Workspace]) -> None:
@@ -247,5 +226,16 @@ class PreparedCall:
         if status:
             native.check(status, "rfsn_archive_attend")
 
+    def select(self, cache, q_ptr: int, q_start_pos: int, workspace: Optional[native.Workspace]) -> torch.Tensor:
+        """Numbers of the selected tiles, int32 [B, Hkv, q_len, top_tiles]."""
+        out = torch.empty_like(self.numbers)
+        ws = workspace if workspace is not None else native.default_workspace(cache.device)
+        buf = ws.get(self.nbytes)
+        status = native.lib().rfsn_archive_select(self.ref, q_ptr, q_start_pos, out.data_ptr(), buf.data_ptr(),
+                                                  buf.numel(), native.stream_ptr())
+        if status:
+            native.check(status, "rfsn_archive_select")
+        return out
 
-__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "PreparedCall", "PreparedSelection", "workspace_bytes"]
+
+__all__ = ["ARCHIVE_DTYPES", "PackedArchive", "PreparedCall", "workspace_bytes"]

@@ -46,7 +46,7 @@ import numpy as np
 import torch
 
 from . import _native as native
-from .archive import PackedArchive, PreparedCall, PreparedSelection, check_archive_options, padded_rows
+from .archive import PackedArchive, PreparedCall, check_archive_options, padded_rows
 from .block_manager import BlockId, BlockLocation, BlockManager, BlockManifest, BlockSpan
 from .config import RFSNConfig, RuntimeMode, resolve_dtype, validate_session_id
 from .residency import ResidencyManager
@@ -287,7 +287,6 @@ class PagedSegments(Sequence):
         self.tile_list = cache.tile_snapshot() if table is not None else (cache.tile_snapshot()[0], 0)
         # prepared calls over these segments, by query shape
         self.calls: dict[tuple, PreparedCall] = {}
-        self.selections: dict[tuple, PreparedSelection] = {}
 
     def __len__(self) -> int:
         return len(self.spans)
@@ -1151,7 +1150,8 @@ class LayerKVCache:
                                top_tiles=top_tiles)
 
     def select_tiles(self, q: torch.Tensor, q_start_pos: int, top_tiles: int,
-                     segments: Optional[PagedSegments] = None) -> torch.Tensor:
+                     segments: Optional[PagedSegments] = None, *,
+                     workspace: Optional[native.Workspace] = None) -> torch.Tensor:
         """Numbers of the archived 64-token tiles (counted through the blocks in
         page-table order) that ``attend(..., top_tiles=n)`` reads: int32
         [B, Hkv, Lq, top_tiles], ascending, -1 behind them. Needs
@@ -1159,13 +1159,14 @@ class LayerKVCache:
         if segments is None:
             segments = self.get_attention_segments()
         qf = _query(self, q)
-        key = (qf.shape[1], qf.shape[2], top_tiles)
-        call = segments.selections.get(key)
-        if call is None or call.keep[3] is not self.tile_bounds:
-            call = segments.selections[key] = PreparedSelection(self, segments, int(qf.shape[1]), int(qf.shape[2]),
-                                                                int(top_tiles))
+        _, H, Lq, _ = qf.shape
+        key = (H, Lq, top_tiles, "select")
+        call = segments.calls.get(key)
+        if call is None or not call.current(self):
+            call = segments.calls[key] = PreparedCall(self, segments, native.HotWindowC(), H, Lq, int(top_tiles), 0,
+                                                      select_only=True)
         with native.on_device(self.device):
-            return call(self, qf, int(q_start_pos)).select(4, 3)
+            return call.select(self, qf.data_ptr(), int(q_start_pos), workspace)
 
 
 def _query(cache: LayerKVCache, q: torch.Tensor) -> torch.Tensor:
@@ -1216,9 +1217,7 @@ def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
     lse = torch.empty(qf.shape[:3], dtype=torch.float32, device=cache.device) if want_lse else None
     key = (H, Lq, top_tiles, max_splits)
     call = segments.calls.get(key) if step_state is None else None
-    if call is None or call.keep[2] is not cache.archive or call.keep[1] is not cache.arena:
-        if top_tiles < 0 or (top_tiles and cache.tile_bounds is None):
-            raise ValueError("top_tiles needs a cache built with tile_index=True and a count >= 0")
+    if call is None or not call.current(cache):
         hot = _hot_window(cache, segments, step_state)
         call = PreparedCall(cache, segments, hot, H, Lq, int(top_tiles), max_splits)
         if step_state is None and segments.hot_state is not None:

@@ -354,7 +354,9 @@ def test_attention_arguments(lib):
     expect(lib.rfsn_archive_attention(None, None, FAKE, 1, 8, 2, 1, 0, ctypes.byref(tiles), ctypes.byref(hot), FAKE, None,
                                       FAKE, 1 << 20, 0, None), BAD, "NULL arena")
     expect(lib.rfsn_archive_attend(None, FAKE, 0, FAKE, None, FAKE, 1 << 20, None), BAD, "NULL call")
+    expect(lib.rfsn_archive_select(None, FAKE, 0, FAKE, FAKE, 1 << 20, None), BAD, "NULL call")
     call = native.ArchiveCallC()
+    expect(lib.rfsn_archive_select(ctypes.byref(call), FAKE, 0, FAKE, FAKE, 1 << 20, None), BAD, "NULL call")
     expect(lib.rfsn_archive_attend(ctypes.byref(call), FAKE, 0, FAKE, None, FAKE, 1 << 20, None), BAD, "NULL call")
 
 

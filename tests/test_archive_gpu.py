@@ -656,10 +656,12 @@ def test_two_streams_with_workspaces_of_their_own():
     caches = [make("bfloat16", 1, 8, 2, 128, (3000,), 20, tile_index=True, seed=i)[0] for i in range(2)]
     q = queries(1, 8, 1, 128)
     want = [[c.attend(q, 3019, top_tiles=top).clone() for top in (0, 5)] for c in caches]
+    tiles = [c.select_tiles(q, 3019, 5).clone() for c in caches]
     streams = [torch.cuda.Stream() for _ in caches]
     spaces = [native.Workspace(c.device) for c in caches]
     segs = [c.get_attention_segments() for c in caches]
     got = [[], []]
+    lists = [[], []]
     for s in streams:
         s.wait_stream(torch.cuda.current_stream())
     for _ in range(20):
@@ -667,10 +669,12 @@ def test_two_streams_with_workspaces_of_their_own():
             with torch.cuda.stream(streams[i]):
                 got[i].append([paged_attention(c, q, 3019, segs[i], workspace=spaces[i], top_tiles=top)
                                for top in (0, 5)])
+                lists[i].append(c.select_tiles(q, 3019, 5, segs[i], workspace=spaces[i]))
     torch.cuda.synchronize()
     for i in range(2):
         for pair in got[i]:
             assert torch.equal(pair[0], want[i][0]) and torch.equal(pair[1], want[i][1])
+        assert all(torch.equal(x, tiles[i]) for x in lists[i])
 
 
 def test_the_same_call_gives_the_same_bits():
