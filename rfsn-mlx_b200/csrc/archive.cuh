@@ -63,6 +63,114 @@ struct SelectParams {
     const int* dyn;
 };
 
+// Paired float32 arithmetic (PTX .f32x2): two results per issue slot, each rounded as the scalar operation.
+__device__ __forceinline__ uint64_t pair(float2 a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t r) {
+    float2 a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+    return a;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)), "l"(pair(c)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
+    return unpair(r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Split merge by the last CTA of a list (and block of SL query slots) to
+// arrive; called by threads 0 .. nthreads - 1 of the CTA after they wrote its
+// partials (named barrier 1 is theirs). The partials of all splits are
+// contiguous runs (O, m, l): with room for them in `stage` they come in one
+// round trip of asynchronous copies. wts: room for SL * splits floats.
+template <int D>
+__device__ __forceinline__ void merge_splits(const Params& p, const OutMap& om, int bh, int slot0, int nslots, int SL,
+                                             int counter, uint8_t* stage, size_t stage_bytes, float* wts, float* inv,
+                                             int* flag, int nthreads) {
+    constexpr int V4 = D / 4;  // float4 per row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    named_barrier_sync(1, nthreads);  // the CTA's partials before thread 0's release
+    if (threadIdx.x == 0) *flag = atom_add_acq_rel_gpu(&p.ws.counters[counter], 1) == p.splits - 1;
+    named_barrier_sync(1, nthreads);
+    if (!*flag) return;
+    const size_t part_base = (size_t)counter * p.splits * SL;
+    const int parts = p.splits * SL;
+    const bool staged = (size_t)parts * (D + 2) * 4 <= stage_bytes;
+    const float* src_o = p.ws.o + part_base * D;
+    const float* src_m = p.ws.m + part_base;
+    const float* src_l = p.ws.l + part_base;
+    if (staged) {
+        float4* st_o = reinterpret_cast<float4*>(stage);
+        float4* st_ml = st_o + (size_t)parts * V4;
+        for (int i = threadIdx.x; i < parts / 2; i += nthreads)
+            cp_async_16(st_ml + i, i < parts / 4 ? src_m + 4 * i : src_l + 4 * (i - parts / 4));
+        for (int i = threadIdx.x; i < parts * V4; i += nthreads) cp_async_16(st_o + i, src_o + 4 * (size_t)i);
+        cp_async_commit();
+        cp_async_wait_all();
+        named_barrier_sync(1, nthreads);
+        src_o = reinterpret_cast<const float*>(st_o);
+        src_m = reinterpret_cast<const float*>(st_ml);
+        src_l = src_m + parts;
+    }
+    auto get = [&](const float* x) { return staged ? *x : __ldcg(x); };
+    for (int sl = warp; sl < nslots; sl += nthreads / 32) {
+        float M = -INFINITY, L = 0.f;
+        for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, get(src_m + s * SL + sl));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        for (int s = lane; s < p.splits; s += 32) {
+            const float wt = M == -INFINITY ? 1.f : ex2_approx(get(src_m + s * SL + sl) - M);
+            L += wt * get(src_l + s * SL + sl);
+            wts[sl * p.splits + s] = wt;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        if (lane == 0) {
+            const bool any = L > 0.f || L != L;
+            inv[sl] = any ? 1.f / L : 0.f;
+            if (p.lse != nullptr)
+                p.lse[om.row(bh, slot0 + sl)] = any ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+        }
+    }
+    named_barrier_sync(1, nthreads);
+    for (int i = threadIdx.x; i < nslots * V4; i += nthreads) {
+        const int sl = i / V4, d4 = i % V4;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4* from = reinterpret_cast<const float4*>(src_o) + sl * V4 + d4;
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) {
+            const float4 o = staged ? from[(size_t)s * SL * V4] : __ldcg(from + (size_t)s * SL * V4);
+            const float wt = wts[sl * p.splits + s];
+            O.x += wt * o.x;
+            O.y += wt * o.y;
+            O.z += wt * o.z;
+            O.w += wt * o.w;
+        }
+        const float r = inv[sl];
+        *reinterpret_cast<float4*>(p.out + om.row(bh, slot0 + sl) * D + 4 * d4) =
+            make_float4(O.x * r, O.y * r, O.z * r, O.w * r);
+    }
+    if (threadIdx.x == 0) p.ws.counters[counter] = 0;
+}
+
 }  // namespace archive
 
 // archive_pack.cu
@@ -80,6 +188,11 @@ rfsn_status select_tiles_launch(int bounds_dtype, int head_dim, const archive::S
 int archive_attn_ctas(int nb);
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int nb, int zblocks, cudaStream_t stream);
+// archive_rows.cu: 5 to 16 query slots per CTA (slots 8 or 16) over a packed archive, head_dim 128;
+// Params::items_per_split in units of one archived item (two tiles), hot items of 128 keys count two
+rfsn_status archive_rows_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
+                                int lists, int slots, int zblocks, cudaStream_t stream);
+void preload_rows_kernels();
 
 // archive_chunk.cu: chunks of queries over a packed archive, head_dim 128. Workspace: partials and a copy of the ring.
 bool archive_chunk_fits(int G);

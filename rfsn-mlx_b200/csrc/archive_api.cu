@@ -22,32 +22,37 @@ rfsn_status check_device(int device, const char* what) {
     return RFSN_OK;
 }
 
-// Query slots of one list, column blocks of 4 slots per CTA and CTAs (z) per list.
+// Query slots of one list, slots per CTA, CTAs (z) per list, and the kernel: rows (archive_rows.cu) or tiles
+// (archive_attn.cu, 4 or 8 slots per CTA).
 struct SlotPlan {
-    int lists, slots, nb, zblocks;
+    int lists, slots, per_cta, zblocks;
+    bool rows;
 };
 
-SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, bool per_query) {
+SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, int head_dim, bool packed, bool per_query) {
     SlotPlan s;
     const int G = q_heads / kv_heads;
     s.lists = batch * kv_heads * (per_query ? q_len : 1);
     s.slots = per_query ? G : G * q_len;
-    s.nb = s.slots <= 4 ? 1 : 2;
-    s.zblocks = (s.slots + 4 * s.nb - 1) / (4 * s.nb);
+    s.rows = packed && !per_query && head_dim == 128 && s.slots > 4;
+    s.per_cta = s.slots <= 4 ? 4 : (s.slots <= 8 || !s.rows ? 8 : 16);
+    s.zblocks = (s.slots + s.per_cta - 1) / s.per_cta;
     return s;
 }
+
+int ctas_per_sm(const SlotPlan& sp) { return sp.rows ? 1 : archive_attn_ctas(sp.per_cta / 4); }
 
 // Splits of a list's items: the CTAs that are resident at once, over all lists.
 int split_limit(const SlotPlan& sp, int head_dim, int max_splits) {
     const int sms = std::max(device_sms(), 1);
-    int s = std::max(1, archive_attn_ctas(sp.nb) * sms / std::max(1, sp.lists * sp.zblocks));
+    int s = std::max(1, ctas_per_sm(sp) * sms / std::max(1, sp.lists * sp.zblocks));
     s = std::min(s, head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64);
     if (max_splits > 0) s = std::min(s, max_splits);
     return s;
 }
 
 WsLayout attention_ws(const SlotPlan& sp, int splits, int head_dim) {
-    return ws_layout(splits > 1 ? sp.lists * sp.zblocks : 0, 1, splits, 4 * sp.nb, head_dim);
+    return ws_layout(splits > 1 ? sp.lists * sp.zblocks : 0, 1, splits, sp.per_cta, head_dim);
 }
 
 // Largest attention workspace of a shape: every split count it may choose (at
@@ -56,7 +61,7 @@ size_t attention_ws_limit(const SlotPlan& sp, int head_dim) {
     const int units = std::max(1, sp.lists * sp.zblocks);
     const int limit = std::max(split_limit(sp, head_dim, 0),
                                std::min(head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64,
-                                        std::max(1, archive_attn_ctas(sp.nb) * 148 / units)));
+                                        std::max(1, ctas_per_sm(sp) * 148 / units)));
     return attention_ws(sp, limit, head_dim).total;
 }
 
@@ -138,16 +143,17 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     if (st != RFSN_OK) return st;
     const bool chunk = packed != nullptr && tiles->per_query == 0 && !stepped && tiles->n > 0 &&
                        chunk_shape(arena->head_dim, q_heads / kv_heads, q_len, tiles->n);
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, tiles->per_query != 0);
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, arena->head_dim, packed != nullptr,
+                                  tiles->per_query != 0);
     RFSN_CHECK_ARG(chunk || sp.zblocks <= kMaxLists, "%s: too many query rows", what);
-    const int hk = arena->head_dim == 128 ? 32 : 64;  // 16-bit keys per item
+    const int hk = sp.rows ? 128 : (arena->head_dim == 128 ? 32 : 64);  // 16-bit keys per item
     const int per_tile = packed != nullptr ? 1 : kTile / hk;
     RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
     const int first = std::min(hot->length, hot->capacity - hot->head_index);
     // with a device step state the window is only known when the kernel runs: planned for the largest
     const int hot_items = stepped ? (hot->capacity + hk - 1) / hk + 1
                                   : (first + hk - 1) / hk + (hot->length - first + hk - 1) / hk;
-    const int total = std::max(1, tiles->n * per_tile + hot_items);
+    const int total = std::max(1, sp.rows ? (tiles->n + 1) / 2 + 2 * hot_items : tiles->n * per_tile + hot_items);
     int splits = std::min(split_limit(sp, arena->head_dim, max_splits), total);
     const int per = (total + splits - 1) / splits;
     splits = (total + per - 1) / per;
@@ -189,7 +195,9 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     if (chunk)
         return archive_chunk_launch(arena, packed, p, batch, workspace, workspace_bytes, max_splits,
                                     static_cast<cudaStream_t>(stream));
-    return archive_attn_launch(arena, packed, p, sp.lists, sp.nb, sp.zblocks, static_cast<cudaStream_t>(stream));
+    if (sp.rows)
+        return archive_rows_launch(arena, packed, p, sp.lists, sp.per_cta, sp.zblocks, static_cast<cudaStream_t>(stream));
+    return archive_attn_launch(arena, packed, p, sp.lists, sp.per_cta / 4, sp.zblocks, static_cast<cudaStream_t>(stream));
 }
 
 // numbers: out receives the tiles' numbers ([lists][n_select]) instead of their entries
@@ -368,8 +376,10 @@ rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, in
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0 && hot_capacity >= 0,
                    "rfsn_archive_workspace_size: negative count");
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, n_select > 0);
-    size_t need = attention_ws_limit(sp, head_dim);
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, false, n_select > 0);
+    size_t need = std::max(attention_ws_limit(sp, head_dim),
+                           attention_ws_limit(slot_plan(batch, q_heads, kv_heads, q_len, head_dim, true, n_select > 0),
+                                              head_dim));
     if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
     else if (chunk_shape(head_dim, q_heads / kv_heads, q_len, n_tiles))
         need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity));
@@ -404,7 +414,7 @@ rfsn_status rfsn_archive_attend(const rfsn_archive_call* c, const float* q, int 
     rfsn_status st = check_shape(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, true, what);
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(c->tiles.n > 0 && c->tiles.per_query == 0 && c->top_tiles <= (1 << 20), "%s: bad tile list", what);
-    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, true);
+    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, c->packed != nullptr, true);
     const size_t off = lists_offset(sp, head_dim, c->tiles.n);
     const size_t need = off + sizeof(int4) * (size_t)sp.lists * c->top_tiles;
     if (workspace == nullptr || workspace_bytes < need) {

@@ -728,71 +728,8 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     }
     if (p.splits == 1) return;
 
-    // ---------------- split merge: the last CTA of the list ----------------
-    named_barrier_sync(1, kNCW * 32);  // the CTA's partials before thread 0's release
-    if (threadIdx.x == 0) sm.flag = atom_add_acq_rel_gpu(&p.ws.counters[counter], 1) == p.splits - 1;
-    named_barrier_sync(1, kNCW * 32);
-    if (!sm.flag) return;
-    // The partials of all splits are contiguous runs (O, m, l): with room for
-    // them in the idle stages they come in one round trip of asynchronous copies.
-    float* wts = &sm.red_o[0][0][0];  // [SL][splits] weights
-    const int parts = p.splits * SL;
-    const bool staged = (size_t)parts * (D + 2) * 4 <= (size_t)STAGES * kStageBytes;
-    const float* src_o = p.ws.o + part_base * D;
-    const float* src_m = p.ws.m + part_base;
-    const float* src_l = p.ws.l + part_base;
-    if (staged) {
-        float4* st_o = reinterpret_cast<float4*>(&sm.stage[0][0]);
-        float4* st_ml = st_o + (size_t)parts * V4;
-        for (int i = threadIdx.x; i < parts / 2; i += kNCW * 32)
-            cp_async_16(st_ml + i, i < parts / 4 ? src_m + 4 * i : src_l + 4 * (i - parts / 4));
-        for (int i = threadIdx.x; i < parts * V4; i += kNCW * 32) cp_async_16(st_o + i, src_o + 4 * (size_t)i);
-        cp_async_commit();
-        cp_async_wait_all();
-        named_barrier_sync(1, kNCW * 32);
-        src_o = reinterpret_cast<const float*>(st_o);
-        src_m = reinterpret_cast<const float*>(st_ml);
-        src_l = src_m + parts;
-    }
-    auto get = [&](const float* x) { return staged ? *x : __ldcg(x); };
-    for (int sl = warp; sl < nslots; sl += kNCW) {
-        float M = -CUDART_INF_F, L = 0.f;
-        for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, get(src_m + s * SL + sl));
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-        for (int s = lane; s < p.splits; s += 32) {
-            const float wt = M == -CUDART_INF_F ? 1.f : ex2_approx(get(src_m + s * SL + sl) - M);
-            L += wt * get(src_l + s * SL + sl);
-            wts[sl * p.splits + s] = wt;
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-        if (lane == 0) {
-            const bool any = L > 0.f || L != L;
-            sm.red_l[0][sl] = any ? 1.f / L : 0.f;
-            if (p.lse != nullptr)
-                p.lse[om.row(bh, slot0 + sl)] = any ? (M + log2f(L)) * 0.69314718055994531f : -CUDART_INF_F;
-        }
-    }
-    named_barrier_sync(1, kNCW * 32);
-    for (int i = threadIdx.x; i < nslots * V4; i += kNCW * 32) {
-        const int sl = i / V4, d4 = i % V4;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4* from = reinterpret_cast<const float4*>(src_o) + sl * V4 + d4;
-#pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) {
-            const float4 o = staged ? from[(size_t)s * SL * V4] : __ldcg(from + (size_t)s * SL * V4);
-            const float wt = wts[sl * p.splits + s];
-            O.x += wt * o.x;
-            O.y += wt * o.y;
-            O.z += wt * o.z;
-            O.w += wt * o.w;
-        }
-        const float inv = sm.red_l[0][sl];
-        *reinterpret_cast<float4*>(p.out + om.row(bh, slot0 + sl) * D + 4 * d4) =
-            make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
-    }
-    if (threadIdx.x == 0) p.ws.counters[counter] = 0;
+    merge_splits<D>(p, om, bh, slot0, nslots, SL, counter, &sm.stage[0][0], STAGES * kStageBytes, &sm.red_o[0][0][0],
+                    sm.red_l[0], &sm.flag, kNCW * 32);
 }
 
 // Launch shape by column blocks: consumer groups, stages and CTAs per SM.
@@ -869,6 +806,7 @@ void preload_archive_kernels() {
     using namespace archive;
     preload_pack_kernels();
     preload_select_kernels();
+    preload_rows_kernels();
     preload_chunk_kernels();
     preload<__nv_bfloat16, 128>();
     preload<__nv_bfloat16, 64>();

@@ -129,33 +129,6 @@ __device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                  : "memory");
 }
-// Paired float32 arithmetic (PTX .f32x2): two results per issue slot, each rounded as the scalar operation.
-__device__ __forceinline__ uint64_t pair(float2 a) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
-    return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t r) {
-    float2 a;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
-    return a;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)), "l"(pair(c)));
-    return unpair(r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
-    return unpair(r);
-}
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
-    uint64_t r;
-    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a)), "l"(pair(b)));
-    return unpair(r);
-}
-
 // (a, b) -> two float16 high parts and two float16 remainders. The high part
 // is the value cut to 11 significant bits (exact in float16, and no
 // conversion back is needed for the remainder), the remainder is exact in
