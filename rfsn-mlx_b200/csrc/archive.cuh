@@ -188,8 +188,7 @@ rfsn_status select_tiles_launch(int bounds_dtype, int head_dim, const archive::S
 int archive_attn_ctas(int nb);
 rfsn_status archive_attn_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int nb, int zblocks, cudaStream_t stream);
-// archive_rows.cu: 5 to 16 query slots per CTA (slots 8 or 16) over a packed archive, head_dim 128;
-// Params::items_per_split in units of one archived item (two tiles), hot items of 128 keys count two
+// archive_rows.cu: 5 to 16 query slots per CTA (slots 8 or 16) over a packed archive, head_dim 128
 rfsn_status archive_rows_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& p,
                                 int lists, int slots, int zblocks, cudaStream_t stream);
 void preload_rows_kernels();

@@ -64,12 +64,11 @@ struct Smem {
     static constexpr int kN8 = round16up(kTerms * SL);
     static constexpr int kTerms16 = BF16 ? 3 : 2;
     static constexpr int kN16 = round16up(kTerms16 * SL);
-    static constexpr int kPBytes = kN8 * BN > 2 * kN16 * 128 ? kN8 * BN : 2 * kN16 * 128;
     static constexpr int kRow = D + 4;
     uint8_t stage[kStages][kItemBytes];
     uint8_t q8[kN8 * D];          // Q^T terms, 128-byte-swizzled rows (term, slot)
     uint8_t q16[2][kN16 * 128];   // the same in 16 bits, by channel half
-    uint8_t p[2][(kPBytes + 1023) / 1024 * 1024];  // P^T terms of the two groups; at the end the merge's weights
+    uint8_t p[2][BN * 128];       // P^T terms of the two groups, a row of columns per key; at the end the merge's weights
     uint64_t full[kStages], empty[kStages];
     uint64_t s_full[4], p_full[2], o_full[2], mma_done;
     Info info[kInfo];
@@ -101,11 +100,8 @@ __device__ __forceinline__ float2 minus32(uint32_t codes) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(y) : "r"(codes));
     return __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(-32.f)));
 }
-__device__ __forceinline__ void sts_u8(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void sts_u16(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)v) : "memory");
+__device__ __forceinline__ void sts_v2(uint32_t addr, uint2 v) {
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
 }
 __device__ __forceinline__ void sts_v4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
@@ -123,6 +119,31 @@ __device__ __forceinline__ bool group_any(int group, bool hand) {
         : "r"((uint32_t)hand), "r"(2 + group)
         : "memory");
     return r != 0;
+}
+
+// SL values per lane reduced over the warp's lanes, each step halving the values a lane carries (SL instead of
+// 5 SL shuffles). The result of slot `slot` comes out in every lane with own_slot(lane) == slot.
+template <int SL, typename Op>
+__device__ __forceinline__ float reduce_slots(const float2 (&x)[SL / 2], Op op) {
+    const int lane = threadIdx.x & 31;
+    float v[SL];
+#pragma unroll
+    for (int s = 0; s < SL; ++s) v[s] = (s & 1) ? x[s / 2].y : x[s / 2].x;
+#pragma unroll
+    for (int n = SL / 2, bit = 16; n > 0; n >>= 1, bit >>= 1) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int s = 0; s < n; ++s) {
+            const float other = __shfl_xor_sync(0xffffffffu, up ? v[s] : v[s + n], bit);
+            v[s] = op(up ? v[s + n] : v[s], other);
+        }
+    }
+#pragma unroll
+    for (int bit = 16 / SL; bit > 0; bit >>= 1) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], bit));
+    return v[0];
+}
+template <int SL> __device__ __forceinline__ int own_slot(int lane) {  // bits of the lane from the highest down
+    return SL == 16 ? lane >> 1 : lane >> 2;
 }
 
 // A row of SL * terms sums from TMEM, the terms joined: e4m3 terms by their weights, 16-bit ones as they are.
@@ -175,18 +196,17 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
     const int split = blockIdx.x, bh = blockIdx.y, zb = blockIdx.z;
     const int slot0 = zb * SL, nslots = min(SL, p.slots - slot0);
 
-    // Units of one stage: an archived item (two tiles of the list) takes one, a hot item two. A split has the items
-    // that begin in its run of units.
+    // Items: two tiles of the list, then 128 ring keys. A split has its share of both.
+    auto share = [&](int items, int s) { return (int)((long long)items * s / p.splits); };
     const int arch_items = (p.n_tiles + 1) / 2;
-    const int u0 = split * p.items_per_split, u1 = u0 + p.items_per_split;
-    const int a0 = min(u0, arch_items), na = min(u1, arch_items) - a0;
+    const int a0 = share(arch_items, split), na = share(arch_items, split + 1) - a0;
     int q_pos0 = p.q_pos0, head = p.head, hlen = p.hlen, hstart = p.hstart;
     int first = 0, h0 = 0, nh = 0;
     auto plan = [&]() {
         first = min(hlen, p.capacity - head);
         const int items = (first + BN - 1) / BN + (hlen - first + BN - 1) / BN;
-        h0 = min(items, max(0, u0 - arch_items + 1) / 2);
-        nh = min(items, max(0, u1 - arch_items + 1) / 2) - h0;
+        h0 = share(items, split);
+        nh = share(items, split + 1) - h0;
     };
     auto read_state = [&](bool report) {
         if (p.dyn != nullptr) {
@@ -290,7 +310,7 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
                 stop = __shfl_sync(0xffffffffu, stop, 0);
             }
         }
-        if (!stop && u1 > arch_items) {
+        if (!stop && (p.dyn != nullptr || p.hlen > 0)) {
             griddep_wait();
             read_state(false);
             const int items_a = (first + BN - 1) / BN;
@@ -341,9 +361,9 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
         read_state(false);
         named_barrier_sync(4, kSoftmaxThreads + 32);  // q is in shared memory
         const bool leader = tc::elect_leader();  // the whole warp waits and counts, one lane issues
-        constexpr uint32_t id_s8 = tc::idesc_e4m3(false, false, BN, kN8), id_o8 = tc::idesc_e4m3(true, false, D, kN8);
+        constexpr uint32_t id_s8 = tc::idesc_e4m3(false, false, BN, kN8), id_o8 = tc::idesc_e4m3(true, true, D, kN8);
         constexpr uint32_t id_s16 = tc::idesc_f16(BF16, false, false, BN, kN16);
-        constexpr uint32_t id_o16 = tc::idesc_f16(BF16, true, false, D, kN16);
+        constexpr uint32_t id_o16 = tc::idesc_f16(BF16, true, true, D, kN16);
         const int n = na + nh;
         auto k_slot = [&](int t) { return t < na ? t : na + 2 * (t - na); };
         bool ok = true;
@@ -381,12 +401,12 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
 #pragma unroll
                     for (int kk = 0; kk < BN / 32; ++kk)
                         tc::mma_e4m3_ss(leader, tO, tc::smem_desc_sw128(v + BN * D + 32 * 128 * kk, 16, 1024),
-                                        tc::smem_desc_sw128(pb + 32 * kk, 16, 1024), id_o8, kk > 0);
+                                        tc::smem_desc_sw128(pb + 32 * 128 * kk, 16, 1024), id_o8, kk > 0);
                 } else {
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk)
                         tc::mma_f16_ss(leader, tO, tc::smem_desc_sw128(v + 16 * 128 * kk, BN * 128, 1024),
-                                       tc::smem_desc_sw128(pb + (kk >> 2) * kN16 * 128 + 32 * (kk & 3), 16, 1024),
+                                       tc::smem_desc_sw128(pb + 16 * 128 * kk, 16, 1024),
                                        id_o16, kk > 0);
                 }
                 tc::commit(leader, &sm.o_full[w]);
@@ -530,13 +550,8 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
 #pragma unroll
             for (int s = 0; s < H; ++s) top = fmaxf(top, fmaxf(x[s].x, x[s].y));
             if (group_any(w, top > kLazy || fresh != 0 || !ok)) {  // a maximum moves, or a wait gave up
-#pragma unroll
-                for (int s = 0; s < SL; ++s) {
-                    float tm = (s & 1) ? x[s / 2].y : x[s / 2].x;
-#pragma unroll
-                    for (int off = 16; off > 0; off >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, off));
-                    if (lane == 0) sm.red[w][gw][s] = tm;
-                }
+                const float tm = reduce_slots<SL>(x, [](float a, float b) { return fmaxf(a, b); });
+                if ((lane & (32 / SL - 1)) == 0) sm.red[w][gw][own_slot<SL>(lane)] = tm;
                 if (lane == 0) sm.bad[w][gw] = !ok;
                 named_barrier_sync(2 + w, 128);
                 if (sm.bad[w][0] | sm.bad[w][1] | sm.bad[w][2] | sm.bad[w][3]) {
@@ -569,35 +584,37 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
                 l[s] = add2(l[s], pr);
                 x[s] = mul2(pr, both(f));
             }
+            // P^T, N-major: the key's row of columns (term, slot)
+            const uint32_t prow = pb + r * 128;
+            auto chunk = [&](int c) { return prow + ((c ^ (r & 7)) << 4); };
             if (arch) {
-                uint32_t at[8];  // the key's byte in rows 0 .. 7 of the swizzle pattern
 #pragma unroll
-                for (int i = 0; i < 8; ++i) at[i] = pb + (r ^ (i << 4));
-#pragma unroll
-                for (int j = 0; j < kTerms; ++j)
+                for (int j = 0; j < kTerms; ++j) {
+                    uint32_t c[H];
 #pragma unroll
                     for (int s = 0; s < H; ++s) {
-                        const uint32_t c = e4m3x2(x[s].x, x[s].y);
-                        const int row = j * SL + 2 * s;
-                        sts_u8(at[row & 7] + row * 128, c);
-                        sts_u8(at[(row + 1) & 7] + (row + 1) * 128, c >> 8);
-                        if (j < kTerms - 1) x[s] = fma2(x[s], both(32.f), minus32(c));
+                        c[s] = e4m3x2(x[s].x, x[s].y);
+                        if (j < kTerms - 1) x[s] = fma2(x[s], both(32.f), minus32(c[s]));
                     }
+                    if constexpr (SL == 16)
+                        sts_v4(chunk(j), make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16));
+                    else
+                        sts_v2(chunk(j >> 1) + 8 * (j & 1), make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16));
+                }
             } else {
-                uint32_t at[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) at[i] = pb + half * kN16 * 128 + ((2 * ki) ^ (i << 4));
-#pragma unroll
-                for (int j = 0; j < kTerms16; ++j)
+                for (int j = 0; j < kTerms16; ++j) {
+                    uint32_t c[H];
 #pragma unroll
                     for (int s = 0; s < H; ++s) {
                         const float2 y = make_float2(round16<T>(x[s].x), round16<T>(x[s].y));
-                        const uint32_t c = pack2<T>(y.x, y.y);
-                        const int row = j * SL + 2 * s;
-                        sts_u16(at[row & 7] + row * 128, c);
-                        sts_u16(at[(row + 1) & 7] + (row + 1) * 128, c >> 16);
+                        c[s] = pack2<T>(y.x, y.y);
                         x[s] = sub2(x[s], y);
                     }
+#pragma unroll
+                    for (int i = 0; i < H / 4; ++i)
+                        sts_v4(chunk(j * (H / 4) + i), make_uint4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]));
+                }
             }
             if (seen < kTile && ki >= seen) {  // V of keys that no slot sees may hold anything: zeroed
                 // a hot item's V comes behind its K: the copy must have landed
@@ -626,14 +643,12 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
         }
         griddep_launch_dependents();
         // row sums over the group's keys
+        const float sum = reduce_slots<SL>(l, [](float a, float b) { return a + b; });
+        if ((lane & (32 / SL - 1)) == 0) sm.red[w][gw][own_slot<SL>(lane)] = sum;
+        if (r == 0) {
 #pragma unroll
-        for (int s = 0; s < SL; ++s) {
-            float sum = (s & 1) ? l[s / 2].y : l[s / 2].x;
-            const float neg = (s & 1) ? nm[s / 2].y : nm[s / 2].x;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            if (lane == 0) sm.red[w][gw][s] = sum;
-            if (r == 0) sm.m[w][s] = (fresh >> s) & 1 ? -CUDART_INF_F : -neg;
+            for (int s = 0; s < SL; ++s)
+                sm.m[w][s] = (fresh >> s) & 1 ? -CUDART_INF_F : -((s & 1) ? nm[s / 2].y : nm[s / 2].x);
         }
         tc::fence_before_sync();
         named_barrier_sync(1, kSoftmaxThreads);
