@@ -42,6 +42,7 @@ struct Params {
     int q_heads, kv_heads, q_len, q_pos0, G;
     int slots;              // query slots of one list: q_len * G, or G per query row
     int items_per_split, splits;
+    int hot_items;          // archive_rows.cu: items of 128 ring keys, at most
     float qscale;           // 1/sqrt(D) * log2(e)
     WsView ws;
     const int* dyn;         // device step state (RFSN_STEP_*) or nullptr

@@ -189,6 +189,7 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     p.slots = sp.slots;
     p.items_per_split = per;
     p.splits = splits;
+    p.hot_items = hot_items;
     p.qscale = (float)(1.0 / std::sqrt((double)arena->head_dim)) * 1.4426950408889634f;
     p.ws = ws_view(workspace, w);
     p.dyn = hot->step_state;

@@ -196,10 +196,16 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
     const int split = blockIdx.x, bh = blockIdx.y, zb = blockIdx.z;
     const int slot0 = zb * SL, nslots = min(SL, p.slots - slot0);
 
-    // Items: two tiles of the list, then 128 ring keys. A split has its share of both.
+    // Items: two tiles of the list, then 128 ring keys, of twice the bytes. A split has its share of the ring items,
+    // and archived items up to its share of the whole. (That count is fixed on the host from the longest window where
+    // the window is only known now: the loads of archived tiles begin before.)
     auto share = [&](int items, int s) { return (int)((long long)items * s / p.splits); };
     const int arch_items = (p.n_tiles + 1) / 2;
-    const int a0 = share(arch_items, split), na = share(arch_items, split + 1) - a0;
+    auto arch_before = [&](int s) {
+        const int fair = share(arch_items + 2 * p.hot_items, s) - 2 * share(p.hot_items, s);
+        return arch_items >= 2 * p.splits ? max(0, min(arch_items, fair)) : share(arch_items, s);
+    };
+    const int a0 = arch_before(split), na = arch_before(split + 1) - a0;
     int q_pos0 = p.q_pos0, head = p.head, hlen = p.hlen, hstart = p.hstart;
     int first = 0, h0 = 0, nh = 0;
     auto plan = [&]() {
@@ -621,10 +627,10 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
                 if (!arch && !mbar_wait_bounded(&sm.full[vs % kStages], (vs / kStages) & 1, &sm.abort)) fail(&sm.abort, p);
                 const uint32_t v = smem_u32(sm.stage[vs % kStages]) + (arch ? BN * D : 0) + r * 128;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sts_v4(v + 16 * i, make_uint4(0, 0, 0, 0));
+                for (int i = 0; i < 8; ++i) sts_v4(v + ((16 * i) ^ ((r & 7) << 4)), make_uint4(0, 0, 0, 0));
                 if (!arch) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sts_v4(v + BN * 128 + 16 * i, make_uint4(0, 0, 0, 0));
+                    for (int i = 0; i < 8; ++i) sts_v4(v + BN * 128 + ((16 * i) ^ ((r & 7) << 4)), make_uint4(0, 0, 0, 0));
                 }
             }
             unit = arch ? u : 1.f / kPScale;
