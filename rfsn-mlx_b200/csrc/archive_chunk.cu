@@ -212,7 +212,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         return;
     }
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int G = p.G, ppc = BM / G;
     // Units (query block, KV head): latest query blocks first, the heads
     // interleaved; the splits of a unit's keys are consecutive CTAs.
@@ -426,7 +426,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             // ---------------- MMA issuer ----------------
             named_barrier_sync(1, kSoftmaxThreads + 32);  // q is in TMEM
             tc::fence_after_sync();
-            if (lane == 0 && nt > 0) {
+            if (nt > 0) {  // the whole warp waits and counts, one lane issues
+                const bool leader = tc::elect_leader();
                 const uint32_t id_qk = tc::idesc_f16(false, false, false, BM, BN);
                 const uint32_t id_pv = tc::idesc_f16(false, false, true, BM, D);
                 const uint32_t tO = tmem + kColO;
@@ -436,8 +437,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                     const uint32_t ph = (t >> 1) & 1;
                     if (t < nt) {
                         // S buffer t % 2 last held P(t - 2)
-                        ok = mbar_wait_bounded(&sm.k_full[s], ph, &sm.abort) &&
-                             (t < kStages || mbar_wait_bounded(&sm.pv_done[s], ph ^ 1, &sm.abort));
+                        ok = warp_wait(&sm.k_full[s], ph, &sm.abort) &&
+                             (t < kStages || warp_wait(&sm.pv_done[s], ph ^ 1, &sm.abort));
                         if (!ok) break;
                         tc::fence_after_sync();
                         const uint32_t tS = tmem + 128 * s;
@@ -446,20 +447,20 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                             const uint32_t tQ = tmem + (part ? kColQlo : kColQhi);
 #pragma unroll
                             for (int kk = 0; kk < 8; ++kk)
-                                tc::mma_f16_ts(tS, tQ + 8 * kk,
+                                tc::mma_f16_ts(leader, tS, tQ + 8 * kk,
                                                tc::smem_desc_sw128(smem_u32(sm.k[s][kk >> 2]) + (kk & 3) * 32, 16, 1024),
                                                id_qk, part > 0 || kk > 0);
                         }
-                        tc::commit(&sm.s_full[s]);
-                        tc::commit(&sm.k_empty[s]);
+                        tc::commit(leader, &sm.s_full[s]);
+                        tc::commit(leader, &sm.k_empty[s]);
                     }
                     if (t > 0) {
                         const int u = t - 1, us = u & 1;
                         const uint32_t uph = (u >> 1) & 1;
                         // P(u) written, V(u) there, O(u - 1) read out
-                        ok = mbar_wait_bounded(&sm.p_full[us], uph, &sm.abort) &&
-                             mbar_wait_bounded(&sm.v_full[us], uph, &sm.abort) &&
-                             (u == 0 || mbar_wait_bounded(&sm.o_empty, (u - 1) & 1, &sm.abort));
+                        ok = warp_wait(&sm.p_full[us], uph, &sm.abort) &&
+                             warp_wait(&sm.v_full[us], uph, &sm.abort) &&
+                             (u == 0 || warp_wait(&sm.o_empty, (u - 1) & 1, &sm.abort));
                         if (!ok) break;
                         tc::fence_after_sync();
                         const uint32_t tP = tmem + 128 * us;
@@ -467,17 +468,17 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                         for (int part = 0; part < 2; ++part) {
 #pragma unroll
                             for (int kk = 0; kk < 8; ++kk)
-                                tc::mma_f16_ts(tO, tP + 64 * part + 8 * kk,
+                                tc::mma_f16_ts(leader, tO, tP + 64 * part + 8 * kk,
                                                tc::smem_desc_sw128(smem_u32(sm.v[us][0]) + kk * 16 * 128, kHalfBytes, 1024),
                                                id_pv, part > 0 || kk > 0);
                         }
-                        tc::commit(&sm.pv_done[us]);
-                        tc::commit(&sm.v_empty[us]);
+                        tc::commit(leader, &sm.pv_done[us]);
+                        tc::commit(leader, &sm.v_empty[us]);
                     }
                 }
-                if (!ok) fail(&sm.abort, p);
+                if (!ok && lane == 0) fail(&sm.abort, p);
                 // no tensor-core work may be in flight when TMEM is released
-                tc::commit(&sm.mma_done);
+                tc::commit(leader, &sm.mma_done);
                 mbar_wait_bounded(&sm.mma_done, 0, nullptr);
             }
         }
