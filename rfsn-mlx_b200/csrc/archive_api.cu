@@ -29,14 +29,14 @@ struct SlotPlan {
     bool rows;
 };
 
-SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, int head_dim, bool packed, bool per_query) {
+SlotPlan make_plan(int batch, int q_heads, int kv_heads, int q_len, bool per_query, int per_cta, bool rows) {
     SlotPlan s;
     const int G = q_heads / kv_heads;
     s.lists = batch * kv_heads * (per_query ? q_len : 1);
     s.slots = per_query ? G : G * q_len;
-    s.rows = packed && !per_query && head_dim == 128 && s.slots > 4;
-    s.per_cta = s.slots <= 4 ? 4 : (s.slots <= 8 || !s.rows ? 8 : 16);
-    s.zblocks = (s.slots + s.per_cta - 1) / s.per_cta;
+    s.per_cta = per_cta;
+    s.zblocks = (s.slots + per_cta - 1) / per_cta;
+    s.rows = rows;
     return s;
 }
 
@@ -49,6 +49,23 @@ int split_limit(const SlotPlan& sp, int head_dim, int max_splits) {
     s = std::min(s, head_dim == 128 ? archive::kMaxSplits128 : archive::kMaxSplits64);
     if (max_splits > 0) s = std::min(s, max_splits);
     return s;
+}
+
+// The rows kernel runs from 5 slots on (8 slots, 8 heads: 33K keys 20 us, the tile kernel 23; 131K 53 / 59). It takes 8
+// or 16 slots a CTA: 16 halve the passes over K/V, but their merge reads twice the partials. Measured (us, 8 / 16
+// slots): 16 slots, 8 heads (18 splits of 16): 4K keys 10.7 / 13.3, 16K 18.5 / 17.8, 33K 29 / 25, 131K 88 / 61;
+// 32 slots: 4K 13.8 / 13.9, 16K 31 / 24; 1 head (74 splits): 33K 14 / 23. units: a split's work, below.
+SlotPlan slot_plan(int batch, int q_heads, int kv_heads, int q_len, int head_dim, bool packed, bool per_query,
+                   long long units) {
+    const int slots = q_heads / kv_heads * (per_query ? 1 : q_len);
+    auto plan = [&](int per_cta, bool rows) {
+        return make_plan(batch, q_heads, kv_heads, q_len, per_query, per_cta, rows);
+    };
+    if (slots <= 4) return plan(4, false);
+    if (!packed || per_query || head_dim != 128) return plan(8, false);
+    const SlotPlan wide = plan(16, true);
+    const long long splits = std::min<long long>(split_limit(wide, head_dim, 0), std::max(units, 1LL));
+    return slots > 8 && units > splits * (2 + splits / 4) ? wide : plan(8, true);
 }
 
 WsLayout attention_ws(const SlotPlan& sp, int splits, int head_dim) {
@@ -65,16 +82,17 @@ size_t attention_ws_limit(const SlotPlan& sp, int head_dim) {
     return attention_ws(sp, limit, head_dim).total;
 }
 
-// Chunks run on the tcgen05 kernel. It works on 128 query rows whatever the
-// call has and takes about 24 us at least; the tile kernel reads K/V again for
-// every 8 slots. Measured (32 q / 8 KV heads, us, tile / chunk kernel): 32
-// slots over 4K keys 16 / 24, 16K 37 / 38, 132K 217 / 141; 64 slots over 4K
-// 27 / 24, 16K 72 / 38.
-constexpr int kChunkSlots = 64, kChunkSlotsLong = 24, kChunkLongTiles = 256;
-bool chunk_shape(int head_dim, int G, int q_len, int n_tiles) {
+// Packed archives with head_dim 128: the rows kernel reads K/V again for every
+// 16 query slots, the chunk kernel for every 128, at about 2.1 times the cost
+// of a pass, and 9 us more to begin with. Measured (8 KV heads, us, rows /
+// chunk kernel): 32 slots over 16K keys 24 / 35, 131K 107 / 125; 48 slots over
+// 16K 30 / 35, 33K 49 / 52, 131K 155 / 126; 64 slots over 4K 18 / 22, 16K 39 / 36,
+// 33K 69 / 53; 1 KV head: 96 slots over 33K 22 / 35.
+constexpr long long kChunkGain = 38000;  // 10 * 64-token tiles of all heads * passes saved
+bool chunk_shape(int head_dim, int groups, int G, int q_len, int n_tiles) {
     const long long slots = q_len * (long long)G;
-    return head_dim == 128 && archive_chunk_fits(G) &&
-           (slots >= kChunkSlots || (slots >= kChunkSlotsLong && n_tiles >= kChunkLongTiles));
+    const long long passes = 10 * ((slots + 15) / 16) - 21 * ((slots + 127) / 128);
+    return head_dim == 128 && archive_chunk_fits(G) && passes * n_tiles * groups > kChunkGain;
 }
 
 size_t select_scores_offset();
@@ -142,19 +160,26 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     st = check_device(arena->device, what);
     if (st != RFSN_OK) return st;
     const bool chunk = packed != nullptr && tiles->per_query == 0 && !stepped && tiles->n > 0 &&
-                       chunk_shape(arena->head_dim, q_heads / kv_heads, q_len, tiles->n);
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, arena->head_dim, packed != nullptr,
-                                  tiles->per_query != 0);
-    RFSN_CHECK_ARG(chunk || sp.zblocks <= kMaxLists, "%s: too many query rows", what);
-    const int hk = sp.rows ? 128 : (arena->head_dim == 128 ? 32 : 64);  // 16-bit keys per item
-    const int per_tile = packed != nullptr ? 1 : kTile / hk;
-    RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
+                       chunk_shape(arena->head_dim, groups, q_heads / kv_heads, q_len, tiles->n);
     const int first = std::min(hot->length, hot->capacity - hot->head_index);
     // with a device step state the window is only known when the kernel runs: planned for the largest
-    const int hot_items = stepped ? (hot->capacity + hk - 1) / hk + 1
-                                  : (first + hk - 1) / hk + (hot->length - first + hk - 1) / hk;
+    auto hot_of = [&](int keys) {  // items of that many ring keys
+        return stepped ? (hot->capacity + keys - 1) / keys + 1
+                       : (first + keys - 1) / keys + (hot->length - first + keys - 1) / keys;
+    };
+    // rows kernel: an item of two tiles is one unit, one of 128 ring keys (twice the bytes) two
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, arena->head_dim, packed != nullptr,
+                                  tiles->per_query != 0, (tiles->n + 1) / 2 + 2LL * hot_of(128));
+    RFSN_CHECK_ARG(chunk || sp.zblocks <= kMaxLists, "%s: too many query rows", what);
+    const int hk = sp.rows ? 128 : (arena->head_dim == 128 ? 32 : 64);
+    const int per_tile = packed != nullptr ? 1 : kTile / hk;
+    RFSN_CHECK_ARG((long long)tiles->n * per_tile < (1LL << 30), "%s: too many tiles", what);
+    const int hot_items = hot_of(hk);
     const int total = std::max(1, sp.rows ? (tiles->n + 1) / 2 + 2 * hot_items : tiles->n * per_tile + hot_items);
     int splits = std::min(split_limit(sp, arena->head_dim, max_splits), total);
+    // The last CTA reads every split's partial: with few lists, more splits than about sqrt(72 units / slots) cost
+    // more there than they save (fitted: 0.8 us a unit, 11 ns a partial row).
+    if (sp.rows) splits = std::min(splits, std::max(1, (int)std::sqrt(72.0 * total / sp.per_cta)));
     const int per = (total + splits - 1) / splits;
     splits = (total + per - 1) / per;
     // more than one split only where all lists leave SMs idle: far fewer lists than arrival counters
@@ -377,12 +402,17 @@ rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, in
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0 && hot_capacity >= 0,
                    "rfsn_archive_workspace_size: negative count");
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, false, n_select > 0);
-    size_t need = std::max(attention_ws_limit(sp, head_dim),
-                           attention_ws_limit(slot_plan(batch, q_heads, kv_heads, q_len, head_dim, true, n_select > 0),
-                                              head_dim));
+    // every plan that a call over up to that many tiles may take
+    auto plan = [&](int per_cta, bool rows) {
+        return make_plan(batch, q_heads, kv_heads, q_len, n_select > 0, per_cta, rows);
+    };
+    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, false, n_select > 0, 0);
+    size_t need = attention_ws_limit(sp, head_dim);
+    if (sp.slots > 4 && n_select == 0 && head_dim == 128)
+        for (int per_cta = 8; per_cta <= 16; per_cta += 8)
+            need = std::max(need, attention_ws_limit(plan(per_cta, true), head_dim));
     if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
-    else if (chunk_shape(head_dim, q_heads / kv_heads, q_len, n_tiles))
+    else if (chunk_shape(head_dim, batch * kv_heads, q_heads / kv_heads, q_len, n_tiles))
         need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity));
     *bytes = need;
     return RFSN_OK;
@@ -415,7 +445,7 @@ rfsn_status rfsn_archive_attend(const rfsn_archive_call* c, const float* q, int 
     rfsn_status st = check_shape(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, true, what);
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(c->tiles.n > 0 && c->tiles.per_query == 0 && c->top_tiles <= (1 << 20), "%s: bad tile list", what);
-    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, c->packed != nullptr, true);
+    const SlotPlan sp = slot_plan(c->batch, c->q_heads, c->kv_heads, c->q_len, head_dim, c->packed != nullptr, true, 0);
     const size_t off = lists_offset(sp, head_dim, c->tiles.n);
     const size_t need = off + sizeof(int4) * (size_t)sp.lists * c->top_tiles;
     if (workspace == nullptr || workspace_bytes < need) {
