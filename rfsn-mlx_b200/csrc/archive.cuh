@@ -56,6 +56,7 @@ struct SelectParams {
     int q_heads, kv_heads, q_len, q_pos0, G;
     const int4* tiles;
     int n_tiles, n_select, tiles_per_cta;
+    int head_groups;        // of four q heads, scored side by side: 1, 2, 4 or 8
     int4* out;              // [groups * q_len][n_select] tiles, or
     int* numbers;           // their numbers only (out is nullptr)
     float* scores;          // workspace [groups * q_len][n_tiles]

@@ -272,9 +272,10 @@ rfsn_status select(const char* what, const void* bounds, int bounds_dtype, const
     p.counters = reinterpret_cast<int*>(ws + 256);
     p.error = reinterpret_cast<int*>(ws);
     p.dyn = step_state;
-    // one CTA per SM over all lists, in steps of the 128 tiles that a CTA scores at once
-    const int want = std::max(1, device_sms() / lists);
-    p.tiles_per_cta = std::max(128, ((tiles->n + want - 1) / want + 127) / 128 * 128);
+    // one CTA per SM over all lists, in steps of the tiles that a CTA scores at once (128 over the head groups)
+    p.head_groups = p.G <= 4 ? 1 : (p.G <= 8 ? 2 : (p.G <= 16 ? 4 : 8));
+    const int want = std::max(1, device_sms() / lists), step = 128 / p.head_groups;
+    p.tiles_per_cta = std::max(step, ((tiles->n + want - 1) / want + step - 1) / step * step);
     const int chunks = std::max(1, (tiles->n + p.tiles_per_cta - 1) / p.tiles_per_cta);
     return select_tiles_launch(bounds_dtype, head_dim, p, lists, chunks, static_cast<cudaStream_t>(stream));
 }

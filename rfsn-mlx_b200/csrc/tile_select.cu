@@ -24,7 +24,19 @@ namespace archive {
 
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kHeadsPerPass = 4;
+constexpr int kHeadsPerPass = 4;  // of a warp
+
+// Eight lanes score kTilesPerLane tiles side by side (each q pair fetched from
+// shared memory serves all of them), kPassTiles at a time per CTA. With more
+// than four q heads per KV head the warps are shared out over up to eight
+// groups of four heads, and a CTA takes as many tiles less at a time (32 heads
+// of 1 KV head, 78 tiles: 31.3 us with the groups one after the other in one
+// CTA, 8.5 us side by side in five). The first pass's bounds are requested
+// before the wait for q: they never come from the kernel that this launch
+// overlaps (packing and bounding are launched without that overlap).
+constexpr int kTilesPerLane = 2;
+constexpr int kPassTiles = kSelWarps * 4 * kTilesPerLane;
+constexpr int kMaxHeadGroups = 8;
 
 template <typename T> struct BoundVec;  // 8 bounds -> float
 template <> struct BoundVec<__nv_bfloat16> {
@@ -77,6 +89,7 @@ struct SelShared {
     int bucket, above, inside;
     int hist[kBuckets];
     alignas(16) int tally[kSelRegKeys * kSelWarps];  // tiles above (low half) and at (high half) the threshold
+    float part[kSelWarps * 4 * kTilesPerLane];       // scores by head group
 };
 
 // The n-th largest key by narrowing a key range: a histogram of 1,024 equal
@@ -258,14 +271,6 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
     for (int i = n + tid; i < p.n_select; i += kSelThreads) put(i, -1);
 }
 
-// Eight lanes score kTilesPerLane tiles side by side (each q pair fetched from
-// shared memory serves all of them), kPassTiles at a time per CTA. The first
-// pass's bounds are requested before the wait for q: they never come from the
-// kernel that this launch overlaps (packing and bounding are launched without
-// that overlap).
-constexpr int kTilesPerLane = 2;
-constexpr int kPassTiles = kSelWarps * 4 * kTilesPerLane;
-
 // A bound as a double has an empty low word (8 or 11 significant bits), so the
 // choice between lo and hi by the sign of q is one word.
 __device__ __forceinline__ double pick(bool up, int hi_hi, int hi_lo) { return __hiloint2double(up ? hi_hi : hi_lo, 0); }
@@ -274,7 +279,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
     constexpr int NV = D / 64;  // vectors of 8 channels per lane
     constexpr int U = kTilesPerLane;
-    __shared__ double2 qs[kHeadsPerPass * D / 2];
+    __shared__ double2 qs[kMaxHeadGroups * kHeadsPerPass * D / 2];
     __shared__ SelShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int list = blockIdx.y;
@@ -317,7 +322,9 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         }
         return f;
     };
-    const int t_lane = t_begin + U * (4 * warp + sub);
+    const int groups = p.head_groups, group_warps = kSelWarps / groups, pass_tiles = kPassTiles / groups;
+    const int group = warp / group_warps, slot = U * (4 * (warp % group_warps) + sub);  // of the pass's tiles
+    const int t_lane = t_begin + slot;
     Fetched f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) f[u] = fetch(t_lane + u);
@@ -325,21 +332,21 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
     griddep_wait();  // q, the step state and the workspace may belong to the kernel this one overlaps
     griddep_launch_dependents();
     const int qpos = (p.dyn != nullptr ? p.dyn[RFSN_STEP_POS] : p.q_pos0) + row;
-    for (int g0 = 0; g0 < p.G; g0 += kHeadsPerPass) {
-        const int heads = min(kHeadsPerPass, p.G - g0);
+    for (int g0 = 0; g0 < p.G; g0 += kHeadsPerPass * groups) {
+        const int heads = p.G - g0 - kHeadsPerPass * group;  // of the warp's group (and more)
         if (g0 > 0) __syncthreads();
-        for (int i = tid; i < kHeadsPerPass * D / 2; i += kSelThreads) {
+        for (int i = tid; i < groups * kHeadsPerPass * D / 2; i += kSelThreads) {
             // pairs of channels 8 (l8 + 8 v) + 2 j, + 1 of a head at [head][4 v + j][l8]: lanes side by side
             const int g = i / (D / 2), pr = i % (D / 2);
             const int d = 8 * ((pr & 7) + 8 * (pr >> 5)) + 2 * ((pr >> 3) & 3);
             float2 x = make_float2(0.f, 0.f);
-            if (g < heads)
+            if (g0 + g < p.G)
                 x = *reinterpret_cast<const float2*>(
                     p.q + (((size_t)b * p.q_heads + hk * p.G + g0 + g) * p.q_len + row) * D + d);
             qs[i] = make_double2((double)x.x, (double)x.y);
         }
         __syncthreads();
-        for (int t0 = 0; t_begin + t0 < t_end; t0 += kPassTiles) {
+        for (int t0 = 0; t_begin + t0 < t_end; t0 += pass_tiles) {
             if (t0 > 0 || g0 > 0) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) f[u] = fetch(t_lane + t0 + u);
@@ -363,7 +370,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
                     }
 #pragma unroll
                     for (int g = 0; g < kHeadsPerPass; ++g) {
-                        const double2 q2 = qs[g * (D / 2) + (4 * v + j) * 8 + l8];
+                        const double2 q2 = qs[(kHeadsPerPass * group + g) * (D / 2) + (4 * v + j) * 8 + l8];
                         const bool up0 = q2.x >= 0.0, up1 = q2.y >= 0.0;
 #pragma unroll
                         for (int u = 0; u < U; ++u) {
@@ -388,15 +395,24 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
                 const unsigned nan = __ballot_sync(0xffffffffu, best != best);
                 best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
                 best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-                if (l8 == 0 && t < t_end) {
-                    if ((nan >> (8 * sub)) & 0xffu) best = CUDART_NAN_F;
-                    if (f[u].e.z <= 0 || f[u].e.y > qpos) best = -CUDART_INF_F;
-                    if (g0 > 0) {  // heads of the earlier passes
-                        const float prev = scores[t];
-                        best = (prev != prev || best != best) ? CUDART_NAN_F : fmaxf(prev, best);
-                    }
+                if ((nan >> (8 * sub)) & 0xffu) best = CUDART_NAN_F;
+                if (f[u].e.z <= 0 || f[u].e.y > qpos) best = -CUDART_INF_F;
+                if (groups > 1) {
+                    if (l8 == 0) sh.part[group * pass_tiles + slot + u] = best;
+                } else if (l8 == 0 && t < t_end) {
                     scores[t] = best;
                 }
+            }
+            if (groups > 1) {  // the head groups of this pass, and those of earlier ones
+                __syncthreads();
+                const int t = t_begin + t0 + tid;
+                if (tid < pass_tiles && t < t_end) {
+                    auto larger = [](float a, float b) { return a != a || b != b ? CUDART_NAN_F : fmaxf(a, b); };
+                    float best = sh.part[tid];
+                    for (int g = 1; g < groups; ++g) best = larger(best, sh.part[g * pass_tiles + tid]);
+                    scores[t] = g0 > 0 ? larger(scores[t], best) : best;
+                }
+                __syncthreads();
             }
         }
     }

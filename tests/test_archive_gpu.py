@@ -326,6 +326,10 @@ SELECT = [
     ("bfloat16", False, 1, 32, 1, 128, (500,), 3, 4, 3),     # 32 heads of one KV head
     ("bfloat16", True, 1, 4, 2, 128, (1,), 1, 1, 1),
     ("bfloat16", False, 1, 4, 2, 128, (64,) * 300, 1, 1, 37),
+    ("float16", False, 1, 10, 2, 64, (64,) * 70, 1, 2, 9),   # head groups side by side: 5, 12, 24 and 40 q heads each
+    ("bfloat16", True, 1, 24, 2, 128, (640, 33, 64), 7, 1, 5),
+    ("bfloat16", False, 2, 24, 1, 64, (1000, 20), 7, 1, 6),
+    ("bfloat16", True, 1, 40, 1, 128, (64,) * 40, 1, 3, 12),
 ]
 
 
