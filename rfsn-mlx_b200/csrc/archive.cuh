@@ -101,13 +101,16 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // Split merge by the last CTA of a list (and block of SL query slots) to
 // arrive; called by threads 0 .. nthreads - 1 of the CTA after they wrote its
 // partials (named barrier 1 is theirs). The partials of all splits are
-// contiguous runs (O, m, l): with room for them in `stage` they come in one
-// round trip of asynchronous copies. wts: room for SL * splits floats.
+// contiguous runs (m, l, O) and come by asynchronous copies through `stage`:
+// m and l with as many splits' O as fit in one round trip, the rest in further
+// ones. Reading them one by one took 13 us for 240 splits of 4 slots. wts: room
+// for SL * splits floats.
 template <int D>
 __device__ __forceinline__ void merge_splits(const Params& p, const OutMap& om, int bh, int slot0, int nslots, int SL,
-                                             int counter, uint8_t* stage, size_t stage_bytes, float* wts, float* inv,
+                                             int counter, uint8_t* stage, int stage_bytes, float* wts, float* inv,
                                              int* flag, int nthreads) {
-    constexpr int V4 = D / 4;  // float4 per row
+    constexpr int V4 = D / 4;   // float4 per row
+    constexpr int kOwn = 2;     // float4 of the result per thread, at most
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     named_barrier_sync(1, nthreads);  // the CTA's partials before thread 0's release
     if (threadIdx.x == 0) *flag = atom_add_acq_rel_gpu(&p.ws.counters[counter], 1) == p.splits - 1;
@@ -115,60 +118,72 @@ __device__ __forceinline__ void merge_splits(const Params& p, const OutMap& om, 
     if (!*flag) return;
     const size_t part_base = (size_t)counter * p.splits * SL;
     const int parts = p.splits * SL;
-    const bool staged = (size_t)parts * (D + 2) * 4 <= stage_bytes;
-    const float* src_o = p.ws.o + part_base * D;
-    const float* src_m = p.ws.m + part_base;
-    const float* src_l = p.ws.l + part_base;
-    if (staged) {
-        float4* st_o = reinterpret_cast<float4*>(stage);
-        float4* st_ml = st_o + (size_t)parts * V4;
-        for (int i = threadIdx.x; i < parts / 2; i += nthreads)
-            cp_async_16(st_ml + i, i < parts / 4 ? src_m + 4 * i : src_l + 4 * (i - parts / 4));
-        for (int i = threadIdx.x; i < parts * V4; i += nthreads) cp_async_16(st_o + i, src_o + 4 * (size_t)i);
+    float4* st_ml = reinterpret_cast<float4*>(stage);
+    float4* st_o = st_ml + parts / 2;
+    const int round = min(p.splits, (stage_bytes - parts * 8) / (SL * D * 4));  // splits per round trip
+    const float* gm = p.ws.m + part_base;
+    const float* gl = p.ws.l + part_base;
+    const float4* go = reinterpret_cast<const float4*>(p.ws.o + part_base * D);
+    for (int i = threadIdx.x; i < parts / 2; i += nthreads)
+        cp_async_16(st_ml + i, i < parts / 4 ? gm + 4 * i : gl + 4 * (i - parts / 4));
+    float4 acc[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < p.splits; s0 += round) {
+        const int n = min(round, p.splits - s0);
+        if (s0 > 0) named_barrier_sync(1, nthreads);  // the stage has been read
+        for (int i = threadIdx.x; i < n * SL * V4; i += nthreads) cp_async_16(st_o + i, go + (size_t)s0 * SL * V4 + i);
         cp_async_commit();
         cp_async_wait_all();
         named_barrier_sync(1, nthreads);
-        src_o = reinterpret_cast<const float*>(st_o);
-        src_m = reinterpret_cast<const float*>(st_ml);
-        src_l = src_m + parts;
-    }
-    auto get = [&](const float* x) { return staged ? *x : __ldcg(x); };
-    for (int sl = warp; sl < nslots; sl += nthreads / 32) {
-        float M = -INFINITY, L = 0.f;
-        for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, get(src_m + s * SL + sl));
+        if (s0 == 0) {
+            const float* src_m = reinterpret_cast<const float*>(st_ml);
+            const float* src_l = src_m + parts;
+            for (int sl = warp; sl < nslots; sl += nthreads / 32) {
+                float M = -INFINITY, L = 0.f;
+                for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, src_m[s * SL + sl]);
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-        for (int s = lane; s < p.splits; s += 32) {
-            const float wt = M == -INFINITY ? 1.f : ex2_approx(get(src_m + s * SL + sl) - M);
-            L += wt * get(src_l + s * SL + sl);
-            wts[sl * p.splits + s] = wt;
+                for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+                for (int s = lane; s < p.splits; s += 32) {
+                    const float wt = M == -INFINITY ? 1.f : ex2_approx(src_m[s * SL + sl] - M);
+                    L += wt * src_l[s * SL + sl];
+                    wts[sl * p.splits + s] = wt;
+                }
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+                if (lane == 0) {
+                    const bool any = L > 0.f || L != L;
+                    inv[sl] = any ? 1.f / L : 0.f;
+                    if (p.lse != nullptr)
+                        p.lse[om.row(bh, slot0 + sl)] = any ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
+                }
+            }
+            named_barrier_sync(1, nthreads);
         }
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-        if (lane == 0) {
-            const bool any = L > 0.f || L != L;
-            inv[sl] = any ? 1.f / L : 0.f;
-            if (p.lse != nullptr)
-                p.lse[om.row(bh, slot0 + sl)] = any ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
-        }
-    }
-    named_barrier_sync(1, nthreads);
-    for (int i = threadIdx.x; i < nslots * V4; i += nthreads) {
-        const int sl = i / V4, d4 = i % V4;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4* from = reinterpret_cast<const float4*>(src_o) + sl * V4 + d4;
+        for (int k = 0; k < kOwn; ++k) {
+            const int i = threadIdx.x + k * nthreads, sl = i / V4;
+            if (i >= nslots * V4) break;
+            const float4* from = st_o + i;
+            const float* w = wts + sl * p.splits + s0;
 #pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) {
-            const float4 o = staged ? from[(size_t)s * SL * V4] : __ldcg(from + (size_t)s * SL * V4);
-            const float wt = wts[sl * p.splits + s];
-            O.x += wt * o.x;
-            O.y += wt * o.y;
-            O.z += wt * o.z;
-            O.w += wt * o.w;
+            for (int s = 0; s < n; ++s) {
+                const float4 o = from[s * SL * V4];
+                const float wt = w[s];
+                acc[k].x += wt * o.x;
+                acc[k].y += wt * o.y;
+                acc[k].z += wt * o.z;
+                acc[k].w += wt * o.w;
+            }
         }
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+        const int i = threadIdx.x + k * nthreads, sl = i / V4;
+        if (i >= nslots * V4) break;
         const float r = inv[sl];
-        *reinterpret_cast<float4*>(p.out + om.row(bh, slot0 + sl) * D + 4 * d4) =
-            make_float4(O.x * r, O.y * r, O.z * r, O.w * r);
+        *reinterpret_cast<float4*>(p.out + om.row(bh, slot0 + sl) * D + 4 * (i % V4)) =
+            make_float4(acc[k].x * r, acc[k].y * r, acc[k].z * r, acc[k].w * r);
     }
     if (threadIdx.x == 0) p.ws.counters[counter] = 0;
 }

@@ -177,9 +177,10 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     const int hot_items = hot_of(hk);
     const int total = std::max(1, sp.rows ? (tiles->n + 1) / 2 + 2 * hot_items : tiles->n * per_tile + hot_items);
     int splits = std::min(split_limit(sp, arena->head_dim, max_splits), total);
-    // The last CTA reads every split's partial: with few lists, more splits than about sqrt(72 units / slots) cost
-    // more there than they save (fitted: 0.8 us a unit, 11 ns a partial row).
-    if (sp.rows) splits = std::min(splits, std::max(1, (int)std::sqrt(72.0 * total / sp.per_cta)));
+    // The last CTA reads every split's partials: with few lists, more splits than about sqrt(c items / slots) cost more
+    // there than they save. Measured (1 KV head, 4 slots, 49K keys, us): 32 splits 18.5, 64 14.0, 96 13.3, 240 17.1;
+    // 5K keys: 16 8.0, 48 7.5, 80 9.3; two heads of 8 slots, 43 tiles: 8 20.1, 24 19.0, 43 20.6.
+    splits = std::min(splits, std::max(1, (int)std::sqrt((sp.rows ? 72.0 : 50.0) * total / sp.per_cta)));
     const int per = (total + splits - 1) / splits;
     splits = (total + per - 1) / per;
     // more than one split only where all lists leave SMs idle: far fewer lists than arrival counters

@@ -728,6 +728,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     }
     if (p.splits == 1) return;
 
+    static_assert(SL * (D / 4) <= 2 * kNCW * 32, "two float4 of the result per thread");
     merge_splits<D>(p, om, bh, slot0, nslots, SL, counter, &sm.stage[0][0], STAGES * kStageBytes, &sm.red_o[0][0][0],
                     sm.red_l[0], &sm.flag, kNCW * 32);
 }

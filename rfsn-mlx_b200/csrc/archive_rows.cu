@@ -708,6 +708,7 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
     }
     if (p.splits == 1) return;
     static_assert(sizeof(sm.p) >= SL * kMaxSplits128 * sizeof(float), "room for the merge's weights");
+    static_assert(SL * V4 <= 2 * kSoftmaxThreads, "two float4 of the result per thread");
     merge_splits<D>(p, om, bh, slot0, nslots, SL, counter, &sm.stage[0][0], sizeof(sm.stage),
                     reinterpret_cast<float*>(sm.p[0]), sm.inv, &sm.flag, kSoftmaxThreads);
 }
