@@ -33,6 +33,11 @@
 // The softmax keeps a reference maximum per query slot that moves only when a
 // logit exceeds it by more than 2^8 (in powers of two), so most strips need
 // one vote instead of a reduction over the lanes and a rescale.
+//
+// Measured, 32 q / 8 KV heads, head_dim 128: 128K packed tokens and 4K ring
+// 50.3 us (5.5 TB/s; 43.2 at the copy rate), 6K and 2K fp16 9.6 us, where the
+// wait for the SMs, q, one round of tiles and the merge are 1 to 2 us each. 8
+// and 16 consumer warps per SM take the same time as 8 (two CTAs of four).
 #include <atomic>
 
 #include <math_constants.h>
@@ -733,7 +738,8 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                     sm.red_l[0], &sm.flag, kNCW * 32);
 }
 
-// Launch shape by column blocks: consumer groups, stages and CTAs per SM.
+// Launch shape by column blocks: consumer groups, stages and CTAs per SM. With two column blocks a CTA needs the
+// registers of a whole SM's share; two CTAs of four warps with one block are 50 us at 128K, one of eight 53.
 template <int NB> struct Shape;
 template <> struct Shape<1> { static constexpr int kGroups = 1, kStages = 6, kCtas = 2; };
 template <> struct Shape<2> { static constexpr int kGroups = 2, kStages = 8, kCtas = 1; };
