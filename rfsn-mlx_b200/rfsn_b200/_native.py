@@ -323,8 +323,14 @@ _nothing = _Nothing()
 def on_device(device: torch.device):
     """Context in which ``device`` is the current CUDA device (a no-op when it
     already is): launches go to its current stream."""
-    current = _current_device() if _current_device is not None else torch.cuda.current_device()
-    return _nothing if device.index is None or device.index == current else torch.cuda.device(device)
+    return _nothing if is_current(device) else torch.cuda.device(device)
+
+
+def is_current(device: torch.device) -> bool:
+    """``device`` is the current CUDA device (or names none)."""
+    index = device.index
+    return index is None or index == (_current_device() if _current_device is not None
+                                      else torch.cuda.current_device())
 
 
 def host_device_pointer(t: torch.Tensor) -> int:

@@ -1146,6 +1146,9 @@ class LayerKVCache:
         (``paged_attention``)."""
         if segments is None:
             segments = self.get_attention_segments()
+        if (top_tiles or self.archive is not None) and segments.spans:  # without the detour: short calls are host-bound
+            return _tile_attention(self, q, q_start_pos, segments, want_lse, max_splits, None, None, None, None,
+                                   top_tiles)
         return paged_attention(self, q, q_start_pos, segments, want_lse=want_lse, max_splits=max_splits,
                                top_tiles=top_tiles)
 
@@ -1170,7 +1173,8 @@ class LayerKVCache:
 
 
 def _query(cache: LayerKVCache, q: torch.Tensor) -> torch.Tensor:
-    if q.dim() != 4 or q.shape[0] != cache.batch_size or q.shape[3] != cache.config.head_dim:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != cache.batch_size or shape[3] != cache.config.head_dim:
         raise ValueError(f"q must be [batch={cache.batch_size}, heads, q_len, head_dim={cache.config.head_dim}]")
     return _as(q, cache.device, torch.float32)
 
@@ -1215,6 +1219,7 @@ def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
         out_ptr = _out_pointer(cache, out, tuple(qf.shape))
     _, H, Lq, _ = qf.shape
     lse = torch.empty(qf.shape[:3], dtype=torch.float32, device=cache.device) if want_lse else None
+    lse_ptr = lse.data_ptr() if want_lse else None
     key = (H, Lq, top_tiles, max_splits)
     call = segments.calls.get(key) if step_state is None else None
     if call is None or not call.current(cache):
@@ -1222,8 +1227,11 @@ def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
         call = PreparedCall(cache, segments, hot, H, Lq, int(top_tiles), max_splits)
         if step_state is None and segments.hot_state is not None:
             segments.calls[key] = call
-    with native.on_device(cache.device):
-        call(cache, qf.data_ptr(), int(q_start_pos), out_ptr, lse.data_ptr() if want_lse else None, workspace)
+    if native.is_current(cache.device):
+        call(cache, qf.data_ptr(), int(q_start_pos), out_ptr, lse_ptr, workspace)
+    else:
+        with torch.cuda.device(cache.device):
+            call(cache, qf.data_ptr(), int(q_start_pos), out_ptr, lse_ptr, workspace)
     return (out, lse) if want_lse else out
 
 
