@@ -556,10 +556,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             if (!warp_wait(&sm.info_full[t % kInfo], (t / kInfo) & 1, &sm.abort)) { failed = true; break; }
             const Info& inf = sm.info[t % kInfo];
             const int pos = inf.pos[ch], len = inf.len[ch];
-            const float u = fmaxf(inf.sv[0], inf.sv[1]);
+            // the larger scale of the halves that some row of the CTA sees
+            const float u = fmaxf(inf.pos[0] <= qlast ? inf.sv[0] : kTiny, inf.pos[1] <= qlast ? inf.sv[1] : kTiny);
             // p comes out of the exponential times f = 2^7 s_v / u; the row sum takes f off again once per tile. Both
             // factors stay normal numbers: a product below them is lost beside the other half (f) or a logit of 0 (c).
-            const float f = fmaxf(inf.sv[ch] / u * kPScale, kMinF), c = fmaxf(qmul * inf.sk[ch], kTiny);
+            const float f = fminf(fmaxf(inf.sv[ch] / u, kMinF), 1.f) * kPScale, c = fmaxf(qmul * inf.sk[ch], kTiny);
             const float lf = log2f(f);
             if (!warp_wait(&sm.s_full[s], (t >> 1) & 1, &sm.abort)) { failed = true; break; }
             tc::fence_after_sync();

@@ -545,9 +545,11 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
             const Info& inf = sm.info[t % kInfo];
             const int len = inf.len[half], pos = inf.pos[half];
             const float sk = inf.sk[half];
-            const float u = fmaxf(inf.sv[0], inf.sv[1]);
-            // p times f: the key's share of the item's unit (16-bit items: a power of two that fits float16)
-            const float f = arch ? fmaxf(inf.sv[half] / u, kMinF) : kPScale;
+            // the item's unit: the larger scale of the halves that some slot sees
+            const float u = fmaxf(inf.pos[0] <= qlast ? inf.sv[0] : kTiny, inf.pos[1] <= qlast ? inf.sv[1] : kTiny);
+            // p times f: the key's share of the unit, nothing to a half behind it (16-bit items: a power of two that
+            // fits float16)
+            const float f = arch ? fminf(fmaxf(inf.sv[half] / u, kMinF), 1.f) : kPScale;
             // logits in log2 units below the reference maximum
 #pragma unroll
             for (int s = 0; s < H; ++s) x[s] = fma2(x[s], mul2(qm[s], both(sk)), nm[s]);

@@ -1050,6 +1050,17 @@ class LayerKVCache:
             self._tiles_dev = self._ops.new_table(64)
         return self._tiles_dev, self._n_tiles
 
+    def takes_step_state(self, q_heads: int) -> bool:
+        """The decode attention of this cache can read the query position and
+        the ring from a device step state (a captured step). Packed caches and
+        selecting ones take any head ratio and head_dim 64 or 128."""
+        D, Hkv = self.config.head_dim, self.num_kv_heads
+        if self.dtype not in (torch.bfloat16, torch.float16) or q_heads % Hkv:
+            return False
+        if self.archive is not None or self.top_tiles:
+            return D in (64, 128)
+        return D == 128 and q_heads // Hkv <= 4
+
     def capture_key(self) -> tuple:
         """Device addresses, beyond the arena's and the page table's, that a
         captured attention call of this layer holds by value."""

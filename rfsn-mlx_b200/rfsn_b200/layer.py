@@ -96,7 +96,8 @@ class GraphedDecodeStep:
     page table or the arena changes; when archived blocks are cold or a
     prefetch is in flight the step runs ``attention_step`` op by op instead.
     Needs bf16/f16 K/V, head_dim 128 and <= 4 query heads per KV head (the
-    tensor-core decode kernel)."""
+    tensor-core decode kernel), or a packed or selecting cache with head_dim 64
+    or 128 (``LayerKVCache.takes_step_state``)."""
 
     def __init__(self, cache: LayerKVCache, q_heads: int) -> None:
         from . import _native as native
@@ -105,8 +106,7 @@ class GraphedDecodeStep:
         B, Hkv, D = cache.batch_size, cache.num_kv_heads, cache.config.head_dim
         self.shape_q = (B, q_heads, 1, D)
         shape_kv = (B, Hkv, 1, D)
-        self.supported = (cache.dtype in (torch.bfloat16, torch.float16) and D == 128 and q_heads % Hkv == 0
-                          and q_heads // Hkv <= 4)
+        self.supported = cache.takes_step_state(q_heads)
         dev = cache.device
         es = torch.empty((), dtype=cache.dtype).element_size()
         align = lambda n: (n + 255) // 256 * 256  # noqa: E731

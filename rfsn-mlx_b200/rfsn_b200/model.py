@@ -387,7 +387,7 @@ class RFSNModel:
         """model.py:167-189: token_id (B,) -> logits (B, vocab).
 
         When the cache allows it (bf16/f16, head_dim 128, <= 4 query heads per KV
-        head, every archived block resident in HBM, no prefetch in flight) the
+        head, or a packed or selecting cache; every archived block resident in HBM, no prefetch in flight) the
         step replays a CUDA graph of the whole network, captured once and again
         after every page-table change; the host only runs the cache bookkeeping.
         Otherwise (or with ``use_graphs = False``) it runs op by op."""
@@ -483,8 +483,7 @@ class _DecodeGraph:
     def supported(model: "RFSNModel", cache: RFSNCache) -> bool:
         cfg = model.config
         return (model.device.type == "cuda" and model.dtype in (torch.bfloat16, torch.float16)
-                and cfg.head_dim == 128 and cfg.num_heads // cfg.num_kv_heads <= 4
-                and all(lc.dtype == model.dtype for lc in cache.layers))
+                and all(lc.dtype == model.dtype and lc.takes_step_state(cfg.num_heads) for lc in cache.layers))
 
     def __init__(self, model: "RFSNModel", cache: RFSNCache) -> None:
         self.model = model

@@ -233,7 +233,7 @@ def test_attention_over_the_archive_and_the_ring(dtype, B, H, Hkv, D, lens, hot,
             check_out(out, lse, want, want_lse, vv)
 
 
-@pytest.mark.parametrize("Lq", [3, 40])  # the tile kernel and the chunk kernel
+@pytest.mark.parametrize("Lq", [3, 40])  # one and several passes of the rows kernel
 @pytest.mark.parametrize("q_pos", [-1, 0, 63, 64, 100, 250])
 def test_queries_among_the_keys_see_the_earlier_ones_only(q_pos, Lq):
     """Positions inside the archive mask part of a tile, whole tiles and the ring; a row before every key gives zeros
@@ -472,19 +472,20 @@ def test_calls_on_another_stream_and_back():
 
 @pytest.mark.parametrize("top_tiles", [0, 3])
 @pytest.mark.parametrize("packed", [True, False])
-def test_graphed_decode_step_equals_the_op_by_op_step(packed, top_tiles):
+@pytest.mark.parametrize("H,D", [(8, 128), (16, 128), (40, 128), (8, 64), (40, 64)])  # 4 to 20 query heads per KV head
+def test_graphed_decode_step_equals_the_op_by_op_step(packed, top_tiles, H, D):
     """Tokens through the seal rule, captured steps against attention_step on a second cache."""
     torch = _torch()
     if not packed and not top_tiles:
         pytest.skip("the exact dense path has its own tests")
     from rfsn_b200.layer import GraphedDecodeStep, attention_step
 
-    caches = [make("bfloat16", 1, 8, 2, 128, (), 0, hot_cap=96, wrap=0, top_tiles=top_tiles,
+    caches = [make("bfloat16", 1, H, 2, D, (), 0, hot_cap=96, wrap=0, top_tiles=top_tiles,
                    archive_dtype="float8_e4m3fn" if packed else None, pool_tokens=2048)[0] for _ in range(2)]
-    step = GraphedDecodeStep(caches[0], 8)
+    step = GraphedDecodeStep(caches[0], H)
     g = torch.Generator().manual_seed(11)
     for pos in range(330):
-        q, k, v = (torch.randn(1, h, 1, 128, generator=g).to(torch.bfloat16) for h in (8, 2, 2))
+        q, k, v = (torch.randn(1, h, 1, D, generator=g).to(torch.bfloat16) for h in (H, 2, 2))
         step.q_host.copy_(q)
         step.k_host.copy_(k)
         step.v_host.copy_(v)
@@ -770,3 +771,204 @@ def test_a_selection_from_no_tiles_reports_nothing():
     assert bool((cache.select_tiles(q, 19, 3) == -1).all())
     assert torch.equal(cache.attend(q, 19, top_tiles=3), cache.attend(q, 19))
     native.default_workspace(cache.device).check()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("H,Hkv,Lq", [(6, 1, 1), (8, 1, 1), (3, 1, 3), (9, 1, 1), (7, 1, 2), (16, 1, 1), (17, 1, 1),
+                                      (5, 1, 7), (33, 1, 1), (130, 1, 1)])
+@pytest.mark.parametrize("lens,hot,wrap", [((64,), 1, 0), ((1, 63, 64, 65, 130), 200, 90), ((1000,) * 5, 300, 299),
+                                           ((), 40, 5)])
+def test_every_count_of_query_slots(dtype, H, Hkv, Lq, lens, hot, wrap):
+    """5 and more query slots of a packed cache, one or several CTAs deep, odd counts and rings that wrap."""
+    torch = _torch()
+    import archive_ref as ref
+
+    cap = hot if wrap else max(hot, 64)
+    cache, k, v = make(dtype, 1, H, Hkv, 128, lens, hot, hot_cap=cap, wrap=wrap % cap)
+    n = sum(lens) + hot
+    q = queries(1, H, Lq, 128)
+    kk, vv = held(cache, k, v, lens)
+    for last in (n - 1, n + 50, n // 2):
+        first = last - Lq + 1
+        if first < 0:
+            continue
+        want, lse = ref.attention(q, kk, vv, torch.arange(n), first)
+        out, got = cache.attend(q, first, want_lse=True)
+        check_out(out, got, want, lse, vv)
+
+
+@pytest.mark.parametrize("Lq", [1, 2, 4, 9, 40])
+def test_captured_calls_replay_on_new_queries(Lq):
+    """A captured call of every kernel gives what the eager call gives, on queries written before each replay."""
+    torch = _torch()
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (1000, 500), 60, tile_index=True)
+    segs = cache.get_attention_segments()
+    q = queries(1, 8, Lq, 128)
+    first = 1560 - Lq
+    from rfsn_b200 import _native as native
+    from rfsn_b200.cache import paged_attention
+
+    ws = [native.Workspace(cache.device) for _ in range(2)]  # a graph keeps the workspace it was captured with
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for i, top in enumerate((0, 3)):
+        with torch.cuda.stream(side):
+            paged_attention(cache, q, first, segs, workspace=ws[i], top_tiles=top)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append([paged_attention(cache, q, first, segs, workspace=ws[i], top_tiles=top) for _ in range(2)])
+        graphs.append(g)
+    for seed in range(3):
+        q.copy_(queries(1, 8, Lq, 128, seed=seed + 20))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for i, top in enumerate((0, 3)):
+            want = cache.attend(q, first, segs, top_tiles=top)
+            assert all(torch.equal(o, want) for o in outs[i])
+
+
+def test_values_of_very_different_size_in_one_call():
+    """Tiles whose V scales are 2^20 apart: the error is measured against the largest value that is seen."""
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (64, 64, 64, 64, 64)
+    for Lq in (1, 4, 40):
+        torch.manual_seed(3)
+        cache, k, v = make("bfloat16", 1, 4, 1, 128, (), 0, hot_cap=64, pool_tokens=2048)
+        v = torch.randn(1, 1, 320, 128, device="cuda")
+        k = torch.randn(1, 1, 320, 128, device="cuda").to(torch.bfloat16)
+        for i, s in enumerate((1.0, 2.0 ** 20, 2.0 ** -20, 1.0, 2.0 ** 10)):
+            v[:, :, 64 * i:64 * i + 64] *= s
+            cache.import_block(k[:, :, 64 * i:64 * i + 64], v[:, :, 64 * i:64 * i + 64].to(torch.bfloat16), 64 * i)
+        v = v.to(torch.bfloat16)
+        kk, vv = held(cache, k, v, lens)
+        q = queries(1, 4, Lq, 128)
+        for last in (63, 319):
+            if last - Lq + 1 < 0:
+                continue
+            want, lse = ref.attention(q, kk, vv, torch.arange(320), last - Lq + 1)
+            out, got = cache.attend(q, last - Lq + 1, want_lse=True)
+            check_out(out, got, want, lse, vv[:, :, :last + 1])
+
+
+# ------------------------------------------------------------------ chunks (128 query slots per CTA)
+def in_chunks(cache, q, first, **kw):
+    """``attend``, checked to run the chunk kernel: the ring's copy or the merge is a launch of its own."""
+    from rfsn_b200 import _native as native
+
+    before = native.launch_count()
+    out = cache.attend(q, first, **kw)
+    assert native.launch_count() - before >= 2
+    return out
+
+
+@pytest.mark.parametrize("dtype,B,H,Hkv,lens,hot,wrap,Lq", [
+    ("bfloat16", 1, 8, 2, (64,) * 81, 100, 0, 128),            # an odd number of tiles
+    ("float16", 2, 8, 2, (70,) * 30 + (64,) * 2, 33, 20, 100),  # ragged tiles, a wrapped ring
+    ("bfloat16", 1, 40, 1, (1000,) * 8, 64, 0, 77),             # 40 heads a row: 3 rows in a CTA, 8 slots idle
+    ("bfloat16", 1, 4, 4, (6000,), 300, 0, 300),
+    ("float16", 1, 128, 1, (5000,), 10, 0, 9),                  # a row per CTA
+])
+def test_chunks_of_queries(dtype, B, H, Hkv, lens, hot, wrap, Lq):
+    torch = _torch()
+    import archive_ref as ref
+
+    cache, k, v = make(dtype, B, H, Hkv, 128, lens, hot, hot_cap=max(hot, 64), wrap=wrap)
+    n = sum(lens) + hot
+    q = queries(B, H, Lq, 128)
+    kk, vv = held(cache, k, v, lens)
+    for first in (n - Lq, n + 7, n // 2, 0, -5):
+        want, lse = ref.attention(q, kk, vv, torch.arange(n), first)
+        out, got = in_chunks(cache, q, first, want_lse=True)
+        check_out(out, got, want, lse, vv)
+    assert torch.equal(in_chunks(cache, q, n - Lq), in_chunks(cache, q, n - Lq))
+
+
+def test_chunks_and_what_lies_behind_them():
+    """NaN K and V behind the last query of a chunk, in its own tile too, in the archive and in the ring. (Against the
+    64-bit form: the scale of a ring tile, and with it the roundings of p, depends on its finite values.)"""
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (64,) * 81
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, lens, 100)
+    q = queries(1, 8, 128, 128)
+    kk, vv = held(cache, k, v, lens)
+    spans = cache.get_attention_segments().spans
+    for last in (5184 + 70, 5183, 5170, 5120, 3000):  # NaN stays from one to the next
+        first = last + 1 - 128
+        for codes in (cache.archive.k.view(torch.uint8), cache.archive.v.view(torch.uint8)):
+            for row, start, n in spans[:81]:
+                if start + n > last + 1:
+                    codes[:, row + max(0, last + 1 - start):row + n] = 0x7F
+        for arena in (cache._arena_k, cache._arena_v):
+            arena[:, max(0, last + 1 - 5184):100] = math.nan
+        want, want_lse = ref.attention(q, kk, vv, torch.arange(5284), first)
+        out, lse = in_chunks(cache, q, first, want_lse=True)
+        check_out(out, lse, want, want_lse, vv)
+
+
+def test_chunks_with_nan_that_is_seen():
+    torch = _torch()
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (64,) * 81, 100)
+    q = queries(1, 8, 128, 128)
+    row = cache.get_attention_segments().spans[7][0]
+    kn, vn = k[:, :, 448:512].clone(), v[:, :, 448:512].clone()
+    kn[0, 1, 3, 5] = math.inf  # packed as NaN: every row of KV head 1
+    vn[0, 0, 4, 7] = math.nan  # channel 7 of KV head 0
+    cache.archive.pack(kn, vn, row)
+    out = in_chunks(cache, q, 5284 - 128)
+    assert bool(torch.isnan(out[0, 4:]).all())
+    fine = torch.ones(128, dtype=torch.bool, device="cuda")
+    fine[7] = False
+    assert bool(torch.isfinite(out[0, :4][..., fine]).all()) and bool(torch.isnan(out[0, :4, :, 7]).all())
+
+
+@pytest.mark.parametrize("v_scale,q_scale", [(1e-6, 1.0), (1e-30, 0.0), (1e30, 60.0), (1.0, 1e-30)])
+def test_chunks_of_extreme_sizes(v_scale, q_scale):
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (64,) * 81
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, lens, 100, v_scale=v_scale)
+    q = queries(1, 8, 128, 128, scale=q_scale)
+    kk, vv = held(cache, k, v, lens)
+    want, lse = ref.attention(q, kk, vv, torch.arange(5284), 5284 - 128)
+    out, got = in_chunks(cache, q, 5284 - 128, want_lse=True)
+    tol = REL * max(1.0, q_scale)  # logits of q_scale times the usual size carry that many times the error
+    assert float((out.double().cpu() - want).abs().max()) <= tol * float(vv.abs().max())
+    assert float((got.double().cpu() - lse).abs().max()) <= tol * 4
+
+
+def test_chunks_captured_and_on_two_streams():
+    torch = _torch()
+    from rfsn_b200 import _native as native
+    from rfsn_b200.cache import paged_attention
+
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (64,) * 81, 100)
+    segs = cache.get_attention_segments()
+    q = queries(1, 8, 128, 128)
+    first = 5284 - 128
+    spaces = [native.Workspace(cache.device) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    for ws, s in zip(spaces, streams):
+        with torch.cuda.stream(s):
+            paged_attention(cache, q, first, segs, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(paged_attention(cache, q, first, segs, workspace=ws))
+        graphs.append(g)
+    for seed in range(3):
+        q.copy_(queries(1, 8, 128, 128, seed=seed + 3))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        want = in_chunks(cache, q, first, segments=segs)
+        assert all(torch.equal(o, want) for o in outs)
