@@ -1195,7 +1195,7 @@ def _out_pointer(cache: LayerKVCache, out: torch.Tensor, shape: tuple) -> int:
         raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
     if out.device.type == "cpu":
         return native.host_device_pointer(out)
-    if out.device == cache.device:
+    if out.device == cache.device or (cache.device.index is None and out.device.type == cache.device.type):
         return out.data_ptr()
     raise ValueError(f"out must be on {cache.device} or pinned host memory")
 
@@ -1280,7 +1280,9 @@ def paged_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
     B, H, Lq, D = (int(x) for x in qf.shape)
     if out is None:
         out = torch.empty((B, H, Lq, D), dtype=torch.float32, device=cache.device)
-    out_ptr = _out_pointer(cache, out, (B, H, Lq, D))
+        out_ptr = out.data_ptr()
+    else:
+        out_ptr = _out_pointer(cache, out, (B, H, Lq, D))
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=cache.device) if want_lse else None
     if segments.table is not None:
         table_dev, n_blocks, toks, tiles = segments.table

@@ -972,3 +972,23 @@ def test_chunks_captured_and_on_two_streams():
         torch.cuda.synchronize()
         want = in_chunks(cache, q, first, segments=segs)
         assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_a_device_without_an_index(packed):
+    """device="cuda" names the current device, for the cache, its archive and results given by the caller."""
+    torch = _torch()
+    from rfsn_b200.cache import paged_attention
+
+    kw = dict(archive_dtype="float8_e4m3fn" if packed else None, tile_index=True)
+    caches = [make("bfloat16", 1, 8, 2, 128, (300,), 20, device=d, **kw)[0] for d in ("cuda", "cuda:0")]
+    q = queries(1, 8, 1, 128)
+    for top in (0, 2):
+        outs = []
+        for c in caches:
+            segs = c.get_attention_segments()
+            outs.append(c.attend(q, 319, segs, top_tiles=top))
+            given = torch.empty_like(q)
+            outs.append(paged_attention(c, q, 319, segs, out=given, top_tiles=top))
+        assert all(torch.equal(o, outs[0]) for o in outs)
+    assert torch.equal(caches[0].select_tiles(q, 319, 2), caches[1].select_tiles(q, 319, 2))
