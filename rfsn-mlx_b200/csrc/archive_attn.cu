@@ -261,7 +261,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = blockIdx.x, list = blockIdx.y, zb = blockIdx.z;
+    const int list = blockIdx.x, split = blockIdx.y, zb = blockIdx.z;
     const int row0 = p.per_query ? list % p.q_len : 0;             // query row of a list of its own
     const int bh = p.per_query ? list / p.q_len : list;
     const int slot0 = (p.per_query ? row0 * p.G : 0) + zb * SL;    // first query slot handled: slot = row * G + head
@@ -758,7 +758,7 @@ rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, c
     }
     const CUtensorMap& k8 = PACKED ? packed->maps[0] : arena->item_maps[0];
     const CUtensorMap& v8 = PACKED ? packed->maps[1] : arena->item_maps[1];
-    RFSN_CUDA(launch_pdl(kern, dim3(p.splits, lists, zblocks), dim3((4 * Sh::kGroups + 1) * 32), smem, s,
+    RFSN_CUDA(launch_pdl(kern, dim3(lists, p.splits, zblocks), dim3((4 * Sh::kGroups + 1) * 32), smem, s,
                          arena->item_maps[0], arena->item_maps[1], k8, v8, p));
     note_launch();
     return RFSN_OK;

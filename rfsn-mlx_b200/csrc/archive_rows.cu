@@ -201,7 +201,7 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
     }
     Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int split = blockIdx.x, bh = blockIdx.y, zb = blockIdx.z;
+    const int bh = blockIdx.x, split = blockIdx.y, zb = blockIdx.z;
     const int slot0 = zb * SL, nslots = min(SL, p.slots - slot0);
 
     // Items: two tiles of the list, then 128 ring keys, of twice the bytes. A split has its share of the ring items,
@@ -733,7 +733,7 @@ rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, c
         RFSN_CUDA(cudaFuncSetAttribute(rows_kernel<T, SL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Sm)));
         if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
-    RFSN_CUDA(launch_pdl(rows_kernel<T, SL>, dim3(p.splits, lists, zblocks), dim3(kThreads), sizeof(Sm), s,
+    RFSN_CUDA(launch_pdl(rows_kernel<T, SL>, dim3(lists, p.splits, zblocks), dim3(kThreads), sizeof(Sm), s,
                          packed->maps[0], packed->maps[1], arena->maps[0], arena->maps[1], p));
     note_launch();
     return RFSN_OK;
