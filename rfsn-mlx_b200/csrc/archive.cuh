@@ -126,6 +126,7 @@ __device__ __forceinline__ void merge_splits(const Params& p, const OutMap& om, 
     const float4* go = reinterpret_cast<const float4*>(p.ws.o + part_base * D);
     for (int i = threadIdx.x; i < parts / 2; i += nthreads)
         cp_async_16(st_ml + i, i < parts / 4 ? gm + 4 * i : gl + 4 * (i - parts / 4));
+    cp_async_commit();
     float4 acc[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -134,9 +135,9 @@ __device__ __forceinline__ void merge_splits(const Params& p, const OutMap& om, 
         if (s0 > 0) named_barrier_sync(1, nthreads);  // the stage has been read
         for (int i = threadIdx.x; i < n * SL * V4; i += nthreads) cp_async_16(st_o + i, go + (size_t)s0 * SL * V4 + i);
         cp_async_commit();
-        cp_async_wait_all();
-        named_barrier_sync(1, nthreads);
-        if (s0 == 0) {
+        if (s0 == 0) {  // the weights while O is on its way
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            named_barrier_sync(1, nthreads);
             const float* src_m = reinterpret_cast<const float*>(st_ml);
             const float* src_l = src_m + parts;
             for (int sl = warp; sl < nslots; sl += nthreads / 32) {
@@ -158,8 +159,9 @@ __device__ __forceinline__ void merge_splits(const Params& p, const OutMap& om, 
                         p.lse[om.row(bh, slot0 + sl)] = any ? (M + log2f(L)) * 0.69314718055994531f : -INFINITY;
                 }
             }
-            named_barrier_sync(1, nthreads);
         }
+        cp_async_wait_all();
+        named_barrier_sync(1, nthreads);
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
             const int i = threadIdx.x + k * nthreads, sl = i / V4;
