@@ -154,35 +154,38 @@ template <int SL> __device__ __forceinline__ int own_slot(int lane) {  // bits o
     return SL == 16 ? lane >> 1 : lane >> 2;
 }
 
-// A row of SL * terms sums from TMEM, the terms joined: e4m3 terms by their weights, 16-bit ones as they are.
+// A row of SL * terms sums from TMEM, the terms joined: e4m3 terms by their weights (in two loads: the registers of
+// all five at once would not stay in place), 16-bit ones as they are.
 template <int SL, int TERMS16>
 __device__ __forceinline__ void load_joined(uint32_t taddr, bool codes, float2 (&x)[SL / 2]) {
-    uint32_t r[4 * SL], r4[SL];
+    static_assert(kTerms == 5 && TERMS16 <= 3, "columns");
+    uint32_t r[2 * SL], r4[SL];
     auto two = [](const uint32_t* w) { return make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])); };
+    auto pair_of_terms = [&](uint32_t at) {
+        if constexpr (SL == 16) tc::ld_32x32b_x32_sync(at, r);
+        else tc::ld_32x32b_x16_sync(at, r);
+    };
+    auto term = [&](uint32_t at) {
+        if constexpr (SL == 16) tc::ld_32x32b_x16_sync(at, r4);
+        else tc::ld_32x32b_x8_sync(at, r4);
+    };
+    const float2 down = both(0.03125f);
     if (codes) {
-        if constexpr (SL == 16) {
-            tc::ld_32x32b_x64_sync(taddr, r);
-            tc::ld_32x32b_x16_sync(taddr + 64, r4);
-        } else {
-            tc::ld_32x32b_x32_sync(taddr, r);
-            tc::ld_32x32b_x8_sync(taddr + 32, r4);
-        }
+        term(taddr + 4 * SL);
+        pair_of_terms(taddr + 2 * SL);
 #pragma unroll
-        for (int s = 0; s < SL / 2; ++s) {
-            float2 v = two(r4 + 2 * s);
+        for (int s = 0; s < SL / 2; ++s)
+            x[s] = fma2(fma2(two(r4 + 2 * s), down, two(r + SL + 2 * s)), down, two(r + 2 * s));
+        pair_of_terms(taddr);
 #pragma unroll
-            for (int j = kTerms - 2; j >= 0; --j) v = fma2(v, both(0.03125f), two(r + j * SL + 2 * s));
-            x[s] = v;
-        }
+        for (int s = 0; s < SL / 2; ++s) x[s] = fma2(fma2(x[s], down, two(r + SL + 2 * s)), down, two(r + 2 * s));
     } else {
-        if constexpr (SL == 16) tc::ld_32x32b_x64_sync(taddr, r);
-        else tc::ld_32x32b_x32_sync(taddr, r);
+        pair_of_terms(taddr);
+        if (TERMS16 == 3) term(taddr + 2 * SL);
 #pragma unroll
         for (int s = 0; s < SL / 2; ++s) {
-            float2 v = two(r + (TERMS16 - 1) * SL + 2 * s);
-#pragma unroll
-            for (int j = TERMS16 - 2; j >= 0; --j) v = add2(v, two(r + j * SL + 2 * s));
-            x[s] = v;
+            const float2 low = TERMS16 == 3 ? add2(two(r4 + 2 * s), two(r + SL + 2 * s)) : two(r + SL + 2 * s);
+            x[s] = add2(low, two(r + 2 * s));
         }
     }
 }
