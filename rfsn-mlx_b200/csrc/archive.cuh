@@ -17,7 +17,7 @@ struct rfsn_packed_archive {
     int rows;
     int head_dim;
     int device;
-    CUtensorMap maps[2];  // K and V, boxes of one 64-token tile
+    CUtensorMap maps[4];  // K and V: boxes of one 64-token tile, boxes of 16 rows
 };
 
 namespace rfsn {

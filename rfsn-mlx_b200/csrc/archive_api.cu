@@ -326,6 +326,8 @@ rfsn_status rfsn_packed_archive_create(void* k_codes, void* v_codes, float* scal
     cudaGetDevice(&a->device);
     rfsn_status st = encode_rows_map(&a->maps[0], k_codes, RFSN_E4M3, batch_kv_heads, rows, head_dim, kTile);
     if (st == RFSN_OK) st = encode_rows_map(&a->maps[1], v_codes, RFSN_E4M3, batch_kv_heads, rows, head_dim, kTile);
+    if (st == RFSN_OK) st = encode_rows_map(&a->maps[2], k_codes, RFSN_E4M3, batch_kv_heads, rows, head_dim, 16);
+    if (st == RFSN_OK) st = encode_rows_map(&a->maps[3], v_codes, RFSN_E4M3, batch_kv_heads, rows, head_dim, 16);
     if (st != RFSN_OK) {
         delete a;
         return st;

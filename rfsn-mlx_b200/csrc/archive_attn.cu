@@ -249,6 +249,7 @@ template <typename T, int D, int NB, int GROUPS, int STAGES, int CTAS, bool PACK
 __global__ void __launch_bounds__((4 * GROUPS + 1) * 32, CTAS)
 archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_constant__ CUtensorMap mapV16,
                     const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ CUtensorMap mapV8,
+                    const __grid_constant__ CUtensorMap stripK8, const __grid_constant__ CUtensorMap stripV8,
                     const Params p) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using Geo = Geometry<D>;
@@ -332,10 +333,18 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                     if (d.z <= 0) {
                         mbar_arrive(&sm.full[s]);  // nothing to load
                     } else if (PACKED && packed) {
-                        mbar_arrive_expect_tx(&sm.full[s], 2 * kTile * D + 16);
-                        const int r = bh * p.packed_rows + d.x;
-                        tma_load_2d(st, &mapK8, 0, r, &sm.full[s]);
-                        tma_load_2d(st + Geo::kVPacked, &mapV8, 0, r, &sm.full[s]);
+                        // of a tile at a block's end only the strips of 16 keys that it has
+                        const int strips = (d.z + 15) / 16, r = bh * p.packed_rows + d.x;
+                        mbar_arrive_expect_tx(&sm.full[s], strips * 32 * D + 16);
+                        if (strips == 4) {
+                            tma_load_2d(st, &mapK8, 0, r, &sm.full[s]);
+                            tma_load_2d(st + Geo::kVPacked, &mapV8, 0, r, &sm.full[s]);
+                        } else {
+                            for (int i = 0; i < strips; ++i) {
+                                tma_load_2d(st + 16 * D * i, &stripK8, 0, r + 16 * i, &sm.full[s]);
+                                tma_load_2d(st + Geo::kVPacked + 16 * D * i, &stripV8, 0, r + 16 * i, &sm.full[s]);
+                            }
+                        }
                         bulk_load(&sm.meta[s], p.scales + (size_t)bh * (p.packed_rows / kTile) + d.x / kTile, 16,
                                   &sm.full[s]);
                     } else {
@@ -465,7 +474,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
         const int4 inf = sm.info[s];
         const uint32_t sb = smem_u32(sm.stage[s]);
         if (PACKED && inf.x) {
-            const int k_strip = 16 * gwarp;
+            const int k_strip = 16 * ((gwarp + it / GROUPS) & 3);  // in turn: a block's short last tile is not always warp 0's
             const int seen = min(inf.z, qlast - inf.y + 1) - k_strip;
             const bool mine = seen > 0;
             if (mine) {
@@ -565,7 +574,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
             }
         } else {
             // 16-bit item: HK / 16 strips; with two strips the group's warp pairs take turns
-            const int strip = HK == 64 ? gwarp : (gwarp & 1);
+            const int strip = HK == 64 ? (gwarp + it / GROUPS) & 3 : (gwarp & 1);
             const bool mine = HK == 64 || (gwarp >> 1) == ((it / GROUPS) & 1);
             const int sv = min(inf.z, qlast - inf.y + 1) - 16 * strip;  // keys of the strip that some slot sees
             if (mine && sv > 0) {
@@ -758,8 +767,10 @@ rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, c
     }
     const CUtensorMap& k8 = PACKED ? packed->maps[0] : arena->item_maps[0];
     const CUtensorMap& v8 = PACKED ? packed->maps[1] : arena->item_maps[1];
+    const CUtensorMap& ks = PACKED ? packed->maps[2] : arena->item_maps[0];
+    const CUtensorMap& vs = PACKED ? packed->maps[3] : arena->item_maps[1];
     RFSN_CUDA(launch_pdl(kern, dim3(lists, p.splits, zblocks), dim3((4 * Sh::kGroups + 1) * 32), smem, s,
-                         arena->item_maps[0], arena->item_maps[1], k8, v8, p));
+                         arena->item_maps[0], arena->item_maps[1], k8, v8, ks, vs, p));
     note_launch();
     return RFSN_OK;
 }

@@ -193,6 +193,7 @@ __device__ __forceinline__ void load_joined(uint32_t taddr, bool codes, float2 (
 template <typename T, int SL>
 __global__ void __launch_bounds__(kThreads, 1)
 rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ CUtensorMap mapV8,
+            const __grid_constant__ CUtensorMap stripK8, const __grid_constant__ CUtensorMap stripV8,
             const __grid_constant__ CUtensorMap mapK16, const __grid_constant__ CUtensorMap mapV16, const Params p) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     using Sm = Smem<SL, BF16>;
@@ -309,17 +310,26 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
                         sm.info[it % kInfo] = inf;
                         uint64_t* full = &sm.full[slot % kStages];
                         uint8_t* dst = sm.stage[slot % kStages];
-                        const int parts = (inf.len[0] > 0) + (inf.len[1] > 0);
-                        if (parts > 0)
-                            mbar_arrive_expect_tx(full, parts * 2 * kTile * D);
+                        // of a tile at a block's end only the strips of 16 keys that it has
+                        const int strips[2] = {(inf.len[0] + 15) / 16, (inf.len[1] + 15) / 16};
+                        if (strips[0] + strips[1] > 0)
+                            mbar_arrive_expect_tx(full, (strips[0] + strips[1]) * 32 * D);
                         else
                             mbar_arrive(full);
-                        for (int h = 0; h < 2; ++h)
-                            if (inf.len[h] > 0) {
-                                const int g = bh * p.packed_rows + r[h];
-                                tma_load_2d(dst + h * kTile * D, &mapK8, 0, g, full);
-                                tma_load_2d(dst + BN * D + h * kTile * D, &mapV8, 0, g, full);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int g = bh * p.packed_rows + r[h];
+                            uint8_t* k = dst + h * kTile * D;
+                            if (strips[h] == 4) {
+                                tma_load_2d(k, &mapK8, 0, g, full);
+                                tma_load_2d(k + BN * D, &mapV8, 0, g, full);
+                            } else {
+                                for (int i = 0; i < strips[h]; ++i) {
+                                    tma_load_2d(k + 16 * D * i, &stripK8, 0, g + 16 * i, full);
+                                    tma_load_2d(k + BN * D + 16 * D * i, &stripV8, 0, g + 16 * i, full);
+                                }
                             }
+                        }
                     }
                 }
                 ++slot;
@@ -737,7 +747,8 @@ rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, c
         if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
     RFSN_CUDA(launch_pdl(rows_kernel<T, SL>, dim3(lists, p.splits, zblocks), dim3(kThreads), sizeof(Sm), s,
-                         packed->maps[0], packed->maps[1], arena->maps[0], arena->maps[1], p));
+                         packed->maps[0], packed->maps[1], packed->maps[2], packed->maps[3], arena->maps[0],
+                         arena->maps[1], p));
     note_launch();
     return RFSN_OK;
 }
