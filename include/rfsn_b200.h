@@ -493,10 +493,10 @@ RFSN_API rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* archive, int sr
  *   - the archived keys are the listed tiles: of `packed` when it is given
  *     (K = code * scale, V = code * scale), else of `arena` itself;
  *   - the hot window is always `arena`'s (the cache's 16-bit type);
- *   - head_dim 64 or 128, bf16/f16 arenas; any q_len and GQA ratio. From 64
- *     query slots (q_len * q_heads / kv_heads) on, 24 over 256 tiles and more,
- *     a packed archive with head_dim 128 runs the tcgen05 kernel; else K/V are
- *     read again for every 8 query slots.
+ *   - head_dim 64 or 128, bf16/f16 arenas; any q_len and GQA ratio. Over a
+ *     packed archive K/V are read once for every 16 query slots (q_len *
+ *     q_heads / kv_heads; 8 with head_dim 64 or short contexts), for every 128
+ *     where that is faster; else once for every 8.
  * Scores are accurate to float32 rounding (q and p are split into two float16
  * or three bfloat16 terms for the tensor cores).
  * A key behind a row's position changes nothing in it, with one exception: a

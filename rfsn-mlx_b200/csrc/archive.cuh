@@ -212,9 +212,9 @@ rfsn_status archive_rows_launch(const rfsn_arena* arena, const rfsn_packed_archi
                                 int lists, int slots, int zblocks, cudaStream_t stream);
 void preload_rows_kernels();
 
-// archive_chunk.cu: chunks of queries over a packed archive, head_dim 128. Workspace: partials and a copy of the ring.
+// archive_chunk.cu: chunks of queries over a packed archive. Workspace: partials and a copy of the ring.
 bool archive_chunk_fits(int G);
-size_t archive_chunk_ws(int groups, int hot_capacity);
+size_t archive_chunk_ws(int groups, int hot_capacity, int head_dim);
 rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& a,
                                  int batch, void* workspace, size_t workspace_bytes, int max_splits,
                                  cudaStream_t stream);

@@ -82,17 +82,21 @@ size_t attention_ws_limit(const SlotPlan& sp, int head_dim) {
     return attention_ws(sp, limit, head_dim).total;
 }
 
-// Packed archives with head_dim 128: the rows kernel reads K/V again for every
-// 16 query slots, the chunk kernel for every 128, at about 2.1 times the cost
-// of a pass, and 9 us more to begin with. Measured (8 KV heads, us, rows /
-// chunk kernel): 32 slots over 16K keys 24 / 35, 131K 107 / 125; 48 slots over
-// 16K 30 / 35, 33K 49 / 52, 131K 155 / 126; 64 slots over 4K 18 / 22, 16K 39 / 36,
-// 33K 69 / 53; 1 KV head: 96 slots over 33K 22 / 35.
-constexpr long long kChunkGain = 38000;  // 10 * 64-token tiles of all heads * passes saved
+// Packed archives: the rows kernel (head_dim 128) reads K/V again for every 16
+// query slots, the tile kernel (head_dim 64) for every 8, the chunk kernel for
+// every 128, at about 2.1 (1.95) times the cost of a pass, and 9 us more to
+// begin with. Measured (8 KV heads, us, rows / chunk kernel): 32 slots over 16K
+// keys 24 / 35, 131K 107 / 125; 48 slots over 16K 30 / 35, 33K 49 / 52, 131K 155 /
+// 126; 64 slots over 4K 18 / 22, 16K 39 / 36, 33K 69 / 53; 1 KV head: 96 slots over
+// 33K 22 / 35. head_dim 64 (tile / chunk kernel): 24 slots over 16K 23 / 26, 33K 41 /
+// 39; 64 over 4K 19 / 18, 16K 57 / 27; 1,024 over 16K 743 / 116; 1 KV head: 128 over
+// 16K 17 / 23, 256 31 / 23.
+// With fewer than 5 units of 128 slots (times 32 key ranges) it leaves SMs idle and a unit's pass costs as much as 5's.
 bool chunk_shape(int head_dim, int groups, int G, int q_len, int n_tiles) {
-    const long long slots = q_len * (long long)G;
-    const long long passes = 10 * ((slots + 15) / 16) - 21 * ((slots + 127) / 128);
-    return head_dim == 128 && archive_chunk_fits(G) && passes * n_tiles * groups > kChunkGain;
+    const long long slots = q_len * (long long)G, units = std::max(5LL, (slots + 127) / 128 * groups);
+    const long long saved = head_dim == 128 ? 20 * ((slots + 15) / 16) * groups - 42 * units   // 20 * passes of a head
+                                            : 20 * ((slots + 7) / 8) * groups - 39 * units;
+    return archive_chunk_fits(G) && saved * n_tiles > 76000;  // * 64-token tiles
 }
 
 size_t select_scores_offset();
@@ -417,7 +421,7 @@ rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, in
             need = std::max(need, attention_ws_limit(plan(per_cta, true), head_dim));
     if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
     else if (chunk_shape(head_dim, batch * kv_heads, q_heads / kv_heads, q_len, n_tiles))
-        need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity));
+        need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity, head_dim));
     *bytes = need;
     return RFSN_OK;
 }

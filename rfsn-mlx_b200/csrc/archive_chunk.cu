@@ -1,5 +1,5 @@
 // Attention of a chunk of queries over a packed archive and the hot window on
-// tcgen05 tensor cores (head_dim 128).
+// tcgen05 tensor cores.
 //
 //   out = softmax(q K^T / sqrt(D) + causal) V,  K = code * s_k(tile), V = code * s_v(tile)
 //
@@ -51,11 +51,9 @@ namespace rfsn {
 namespace archive {
 namespace chunk {
 
-constexpr int D = 128;
 constexpr int BM = 128;               // query rows per CTA
 constexpr int BN = 128;               // keys per tile
-constexpr int kHalfBytes = BN * 128;  // one 64-channel half of a float16 operand tile
-constexpr int kCodeBytes = BN * D;    // codes of K or V of a tile
+constexpr int kHalfBytes = BN * 128;  // 64 channels of a float16 operand tile
 constexpr int kStages = 2;            // staging, operand and S/P buffers alike
 // Tile infos in flight. Tile t + 8 is posted when the staging slot two before its own is free, at the earliest after
 // K(t + 7) was copied: S(t + 5) was done then, which needs P V (t + 3) and so the softmax of tile t to be over.
@@ -67,16 +65,18 @@ constexpr int kConvWarp = 8, kProducerWarp = 12, kMmaWarp = 13;
 constexpr int kMaxSplit = 32;  // key ranges of a unit
 constexpr float kTiny = 1.17549435e-38f;  // 2^-126
 constexpr float kMinF = 7.8886091e-31f;   // 2^-100
-constexpr uint32_t kTmemCols = 512, kColO = 256, kColQhi = 384, kColQlo = 448;
+constexpr uint32_t kTmemCols = 512, kColO = 256, kColQ = 384;  // q: hi, then lo, head_dim / 2 columns each
 
 struct Info {
     int pos[2], len[2];
     float sk[2], sv[2];
 };
 
+template <int D>
 struct Smem {
-    uint8_t k[kStages][2][kHalfBytes];   // float16 operands
-    uint8_t v[kStages][2][kHalfBytes];
+    static constexpr int kCodeBytes = BN * D;  // codes of K or V of a tile
+    uint8_t k[kStages][D / 64][kHalfBytes];   // float16 operands
+    uint8_t v[kStages][D / 64][kHalfBytes];
     uint8_t staged[kStages][2 * kCodeBytes];  // codes of K and V of a tile, or K or V of a float16 hot tile
     uint64_t c_full[kStages], c_empty[kStages];
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
@@ -155,40 +155,45 @@ __device__ __forceinline__ void split_half_rn(float a, float b, uint32_t& hi, ui
 }
 
 // Codes of 128 keys -> float16 operand tile: a thread widens 16 codes (one
-// 16-byte chunk of a row) at a time. Eight lanes cover a row, and the lanes of
-// the upper channel half store their two chunks in the other order, so that
-// both the load and the stores meet every bank once. Rows from first (second)
-// of the two 64-key halves on are zeroed: a half without keys (its staging
-// holds an earlier tile), and V of keys that no query row of the CTA sees.
+// 16-byte chunk of a row) at a time. The lanes of a phase cover whole rows of
+// codes; with head_dim 128 those of the upper channel half store their two
+// chunks in the other order, so that both the load and the stores meet every
+// bank once. Rows from first (second) of the two 64-key halves on are zeroed: a
+// half without keys (its staging holds an earlier tile), and V of keys that no
+// query row of the CTA sees.
+template <int D>
 __device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t op, int first, int second) {
-    const int th = threadIdx.x & 127, c = th & 7, r0 = th >> 3;
-    const int c0 = (2 * c) & 7, swap = c >> 2;
-    // rows r0 + 16 i share r & 7, so the swizzled chunk offsets are the thread's own
-    const uint32_t from = codes + r0 * 128 + ((c ^ (r0 & 7)) << 4);
-    const uint32_t to = op + (c >> 2) * kHalfBytes + r0 * 128;
+    constexpr int kChunks = D / 16, kRows = 128 / kChunks;  // chunks of a row, rows at a time
+    const int th = threadIdx.x & 127, c = th % kChunks, r0 = th / kChunks;
+    const int c0 = (2 * c) & 7, half = c >> 2, swap = D == 128 ? half : 0;
+    // rows r0 + kRows i share r & 7, so the swizzled chunk offsets are the thread's own
+    const uint32_t from = codes + r0 * D + ((D == 128 ? c ^ (r0 & 7) : c ^ ((r0 >> 1) & 3)) << 4);
+    const uint32_t to = op + half * kHalfBytes + r0 * 128;
     const uint32_t to0 = to + (((c0 + swap) ^ (r0 & 7)) << 4), to1 = to + (((c0 + 1 - swap) ^ (r0 & 7)) << 4);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // the two 64-key halves, four loads in flight
-        uint4 x[4];
+    for (int h = 0; h < 2; ++h) {  // the two 64-key halves, their loads in flight together
+        constexpr int kLoads = kTile / kRows;
+        uint4 x[kLoads];
         const int live = (h ? second : first) - r0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            x[i] = 16 * i < live ? lds_u4(from + (64 * h + 16 * i) * 128) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kLoads; ++i)
+            x[i] = kRows * i < live ? lds_u4(from + (64 * h + kRows * i) * D) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kLoads; ++i) {
             const uint4 a = make_uint4(widen(x[i].x), widen_hi(x[i].x), widen(x[i].y), widen_hi(x[i].y));
             const uint4 b = make_uint4(widen(x[i].z), widen_hi(x[i].z), widen(x[i].w), widen_hi(x[i].w));
-            sts_u4(to0 + (64 * h + 16 * i) * 128, swap ? b : a);
-            sts_u4(to1 + (64 * h + 16 * i) * 128, swap ? a : b);
+            sts_u4(to0 + (64 * h + kRows * i) * 128, swap ? b : a);
+            sts_u4(to1 + (64 * h + kRows * i) * 128, swap ? a : b);
         }
     }
 }
 
 // A float16 tile that is already in the operand's layout; rows zeroed as above.
+template <int D>
 __device__ __forceinline__ void copy_tile(uint32_t from, uint32_t op, int first, int second) {
     const int th = threadIdx.x & 127;
 #pragma unroll
-    for (int i = 0; i < 2 * kHalfBytes / 16 / 128; i += 8) {
+    for (int i = 0; i < D / 64 * kHalfBytes / 16 / 128; i += 8) {
         uint4 x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -208,6 +213,7 @@ __device__ __forceinline__ void publish(uint64_t* bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ CUtensorMap mapV8,
              const __grid_constant__ CUtensorMap mapKh, const __grid_constant__ CUtensorMap mapVh, const Params p) {
@@ -216,7 +222,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         if (threadIdx.x == 0) atomicExch(p.ws.error, kDevErrBadTable);
         return;
     }
-    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    constexpr int kCodeBytes = Smem<D>::kCodeBytes;
+    constexpr uint32_t kColQlo = kColQ + D / 2;
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>(smem_raw);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int G = p.G, ppc = BM / G;
     // Units (query block, KV head): latest query blocks first, the heads
@@ -296,9 +304,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                 const int v_first = min(inf.len[0], qlast - inf.pos[0] + 1), v_second = min(inf.len[1], qlast - inf.pos[1] + 1);
                 const uint32_t k_op = smem_u32(sm.k[s][0]), v_op = smem_u32(sm.v[s][0]);
                 if (arch) {
-                    convert_tile(smem_u32(sm.staged[slot & 1]), k_op, first, second);
+                    convert_tile<D>(smem_u32(sm.staged[slot & 1]), k_op, first, second);
                 } else {
-                    copy_tile(smem_u32(sm.staged[slot & 1]), k_op, first, second);
+                    copy_tile<D>(smem_u32(sm.staged[slot & 1]), k_op, first, second);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.c_empty[slot & 1]);
                     ++slot;
@@ -308,9 +316,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                      (t < kStages || warp_wait(&sm.v_empty[s], ph ^ 1, &sm.abort));
                 if (!ok) break;
                 if (arch)
-                    convert_tile(smem_u32(sm.staged[slot & 1]) + kCodeBytes, v_op, v_first, v_second);
+                    convert_tile<D>(smem_u32(sm.staged[slot & 1]) + kCodeBytes, v_op, v_first, v_second);
                 else
-                    copy_tile(smem_u32(sm.staged[slot & 1]), v_op, v_first, v_second);
+                    copy_tile<D>(smem_u32(sm.staged[slot & 1]), v_op, v_first, v_second);
                 publish(&sm.v_full[s]);
                 if (lane == 0) mbar_arrive(&sm.c_empty[slot & 1]);
                 ++slot;
@@ -409,8 +417,8 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                                         full = &sm.c_full[slot & 1];
                                         dst = sm.staged[slot & 1];
                                     }
-                                    mbar_arrive_expect_tx(full, 2 * kHalfBytes);
-                                    for (int c = 0; c < 2; ++c)
+                                    mbar_arrive_expect_tx(full, D / 64 * kHalfBytes);
+                                    for (int c = 0; c < D / 64; ++c)
                                         for (int h = 0; h < 2; ++h)
                                             tma_load_2d(dst + c * kHalfBytes + h * kTile * 128, w ? &mapVh : &mapKh,
                                                         64 * c, g + h * kTile, full);
@@ -449,9 +457,9 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                         const uint32_t tS = tmem + 128 * s;
 #pragma unroll 1
                         for (int part = 0; part < 2; ++part) {
-                            const uint32_t tQ = tmem + (part ? kColQlo : kColQhi);
+                            const uint32_t tQ = tmem + (part ? kColQlo : kColQ);
 #pragma unroll
-                            for (int kk = 0; kk < 8; ++kk)
+                            for (int kk = 0; kk < D / 16; ++kk)
                                 tc::mma_f16_ts(leader, tS, tQ + 8 * kk,
                                                tc::smem_desc_sw128(smem_u32(sm.k[s][kk >> 2]) + (kk & 3) * 32, 16, 1024),
                                                id_qk, part > 0 || kk > 0);
@@ -498,11 +506,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         float qmul;
         {
             const float* src =
-                p.q + (((size_t)b * p.q_heads + hk * G + g) * p.q_len + (row_ok ? qrow : 0)) * D + 64 * ch;
-            float4 x[16];
+                p.q + (((size_t)b * p.q_heads + hk * G + g) * p.q_len + (row_ok ? qrow : 0)) * D + D / 2 * ch;
+            float4 x[D / 8];
             float a = 0.f;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
+            for (int c = 0; c < D / 8; ++c) {
                 x[c] = row_ok ? *reinterpret_cast<const float4*>(src + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
                 a = fmaxf(a, fmaxf(fmaxf(fabsf(x[c].x), fabsf(x[c].y)), fmaxf(fabsf(x[c].z), fabsf(x[c].w))));
             }
@@ -514,24 +522,29 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             e = max(-126, min(126, e));
             const float up = __uint_as_float((uint32_t)(e + 127) << 23);
             qmul = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
-            uint32_t hi[32], lo[32];
+            uint32_t hi[D / 4], lo[D / 4];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
+            for (int c = 0; c < D / 8; ++c) {
                 split_half_rn(x[c].x * up, x[c].y * up, hi[2 * c], lo[2 * c]);
                 split_half_rn(x[c].z * up, x[c].w * up, hi[2 * c + 1], lo[2 * c + 1]);
             }
-            tc::st_32x32b_x32(tmem + lane_base + kColQhi + 32 * ch, hi);
-            tc::st_32x32b_x32(tmem + lane_base + kColQlo + 32 * ch, lo);
+            if constexpr (D == 128) {
+                tc::st_32x32b_x32(tmem + lane_base + kColQ + 32 * ch, hi);
+                tc::st_32x32b_x32(tmem + lane_base + kColQlo + 32 * ch, lo);
+            } else {
+                tc::st_32x32b_x16(tmem + lane_base + kColQ + 16 * ch, hi);
+                tc::st_32x32b_x16(tmem + lane_base + kColQlo + 16 * ch, lo);
+            }
             tc::wait_st();
         }
         tc::fence_before_sync();
         named_barrier_sync(1, kSoftmaxThreads + 32);
 
         const int qpos = p.q_pos0 + qrow;
-        const uint32_t tO = tmem + kColO + lane_base + 64 * ch;
-        float2 acc[32];  // O of the row's channels 64 ch .. 64 ch + 63
+        const uint32_t tO = tmem + kColO + lane_base + D / 2 * ch;
+        float2 acc[D / 4];  // O of the row's channel half ch
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
+        for (int i = 0; i < D / 4; ++i) acc[i] = make_float2(0.f, 0.f);
         float m = -CUDART_INF_F, l = 0.f, w_prev = 0.f;
         bool failed = false;
         // acc += w O(t): P V of tile t out of TMEM, 32 columns at a time
@@ -539,7 +552,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             if (!warp_wait(&sm.pv_done[t & 1], (t >> 1) & 1, &sm.abort)) return false;
             tc::fence_after_sync();
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < D / 64; ++c) {
                 uint32_t o[32];
                 tc::ld_32x32b_x32_sync(tO + 32 * c, o);
 #pragma unroll
@@ -616,7 +629,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
             w_prev = u * (1.f / kPScale);
             if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) acc[i] = make_float2(acc[i].x * alpha, acc[i].y * alpha);
+                for (int i = 0; i < D / 4; ++i) acc[i] = make_float2(acc[i].x * alpha, acc[i].y * alpha);
             }
         }
         if (!failed && nt > 0 && !drain(nt - 1, w_prev)) failed = true;
@@ -637,11 +650,11 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
         // the call's output, or this split's normalised output and log-sum-exp for chunk_merge_kernel
         const bool whole = p.nsplit == 1;
         const size_t orow = whole ? ((size_t)b * p.q_heads + hk * G + g) * p.q_len + qrow : (size_t)blockIdx.x * BM + r;
-        float* dst = (whole ? p.out : p.ws.o) + (!whole || row_ok ? orow : 0) * D + 64 * ch;
+        float* dst = (whole ? p.out : p.ws.o) + (!whole || row_ok ? orow : 0) * D + D / 2 * ch;
         float* dst_lse = whole ? p.lse : p.ws.m;
         if (!whole || row_ok) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
+            for (int i = 0; i < D / 4; i += 2)
                 *reinterpret_cast<float4*>(dst + 2 * i) =
                     make_float4(acc[i].x * inv, acc[i].y * inv, acc[i + 1].x * inv, acc[i + 1].y * inv);
             if (ch == 0 && dst_lse != nullptr) dst_lse[orow] = lse;
@@ -659,6 +672,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
 // out = sum_s e^(lse_s - M) O_s / sum_s e^(lse_s - M) over the splits of a unit's
 // keys: one warp per query row, a lane holding 4 channels. Bound by the
 // partials' bytes (64 KB per part, from L2).
+template <int D>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(const Params p) {
     griddep_wait();
     const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -679,7 +693,8 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const Params p) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4* src = reinterpret_cast<const float4*>(p.ws.o + base * D) + lane;
+    const int c = lane % (D / 4);  // with head_dim 64 the upper half of the lanes repeats the lower one
+    const float4* src = reinterpret_cast<const float4*>(p.ws.o + base * D) + c;
 #pragma unroll 8
     for (int s = 0; s < p.nsplit; ++s) {
         const float4 o = __ldcg(src + (size_t)s * BM * (D / 4));
@@ -692,27 +707,28 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const Params p) {
     const bool some = L > 0.f || L != L;
     const float inv = some ? 1.f / L : 0.f;
     const size_t orow = ((size_t)(bh / p.kv_heads) * p.q_heads + (bh % p.kv_heads) * p.G + g) * p.q_len + qrow;
-    reinterpret_cast<float4*>(p.out + orow * D)[lane] =
-        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (lane < D / 4)
+        reinterpret_cast<float4*>(p.out + orow * D)[c] = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     if (lane == 0 && p.lse != nullptr) p.lse[orow] = some ? M + logf(L) : -CUDART_INF_F;
 }
 
 // The live ring tokens as float16 tiles of 64 with a power-of-two scale s each
 // (largest magnitude / s in [2^14, 2^15)), zero rows behind the last token.
 // One CTA per (tile, KV head, K or V).
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) hot_half_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                        __half* __restrict__ kh, __half* __restrict__ vh,
                                                        float* __restrict__ scales, int rows, int ring_row0,
                                                        int capacity, int head, int hlen, int hot_rows) {
     const int tile = blockIdx.x, bh = blockIdx.y, is_v = blockIdx.z;
-    const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+    constexpr int kPerRow = D / 8, kRows = 256 / kPerRow, kIters = kTile / kRows;
+    const int c8 = threadIdx.x % kPerRow, r0 = threadIdx.x / kPerRow;
     const T* src = (is_v ? v : k) + (size_t)bh * rows * D + 8 * c8;
-    float x[4][8];
+    float x[kIters][8];
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t = tile * kTile + r0 + 16 * i;
+    for (int i = 0; i < kIters; ++i) {
+        const int t = tile * kTile + r0 + kRows * i;
         uint4 w = make_uint4(0, 0, 0, 0);
         if (t < hlen) w = *reinterpret_cast<const uint4*>(src + (size_t)(ring_row0 + (head + t) % capacity) * D);
         const T* e = reinterpret_cast<const T*>(&w);
@@ -735,11 +751,11 @@ __global__ void __launch_bounds__(256) hot_half_kernel(const T* __restrict__ k, 
     const float s = __uint_as_float((uint32_t)(e + 127) << 23), inv = 1.f / s;
     __half* dst = (is_v ? vh : kh) + ((size_t)bh * hot_rows + tile * kTile) * D + 8 * c8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kIters; ++i) {
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = pack2<__half>(x[i][2 * j] * inv, x[i][2 * j + 1] * inv);
-        *reinterpret_cast<uint4*>(dst + (size_t)(r0 + 16 * i) * D) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + (size_t)(r0 + kRows * i) * D) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     if (threadIdx.x == 0) scales[2 * ((size_t)bh * (hot_rows / kTile) + tile) + is_v] = s;
 }
@@ -766,35 +782,34 @@ int choose_split(int units, double tiles, int sms, int max_splits) {
     return best;
 }
 
-size_t hot_offset(int sms) { return align_up(ws_layout(1, 1, kMaxParts * sms, BM, D).total, 1024); }
+size_t hot_offset(int sms, int head_dim) {
+    return align_up(ws_layout(1, 1, kMaxParts * sms, BM, head_dim).total, 1024);
+}
 int hot_rows_for(int tokens) { return (tokens + BN - 1) / BN * BN; }
-size_t hot_bytes(int groups, int tokens) {
+size_t hot_bytes(int groups, int tokens, int head_dim) {
     const size_t rows = (size_t)groups * hot_rows_for(tokens);
-    return 2 * rows * D * 2 + rows / kTile * sizeof(float2);
+    return 2 * rows * head_dim * 2 + rows / kTile * sizeof(float2);
 }
 
-}  // namespace chunk
-}  // namespace archive
-
-size_t archive_chunk_ws(int groups, int hot_capacity) {
-    using namespace archive::chunk;
-    return hot_offset(std::max(device_sms(), 148)) + hot_bytes(groups, hot_capacity);
+template <typename T, int D>
+void launch_hot_half(const rfsn_arena* arena, const archive::Params& a, int groups, int hot_rows, __half* kh, __half* vh,
+                     float* scales, cudaStream_t s) {
+    hot_half_kernel<T, D><<<dim3(hot_rows / kTile, groups, 2), 256, 0, s>>>(
+        static_cast<const T*>(arena->k), static_cast<const T*>(arena->v), kh, vh, scales, a.rows, a.ring_row0, a.capacity,
+        a.head, a.hlen, hot_rows);
 }
 
-bool archive_chunk_fits(int G) { return G <= archive::chunk::BM; }
-
-rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& a,
+template <int D>
+rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& a,
                                  int batch, void* workspace, size_t workspace_bytes, int max_splits, cudaStream_t s) {
-    using namespace archive;
-    using namespace archive::chunk;
     const int groups = batch * a.kv_heads;
     const int sms = std::max(device_sms(), 148);
-    const size_t off = hot_offset(sms), need = off + hot_bytes(groups, a.hlen);
+    const size_t off = hot_offset(sms, D), need = off + hot_bytes(groups, a.hlen, D);
     if (workspace_bytes < need) {
         set_error("rfsn_archive_attention: workspace too small: need %zu bytes, have %zu", need, workspace_bytes);
         return RFSN_ERR_OVERFLOW;
     }
-    chunk::Params p;
+    Params p;
     memset(&p, 0, sizeof(p));
     p.q = a.q;
     p.out = a.out;
@@ -823,17 +838,17 @@ rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_arch
     if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
         // setmaxnreg moves registers between the warpgroups of what the block was launched with
         cudaFuncAttributes attr;
-        RFSN_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel));
+        RFSN_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel<D>));
         if (attr.numRegs * kThreads < 256 * (kSoftmaxRegs + kOtherRegs)) {
             set_error("rfsn_archive_attention: built with %d registers per thread, the chunk kernel needs %d",
                       attr.numRegs, 256 * (kSoftmaxRegs + kOtherRegs) / kThreads);
             return RFSN_ERR_UNSUPPORTED;
         }
-        RFSN_CUDA(cudaFuncSetAttribute(chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(chunk::Smem)));
+        RFSN_CUDA(cudaFuncSetAttribute(chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>)));
         // the small kernels around it with the same split of the SM's memory, or each change of split drains the SMs
-        for (const void* f : {reinterpret_cast<const void*>(hot_half_kernel<__half>),
-                              reinterpret_cast<const void*>(hot_half_kernel<__nv_bfloat16>),
-                              reinterpret_cast<const void*>(chunk_merge_kernel)})
+        for (const void* f : {reinterpret_cast<const void*>(hot_half_kernel<__half, D>),
+                              reinterpret_cast<const void*>(hot_half_kernel<__nv_bfloat16, D>),
+                              reinterpret_cast<const void*>(chunk_merge_kernel<D>)})
             RFSN_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout,
                                            cudaSharedmemCarveoutMaxShared));
         if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
@@ -846,15 +861,10 @@ rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_arch
         __half* vh = kh + rows * D;
         float* hs = reinterpret_cast<float*>(vh + rows * D);
         p.hot_scales = reinterpret_cast<const float2*>(hs);
-        const dim3 grid(p.hot_rows / kTile, groups, 2);
         if (arena->dtype == RFSN_BF16)
-            hot_half_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(
-                static_cast<const __nv_bfloat16*>(arena->k), static_cast<const __nv_bfloat16*>(arena->v), kh, vh, hs,
-                a.rows, a.ring_row0, a.capacity, a.head, a.hlen, p.hot_rows);
+            launch_hot_half<__nv_bfloat16, D>(arena, a, groups, p.hot_rows, kh, vh, hs, s);
         else
-            hot_half_kernel<__half><<<grid, 256, 0, s>>>(static_cast<const __half*>(arena->k),
-                                                         static_cast<const __half*>(arena->v), kh, vh, hs, a.rows,
-                                                         a.ring_row0, a.capacity, a.head, a.hlen, p.hot_rows);
+            launch_hot_half<__half, D>(arena, a, groups, p.hot_rows, kh, vh, hs, s);
         RFSN_CUDA(cudaGetLastError());
         note_launch();
         rfsn_status st = encode_rows_map(&mk, kh, RFSN_F16, groups, p.hot_rows, D, kTile);
@@ -864,22 +874,45 @@ rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_arch
         mk = arena->item_maps[0];  // not used
         mv = arena->item_maps[1];
     }
-    RFSN_CUDA(launch_pdl(chunk_kernel, dim3(p.units * p.nsplit), dim3(chunk::kThreads), sizeof(chunk::Smem), s,
+    RFSN_CUDA(launch_pdl(chunk_kernel<D>, dim3(p.units * p.nsplit), dim3(kThreads), sizeof(Smem<D>), s,
                          packed->maps[0], packed->maps[1], mk, mv, p));
     note_launch();
     if (p.nsplit > 1) {
-        RFSN_CUDA(launch_pdl(chunk_merge_kernel, dim3(p.units * (BM / 8)), dim3(256), 0, s, p));
+        RFSN_CUDA(launch_pdl(chunk_merge_kernel<D>, dim3(p.units * (BM / 8)), dim3(256), 0, s, p));
         note_launch();
     }
     return RFSN_OK;
 }
 
-void preload_chunk_kernels() {
+template <int D>
+void preload() {
     cudaFuncAttributes a;
-    cudaFuncGetAttributes(&a, archive::chunk::chunk_kernel);
-    cudaFuncGetAttributes(&a, archive::chunk::chunk_merge_kernel);
-    cudaFuncGetAttributes(&a, archive::chunk::hot_half_kernel<__half>);
-    cudaFuncGetAttributes(&a, archive::chunk::hot_half_kernel<__nv_bfloat16>);
+    cudaFuncGetAttributes(&a, chunk_kernel<D>);
+    cudaFuncGetAttributes(&a, chunk_merge_kernel<D>);
+    cudaFuncGetAttributes(&a, hot_half_kernel<__half, D>);
+    cudaFuncGetAttributes(&a, hot_half_kernel<__nv_bfloat16, D>);
+}
+
+}  // namespace chunk
+}  // namespace archive
+
+size_t archive_chunk_ws(int groups, int hot_capacity, int head_dim) {
+    using namespace archive::chunk;
+    return hot_offset(std::max(device_sms(), 148), head_dim) + hot_bytes(groups, hot_capacity, head_dim);
+}
+
+bool archive_chunk_fits(int G) { return G <= archive::chunk::BM; }
+
+rfsn_status archive_chunk_launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, const archive::Params& a,
+                                 int batch, void* workspace, size_t workspace_bytes, int max_splits, cudaStream_t s) {
+    using namespace archive::chunk;
+    return arena->head_dim == 128 ? launch<128>(arena, packed, a, batch, workspace, workspace_bytes, max_splits, s)
+                                  : launch<64>(arena, packed, a, batch, workspace, workspace_bytes, max_splits, s);
+}
+
+void preload_chunk_kernels() {
+    archive::chunk::preload<128>();
+    archive::chunk::preload<64>();
 }
 
 }  // namespace rfsn

@@ -865,6 +865,7 @@ def in_chunks(cache, q, first, **kw):
     return out
 
 
+@pytest.mark.parametrize("D", [128, 64])
 @pytest.mark.parametrize("dtype,B,H,Hkv,lens,hot,wrap,Lq", [
     ("bfloat16", 1, 8, 2, (64,) * 81, 100, 0, 128),            # an odd number of tiles
     ("float16", 2, 8, 2, (70,) * 30 + (64,) * 2, 33, 20, 100),  # ragged tiles, a wrapped ring
@@ -872,13 +873,13 @@ def in_chunks(cache, q, first, **kw):
     ("bfloat16", 1, 4, 4, (6000,), 300, 0, 300),
     ("float16", 1, 128, 1, (5000,), 10, 0, 9),                  # a row per CTA
 ])
-def test_chunks_of_queries(dtype, B, H, Hkv, lens, hot, wrap, Lq):
+def test_chunks_of_queries(dtype, B, H, Hkv, lens, hot, wrap, Lq, D):
     torch = _torch()
     import archive_ref as ref
 
-    cache, k, v = make(dtype, B, H, Hkv, 128, lens, hot, hot_cap=max(hot, 64), wrap=wrap)
+    cache, k, v = make(dtype, B, H, Hkv, D, lens, hot, hot_cap=max(hot, 64), wrap=wrap)
     n = sum(lens) + hot
-    q = queries(B, H, Lq, 128)
+    q = queries(B, H, Lq, D)
     kk, vv = held(cache, k, v, lens)
     for first in (n - Lq, n + 7, n // 2, 0, -5):
         want, lse = ref.attention(q, kk, vv, torch.arange(n), first)
@@ -887,15 +888,16 @@ def test_chunks_of_queries(dtype, B, H, Hkv, lens, hot, wrap, Lq):
     assert torch.equal(in_chunks(cache, q, n - Lq), in_chunks(cache, q, n - Lq))
 
 
-def test_chunks_and_what_lies_behind_them():
+@pytest.mark.parametrize("D", [128, 64])
+def test_chunks_and_what_lies_behind_them(D):
     """NaN K and V behind the last query of a chunk, in its own tile too, in the archive and in the ring. (Against the
     64-bit form: the scale of a ring tile, and with it the roundings of p, depends on its finite values.)"""
     torch = _torch()
     import archive_ref as ref
 
     lens = (64,) * 81
-    cache, k, v = make("bfloat16", 1, 8, 2, 128, lens, 100)
-    q = queries(1, 8, 128, 128)
+    cache, k, v = make("bfloat16", 1, 8, 2, D, lens, 100)
+    q = queries(1, 8, 128, D)
     kk, vv = held(cache, k, v, lens)
     spans = cache.get_attention_segments().spans
     for last in (5184 + 70, 5183, 5170, 5120, 3000):  # NaN stays from one to the next
@@ -911,10 +913,11 @@ def test_chunks_and_what_lies_behind_them():
         check_out(out, lse, want, want_lse, vv)
 
 
-def test_chunks_with_nan_that_is_seen():
+@pytest.mark.parametrize("D", [128, 64])
+def test_chunks_with_nan_that_is_seen(D):
     torch = _torch()
-    cache, k, v = make("bfloat16", 1, 8, 2, 128, (64,) * 81, 100)
-    q = queries(1, 8, 128, 128)
+    cache, k, v = make("bfloat16", 1, 8, 2, D, (64,) * 81, 100)
+    q = queries(1, 8, 128, D)
     row = cache.get_attention_segments().spans[7][0]
     kn, vn = k[:, :, 448:512].clone(), v[:, :, 448:512].clone()
     kn[0, 1, 3, 5] = math.inf  # packed as NaN: every row of KV head 1
@@ -922,19 +925,20 @@ def test_chunks_with_nan_that_is_seen():
     cache.archive.pack(kn, vn, row)
     out = in_chunks(cache, q, 5284 - 128)
     assert bool(torch.isnan(out[0, 4:]).all())
-    fine = torch.ones(128, dtype=torch.bool, device="cuda")
+    fine = torch.ones(D, dtype=torch.bool, device="cuda")
     fine[7] = False
     assert bool(torch.isfinite(out[0, :4][..., fine]).all()) and bool(torch.isnan(out[0, :4, :, 7]).all())
 
 
 @pytest.mark.parametrize("v_scale,q_scale", [(1e-6, 1.0), (1e-30, 0.0), (1e30, 60.0), (1.0, 1e-30)])
-def test_chunks_of_extreme_sizes(v_scale, q_scale):
+@pytest.mark.parametrize("D", [128, 64])
+def test_chunks_of_extreme_sizes(v_scale, q_scale, D):
     torch = _torch()
     import archive_ref as ref
 
     lens = (64,) * 81
-    cache, k, v = make("bfloat16", 1, 8, 2, 128, lens, 100, v_scale=v_scale)
-    q = queries(1, 8, 128, 128, scale=q_scale)
+    cache, k, v = make("bfloat16", 1, 8, 2, D, lens, 100, v_scale=v_scale)
+    q = queries(1, 8, 128, D, scale=q_scale)
     kk, vv = held(cache, k, v, lens)
     want, lse = ref.attention(q, kk, vv, torch.arange(5284), 5284 - 128)
     out, got = in_chunks(cache, q, 5284 - 128, want_lse=True)
