@@ -35,7 +35,7 @@
 // one vote instead of a reduction over the lanes and a rescale.
 //
 // Measured, 32 q / 8 KV heads, head_dim 128: 128K packed tokens and 4K ring
-// 50.3 us (5.5 TB/s; 43.2 at the copy rate), 6K and 2K fp16 9.6 us, where the
+// 48.7 us (5.7 TB/s; 43.2 at the copy rate), 6K and 2K fp16 9.2 us, where the
 // wait for the SMs, q, one round of tiles and the merge are 1 to 2 us each. 8
 // and 16 consumer warps per SM take the same time as 8 (two CTAs of four).
 #include <atomic>

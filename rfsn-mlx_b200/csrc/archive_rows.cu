@@ -27,8 +27,8 @@
 // terms of weight 1.
 //
 // Measured, 32 q / 8 KV heads: 4 rows (16 slots) over 31K packed tokens and 2K
-// ring 24.3 us (two passes of the tile kernel 33.8; 11.1 at the copy rate), 131K
-// 60.8 (107); 2 rows over 131K 53.5 (59). About 11 us of it (16 slots; 8.5 with
+// ring 23.3 us (two passes of the tile kernel 33.8; 11.1 at the copy rate), 131K
+// 59.5 (107); 2 rows over 131K 53.4 (59). About 11 us of it (16 slots; 8.5 with
 // 8) is there without keys: q, the first item, the merge. Above that an item of
 // 128 keys takes 0.85 us of a CTA (0.66 of HBM time): the softmax warps' issue
 // slots. Four groups of 8 slots in 640 threads took 29.8 us.
