@@ -240,7 +240,7 @@ def load_library() -> ctypes.CDLL:
         "rfsn_noalloc_check": (i32, [vp, i64]),
         "rfsn_packed_archive_create": (i32, [vp, vp, vp, i32, i32, i32, ctypes.POINTER(vp)]),
         "rfsn_packed_archive_destroy": (i32, [vp]),
-        "rfsn_pack_rows": (i32, [vp, i32, ctypes.POINTER(KvRowsC), i32, vp, vp]),
+        "rfsn_pack_rows": (i32, [vp, i32, vp, i32, vp, vp]),  # KvRowsC by reference, or its bytes
         "rfsn_unpack_rows": (i32, [vp, i32, i32, vp, vp, i32, i64, vp]),
         "rfsn_tile_bounds": (i32, [vp, i32, i32, vp, vp]),
         "rfsn_select_tiles": (i32, [vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, ctypes.POINTER(TileListC), i32,

@@ -21,6 +21,7 @@ Everything runs on ``librfsn_b200.so``; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 from functools import lru_cache
 from typing import Optional
 
@@ -48,12 +49,15 @@ def check_archive_options(dtype: torch.dtype, head_dim: int, archive_dtype: Opti
                          f"128, got {dtype} and {head_dim}")
 
 
-def kv_rows(k: torch.Tensor, v: torch.Tensor, offset: int = 0, wrap: int = 0) -> native.KvRowsC:
-    """Description of K/V [B, Hkv, n, D] for ``rfsn_pack_rows`` (innermost stride 1)."""
+_KV_ROWS = struct.Struct("@PPqqqqqqiiii")  # rfsn_kv_rows; packed bytes cost half of a ctypes structure
+
+
+def kv_rows(k: torch.Tensor, v: torch.Tensor, offset: int = 0, wrap: int = 0) -> bytes:
+    """``rfsn_kv_rows`` of K/V [B, Hkv, n, D] (innermost stride 1)."""
     kb, kh, kt, _ = k.stride()
     vb, vh, vt, _ = v.stride()
-    return native.KvRowsC(k.data_ptr(), v.data_ptr(), kb, kh, kt, vb, vh, vt, native.dtype_code(k.dtype), k.shape[1],
-                          offset, wrap)
+    return _KV_ROWS.pack(k.data_ptr(), v.data_ptr(), kb, kh, kt, vb, vh, vt, native.dtype_code(k.dtype), k.shape[1],
+                         offset, wrap)
 
 
 class PackedArchive:
@@ -142,9 +146,9 @@ class PackedArchive:
                 or not bounds.is_contiguous():
             raise ValueError(f"bounds must be a contiguous uint8 tensor of shape {shape} on {self.device}")
 
-    def _pack(self, rows: native.KvRowsC, row: int, count: int, bounds: Optional[torch.Tensor]) -> None:
+    def _pack(self, rows: bytes, row: int, count: int, bounds: Optional[torch.Tensor]) -> None:
         with native.on_device(self.device):
-            status = native.lib().rfsn_pack_rows(self.handle, row, ctypes.byref(rows), count,
+            status = native.lib().rfsn_pack_rows(self.handle, row, rows, count,
                                                  bounds.data_ptr() if bounds is not None else None,
                                                  native.stream_ptr())
         if status:

@@ -12,7 +12,7 @@ import archive_ref as ref
 from fake_ops import FakeDeviceOps
 from rfsn_b200 import LayerKVCache, RFSNCache, RFSNConfig
 from rfsn_b200 import _native as native
-from rfsn_b200.archive import padded_rows, workspace_bytes
+from rfsn_b200.archive import kv_rows, padded_rows, workspace_bytes
 
 BAD, UNSUPPORTED, OVERFLOW = native.RFSN_ERR_INVALID_ARG, native.RFSN_ERR_UNSUPPORTED, native.RFSN_ERR_OVERFLOW
 FAKE = 0x10000  # a non-NULL, 16-byte aligned address that is never dereferenced
@@ -298,6 +298,10 @@ def expect(status, code, fragment):
 
 def test_struct_layouts_match_header():
     assert ctypes.sizeof(native.KvRowsC) == 80
+    k, v = torch.zeros(2, 3, 5, 64).transpose(1, 2), torch.ones(2, 5, 3, 64)
+    rows = native.KvRowsC.from_buffer_copy(kv_rows(k, v, 4, 9))
+    assert [getattr(rows, f) for f, _ in rows._fields_] == [k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+                                                            native.dtype_code(torch.float32), 5, 4, 9]
     assert ctypes.sizeof(native.TileListC) == 16
     assert ctypes.sizeof(native.ArchiveCallC) == 96
 
