@@ -474,8 +474,9 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
                 sm.qmul[s] = p.qscale * __uint_as_float((uint32_t)(127 - e) << 23);
                 sm.row[s] = live ? (slot0 + s) / p.G : INT_MIN;
             }
+            // an infinity makes every logit of the row infinite or NaN; e4m3 has none
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= up;
+            for (int i = 0; i < 8; ++i) x[i] = a == CUDART_INF_F ? CUDART_NAN_F : x[i] * up;
             if (na > 0) {
                 float y[8];
 #pragma unroll

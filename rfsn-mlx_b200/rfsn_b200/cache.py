@@ -1154,7 +1154,8 @@ class LayerKVCache:
         """Exact attention of float32 q [B, H, Lq, D] against this layer's
         archived blocks and hot window (the work of layer.py:139-162). With
         ``top_tiles`` only the best tiles of each query and KV head are read
-        (``paged_attention``)."""
+        (``paged_attention``; calls that may run at once, on several streams or
+        in several graphs, give it a workspace each)."""
         if segments is None:
             segments = self.get_attention_segments()
         if (top_tiles or self.archive is not None) and segments.spans:  # without the detour: short calls are host-bound

@@ -996,3 +996,32 @@ def test_a_device_without_an_index(packed):
             outs.append(paged_attention(c, q, 319, segs, out=given, top_tiles=top))
         assert all(torch.equal(o, outs[0]) for o in outs)
     assert torch.equal(caches[0].select_tiles(q, 319, 2), caches[1].select_tiles(q, 319, 2))
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("Lq", [1, 2, 4, 40, 128])
+@pytest.mark.parametrize("lens,scale", [((64,) * 81, 1.0), ((64,), 0.01)])
+def test_infinities_and_nan_in_queries_stay_in_their_rows(Lq, packed, D, lens, scale):
+    """A query row with an infinity or a NaN becomes NaN, the others do not change beyond rounding."""
+    torch = _torch()
+    import archive_ref as ref
+
+    if not packed and Lq > 64:
+        pytest.skip("a selecting call takes up to 64 rows")
+    cache, k, v = make("bfloat16", 1, 8, 2, D, lens, 100, tile_index=True, scale=scale,
+                       archive_dtype="float8_e4m3fn" if packed else None)
+    q = queries(1, 8, Lq, D)
+    kk, vv = held(cache, k, v, lens)
+    n = sum(lens) + 100
+    first = n - Lq
+    want, lse = ref.attention(q, kk, vv, torch.arange(n), first)
+    bad = torch.zeros(8, Lq, dtype=torch.bool)
+    for h, r, x in ((3, 0, math.inf), (6, Lq - 1, math.nan), (4, Lq // 2, -math.inf)):
+        q[0, h, r, 5] = x
+        bad[h, r] = True
+    for top in ([0] if packed else []) + ([200] if Lq <= 64 else []):
+        out, got = cache.attend(q, first, top_tiles=top, want_lse=True)
+        out, got = out.cpu(), got.cpu()
+        assert bool(torch.isnan(out[0][bad]).all()) and bool(torch.isnan(got[0][bad]).all())
+        check_out(out[0][~bad], got[0][~bad], want[0][~bad], lse[0][~bad], vv)
