@@ -199,22 +199,24 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(RowSource ks, RowSou
         }
         const size_t slot = (size_t)bh * (rows / kTile) + row0 / kTile;
         if (threadIdx.x == 0) scales[4 * slot + is_v] = s;
-        if (!BOUNDS || !bound) continue;
-        // channel-wise smallest and largest code of the tile's keys
+        if constexpr (BOUNDS) {
+            if (!bound) continue;
+            // channel-wise smallest and largest code of the tile's keys
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            red[0][r0][4 * c8 + j] = lo[j];
-            red[1][r0][4 * c8 + j] = hi[j];
-        }
-        __syncthreads();
-        if (threadIdx.x < D) {  // 2 bounds x D / 2 channel pairs
-            const int w = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
-            __half2 m = red[w][0][j];
+            for (int j = 0; j < 4; ++j) {
+                red[0][r0][4 * c8 + j] = lo[j];
+                red[1][r0][4 * c8 + j] = hi[j];
+            }
+            __syncthreads();
+            if (threadIdx.x < D) {  // 2 bounds x D / 2 channel pairs
+                const int w = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
+                __half2 m = red[w][0][j];
 #pragma unroll 4
-            for (int r = 1; r < (BOUNDS ? RPP : 1); ++r)
-                m = w ? __hmax2_nan(m, red[w][r][j]) : __hmin2_nan(m, red[w][r][j]);
-            const float2 f = __half22float2(m);
-            reinterpret_cast<uint16_t*>(bounds)[(slot * 2 + w) * (D / 2) + j] = (uint16_t)e4m3x2(f.x, f.y);
+                for (int r = 1; r < RPP; ++r)
+                    m = w ? __hmax2_nan(m, red[w][r][j]) : __hmin2_nan(m, red[w][r][j]);
+                const float2 f = __half22float2(m);
+                reinterpret_cast<uint16_t*>(bounds)[(slot * 2 + w) * (D / 2) + j] = (uint16_t)e4m3x2(f.x, f.y);
+            }
         }
     }
 }
