@@ -93,9 +93,11 @@ struct SelShared {
     float part[kSelWarps * 4 * kTilesPerLane];       // scores by head group
 };
 
-// The n-th largest key by narrowing a key range: a histogram of 1,024 equal
-// buckets, the bucket in which the count from the top passes n becomes the
-// range. Two passes as a rule (the first bucket holds a few keys, the second
+// The n-th largest key by narrowing a key range [lo, lo + span]: a histogram of
+// up to 1,024 equal buckets of 2^shift keys, the bucket in which the count from
+// the top passes n becomes the range, and the keys above it, which are taken,
+// are not counted again (a range of fewer than 1,024 keys has fewer buckets).
+// Two passes as a rule (the first bucket holds a few scores, the second
 // separates them), four at most; integer counts, so any order gives the same.
 template <bool REGS>
 __device__ __forceinline__ void select_list(const SelectParams& p, const float* scores, int list, SelShared& sh) {
@@ -148,11 +150,11 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
     uint32_t thr = 1u;  // every visible tile
     if (n < visible) {
         int need = n;
-        int shift = max(0, 32 - __clz(hi - lo) - 10);  // hi - lo + 1 keys in at most 1,024 buckets
+        uint32_t span = hi - lo;
+        int shift = max(0, 32 - __clz(span) - 10);  // span + 1 keys in at most 1,024 buckets
         for (;;) {
             each([&](uint32_t k) {
-                const uint32_t d = (k - lo) >> shift;
-                if (k >= lo && d < kBuckets) atomicAdd(&sh.hist[d], 1);
+                if (k - lo <= span) atomicAdd(&sh.hist[(k - lo) >> shift], 1);  // keys below lo wrap around
             });
             __syncthreads();
             // counts from the top: thread i has buckets 1023 - 2 i and 1022 - 2 i
@@ -180,12 +182,15 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
             lo += (uint32_t)sh.bucket << shift;
             need -= sh.above;
             if (sh.inside == need || shift == 0) break;
+            span = min((1u << shift) - 1u, hi - lo);  // the last bucket may reach beyond the largest key
             shift = max(0, shift - 10);
         }
         thr = lo;
     }
     // Write in tile order: keys above the threshold all, keys equal to it from
-    // the lowest tile on (all of them, unless the bucket was one key).
+    // the lowest tile on (all of them, unless the bucket was one key). Entries
+    // behind the ones written, by their own count, are filled.
+    int written;
     const unsigned below = (1u << lane) - 1u;
     const size_t base = (size_t)list * p.n_select;
     auto put = [&](int i, int t) {
@@ -217,7 +222,9 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
             const int v = __shfl_up_sync(0xffffffffu, incl, off);
             if (lane >= off) incl += v;
         }
-        const int need = n - (__shfl_sync(0xffffffffu, incl, 31) & 0xffff);  // taken among those at the threshold
+        const int all = __shfl_sync(0xffffffffu, incl, 31);
+        const int need = n - (all & 0xffff);  // taken among those at the threshold
+        written = (all & 0xffff) + min(all >> 16, need);
         const int w3 = warp & 3;
         const int part = (w3 > 0 ? four.x : 0) + (w3 > 1 ? four.y : 0) + (w3 > 2 ? four.z : 0);
         const int mine = incl - own + part;  // tallies before (i, warp), in the lane that holds that entry
@@ -248,7 +255,7 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
             sh.tally[kSelWarps + warp] = eq;
         }
         __syncthreads();
-        int gt_before = 0, eq_before = 0, gt_all = 0;
+        int gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
 #pragma unroll
         for (int w = 0; w < kSelWarps; ++w) {
             if (w < warp) {
@@ -256,8 +263,10 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
                 eq_before += sh.tally[kSelWarps + w];
             }
             gt_all += sh.tally[w];
+            eq_all += sh.tally[kSelWarps + w];
         }
         const int need = n - gt_all;
+        written = gt_all + min(eq_all, need);
         for (int t0 = r0; t0 < r1; t0 += 32) {
             const int t = t0 + lane;
             const uint32_t k = t < r1 ? score_key(__ldcg(scores + t)) : 0u;
@@ -269,7 +278,7 @@ __device__ __forceinline__ void select_list(const SelectParams& p, const float* 
             eq_before += __popc(me);
         }
     }
-    for (int i = n + tid; i < p.n_select; i += kSelThreads) put(i, -1);
+    for (int i = written + tid; i < p.n_select; i += kSelThreads) put(i, -1);
 }
 
 // A bound as a double has an empty low word (8 or 11 significant bits), so the
