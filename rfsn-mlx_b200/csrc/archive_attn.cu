@@ -367,7 +367,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
             if (i < arch_end) {
                 d = __ldcg(tiles + i / kPer);
                 const int rows = PACKED ? p.packed_rows : p.rows;
-                if (d.x < 0 || d.z < 0 || d.z > kTile || d.x + d.z > rows || (PACKED && (d.x & (kTile - 1)) != 0)) {
+                if (d.x < 0 || d.z < 0 || d.z > kTile || d.x > rows - d.z || (PACKED && (d.x & (kTile - 1)) != 0)) {
                     atomicExch(p.ws.error, kDevErrBadTable);  // a tile outside the arena: skipped
                     d = make_int4(0, 0, 0, 0);
                 }

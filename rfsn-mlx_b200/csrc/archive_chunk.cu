@@ -344,7 +344,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                         if (i < sm.n_arch) {
                             const int4 e = __ldcg(p.tiles + i);
                             if (e.x < 0 || e.z < 0 || e.z > kTile || (e.x & (kTile - 1)) != 0 ||
-                                e.x + e.z > p.packed_rows) {
+                                e.x > p.packed_rows - e.z) {
                                 atomicExch(p.ws.error, kDevErrBadTable);  // outside the archive: skipped
                             } else {
                                 row = e.x;

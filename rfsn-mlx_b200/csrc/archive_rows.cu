@@ -282,7 +282,7 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
             float sk = 1.f, sv = kTiny;  // a half without keys leaves the unit to the other one
             if (base + (lane >> 1) < na && i < p.n_tiles) {
                 e = __ldcg(p.tiles + i);
-                if (e.x < 0 || e.z < 0 || e.z > kTile || (e.x & (kTile - 1)) != 0 || e.x + e.z > p.packed_rows) {
+                if (e.x < 0 || e.z < 0 || e.z > kTile || (e.x & (kTile - 1)) != 0 || e.x > p.packed_rows - e.z) {
                     atomicExch(p.ws.error, kDevErrBadTable);  // a tile outside the archive: skipped
                     e = make_int4(0, 0, 0, 0);
                 } else if (e.z > 0) {
