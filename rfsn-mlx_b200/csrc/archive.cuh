@@ -18,6 +18,7 @@ struct rfsn_packed_archive {
     int head_dim;
     int device;
     CUtensorMap maps[4];  // K and V: boxes of one 64-token tile, boxes of 16 rows
+    rfsn::FreshWrites fresh;  // codes, scales and key bounds
 };
 
 namespace rfsn {
@@ -46,6 +47,7 @@ struct Params {
     float qscale;           // 1/sqrt(D) * log2(e)
     WsView ws;
     const int* dyn;         // device step state (RFSN_STEP_*) or nullptr
+    bool overlap;           // launched with programmatic overlap (FreshWrites)
 };
 
 struct SelectParams {
@@ -63,6 +65,7 @@ struct SelectParams {
     int* counters;
     int* error;
     const int* dyn;
+    bool overlap;           // as in Params
 };
 
 // Paired float32 arithmetic (PTX .f32x2): two results per issue slot, each rounded as the scalar operation.

@@ -223,6 +223,8 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     p.qscale = (float)(1.0 / std::sqrt((double)arena->head_dim)) * 1.4426950408889634f;
     p.ws = ws_view(workspace, w);
     p.dyn = hot->step_state;
+    // the chunk kernel reads no archived row ahead of the kernel before it, the others do
+    p.overlap = chunk || (packed != nullptr ? packed->fresh : arena->fresh).overlap(static_cast<cudaStream_t>(stream));
     if (chunk)
         return archive_chunk_launch(arena, packed, p, batch, workspace, workspace_bytes, max_splits,
                                     static_cast<cudaStream_t>(stream));
@@ -231,11 +233,12 @@ rfsn_status attention(const rfsn_arena* arena, const rfsn_packed_archive* packed
     return archive_attn_launch(arena, packed, p, sp.lists, sp.per_cta / 4, sp.zblocks, static_cast<cudaStream_t>(stream));
 }
 
-// numbers: out receives the tiles' numbers ([lists][n_select]) instead of their entries
+// numbers: out receives the tiles' numbers ([lists][n_select]) instead of their entries; fresh: of the owner of the
+// bounds and scales, unless it is not known (then nothing is read ahead of the kernel before)
 rfsn_status select(const char* what, const void* bounds, int bounds_dtype, const float* scales, int rows, const float* q,
                    int batch, int q_heads, int kv_heads, int q_len, int head_dim, int q_pos0,
                    const rfsn_tile_list* tiles, int n_select, int32_t* out, bool numbers, const int32_t* step_state,
-                   void* workspace, size_t workspace_bytes, void* stream) {
+                   void* workspace, size_t workspace_bytes, void* stream, const FreshWrites* fresh) {
     rfsn_status st = check_shape(batch, q_heads, kv_heads, q_len, head_dim, true, what);
     if (st == RFSN_OK) st = check_tiles(tiles, what);
     if (st != RFSN_OK) return st;
@@ -277,6 +280,7 @@ rfsn_status select(const char* what, const void* bounds, int bounds_dtype, const
     p.counters = reinterpret_cast<int*>(ws + 256);
     p.error = reinterpret_cast<int*>(ws);
     p.dyn = step_state;
+    p.overlap = fresh != nullptr && fresh->overlap(static_cast<cudaStream_t>(stream));
     // one CTA per SM over all lists, in steps of the tiles that a CTA scores at once (128 over the head groups)
     p.head_groups = p.G <= 4 ? 1 : (p.G <= 8 ? 2 : (p.G <= 16 ? 4 : 8));
     const int want = std::max(1, device_sms() / lists), step = 128 / p.head_groups;
@@ -292,7 +296,7 @@ rfsn_status select_call(const char* what, const rfsn_archive_call* c, const floa
                   pk != nullptr ? reinterpret_cast<const float*>(pk->scales) : nullptr,
                   pk != nullptr ? pk->rows : c->arena->rows, q, c->batch, c->q_heads, c->kv_heads, c->q_len,
                   c->arena->head_dim, q_pos0, &c->tiles, c->top_tiles, out, numbers, c->hot.step_state, workspace,
-                  workspace_bytes, stream);
+                  workspace_bytes, stream, pk != nullptr ? &pk->fresh : &c->arena->fresh);
 }
 
 }  // namespace
@@ -364,6 +368,7 @@ rfsn_status rfsn_pack_rows(const rfsn_packed_archive* a, int dst_row0, const rfs
     RFSN_CHECK_ARG(src->k != nullptr && src->v != nullptr, "rfsn_pack_rows: NULL K or V");
     rfsn_status st = check_device(a->device, "rfsn_pack_rows");
     if (st != RFSN_OK) return st;
+    a->fresh.note(static_cast<cudaStream_t>(stream));
     return pack_rows_launch(a, dst_row0, src, count, bounds, static_cast<cudaStream_t>(stream));
 }
 
@@ -400,6 +405,7 @@ rfsn_status rfsn_tile_bounds(const rfsn_arena* arena, int row0, int count, void*
     if (count == 0) return RFSN_OK;
     rfsn_status st = check_device(arena->device, "rfsn_tile_bounds");
     if (st != RFSN_OK) return st;
+    arena->fresh.note(static_cast<cudaStream_t>(stream));
     return tile_bounds_launch(arena, row0, count, bounds, static_cast<cudaStream_t>(stream));
 }
 
@@ -431,7 +437,7 @@ rfsn_status rfsn_select_tiles(const void* bounds, int bounds_dtype, const float*
                               const rfsn_tile_list* tiles, int n_select, int32_t* out, const int32_t* step_state,
                               void* workspace, size_t workspace_bytes, void* stream) {
     return select("rfsn_select_tiles", bounds, bounds_dtype, scales, rows, q, batch, q_heads, kv_heads, q_len, head_dim,
-                  q_pos0, tiles, n_select, out, false, step_state, workspace, workspace_bytes, stream);
+                  q_pos0, tiles, n_select, out, false, step_state, workspace, workspace_bytes, stream, nullptr);
 }
 
 rfsn_status rfsn_archive_attention(const rfsn_arena* arena, const rfsn_packed_archive* packed, const float* q,

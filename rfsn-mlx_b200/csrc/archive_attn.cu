@@ -769,7 +769,7 @@ rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, c
     const CUtensorMap& v8 = PACKED ? packed->maps[1] : arena->item_maps[1];
     const CUtensorMap& ks = PACKED ? packed->maps[2] : arena->item_maps[0];
     const CUtensorMap& vs = PACKED ? packed->maps[3] : arena->item_maps[1];
-    RFSN_CUDA(launch_pdl(kern, dim3(lists, p.splits, zblocks), dim3((4 * Sh::kGroups + 1) * 32), smem, s,
+    RFSN_CUDA(launch_kernel(p.overlap, kern, dim3(lists, p.splits, zblocks), dim3((4 * Sh::kGroups + 1) * 32), smem, s,
                          arena->item_maps[0], arena->item_maps[1], k8, v8, ks, vs, p));
     note_launch();
     return RFSN_OK;

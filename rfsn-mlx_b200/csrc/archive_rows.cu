@@ -747,9 +747,9 @@ rfsn_status launch(const rfsn_arena* arena, const rfsn_packed_archive* packed, c
         RFSN_CUDA(cudaFuncSetAttribute(rows_kernel<T, SL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Sm)));
         if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
-    RFSN_CUDA(launch_pdl(rows_kernel<T, SL>, dim3(lists, p.splits, zblocks), dim3(kThreads), sizeof(Sm), s,
-                         packed->maps[0], packed->maps[1], packed->maps[2], packed->maps[3], arena->maps[0],
-                         arena->maps[1], p));
+    RFSN_CUDA(launch_kernel(p.overlap, rows_kernel<T, SL>, dim3(lists, p.splits, zblocks), dim3(kThreads), sizeof(Sm), s,
+                            packed->maps[0], packed->maps[1], packed->maps[2], packed->maps[3], arena->maps[0],
+                            arena->maps[1], p));
     note_launch();
     return RFSN_OK;
 }

@@ -487,6 +487,7 @@ rfsn_status rfsn_arena_copy_rows(const rfsn_arena* arena, int src_row0, int src_
     const int row_bytes = arena->head_dim * dtype_size(arena->dtype);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (row_bytes % 16 == 0) {
+        arena->fresh.note(s);
         return copy_rows_launch(arena->k, arena->v, arena->groups, arena->rows, row_bytes, src_row0, src_offset,
                                 src_wrap, dst_row0, count, s);
     }

@@ -137,9 +137,11 @@ __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("grid
 // Launch with programmatic stream serialization: the kernel may start while
 // the previous kernel on the stream runs (once that one triggers its
 // dependents) and must call griddep_wait() before reading what it produced.
+// Without overlap it starts when everything before it in the stream has
+// completed and is visible, and griddep_wait() returns at once.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                              Args... args) {
+inline cudaError_t launch_kernel(bool overlap, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                 cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -149,8 +151,13 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = overlap ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                              Args... args) {
+    return launch_kernel(true, kern, grid, block, smem, stream, args...);
 }
 
 __device__ __forceinline__ void named_barrier_sync(int id, int threads) {

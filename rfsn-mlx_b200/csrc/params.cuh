@@ -2,7 +2,33 @@
 // translation units and the C ABI layer (capi.cu).
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
+
+namespace rfsn {
+// The stream on which a kernel of this library last wrote rows, scales or key
+// bounds that a later kernel reads ahead of its griddep_wait(). Only that wait
+// makes the writes of the kernel before visible under an overlapped launch, so
+// the next such call on that stream is launched without the overlap.
+class FreshWrites {
+  public:
+    void note(cudaStream_t s) const {
+        uintptr_t seen = kNone;
+        if (!stream_.compare_exchange_strong(seen, id(s)) && seen != id(s)) stream_.store(kSeveral);
+    }
+    // May the next call on s overlap with what precedes it? Forgets the writes on s (those on several streams stay).
+    bool overlap(cudaStream_t s) const {
+        uintptr_t seen = id(s);
+        return !stream_.compare_exchange_strong(seen, kNone) && seen != kSeveral;
+    }
+
+  private:
+    static constexpr uintptr_t kNone = 0, kSeveral = ~uintptr_t(0);
+    static uintptr_t id(cudaStream_t s) { return reinterpret_cast<uintptr_t>(s == nullptr ? cudaStreamLegacy : s); }
+    mutable std::atomic<uintptr_t> stream_{kNone};
+};
+}  // namespace rfsn
 
 // One layer's K/V arena and its TMA descriptors (opaque to C ABI users).
 struct rfsn_arena {
@@ -17,6 +43,7 @@ struct rfsn_arena {
     CUtensorMap maps[4];  // K 64-row box, V 64-row box, K 8-row box, V 8-row box
     bool has_items;             // 16-bit K/V, head_dim 64 or 128: maps of archive_attn.cu's items
     CUtensorMap item_maps[2];   // K and V, boxes of 32 rows (head_dim 64: 64 rows)
+    rfsn::FreshWrites fresh;    // archived rows and their key bounds
 };
 
 namespace rfsn {

@@ -32,9 +32,9 @@ constexpr int kHeadsPerPass = 4;  // of a warp
 // than four q heads per KV head the warps are shared out over up to eight
 // groups of four heads, and a CTA takes as many tiles less at a time (32 heads
 // of 1 KV head, 78 tiles: 31.3 us with the groups one after the other in one
-// CTA, 8.5 us side by side in five). The first pass's bounds are requested
-// before the wait for q: they never come from the kernel that this launch
-// overlaps (packing and bounding are launched without that overlap).
+// CTA, 8.5 us side by side in five). The first pass's tiles and bounds are
+// requested before the wait for q: a call whose bounds or scales may have been
+// written by the kernel before it is launched without the overlap.
 constexpr int kTilesPerLane = 2;
 constexpr int kPassTiles = kSelWarps * 4 * kTilesPerLane;
 constexpr int kMaxHeadGroups = 8;
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
 
 template <typename T, int D>
 rfsn_status launch(const SelectParams& p, int lists, int chunks, cudaStream_t s) {
-    RFSN_CUDA(launch_pdl(select_kernel<T, D>, dim3(chunks, lists), dim3(kSelThreads), 0, s, p));
+    RFSN_CUDA(launch_kernel(p.overlap, select_kernel<T, D>, dim3(chunks, lists), dim3(kSelThreads), 0, s, p));
     note_launch();
     return RFSN_OK;
 }

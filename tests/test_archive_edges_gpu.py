@@ -39,3 +39,97 @@ def test_a_row_near_the_end_of_32_bits_is_reported_and_skipped(packed, Lq, top, 
     kk, vv = held(cache, k, v, lens)
     want, want_lse = ref.attention(q, kk, vv, torch.arange(n), n - Lq, seen)
     check_out(out, lse, want, want_lse, vv)
+
+
+# ------------------------------------------------------------------ launch order
+def edge_types(fn, stream=None):
+    """Captures ``fn``, a chain of kernels, and gives the type of its dependencies in order (0: the later kernel
+    starts after the earlier one, 1: they overlap), from the driver's description of the graph."""
+    import ctypes
+
+    torch = _torch()
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g, stream=stream):
+        fn()
+    handle, n = ctypes.c_void_p(g.raw_cuda_graph()), ctypes.c_size_t(0)
+    edges = ctypes.CDLL("libcuda.so.1").cuGraphGetEdges_v2
+    assert edges(handle, None, None, None, ctypes.byref(n)) == 0
+    src, dst = (ctypes.c_void_p * n.value)(), (ctypes.c_void_p * n.value)()
+    data = (ctypes.c_uint8 * 8 * n.value)()  # {from port, to port, type, reserved[5]}
+    assert edges(handle, src, dst, data, ctypes.byref(n)) == 0
+    follow = {src[i]: (dst[i], data[i][2]) for i in range(n.value)}
+    assert len(follow) == n.value  # a chain
+    at, types = (set(src) - set(dst)).pop(), []
+    while at in follow:
+        at, kind = follow[at]
+        types.append(kind)
+    return types
+
+
+@pytest.mark.parametrize("Lq", [1, 4])
+@pytest.mark.parametrize("packed", [True, False])
+def test_what_reads_ahead_does_not_overlap_with_what_wrote(packed, Lq):
+    """Attention and selection read codes, scales and bounds before they wait for the kernel in front of them: the
+    first call behind a kernel that wrote them starts after it, later ones overlap again."""
+    torch = _torch()
+    from rfsn_b200 import _native as native
+    from rfsn_b200.cache import paged_attention
+
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (64,) * 20, 10, tile_index=True,
+                       archive_dtype="float8_e4m3fn" if packed else None)
+    q = queries(1, 8, Lq, 128)
+    segs = cache.get_attention_segments()
+    ws = native.Workspace(cache.device)
+
+    def attend(top):
+        paged_attention(cache, q, 1290 - Lq, segs, workspace=ws, top_tiles=top)
+
+    def write():
+        if packed:
+            cache.archive.pack(k[:, :, :64], v[:, :, :64], 0, bounds=cache.tile_bounds)
+        else:
+            cache._ops.tile_bounds(segs.spans[0][0], 64, cache.tile_bounds)
+
+    tops = [3] + [0] * packed
+    for top in tops:
+        attend(top)  # the workspace is as large as it gets
+    cache.select_tiles(q, 1290 - Lq, 3, segs, workspace=ws)
+    select = lambda: cache.select_tiles(q, 1290 - Lq, 3, segs, workspace=ws)  # noqa: E731
+    assert edge_types(lambda: (attend(3), attend(3))) == [1, 1, 1]  # selection and attention, twice
+    assert edge_types(lambda: (write(), attend(3), attend(3))) == [0, 1, 1, 1]
+    assert edge_types(lambda: (write(), select(), select())) == [0, 1]
+    if packed:
+        assert edge_types(lambda: (attend(0), attend(0))) == [1]
+        assert edge_types(lambda: (write(), write(), attend(0), attend(0))) == [0, 0, 1]
+        assert edge_types(lambda: (write(), attend(0), write(), attend(0), attend(3))) == [0, 0, 0, 1, 1]
+
+
+def test_a_write_on_another_stream_is_not_forgotten():
+    """A call on one stream does not forget what was written on another; writes on several streams stay."""
+    torch = _torch()
+    from rfsn_b200 import _native as native
+    from rfsn_b200.cache import paged_attention
+
+    cache, k, v = make("bfloat16", 1, 8, 2, 128, (64,) * 20, 10)
+    q = queries(1, 8, 1, 128)
+    segs = cache.get_attention_segments()
+    ws = native.Workspace(cache.device)
+    attend = lambda: paged_attention(cache, q, 1289, segs, workspace=ws)  # noqa: E731
+    write = lambda: cache.archive.pack(k[:, :, :64], v[:, :, :64], 0)  # noqa: E731
+    attend()
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (one, two):
+        with torch.cuda.stream(s):
+            attend()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(one):
+        write()
+    torch.cuda.synchronize()
+    assert edge_types(lambda: (attend(), attend()), two) == [1]
+    assert edge_types(lambda: (write(), attend(), attend()), one) == [0, 1]
+    for s in (one, two):
+        with torch.cuda.stream(s):
+            write()
+        torch.cuda.synchronize()
+    assert edge_types(lambda: (attend(), attend()), one) == [0]
