@@ -416,17 +416,17 @@ rfsn_status rfsn_archive_workspace_size(int batch, int q_heads, int kv_heads, in
     if (st != RFSN_OK) return st;
     RFSN_CHECK_ARG(n_tiles >= 0 && n_select >= 0 && hot_capacity >= 0,
                    "rfsn_archive_workspace_size: negative count");
-    // every plan that a call over up to that many tiles may take
-    auto plan = [&](int per_cta, bool rows) {
-        return make_plan(batch, q_heads, kv_heads, q_len, n_select > 0, per_cta, rows);
-    };
-    const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, false, n_select > 0, 0);
-    size_t need = attention_ws_limit(sp, head_dim);
-    if (sp.slots > 4 && n_select == 0 && head_dim == 128)
+    // every plan that a call over up to that many tiles may take; a selecting call over none attends to a shared list
+    const SlotPlan shared = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, false, false, 0);
+    size_t need = attention_ws_limit(shared, head_dim);
+    if (shared.slots > 4 && head_dim == 128)
         for (int per_cta = 8; per_cta <= 16; per_cta += 8)
-            need = std::max(need, attention_ws_limit(plan(per_cta, true), head_dim));
-    if (n_select > 0) need = lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select;
-    else if (chunk_shape(head_dim, batch * kv_heads, q_heads / kv_heads, q_len, n_tiles))
+            need = std::max(need, attention_ws_limit(make_plan(batch, q_heads, kv_heads, q_len, false, per_cta, true),
+                                                     head_dim));
+    if (n_select > 0) {
+        const SlotPlan sp = slot_plan(batch, q_heads, kv_heads, q_len, head_dim, false, true, 0);
+        need = std::max(need, lists_offset(sp, head_dim, n_tiles) + sizeof(int4) * (size_t)sp.lists * n_select);
+    } else if (chunk_shape(head_dim, batch * kv_heads, q_heads / kv_heads, q_len, n_tiles))
         need = std::max(need, archive_chunk_ws(batch * kv_heads, hot_capacity, head_dim));
     *bytes = need;
     return RFSN_OK;

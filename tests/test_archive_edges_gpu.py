@@ -133,3 +133,32 @@ def test_a_write_on_another_stream_is_not_forgotten():
             write()
         torch.cuda.synchronize()
     assert edge_types(lambda: (attend(), attend()), one) == [0]
+
+
+# ------------------------------------------------------------------ workspaces
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("H,Hkv,Lq", [(32, 8, 4), (8, 2, 1), (16, 1, 2)])
+def test_a_selecting_call_over_no_tiles_fits_its_workspace(H, Hkv, Lq, packed):
+    """The C call with top_tiles > 0 and an empty list over a long window, in a workspace of the size asked for."""
+    import ctypes
+
+    torch = _torch()
+    import archive_ref as ref
+    from rfsn_b200 import _native as native
+    from rfsn_b200.archive import workspace_bytes
+
+    hot = 1 << 14
+    cache, k, v = make("bfloat16", 1, H, Hkv, 128, (), hot, hot_cap=hot, tile_index=True,
+                       archive_dtype="float8_e4m3fn" if packed else None)
+    q = queries(1, H, Lq, 128)
+    tiles = torch.zeros(64, 4, dtype=torch.int32, device="cuda")
+    call = native.ArchiveCallC(cache.arena.handle, cache.archive.handle if packed else None,
+                               cache.tile_bounds.data_ptr(), native.TileListC(tiles.data_ptr(), 0, 0),
+                               native.HotWindowC(0, hot, 0, hot, 0, 0, None), 1, H, Hkv, Lq, 4, 0)
+    nbytes = workspace_bytes(1, H, Hkv, Lq, 128, hot, 10, 4)
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(1, H, Lq, device="cuda")
+    native.check(native.lib().rfsn_archive_attend(ctypes.byref(call), q.data_ptr(), hot - Lq, out.data_ptr(),
+                                                  lse.data_ptr(), ws.data_ptr(), nbytes, native.stream_ptr()), "attend")
+    want, want_lse = ref.attention(q, k, v, torch.arange(hot), hot - Lq)
+    check_out(out, lse, want, want_lse, v)
