@@ -1196,9 +1196,10 @@ def _out_pointer(cache: LayerKVCache, out: torch.Tensor, shape: tuple) -> int:
         raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
     if out.device.type == "cpu":
         return native.host_device_pointer(out)
-    if out.device == cache.device or (cache.device.index is None and out.device.type == cache.device.type):
+    device = cache._arena_k.device  # cache.device may name no index
+    if out.device == device:
         return out.data_ptr()
-    raise ValueError(f"out must be on {cache.device} or pinned host memory")
+    raise ValueError(f"out must be on {device} or pinned host memory")
 
 
 def _hot_window(cache: LayerKVCache, segments: PagedSegments,
