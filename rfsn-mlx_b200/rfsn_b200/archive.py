@@ -134,8 +134,17 @@ class PackedArchive:
 
     def pack_ring(self, k: torch.Tensor, v: torch.Tensor, offset: int, wrap: int, row: int, count: int, *,
                   bounds: Optional[torch.Tensor] = None) -> None:
-        """``pack`` of ``count`` ring tokens: k, v [groups, ring rows, D], the
-        oldest token at ``offset``, wrapping at ``wrap``."""
+        """``pack`` of ``count`` ring tokens: k, v [groups, rows, D], the ring in
+        the first ``wrap`` rows, its oldest token at ``offset``."""
+        shape = k.shape
+        if len(shape) != 3 or v.shape != shape or v.dtype != k.dtype or shape[0] != self.groups \
+                or shape[2] != self.head_dim or k.stride(2) != 1 or v.stride(2) != 1:
+            raise ValueError(f"pack_ring needs k and v of one shape [{self.groups}, rows, {self.head_dim}] and one "
+                             "dtype, contiguous along the last dimension")
+        if k.device != self.device or v.device != self.device:
+            raise ValueError(f"K/V must be on {self.device}")
+        if not (0 < wrap <= shape[1] and 0 <= offset < wrap and 0 <= count <= wrap):
+            raise ValueError(f"{count} tokens from {offset} on do not lie in a ring of {wrap} of {shape[1]} rows")
         if bounds is not None:
             self._check_bounds(bounds)
         self._pack(kv_rows(k[None], v[None], offset, wrap), row, count, bounds)

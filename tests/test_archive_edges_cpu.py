@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from rfsn_b200.archive import workspace_bytes
+from rfsn_b200.archive import PackedArchive, workspace_bytes
 from rfsn_b200.cache import _out_pointer
 
 
@@ -40,3 +40,23 @@ def test_results_are_refused_on_another_gpu(named):
     for other in ("cuda:0", "cuda:2"):
         with pytest.raises(ValueError, match="out must be on cuda:1"):
             _out_pointer(cache, Placed(other), (1, 2, 1, 64))
+
+
+def test_ring_tokens_outside_the_tensors_are_refused():
+    """Before anything is launched: the kernel reads what it is told."""
+    a = object.__new__(PackedArchive)
+    a.device, a.groups, a.rows, a.head_dim, a.handle = torch.device("cpu"), 2, 128, 64, None
+    k = torch.zeros(2, 100, 64)
+    for offset, wrap, count in ((0, 101, 10), (100, 100, 1), (-1, 100, 1), (0, 100, 101), (0, 0, 1), (0, -5, 1),
+                                (60, 50, 10), (0, 100, -1)):
+        with pytest.raises(ValueError, match="ring of"):
+            a.pack_ring(k, k, offset, wrap, 0, count)
+    for bad in (k[:1], k[None], k[:, :, :32], k[:, :50], k.half(), k.transpose(1, 2).contiguous().transpose(1, 2)):
+        with pytest.raises(ValueError, match="pack_ring needs"):
+            a.pack_ring(k, bad, 0, 50, 0, 10)
+        with pytest.raises(ValueError, match="pack_ring needs"):
+            a.pack_ring(bad, k, 0, 50, 0, 10)
+    a.device = torch.device("cuda:0")
+    with pytest.raises(ValueError, match="must be on cuda:0"):
+        a.pack_ring(k, k, 0, 100, 0, 10)
+    a.handle = None  # nothing to destroy
