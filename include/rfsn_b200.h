@@ -445,7 +445,9 @@ RFSN_API rfsn_status rfsn_paged_attention_peer(const rfsn_arena* arena,
  * subnormal codes). NaN stays NaN; an infinity becomes NaN.
  *
  * k_codes, v_codes: device uint8 [batch_kv_heads][rows][head_dim], scales:
- * device float32 [batch_kv_heads][rows / 64][4] = {K scale, V scale, 0, 0}.
+ * device float32 [batch_kv_heads][rows / 64][4] = {K scale, V scale, zero, 0},
+ * zero = 1 where rfsn_pack_rows met no V but zeros (and NaN), else 0: such a
+ * tile's scale does not count among the sizes of V. Codes of other origin carry 0.
  * All 16-byte aligned; rows a multiple of 64; head_dim 64 or 128. A block
  * starts at a row that is a multiple of 64 and owns its last tile whole: the
  * rows of that tile behind the block's last token must hold zero codes

@@ -12,7 +12,7 @@
 struct rfsn_packed_archive {
     uint8_t* k;       // [groups][rows][head_dim] e4m3 codes
     uint8_t* v;
-    float4* scales;   // [groups][rows / 64] {K scale, V scale, 0, 0}
+    float4* scales;   // [groups][rows / 64] {K scale, V scale, 1 for a V tile of zeros, 0}
     int groups;
     int rows;
     int head_dim;
@@ -25,6 +25,7 @@ namespace rfsn {
 namespace archive {
 
 constexpr float kPScale = 128.f;  // p <= 2^8 (kLazy), p * 2^7 <= 2^15 fits float16
+constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the smallest scale
 constexpr float kLazy = 8.f;      // log2 units the running maximum may be exceeded by before it moves
 constexpr int kStageBytes = 16384;              // one item: 64 packed keys, or 32 (head_dim 64: 64) 16-bit keys
 constexpr int kMaxSplits128 = 240, kMaxSplits64 = 120;  // bounded by the merge weights kept in shared memory

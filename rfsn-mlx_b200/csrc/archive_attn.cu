@@ -551,7 +551,7 @@ archive_attn_kernel(const __grid_constant__ CUtensorMap mapK16, const __grid_con
                                  ? ((c[nb][0][2] + c[nb][1][2]) + (c[nb][0][3] + c[nb][1][3])) * f : -CUDART_INF_F;
                 }
                 uint32_t b[NB][2], b3[NB][2];
-                softmax_strip<__half, D, NB, false>(st, s0, s1, sc.y, b, b3);
+                softmax_strip<__half, D, NB, false>(st, s0, s1, sc.z == 0.f ? sc.y : kTiny, b, b3);  // z: V all zero
                 if (NB > 1) fetch_v();
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w) {

@@ -20,9 +20,9 @@
 // own unit u.
 //
 // The hot window (bf16 or f16 ring) is first copied by hot_half_kernel into
-// float16 tiles of 64 tokens with a power-of-two scale each: an element keeps
-// its 8 or 11 bits unless it is 2^-29 of its tile's maximum, so the main
-// kernel sees one kind of operand.
+// float16 tiles of 64 tokens with a power-of-two scale each (the smallest for a
+// tile of zeros): an element keeps its 8 or 11 bits unless it is 2^-29 of its
+// tile's maximum, so the main kernel sees one kind of operand.
 //
 // Measured: 512 rows over 16K packed tokens and 1K ring, 32 q / 8 KV heads, 248
 // us = 580 TFLOP/s useful, 1,160 executed; a tile of 128 keys takes 3,300 cycles
@@ -64,7 +64,6 @@ constexpr int kSoftmaxThreads = 256, kThreads = 512;
 constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;
 constexpr int kConvWarp = 8, kProducerWarp = 12, kMmaWarp = 13;
 constexpr int kMaxSplit = 32;  // key ranges of a unit
-constexpr float kTiny = 1.17549435e-38f;  // 2^-126
 constexpr float kMinF = 7.8886091e-31f;   // 2^-100
 constexpr uint32_t kTmemCols = 512, kColO = 256, kColQ = 384;  // q: hi, then lo, head_dim / 2 columns each
 
@@ -337,7 +336,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                 // lanes 2 j, 2 j + 1 fetch the two halves of tile base + j
                 const int t_mine = base + (lane >> 1), gt = t_lo + t_mine, half = lane & 1;
                 int row = 0, pos = 0, len = 0;
-                float sk = 1.f, sv = kTiny;  // a half without keys leaves the unit to the other one
+                float sk = 1.f, sv = kTiny;  // a half without keys or of zero V leaves the unit to the other one
                 if (t_mine < nt) {
                     if (gt < arch_tiles) {
                         const int i = 2 * gt + half;
@@ -352,7 +351,7 @@ chunk_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ 
                                 len = e.z;
                                 const float4 sc = __ldcg(p.scales + (size_t)bh * (p.packed_rows / kTile) + row / kTile);
                                 sk = sc.x;
-                                sv = sc.y;
+                                if (sc.z == 0.f) sv = sc.y;  // else a tile of zeros
                             }
                         }
                     } else {
@@ -727,6 +726,7 @@ __global__ void __launch_bounds__(256) hot_half_kernel(const T* __restrict__ k, 
     const T* src = (is_v ? v : k) + (size_t)bh * rows * D + 8 * c8;
     float x[kIters][8];
     float a = 0.f;
+    bool number = true;
 #pragma unroll
     for (int i = 0; i < kIters; ++i) {
         const int t = tile * kTile + r0 + kRows * i;
@@ -738,17 +738,19 @@ __global__ void __launch_bounds__(256) hot_half_kernel(const T* __restrict__ k, 
             x[i][j] = to_f32<T>(e[j]);
             const float y = fabsf(x[i][j]);
             a = fmaxf(a, y < CUDART_INF_F ? y : 0.f);
+            number &= y < CUDART_INF_F;
         }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
     __shared__ float part[8];
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-    __syncthreads();
+    number = __syncthreads_and(number);
     a = part[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) a = fmaxf(a, part[i]);
-    const int e = a > 0.f ? max((int)(__float_as_uint(a) >> 23) - 127 - 14, -126) : 0;
+    // a tile of zeros leaves the unit of V to the tile beside it
+    const int e = a > 0.f ? max((int)(__float_as_uint(a) >> 23) - 127 - 14, -126) : (number ? -126 : 0);
     const float s = __uint_as_float((uint32_t)(e + 127) << 23), inv = 1.f / s;
     __half* dst = (is_v ? vh : kh) + ((size_t)bh * hot_rows + tile * kTile) * D + 8 * c8;
 #pragma unroll

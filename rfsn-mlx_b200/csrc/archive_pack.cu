@@ -198,7 +198,11 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(RowSource ks, RowSou
             *reinterpret_cast<uint2*>(dst + (size_t)r * D) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
         }
         const size_t slot = (size_t)bh * (rows / kTile) + row0 / kTile;
-        if (threadIdx.x == 0) scales[4 * slot + is_v] = s;
+        if (threadIdx.x == 0) {
+            scales[4 * slot + is_v] = s;
+            // its scale of 1 says nothing about the size of V: the attention kernels leave it out of their units
+            if (is_v) scales[4 * slot + 2] = a > 0.f ? 0.f : 1.f;
+        }
         if constexpr (BOUNDS) {
             if (!bound) continue;
             // channel-wise smallest and largest code of the tile's keys

@@ -57,7 +57,6 @@ constexpr int kSoftmaxThreads = 256, kThreads = 320;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr uint32_t kTmemCols = 512, kBuf = 80;  // four S and two O buffers of up to 80 columns
 constexpr uint32_t kTmemS = 0, kTmemO = 4 * kBuf;
-constexpr float kTiny = 1.17549435e-38f;  // 2^-126
 constexpr float kMinF = 7.8886091e-31f;   // 2^-100
 
 struct Info {
@@ -279,7 +278,7 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
             // lanes 2 j, 2 j + 1 fetch the two halves of item base + j
             const int i = 2 * (a0 + base) + lane;
             int4 e = make_int4(0, 0, 0, 0);
-            float sk = 1.f, sv = kTiny;  // a half without keys leaves the unit to the other one
+            float sk = 1.f, sv = kTiny;  // a half without keys or of zero V leaves the unit to the other one
             if (base + (lane >> 1) < na && i < p.n_tiles) {
                 e = __ldcg(p.tiles + i);
                 if (e.x < 0 || e.z < 0 || e.z > kTile || (e.x & (kTile - 1)) != 0 || e.x > p.packed_rows - e.z) {
@@ -288,7 +287,7 @@ rows_kernel(const __grid_constant__ CUtensorMap mapK8, const __grid_constant__ C
                 } else if (e.z > 0) {
                     const float4 sc = __ldcg(p.scales + (size_t)bh * (p.packed_rows / kTile) + e.x / kTile);
                     sk = sc.x;
-                    sv = sc.y;
+                    if (sc.z == 0.f) sv = sc.y;  // else a tile of zeros
                 }
             }
             const int n = min(16, na - base);

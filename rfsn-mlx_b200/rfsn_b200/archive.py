@@ -82,7 +82,9 @@ class PackedArchive:
         shape = (self.groups, self.rows, self.head_dim)
         self.k = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
         self.v = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
-        self.scales = torch.ones((self.groups, self.rows // TILE, 4), dtype=torch.float32, device=dev)
+        # {K scale, V scale, mark of a V tile packed from zeros, 0} per tile
+        self.scales = torch.zeros((self.groups, self.rows // TILE, 4), dtype=torch.float32, device=dev)
+        self.scales[..., :2] = 1.0
         self.k_scale, self.v_scale = self.scales[..., 0], self.scales[..., 1]
         handle = ctypes.c_void_p()
         with native.on_device(dev):
@@ -108,7 +110,8 @@ class PackedArchive:
         """Zero codes and unit scales (the state of a new archive)."""
         self.k.view(torch.uint8).zero_()
         self.v.view(torch.uint8).zero_()
-        self.scales.fill_(1.0)
+        self.scales.zero_()
+        self.scales[..., :2] = 1.0
 
     def pack(self, k: torch.Tensor, v: torch.Tensor, row: int = 0, *,
              bounds: Optional[torch.Tensor] = None) -> None:

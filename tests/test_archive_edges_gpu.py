@@ -162,3 +162,92 @@ def test_a_selecting_call_over_no_tiles_fits_its_workspace(H, Hkv, Lq, packed):
                                                   lse.data_ptr(), ws.data_ptr(), nbytes, native.stream_ptr()), "attend")
     want, want_lse = ref.attention(q, k, v, torch.arange(hot), hot - Lq)
     check_out(out, lse, want, want_lse, v)
+
+
+# ------------------------------------------------------------------ tiles of zeros
+def with_values(lens, hot, D, change, Lq, dtype="bfloat16"):
+    """A packed cache of 8 / 2 heads whose V went through ``change`` before it was packed, its K and V as held."""
+    torch = _torch()
+    cache, _, _ = make(dtype, 1, 8, 2, D, (), 0, hot_cap=max(hot, 1), pool_tokens=sum(lens) + 64 * len(lens))
+    g = torch.Generator(device="cuda").manual_seed(Lq + D)
+    n = sum(lens) + hot
+    k, v = (torch.randn(1, 2, n, D, generator=g, device="cuda") for _ in range(2))
+    k, v = k.to(cache.dtype), change(v).to(cache.dtype)
+    at = 0
+    for length in lens:
+        cache.import_block(k[:, :, at:at + length], v[:, :, at:at + length], at)
+        at += length
+    cache.hot_start = at
+    if hot:
+        cache.append_exact(k[:, :, at:], v[:, :, at:])
+    return cache, k, v, *held(cache, k, v, lens)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("level", [1.0, 1e-2, 1e-6, 1e-30])
+@pytest.mark.parametrize("zero", [[0], [1], [2, 3], [0, 2, 4, 6, 8], [7], list(range(80)), [81], [82], [80, 81]])
+def test_tiles_of_zero_values_do_not_cost_the_others_precision(zero, level, D):
+    """Padded tokens: the V of whole tiles is zero, in the archive (tiles 0 to 80) or in the ring (81 and 82). Such a
+    tile has a scale of 1, which is no size of its values: with it as the unit, V of 1e-6 would keep a few bits."""
+    torch = _torch()
+    import archive_ref as ref
+
+    lens = (64,) * 81
+
+    def change(v):
+        v = v * level
+        for t in zero:
+            v[:, :, 64 * t:64 * t + 64] = 0
+        return v
+
+    for Lq in (1, 2, 4, 40, 128):  # the decode, rows and chunk kernels
+        cache, k, v, kk, vv = with_values(lens, 140, D, change, Lq)
+        q = queries(1, 8, Lq, D)
+        want, want_lse = ref.attention(q, kk, vv, torch.arange(5324), 5324 - Lq)
+        out, lse = cache.attend(q, 5324 - Lq, want_lse=True)
+        check_out(out, lse, want, want_lse, vv)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Lq", [1, 4, 128])
+@pytest.mark.parametrize("at", [70, 5184 + 70])
+def test_nan_among_zero_values_is_seen(at, Lq, D):
+    """NaN and infinities in a tile whose other values are zero reach their channel (an infinity is NaN in 8 bits)."""
+    torch = _torch()
+    lens = (64,) * 81
+    for bad in (float("nan"), float("inf")):
+        def change(v):
+            v[:, :, at // 64 * 64:at // 64 * 64 + 64] = 0
+            v[:, :, at, 5] = bad
+            return v
+
+        cache, *_ = with_values(lens, 140, D, change, Lq)
+        out = cache.attend(queries(1, 8, Lq, D), 5324 - Lq)
+        fine = torch.arange(D, device="cuda") != 5
+        sees = 5324 - Lq + torch.arange(Lq, device="cuda") >= at
+        assert bool(torch.isfinite(out[..., fine]).all()) and not bool(torch.isfinite(out[:, :, sees, 5]).any())
+
+
+def test_the_mark_of_zero_values():
+    """The third entry of a tile's scales: 1 for a V tile packed from zeros, 0 for any other and for K."""
+    torch = _torch()
+    from rfsn_b200 import PackedArchive
+
+    a = PackedArchive(2, 256, 64)
+    assert not a.scales[..., 2:].any() and bool((a.scales[..., :2] == 1).all())
+    x = torch.ones(1, 2, 200, 64, device="cuda")
+    y = x.clone()
+    y[0, 1, 64:128] = 0
+    y[0, 0, 192:] = 0
+    y[0, 0, 195, 3] = float("nan")
+    a.pack(y, x)
+    assert not a.scales[..., 2].any()
+    a.pack(x, y)
+    want = torch.zeros(2, 4)
+    want[1, 1] = want[0, 3] = 1
+    assert torch.equal(a.scales[..., 2].cpu(), want)
+    a.pack(x, x)
+    assert not a.scales[..., 2:].any()
+    a.pack(x, y)
+    a.clear()
+    assert not a.scales[..., 2:].any() and bool((a.scales[..., :2] == 1).all())
