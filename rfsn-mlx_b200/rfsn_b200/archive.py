@@ -218,6 +218,8 @@ class PreparedCall:
             raise ValueError(f"top_tiles takes up to {SPARSE_MAX_ROWS} query rows a call, got {q_len}")
         tiles_dev, n_tiles = segments.tile_list
         archive, bounds = cache.archive, cache.tile_bounds
+        if not cache.arena.handle or (archive is not None and not archive.handle):
+            raise ValueError("the cache's arena or packed archive has been closed")
         call = native.ArchiveCallC(
             cache.arena.handle, archive.handle if archive is not None else None,
             bounds.data_ptr() if top_tiles else None, native.TileListC(tiles_dev.data_ptr(), n_tiles, 0), hot,
@@ -230,8 +232,10 @@ class PreparedCall:
         self.keep = (call, cache.arena, archive, bounds, tiles_dev)
 
     def current(self, cache) -> bool:
-        """The cache's buffers are still the ones this call points to."""
-        return self.keep[1] is cache.arena and self.keep[2] is cache.archive
+        """The cache's buffers are still the ones this call points to, and open."""
+        arena, archive = self.keep[1], self.keep[2]
+        return arena is cache.arena and archive is cache.archive and bool(arena.handle) \
+            and (archive is None or bool(archive.handle))
 
     def __call__(self, cache, q_ptr: int, q_start_pos: int, out_ptr: int, lse_ptr: Optional[int],
                  workspace: Optional[native.Workspace]) -> None:

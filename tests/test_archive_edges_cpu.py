@@ -1,11 +1,13 @@
 """Packed archives and tile lists without a GPU: sizes and refusals at the edges."""
 
+import ctypes
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from rfsn_b200.archive import PackedArchive, workspace_bytes
+from rfsn_b200 import _native as native
+from rfsn_b200.archive import PackedArchive, PreparedCall, workspace_bytes
 from rfsn_b200.cache import _out_pointer
 
 
@@ -60,3 +62,29 @@ def test_ring_tokens_outside_the_tensors_are_refused():
     with pytest.raises(ValueError, match="must be on cuda:0"):
         a.pack_ring(k, k, 0, 100, 0, 10)
     a.handle = None  # nothing to destroy
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_a_prepared_call_does_not_outlive_what_it_points_to(packed):
+    """Prepared calls hold the handles of the arena and the archive by value: closed ones are refused."""
+    arena = SimpleNamespace(handle=ctypes.c_void_p(4096))
+    archive = SimpleNamespace(handle=ctypes.c_void_p(8192)) if packed else None
+    cache = SimpleNamespace(arena=arena, archive=archive, tile_bounds=torch.zeros(16), batch_size=1, num_kv_heads=2,
+                            config=SimpleNamespace(head_dim=64, hot_capacity=64), device=torch.device("cpu"))
+    segments = SimpleNamespace(tile_list=(torch.zeros(4, 4, dtype=torch.int32), 4))
+
+    def prepare():
+        return PreparedCall(cache, segments, native.HotWindowC(), 8, 1, 2, 0)
+
+    call = prepare()
+    assert call.current(cache)
+    closed = [arena, archive] if packed else [arena]
+    for part in closed:
+        saved, part.handle = part.handle, ctypes.c_void_p()
+        assert not call.current(cache)
+        with pytest.raises(ValueError, match="closed"):
+            prepare()
+        part.handle = saved
+    assert call.current(cache)
+    cache.arena = SimpleNamespace(handle=arena.handle)
+    assert not call.current(cache)
