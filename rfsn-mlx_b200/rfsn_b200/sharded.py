@@ -149,12 +149,18 @@ class PeerGroup:
             self.handle = ctypes.c_void_p()
 
 
+def _refuse_selection(cache: LayerKVCache) -> None:
+    if cache.top_tiles:
+        raise NotImplementedError("sharded decode attends to every tile of its shard: no cache with top_tiles")
+
+
 def sharded_decode_step(cache: LayerKVCache, q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tensor],
                         pos: int, *, owns_hot: bool, group: Optional[dist.ProcessGroup] = None,
                         peers: Optional[PeerGroup] = None) -> torch.Tensor:
     """One decode token of one layer on this rank's shard; returns the merged
     float32 output [B, H, 1, D] on every rank. With ``peers`` the merge is
     fused into the attention kernel (NVLink); otherwise it goes through NCCL."""
+    _refuse_selection(cache)
     if owns_hot:
         cache.evict_for_append(int(k.shape[2]))
         q_rot = cache.append_rope(q, k, v, pos)
@@ -193,6 +199,7 @@ class GraphedShardedDecodeStep:
     def __init__(self, cache: LayerKVCache, q_heads: int, *, owns_hot: bool, peers: PeerGroup) -> None:
         from .layer import GraphedDecodeStep  # staging layout and capture helper
 
+        _refuse_selection(cache)
         self.cache = cache
         self.owns_hot = owns_hot
         self.peers = peers

@@ -9,6 +9,7 @@ import torch
 from rfsn_b200 import _native as native
 from rfsn_b200.archive import PackedArchive, PreparedCall, workspace_bytes
 from rfsn_b200.cache import _out_pointer
+from rfsn_b200.sharded import GraphedShardedDecodeStep, sharded_decode_step
 
 
 @pytest.mark.parametrize("head_dim", [64, 128])
@@ -88,3 +89,14 @@ def test_a_prepared_call_does_not_outlive_what_it_points_to(packed):
     assert call.current(cache)
     cache.arena = SimpleNamespace(handle=arena.handle)
     assert not call.current(cache)
+
+
+def test_sharded_decode_refuses_a_cache_that_selects():
+    """It reads every tile of each rank's shard; dropping the option in silence would be another result."""
+    cache = SimpleNamespace(top_tiles=3)
+    x = torch.zeros(1, 2, 1, 64)
+    for owns_hot in (True, False):
+        with pytest.raises(NotImplementedError, match="top_tiles"):
+            sharded_decode_step(cache, x, x, x, 0, owns_hot=owns_hot)
+        with pytest.raises(NotImplementedError, match="top_tiles"):
+            GraphedShardedDecodeStep(cache, 2, owns_hot=owns_hot, peers=None)
