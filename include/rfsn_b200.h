@@ -500,7 +500,12 @@ RFSN_API rfsn_status rfsn_unpack_rows(const rfsn_packed_archive* archive, int sr
  *     q_heads / kv_heads; 8 with head_dim 64 or short contexts), for every 128
  *     where that is faster; else once for every 8.
  * Scores are accurate to float32 rounding (q and p are split into two float16
- * or three bfloat16 terms for the tensor cores).
+ * or three bfloat16 terms, or five e4m3 ones, for the tensor cores). Over a
+ * packed archive p is split relative to the largest V scale among tiles that are
+ * taken together (pairs of tiles, or those of a warp), so an output is accurate
+ * relative to the largest |V| of the tiles that the rows computed together see:
+ * where a tile's V scale is 2^-r of a neighbour's, its p keeps about 30 - r bits
+ * (22 at most).
  * A key behind a row's position changes nothing in it, with one exception: a
  * NaN or infinity in its V reaches the rows that are computed together with a
  * row that does see it (0 * NaN), so finite V is asked for where q_len > 1.

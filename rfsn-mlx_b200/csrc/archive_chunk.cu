@@ -24,10 +24,11 @@
 // tile of zeros): an element keeps its 8 or 11 bits unless it is 2^-29 of its
 // tile's maximum, so the main kernel sees one kind of operand.
 //
-// Measured: 512 rows over 16K packed tokens and 1K ring, 32 q / 8 KV heads, 248
-// us = 580 TFLOP/s useful, 1,160 executed; a tile of 128 keys takes 3,300 cycles
-// of which the products are 2,050 at full rate. They are issued by a converged
-// warp and its elected lane: from a one-lane branch the same kernel took 287 us.
+// Measured: 512 rows over 16K packed tokens and 1K ring, 32 q / 8 KV heads, 249
+// us back to back = 580 TFLOP/s useful, 1,160 executed (273 us and 527 with other
+// work between the calls); a tile of 128 keys takes 3,300 cycles of which the
+// products are 2,050 at full rate. They are issued by a converged warp and its
+// elected lane: from a one-lane branch the same kernel took 287 us.
 // head_dim 64, 256 rows of 32 heads over 16K: 116 us (743 in passes of 8 slots).
 //
 // Warps (512 threads, registers shifted to the softmax warps by setmaxnreg):

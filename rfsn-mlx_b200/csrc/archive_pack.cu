@@ -23,7 +23,7 @@ namespace rfsn {
 namespace archive {
 
 constexpr int kPackThreads = 256;
-constexpr int kPackCtas = 8;  // per SM: 65,501 tokens of 8 heads 67.8 us (3: 74.5, 4: 72.1, 6: 77.6)
+constexpr int kPackCtas = 8;  // per SM: 65,501 tokens of 8 heads 67.8 us (3: 74.5, 4: 72.1, 6: 77.6, not in order)
 
 struct RowSource {
     const void* p;
@@ -98,7 +98,9 @@ __device__ __forceinline__ float tile_scale(float a) {
 // between the maximum and the conversion, so it is read once, and the next
 // item's tile is requested before this one is converted. Items are numbered K
 // and V fastest, then the heads, so that the CTAs that run together read
-// neighbouring rows of token-major sources. Bound by memory. Rows of the tile
+// neighbouring rows of token-major sources. Bound by memory (65,501 tokens of 8
+// heads 67 us, 93 % of the copy rate); with key bounds by their reduction through
+// shared memory (99 us; 256 tokens 2.5 against 2.1). Rows of the tile
 // behind `count` become zero codes (the attention kernels read whole tiles and
 // multiply them by zero weights).
 template <typename T, int D, bool BOUNDS>
@@ -233,7 +235,8 @@ template <> __device__ __forceinline__ __half unpacked<__half>(float x) {
     return __float2half_rn(x);
 }
 
-// 16 codes per thread: one 16-byte load, 32 (64) bytes stored. Bound by memory.
+// 16 codes per thread: one 16-byte load, 32 (64) bytes stored. Bound by memory:
+// 65,501 tokens of 8 heads to bf16 69.7 us, 89 % of the copy rate.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                      const float4* __restrict__ scales, T* __restrict__ ko,
@@ -264,7 +267,9 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__
 }
 
 // Channel-wise smallest and largest key of each tile of an exact (16-bit)
-// block: one CTA per (tile, KV head); NaN keys give NaN bounds.
+// block: one CTA per (tile, KV head); NaN keys give NaN bounds. Bound by the
+// chain load, reduction, barrier of each CTA: 65,536 tokens of 8 heads 56 us (21 at
+// the copy rate), 256 tokens 3.3.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) bounds_kernel(const T* __restrict__ k, T* __restrict__ bounds, int rows,
                                                      int row0, int count) {

@@ -14,7 +14,7 @@
 //
 // One launch: each CTA scores a range of tiles of one list and the last CTA
 // of the list to arrive selects. Bound by the chain of launch, bounds, arrival
-// and counts: 128 of 2,064 tiles 8.9 us, 16 of 96 6.4 us (32 q / 8 KV heads);
+// and counts: 128 of 2,064 tiles 9.1 us, 16 of 96 6.6 us (32 q / 8 KV heads);
 // the bounds (8.4 MB at 132K tokens) are 1.3 us of HBM time.
 #include <math_constants.h>
 

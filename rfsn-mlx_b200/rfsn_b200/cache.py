@@ -1220,7 +1220,8 @@ def _tile_attention(cache: LayerKVCache, q: torch.Tensor, q_start_pos: int, segm
                     step_state: Optional[torch.Tensor], out: Optional[torch.Tensor], top_tiles: int):
     """``paged_attention`` of packed caches and of calls that select tiles. The
     part of a call that does not depend on the query is prepared once per
-    segments and shape: a decode step's host work is a few microseconds."""
+    segments and shape; a step that takes new segments for each token prepares
+    it again (about 5 us of host work), a captured step does not."""
     if peers is not None:
         raise NotImplementedError("the merge across GPUs inside the kernel reads exact archives in full: no packed "
                                   "archive and no tile selection")
